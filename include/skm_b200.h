@@ -309,6 +309,69 @@ skm_status skm_op_pdxify(int device, const float* in, uint64_t n, uint64_t d, fl
 skm_status skm_op_find_nearest_noalloc(int device, const float* x_dev, const float* y_dev, uint64_t n, uint64_t k, uint64_t d, uint32_t* out_knn_dev, float* out_dist_dev,
                                        void* cuda_stream);
 
+/* ---- operators on rows in device memory, for programs that use clusters inside a model: vectors of a codebook by
+ * assignment and the codebook's gradient, rows to their clusters and back, products in 8 bits.  The reference has no counterpart.
+ *
+ * All pointers are DEVICE memory of `device` (-1 = the current device); cuda_stream is a cudaStream_t of that device (NULL = the
+ * default stream).  The calls return when the work is on the stream: they allocate nothing, wait for nothing and can be captured into
+ * a CUDA graph.  What a call needs beside its arguments is a workspace (256-byte aligned) of the size that the function of the same
+ * name with _workspace answers with; it may be used again as soon as the work on the stream is done with it, so that calls that can
+ * overlap (two streams, two graphs that are replayed at once) have one each.
+ *
+ * Values of rows have one of the types below; sums and products are in fp32 and rounded once.  `ld_*` is the number of elements from
+ * one row to the next; outputs are contiguous.  Cluster numbers (ids) are int32, uint32 (ids_bits 32) or int64 (64); one outside
+ * [0, k) stands for no cluster.  k and the number of ids stay below 2^31. */
+typedef enum skm_dtype { SKM_F32 = 0, SKM_F16 = 1, SKM_BF16 = 2 } skm_dtype;
+
+/* out[i] = scale * row_scales[i] * table[ids[i]] for i < n: table k x d, row_scales n (fp32) or NULL, out n x d.  An id that is no row of
+ * the table gives a row of zeros. */
+skm_status skm_op_lookup(int device, const void* table, uint64_t ld_table, int dtype, uint64_t k, uint64_t d, const void* ids, int ids_bits, uint64_t n, float scale,
+                         const float* row_scales, void* out, void* cuda_stream);
+/* Gradient of the table: out[c] = sum of scale * row_scales[i] * grad[i] over ids[i] = c, zeros for a row that nobody took.  The sums are made
+ * in an order that depends on the ids alone: the same call gives the same bits.  grad n x d of `dtype`, out k x d of `out_dtype`, which is
+ * `dtype` or SKM_F32. */
+uint64_t skm_op_lookup_grad_workspace(uint64_t n, uint64_t k, uint64_t d, int dtype);
+skm_status skm_op_lookup_grad(int device, const void* grad, uint64_t ld_grad, int dtype, uint64_t k, uint64_t d, const void* ids, int ids_bits, uint64_t n, float scale,
+                              const float* row_scales, void* out, int out_dtype, void* workspace, uint64_t workspace_bytes, void* cuda_stream);
+/* Gradient of row_scales: out[i] = scale * <grad[i], table[ids[i]]>, 0 where the id is none. */
+skm_status skm_op_lookup_scale_grad(int device, const void* grad, uint64_t ld_grad, const void* table, uint64_t ld_table, int dtype, uint64_t k, uint64_t d, const void* ids,
+                                    int ids_bits, uint64_t n, float scale, float* out, void* cuda_stream);
+
+/* The order of n ids by cluster, equal ones in their own order, those without a cluster last: order[slot] = which id, position[i] = its
+ * slot, offsets[c] = the first slot of cluster c for c <= k (offsets[k]: how many have a cluster). */
+uint64_t skm_op_group_rows_workspace(uint64_t n, uint64_t k);
+skm_status skm_op_group_rows(int device, const void* ids, int ids_bits, uint64_t n, uint64_t k, uint32_t* order, uint32_t* position, uint32_t* offsets, void* workspace,
+                             uint64_t workspace_bytes, void* cuda_stream);
+/* Rows to the slots of their clusters, m choices to a row: out[position[i * m + j]] = x[i]; x n x d, out n * m x d.  Slots of choices without a
+ * cluster get zeros. */
+skm_status skm_op_to_clusters(int device, const void* x, uint64_t ld_x, int dtype, uint64_t d, const uint32_t* position, const uint32_t* offsets, uint64_t k, uint64_t n, uint64_t m,
+                              void* out, void* cuda_stream);
+/* ... and back: out[i] = sum over j of weights[i * m + j] * y[position[i * m + j]], without the choices that have no cluster; weights n x m
+ * (fp32) or NULL for ones, y n * m x d, out n x d.  With weights NULL it is also the gradient of skm_op_to_clusters. */
+skm_status skm_op_from_clusters(int device, const void* y, uint64_t ld_y, int dtype, uint64_t d, const uint32_t* position, const uint32_t* offsets, uint64_t k, uint64_t n, uint64_t m,
+                                const float* weights, void* out, void* cuda_stream);
+/* Its gradients: grad_y[position[i * m + j]] = weights[i * m + j] * grad[i] (zeros in the slots of choices without a cluster) and
+ * grad_weights[i * m + j] = <grad[i], y[position[i * m + j]]> (fp32; 0 without a cluster).  Either may be NULL; y is read for grad_weights. */
+skm_status skm_op_from_clusters_grad(int device, const void* grad, uint64_t ld_grad, const void* y, uint64_t ld_y, int dtype, uint64_t d, const uint32_t* position,
+                                     const uint32_t* offsets, uint64_t k, uint64_t n, uint64_t m, const float* weights, void* grad_y, float* grad_weights, void* cuda_stream);
+
+/* Rows in 8 bits with a scale each: scales[i] = max_j |x[i][j]| / 127, q[i][j] = x[i][j] * (127 / max) rounded to the nearest whole number (both
+ * steps in fp32).  A row of zeros has scale 0; a row with a value that is no finite number has scale NaN and zeros.  ld_q in bytes: a
+ * multiple of 16 saves skm_op_product_8bit a copy. */
+skm_status skm_op_quantize_rows(int device, const void* x, uint64_t ld_x, int dtype, uint64_t n, uint64_t d, int8_t* q, uint64_t ld_q, float* scales, void* cuda_stream);
+/* out[i][c] = x_scales[i] * w_scales[c] * sum_j x[i][j] * w[c][j]: x n x d, w m x d, signed bytes; d up to 131071, so that every sum is exact
+ * in 32 bits.  With groups > 0, w holds that many matrices, one after the other (m rows of ld_w bytes each), w_scales as many vectors, and rows
+ * offsets[g] .. offsets[g + 1] - 1 of x (offsets ascending, groups + 1 of them, from skm_op_group_rows) are multiplied by matrix g; rows
+ * that belong to no group come out as zeros.  out n x m of out_dtype.
+ *
+ * Every wait inside the kernel is bounded (see skm_debug_wait_injection).  One that runs out is reported as SKM_CUDA_ERROR by the
+ * next call of skm_op_product_8bit on the device that is made after the kernel ended, or by skm_op_product_8bit_status, which waits for the
+ * stream.  A program that captures its first product into a graph may do so: what the report needs is allocated then. */
+uint64_t skm_op_product_8bit_workspace(const int8_t* x, uint64_t ld_x, const int8_t* w, uint64_t ld_w, uint64_t n, uint64_t m, uint64_t d, uint64_t groups);
+skm_status skm_op_product_8bit(int device, const int8_t* x, uint64_t ld_x, const float* x_scales, const int8_t* w, uint64_t ld_w, const float* w_scales, uint64_t n, uint64_t m,
+                               uint64_t d, uint64_t groups, const uint32_t* offsets, void* out, int out_dtype, void* workspace, uint64_t workspace_bytes, void* cuda_stream);
+skm_status skm_op_product_8bit_status(int device, void* cuda_stream);
+
 /* ---- host-side decisions of the path (no GPU needed) ---------------------------------------- */
 
 /* PDXLayout::GetDimensionSplit (layout.h:115-140). */

@@ -123,6 +123,24 @@ SIGNATURES = {
     "skm_op_find_nearest_noalloc": (C.c_int, [C.c_int, C.c_void_p, C.c_void_p, C.c_uint64, C.c_uint64, C.c_uint64, C.c_void_p, C.c_void_p, C.c_void_p]),
     "skm_op_find_nearest_pruned": (C.c_int, [C.c_int, f32p, f32p, C.c_uint64, C.c_uint64, C.c_uint64, C.c_float, C.c_uint32, u32p, f32p, u64p]),
     "skm_op_update_centroids": (C.c_int, [C.c_int, f32p, u32p, C.c_void_p, C.c_uint64, C.c_uint64, C.c_uint64, f32p, u32p, C.POINTER(C.c_double)]),
+    "skm_op_lookup": (C.c_int, [C.c_int, C.c_void_p, C.c_uint64, C.c_int, C.c_uint64, C.c_uint64, C.c_void_p, C.c_int, C.c_uint64, C.c_float, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "skm_op_lookup_grad_workspace": (C.c_uint64, [C.c_uint64, C.c_uint64, C.c_uint64, C.c_int]),
+    "skm_op_lookup_grad": (C.c_int, [C.c_int, C.c_void_p, C.c_uint64, C.c_int, C.c_uint64, C.c_uint64, C.c_void_p, C.c_int, C.c_uint64, C.c_float, C.c_void_p, C.c_void_p, C.c_int,
+                                     C.c_void_p, C.c_uint64, C.c_void_p]),
+    "skm_op_lookup_scale_grad": (C.c_int, [C.c_int, C.c_void_p, C.c_uint64, C.c_void_p, C.c_uint64, C.c_int, C.c_uint64, C.c_uint64, C.c_void_p, C.c_int, C.c_uint64, C.c_float,
+                                           C.c_void_p, C.c_void_p]),
+    "skm_op_group_rows_workspace": (C.c_uint64, [C.c_uint64, C.c_uint64]),
+    "skm_op_group_rows": (C.c_int, [C.c_int, C.c_void_p, C.c_int, C.c_uint64, C.c_uint64, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint64, C.c_void_p]),
+    "skm_op_to_clusters": (C.c_int, [C.c_int, C.c_void_p, C.c_uint64, C.c_int, C.c_uint64, C.c_void_p, C.c_void_p, C.c_uint64, C.c_uint64, C.c_uint64, C.c_void_p, C.c_void_p]),
+    "skm_op_from_clusters": (C.c_int, [C.c_int, C.c_void_p, C.c_uint64, C.c_int, C.c_uint64, C.c_void_p, C.c_void_p, C.c_uint64, C.c_uint64, C.c_uint64, C.c_void_p, C.c_void_p,
+                                       C.c_void_p]),
+    "skm_op_from_clusters_grad": (C.c_int, [C.c_int, C.c_void_p, C.c_uint64, C.c_void_p, C.c_uint64, C.c_int, C.c_uint64, C.c_void_p, C.c_void_p, C.c_uint64, C.c_uint64, C.c_uint64,
+                                            C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "skm_op_quantize_rows": (C.c_int, [C.c_int, C.c_void_p, C.c_uint64, C.c_int, C.c_uint64, C.c_uint64, C.c_void_p, C.c_uint64, C.c_void_p, C.c_void_p]),
+    "skm_op_product_8bit_workspace": (C.c_uint64, [C.c_void_p, C.c_uint64, C.c_void_p, C.c_uint64, C.c_uint64, C.c_uint64, C.c_uint64, C.c_uint64]),
+    "skm_op_product_8bit": (C.c_int, [C.c_int, C.c_void_p, C.c_uint64, C.c_void_p, C.c_void_p, C.c_uint64, C.c_void_p, C.c_uint64, C.c_uint64, C.c_uint64, C.c_uint64, C.c_void_p,
+                                      C.c_void_p, C.c_int, C.c_void_p, C.c_uint64, C.c_void_p]),
+    "skm_op_product_8bit_status": (C.c_int, [C.c_int, C.c_void_p]),
     "skm_op_pdxify": (C.c_int, [C.c_int, f32p, C.c_uint64, C.c_uint64, f32p]),
     "skm_host_dimension_split": (None, [C.c_uint64, C.POINTER(C.c_uint64), C.POINTER(C.c_uint64)]),
     "skm_host_ratios": (None, [C.c_uint64, C.c_float, f32p]),

@@ -1,5 +1,6 @@
 // extern "C" surface of libskm_b200.so (declared in include/skm_b200.h): translates between the C
 // ABI and the Engine class, and between C++ exceptions and status codes.
+#include <algorithm>
 #include <cstring>
 #include <memory>
 #include <new>
@@ -8,6 +9,7 @@
 #include "engine.h"
 #include "noalloc.h"
 #include "kernels_tc.cuh"
+#include "rows.h"
 
 using skmb::Engine;
 
@@ -48,6 +50,79 @@ skm_status guarded(std::string& err, F&& f) {
 }
 
 thread_local std::string g_op_error;
+
+// ---- arguments of the operators on rows in device memory
+namespace rows = skmb::rows;
+
+void need(bool ok, const char* what) {
+    if (!ok) throw std::invalid_argument(what);
+}
+
+rows::Type type_of(int dtype) {
+    need(dtype >= 0 && dtype <= 2, "dtype must be SKM_F32, SKM_F16 or SKM_BF16");
+    return static_cast<rows::Type>(dtype);
+}
+
+rows::Ids ids_of(const void* ids, int bits, uint64_t n) {
+    need(bits == 32 || bits == 64, "ids_bits must be 32 or 64");
+    need(ids || n == 0, "ids must not be NULL");
+    return {ids, bits == 64};
+}
+
+void check_sizes(uint64_t n, uint64_t k) {
+    need(k > 0 && k < 0x7fffffff, "the number of clusters must be positive and below 2^31 - 1");
+    need(n <= 0x7fffffff, "no more than 2^31 - 1 ids");
+}
+
+void check_width(uint64_t d) { need(d > 0 && d <= 0x1fffffff, "the dimensionality must be positive and below 2^29"); }
+
+void check_workspace(const void* workspace, uint64_t given, uint64_t needed) {
+    need(given >= needed, "the workspace is too small");
+    need(needed == 0 || (workspace && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0), "the workspace must be 256-byte aligned device memory");
+}
+
+rows::Places places_of(const uint32_t* position, const uint32_t* offsets, uint64_t k, uint64_t n, uint64_t m) {
+    need(m > 0, "a row must have at least one choice");
+    need(n <= 0x7fffffff / m, "no more than 2^31 - 1 choices");
+    check_sizes(n * m, k);
+    need(n == 0 || (position && offsets), "position and offsets must not be NULL");
+    return {position, offsets ? offsets + k : nullptr, n, m};
+}
+
+rows::Product product_of(const int8_t* x, uint64_t ld_x, const int8_t* w, uint64_t ld_w, uint64_t n, uint64_t m, uint64_t d, uint64_t groups) {
+    need(d > 0 && d <= rows::kMaxProductDepth, "the dimensionality of a product in 8 bits must be positive and at most 131071");
+    need(n <= 0x7fffffff, "no more than 2^31 - 1 rows");
+    need(m <= 0x7fffff80 && (groups == 0 || m * groups <= 0x7fffff80) && groups <= 0x7fffff80, "too many rows of w");
+    rows::Product p{};
+    p.x = x;
+    p.ldx = n > 1 ? ld_x : (d + 15) / 16 * 16;   // (a single row has no next one)
+    p.w = w;
+    p.ldw = m * std::max<uint64_t>(1, groups) > 1 ? ld_w : (d + 15) / 16 * 16;
+    p.n = n;
+    p.m = m;
+    p.d = d;
+    p.groups = groups;
+    return p;
+}
+
+template <class F>
+skm_status row_op(F&& f) {
+    g_create_error.clear();
+    return guarded(g_op_error, f);
+}
+
+// Work of a call whose arguments are fine.
+struct Here {
+    int device = 0;
+    skmb::DeviceScope scope;
+    explicit Here(int wanted) : device(of(wanted)), scope(device) {}
+    static int of(int wanted) {
+        if (wanted < 0) SKM_CUDA(cudaGetDevice(&wanted));
+        return wanted;
+    }
+};
+
+cudaStream_t stream_of(void* s) { return static_cast<cudaStream_t>(s); }
 
 } // namespace
 
@@ -339,6 +414,149 @@ skm_status skm_op_find_nearest_noalloc(int device, const float* x_dev, const flo
                                        void* cuda_stream) {
     g_create_error.clear();
     return guarded(g_op_error, [&] { skmb::noalloc::find_nearest(device, x_dev, y_dev, n, k, d, out_knn_dev, out_dist_dev, static_cast<cudaStream_t>(cuda_stream)); });
+}
+
+// ---- operators on rows in device memory (rows_group.cu, rows_move.cu, rows_sum.cu, product_8bit.cu) ------
+skm_status skm_op_lookup(int device, const void* table, uint64_t ld_table, int dtype, uint64_t k, uint64_t d, const void* ids, int ids_bits, uint64_t n, float scale,
+                         const float* row_scales, void* out, void* cuda_stream) {
+    return row_op([&] {
+        const rows::Type type = type_of(dtype);
+        const rows::Ids at = ids_of(ids, ids_bits, n);
+        check_sizes(n, k);
+        check_width(d);
+        need(n == 0 || (table && out), "table and out must not be NULL");
+        const Here here(device);
+        rows::launch_lookup({table, ld_table}, type, k, d, at, n, scale, row_scales, out, stream_of(cuda_stream));
+    });
+}
+
+uint64_t skm_op_lookup_grad_workspace(uint64_t n, uint64_t k, uint64_t d, int dtype) {
+    return rows::lookup_grad_workspace_bytes(n, k, d, dtype == SKM_F32 ? rows::Type::f32 : rows::Type::f16);
+}
+
+skm_status skm_op_lookup_grad(int device, const void* grad, uint64_t ld_grad, int dtype, uint64_t k, uint64_t d, const void* ids, int ids_bits, uint64_t n, float scale,
+                              const float* row_scales, void* out, int out_dtype, void* workspace, uint64_t workspace_bytes, void* cuda_stream) {
+    return row_op([&] {
+        const rows::Type type = type_of(dtype), out_type = type_of(out_dtype);
+        need(out_type == type || out_type == rows::Type::f32, "the gradient of a table has the type of the rows' gradient or fp32");
+        const rows::Ids at = ids_of(ids, ids_bits, n);
+        check_sizes(n, k);
+        check_width(d);
+        need(out && (grad || n == 0), "grad and out must not be NULL");
+        if (n > 0) check_workspace(workspace, workspace_bytes, rows::lookup_grad_workspace_bytes(n, k, d, type));
+        const Here here(device);
+        rows::launch_lookup_grad({grad, ld_grad}, type, k, d, at, n, scale, row_scales, out, out_type, workspace, stream_of(cuda_stream));
+    });
+}
+
+skm_status skm_op_lookup_scale_grad(int device, const void* grad, uint64_t ld_grad, const void* table, uint64_t ld_table, int dtype, uint64_t k, uint64_t d, const void* ids,
+                                    int ids_bits, uint64_t n, float scale, float* out, void* cuda_stream) {
+    return row_op([&] {
+        const rows::Type type = type_of(dtype);
+        const rows::Ids at = ids_of(ids, ids_bits, n);
+        check_sizes(n, k);
+        check_width(d);
+        need(n == 0 || (grad && table && out), "grad, table and out must not be NULL");
+        const Here here(device);
+        rows::launch_lookup_scale_grad({grad, ld_grad}, {table, ld_table}, type, k, d, at, n, scale, out, stream_of(cuda_stream));
+    });
+}
+
+uint64_t skm_op_group_rows_workspace(uint64_t n, uint64_t k) { return rows::group_workspace_bytes(n, k); }
+
+skm_status skm_op_group_rows(int device, const void* ids, int ids_bits, uint64_t n, uint64_t k, uint32_t* order, uint32_t* position, uint32_t* offsets, void* workspace,
+                             uint64_t workspace_bytes, void* cuda_stream) {
+    return row_op([&] {
+        const rows::Ids at = ids_of(ids, ids_bits, n);
+        check_sizes(n, k);
+        need(offsets && (n == 0 || (order && position)), "order, position and offsets must not be NULL");
+        check_workspace(workspace, workspace_bytes, rows::group_workspace_bytes(n, k));
+        const Here here(device);
+        rows::launch_group(at, n, k, order, position, nullptr, offsets, workspace, stream_of(cuda_stream));
+    });
+}
+
+skm_status skm_op_to_clusters(int device, const void* x, uint64_t ld_x, int dtype, uint64_t d, const uint32_t* position, const uint32_t* offsets, uint64_t k, uint64_t n, uint64_t m,
+                              void* out, void* cuda_stream) {
+    return row_op([&] {
+        const rows::Type type = type_of(dtype);
+        check_width(d);
+        const rows::Places at = places_of(position, offsets, k, n, m);
+        need(n == 0 || (x && out), "x and out must not be NULL");
+        const Here here(device);
+        rows::launch_to_clusters({x, ld_x}, type, d, at, out, stream_of(cuda_stream));
+    });
+}
+
+skm_status skm_op_from_clusters(int device, const void* y, uint64_t ld_y, int dtype, uint64_t d, const uint32_t* position, const uint32_t* offsets, uint64_t k, uint64_t n, uint64_t m,
+                                const float* weights, void* out, void* cuda_stream) {
+    return row_op([&] {
+        const rows::Type type = type_of(dtype);
+        check_width(d);
+        const rows::Places at = places_of(position, offsets, k, n, m);
+        need(n == 0 || (y && out), "y and out must not be NULL");
+        const Here here(device);
+        rows::launch_from_clusters({y, ld_y}, type, d, at, weights, out, stream_of(cuda_stream));
+    });
+}
+
+skm_status skm_op_from_clusters_grad(int device, const void* grad, uint64_t ld_grad, const void* y, uint64_t ld_y, int dtype, uint64_t d, const uint32_t* position,
+                                     const uint32_t* offsets, uint64_t k, uint64_t n, uint64_t m, const float* weights, void* grad_y, float* grad_weights, void* cuda_stream) {
+    return row_op([&] {
+        const rows::Type type = type_of(dtype);
+        check_width(d);
+        const rows::Places at = places_of(position, offsets, k, n, m);
+        need(n == 0 || grad, "grad must not be NULL");
+        need(n == 0 || grad_y || grad_weights, "one of grad_y and grad_weights must not be NULL");
+        need(n == 0 || y || !grad_weights, "y must not be NULL where grad_weights is asked for");
+        const Here here(device);
+        rows::launch_from_clusters_grad({grad, ld_grad}, {y, y ? ld_y : 0}, type, d, at, weights, grad_y, grad_weights, stream_of(cuda_stream));
+    });
+}
+
+skm_status skm_op_quantize_rows(int device, const void* x, uint64_t ld_x, int dtype, uint64_t n, uint64_t d, int8_t* q, uint64_t ld_q, float* scales, void* cuda_stream) {
+    return row_op([&] {
+        const rows::Type type = type_of(dtype);
+        check_width(d);
+        need(n <= 0x7fffffff, "no more than 2^31 - 1 rows");
+        need(n == 0 || (x && q && scales), "x, q and scales must not be NULL");
+        need(n <= 1 || ld_q >= d, "rows of q must not overlap");
+        const Here here(device);
+        rows::launch_quantize_rows({x, ld_x}, type, n, d, q, n > 1 ? ld_q : d, scales, stream_of(cuda_stream));
+    });
+}
+
+uint64_t skm_op_product_8bit_workspace(const int8_t* x, uint64_t ld_x, const int8_t* w, uint64_t ld_w, uint64_t n, uint64_t m, uint64_t d, uint64_t groups) {
+    try {
+        return rows::product_workspace_bytes(product_of(x, ld_x, w, ld_w, n, m, d, groups));
+    } catch (const std::exception&) {
+        return 0;   // (sizes that skm_op_product_8bit refuses)
+    }
+}
+
+skm_status skm_op_product_8bit(int device, const int8_t* x, uint64_t ld_x, const float* x_scales, const int8_t* w, uint64_t ld_w, const float* w_scales, uint64_t n, uint64_t m,
+                               uint64_t d, uint64_t groups, const uint32_t* offsets, void* out, int out_dtype, void* workspace, uint64_t workspace_bytes, void* cuda_stream) {
+    return row_op([&] {
+        rows::Product p = product_of(x, ld_x, w, ld_w, n, m, d, groups);
+        p.out_type = type_of(out_dtype);
+        if (n == 0 || m == 0) return;
+        need(x && w && x_scales && w_scales && out, "x, w, their scales and out must not be NULL");
+        need(groups == 0 || offsets, "offsets must not be NULL where there are groups");
+        check_workspace(workspace, workspace_bytes, rows::product_workspace_bytes(p));
+        p.x_scales = x_scales;
+        p.w_scales = w_scales;
+        p.offsets = offsets;
+        p.out = out;
+        const Here here(device);
+        rows::launch_product(p, workspace, stream_of(cuda_stream));
+    });
+}
+
+skm_status skm_op_product_8bit_status(int device, void* cuda_stream) {
+    return row_op([&] {
+        const Here here(device);
+        rows::check_products(stream_of(cuda_stream));
+    });
 }
 
 // ---- host-side decisions ---------------------------------------------------------------------

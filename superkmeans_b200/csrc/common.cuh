@@ -30,6 +30,19 @@ inline void cuda_check(cudaError_t e, const char* what, const char* file, int li
 }
 #define SKM_CUDA(x) ::skmb::cuda_check((x), #x, __FILE__, __LINE__)
 
+// Makes a device the current one while it is alive.
+struct DeviceScope {
+    int previous = -1;
+    explicit DeviceScope(int device) {
+        SKM_CUDA(cudaGetDevice(&previous));
+        if (previous != device) SKM_CUDA(cudaSetDevice(device));
+        else previous = -1;
+    }
+    ~DeviceScope() {
+        if (previous >= 0) cudaSetDevice(previous);
+    }
+};
+
 unsigned long long kernel_launch_count();
 void note_kernel_launch();
 // Device and pinned-host allocations made by this library in the calling process so far (every cudaMalloc /

@@ -600,6 +600,10 @@ CUtensorMap make_half_tmap(const void* base, size_t cols, size_t rows, uint32_t 
     return make_tmap_of(CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, CU_TENSOR_MAP_SWIZZLE_128B, base, cols, rows, pitch ? pitch : cols, 64, box_rows);
 }
 
+CUtensorMap make_byte_tmap(const void* base, size_t cols, size_t rows, uint32_t box_rows, size_t pitch) {
+    return make_tmap_of(CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, CU_TENSOR_MAP_SWIZZLE_128B, base, cols, rows, pitch, 128, box_rows);
+}
+
 CUtensorMap make_row_major_tmap_128(const float* base, size_t extent, size_t rows, size_t ld, uint32_t box_rows) {
     return make_tmap_of(CU_TENSOR_MAP_DATA_TYPE_FLOAT32, sizeof(float), CU_TENSOR_MAP_SWIZZLE_128B, base, extent, rows, ld, 32, box_rows);
 }

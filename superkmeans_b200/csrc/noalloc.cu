@@ -62,18 +62,6 @@ Scratch* scratch_of_current_device(int device) {
     return g_device_ptr[device];
 }
 
-struct DeviceScope {
-    int previous = -1;
-    explicit DeviceScope(int device) {
-        SKM_CUDA(cudaGetDevice(&previous));
-        if (previous != device) SKM_CUDA(cudaSetDevice(device));
-        else previous = -1;
-    }
-    ~DeviceScope() {
-        if (previous >= 0) cudaSetDevice(previous);
-    }
-};
-
 } // namespace
 
 // x_dev [n][d], y_dev [k][d], out_knn_dev [n], out_dist_dev [n]: device memory of `device`.  Returns after the

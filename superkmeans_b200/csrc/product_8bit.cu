@@ -1,0 +1,502 @@
+// Rows in 8 bits with a scale each, and their product with a matrix in 8 bits with a scale for each of its rows, on the tensor cores:
+// out[i][c] = x_scale[i] * w_scale[c] * sum_j x[i][j] w[c][j].  The sums are whole numbers in 32 bits, hence exact however they are
+// split; a result is rounded when its sum becomes a float, at each of the two scales, and once more to the output's type.
+//
+// tcgen05.mma of kind::i8: the matrix's rows ("channels") are the 128 lanes of the accumulator, the rows of x ("rows") its columns.  That
+// way round one kernel serves a single row as well as many: the accumulator is as narrow as there are rows, and a warp's 32 lanes write
+// 32 neighbouring results of a row.
+#include <cmath>
+#include <mutex>
+#include <string>
+
+#include "rows_access.cuh"
+#include "tc_ptx.cuh"
+#include "kernels_tc.cuh"
+
+namespace skmb {
+namespace rows {
+
+using namespace tc;
+
+namespace {
+
+// ---------------------------------------------------------------------------------------------- rows to 8 bits
+
+// LANES threads to a row, of which each keeps HELD chunks in registers between finding the largest value and dividing by it; rows that
+// are longer are read twice.
+template <typename T, int BYTES, int LANES, int HELD>
+__global__ void __launch_bounds__(256) quantize_rows_kernel(const void* __restrict__ x, size_t pitch, size_t n, uint32_t width, int8_t* __restrict__ q, size_t ldq,
+                                                            float* __restrict__ scales) {
+    using V = Values<T, BYTES>;
+    const size_t row = static_cast<size_t>(blockIdx.x) * (256 / LANES) + threadIdx.x / LANES;
+    const uint32_t lane = threadIdx.x % LANES;
+    const bool valid = row < n;
+    const Chunk<BYTES>* from = reinterpret_cast<const Chunk<BYTES>*>(static_cast<const char*>(x) + (valid ? row : 0) * pitch);
+    Chunk<BYTES> held[HELD];
+#pragma unroll
+    for (int h = 0; h < HELD; ++h) held[h] = valid && lane + h * LANES < width ? __ldg(from + lane + h * LANES) : zero_chunk<BYTES>();
+    // magnitudes as whole numbers: a NaN is above infinity
+    uint32_t most = 0;
+    auto look = [&](const Chunk<BYTES>& c) {
+        V v;
+        v.from(c);
+#pragma unroll
+        for (int i = 0; i < V::N; ++i) most = max(most, __float_as_uint(v.v[i]) & 0x7fffffffu);
+    };
+#pragma unroll
+    for (int h = 0; h < HELD; ++h) look(held[h]);
+    if (valid)
+        for (uint32_t c = lane + HELD * LANES; c < width; c += LANES) look(__ldg(from + c));
+#pragma unroll
+    for (int o = (LANES < 32 ? LANES : 32) / 2; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+    if constexpr (LANES > 32) {
+        __shared__ uint32_t of_warp[8];
+        if ((threadIdx.x & 31) == 0) of_warp[threadIdx.x >> 5] = most;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < 8; ++w) most = max(most, of_warp[w]);
+    }
+    if (!valid) return;
+    const bool finite = most < 0x7f800000u, some = finite && most != 0;
+    const float largest = __uint_as_float(most);
+    // 127 / largest is a float for all but the smallest, which are taken 2^100 times as large
+    const float up = largest < 0x1p-100f ? 0x1p100f : 1.0f;
+    const float inverse = some ? __fdiv_rn(127.0f, largest * up) : 0.0f;
+    if (lane == 0) scales[row] = finite ? __fdiv_rn(largest, 127.0f) : __uint_as_float(0x7fc00000u);
+    int8_t* to = q + row * ldq;
+    auto put = [&](const Chunk<BYTES>& c, uint32_t at) {
+        V v;
+        v.from(c);
+        int8_t b[V::N];
+#pragma unroll
+        for (int i = 0; i < V::N; ++i) b[i] = some ? static_cast<int8_t>(__float2int_rn(__fmul_rn(v.v[i] * up, inverse))) : int8_t{0};
+        if constexpr (V::N == 1) to[at] = b[0];
+        else {
+            Chunk<V::N> packed;
+            memcpy(&packed, b, V::N);
+            *reinterpret_cast<Chunk<V::N>*>(to + at * V::N) = packed;
+        }
+    };
+#pragma unroll
+    for (int h = 0; h < HELD; ++h)
+        if (lane + h * LANES < width) put(held[h], lane + h * LANES);
+    for (uint32_t c = lane + HELD * LANES; c < width; c += LANES) put(__ldg(from + c), c);
+}
+
+// Rows with a pitch that TMA takes (zeros behind d).
+__global__ void __launch_bounds__(256) pad_bytes_kernel(const int8_t* __restrict__ in, size_t ld, size_t n, uint32_t d, uint32_t pitch, int8_t* __restrict__ out) {
+    const size_t row = static_cast<size_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+    if (row >= n) return;
+    for (uint32_t j = threadIdx.x & 31; j < pitch / 4; j += 32) {
+        uint32_t v = 0;
+#pragma unroll
+        for (uint32_t e = 0; e < 4; ++e)
+            if (4 * j + e < d) v |= static_cast<uint32_t>(static_cast<uint8_t>(__ldg(in + row * ld + 4 * j + e))) << (8 * e);
+        *reinterpret_cast<uint32_t*>(out + row * pitch + 4 * j) = v;
+    }
+}
+
+// ---------------------------------------------------------------------------------------------- the product
+constexpr int P_THREADS = 128;
+constexpr int P_STAGES = 4;
+constexpr uint32_t P_CHANNELS = 128;
+constexpr uint32_t P_DEPTH = 128;                          // columns of a stage, one 128-byte swizzle
+constexpr uint32_t P_W_BYTES = P_CHANNELS * P_DEPTH;
+
+// A tile of rows: row0 .. row1 - 1 of a group; groups and groups + 1 stand for rows that belong to none.
+struct RowTile {
+    uint32_t row0, row1, group;
+};
+
+struct ProductMaps {
+    CUtensorMap w, x;
+};
+
+struct ProductParams {
+    const float* x_scales;
+    const float* w_scales;
+    void* out;
+    uint32_t n, m, depth_blocks;
+    uint32_t channel_tiles;
+    uint32_t groups;             // 0: none
+    const RowTile* tiles;        // with groups
+    const uint32_t* n_tiles;
+    int* error;
+    int* told;                   // in host memory
+    long long wait_limit;
+    uint32_t producer_stop;
+};
+
+template <int ROWS>
+struct ProductControl {
+    uint64_t full[P_STAGES];
+    uint64_t empty[P_STAGES];
+    uint64_t done;
+    uint32_t tmem_base;
+    alignas(16) float x_scales[ROWS];
+};
+template <int ROWS>
+constexpr uint32_t kStageBytes = P_W_BYTES + ROWS * P_DEPTH;
+template <int ROWS>
+constexpr uint32_t kProductSmem = P_STAGES * kStageBytes<ROWS> + sizeof(ProductControl<ROWS>) + 1024;
+
+__device__ __forceinline__ void store_result(float* p, float v) { *p = v; }
+__device__ __forceinline__ void store_result(__half* p, float v) { *p = __float2half_rn(v); }
+__device__ __forceinline__ void store_result(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+
+// One tile of 128 channels x ROWS rows per cluster; the CTAs of a cluster share the depth and add their sums at the end, each for its
+// part of the rows, out of one another's shared memory.
+template <int ROWS, typename O>
+__global__ void __launch_bounds__(P_THREADS) product_kernel(const __grid_constant__ ProductMaps maps, const ProductParams p) {
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t raw_addr = smem_u32(smem_raw);
+    const uint32_t pad = (1024u - (raw_addr & 1023u)) & 1023u;
+    uint8_t* smem = smem_raw + pad;
+    const uint32_t smem_base = raw_addr + pad;
+    auto* ctrl = reinterpret_cast<ProductControl<ROWS>*>(smem + P_STAGES * kStageBytes<ROWS>);
+    constexpr uint32_t COLS = ROWS < 32 ? 32 : ROWS;
+    const WaitCtx wctx{p.error, p.wait_limit};
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t split = cluster_size(), rank = cluster_rank();
+
+    const uint32_t tile = blockIdx.x / split, channel_tile = tile % p.channel_tiles, row_tile = tile / p.channel_tiles;
+    RowTile t;
+    if (p.groups) {
+        if (row_tile >= __ldg(p.n_tiles)) return;   // (the whole cluster)
+        t = p.tiles[row_tile];
+    } else {
+        t = {row_tile * ROWS, min(row_tile * ROWS + ROWS, p.n), 0};
+    }
+    const uint32_t channel = channel_tile * P_CHANNELS + threadIdx.x;
+    O* out = static_cast<O*>(p.out);
+    if (p.groups && t.group >= p.groups) {   // rows of no group
+        if (rank == 0 && channel < p.m)
+            for (uint32_t r = t.row0; r < t.row1; ++r) store_result(out + static_cast<size_t>(r) * p.m + channel, 0.f);
+        return;
+    }
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < P_STAGES; ++s) {
+            mbar_init(&ctrl->full[s], 1);
+            mbar_init(&ctrl->empty[s], 1);
+        }
+        mbar_init(&ctrl->done, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        fence_proxy_async();
+    }
+    if (warp == 0) tmem_alloc(&ctrl->tmem_base, COLS);
+    for (uint32_t r = threadIdx.x; r < ROWS; r += P_THREADS) ctrl->x_scales[r] = t.row0 + r < t.row1 ? __ldg(p.x_scales + t.row0 + r) : 0.f;
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = ctrl->tmem_base;
+    const uint32_t k0 = p.depth_blocks * rank / split, k1 = p.depth_blocks * (rank + 1) / split;
+
+    bool ok = true;
+    if (threadIdx.x == 0) {
+        const int w_row = static_cast<int>(t.group * p.m + channel_tile * P_CHANNELS), x_row = static_cast<int>(t.row0);
+        for (uint32_t k = k0, it = 0; k < k1; ++k, ++it) {
+            const uint32_t s = it % P_STAGES, ph = (it / P_STAGES) & 1u;
+            if ((p.producer_stop != 0 && it >= p.producer_stop) || !mbar_wait(&ctrl->empty[s], ph ^ 1u, wctx, 41)) {
+                ok = false;
+                break;
+            }
+            const uint32_t st = smem_base + s * kStageBytes<ROWS>;
+            mbar_arrive_expect_tx(&ctrl->full[s], kStageBytes<ROWS>);
+            tma_load_2d(st, &maps.w, &ctrl->full[s], static_cast<int>(k * P_DEPTH), w_row);
+            tma_load_2d(st + P_W_BYTES, &maps.x, &ctrl->full[s], static_cast<int>(k * P_DEPTH), x_row);
+        }
+    } else if (threadIdx.x == 32) {
+        constexpr uint32_t idesc = make_idesc_i8(P_CHANNELS, ROWS);
+        for (uint32_t k = k0, it = 0; k < k1; ++k, ++it) {
+            const uint32_t s = it % P_STAGES, ph = (it / P_STAGES) & 1u;
+            if (!mbar_wait(&ctrl->full[s], ph, wctx, 42)) {
+                ok = false;
+                break;
+            }
+            tc_fence_after();
+            const uint32_t st = smem_base + s * kStageBytes<ROWS>;
+#pragma unroll
+            for (uint32_t kk = 0; kk < P_DEPTH / 32; ++kk) umma_i8(tmem_base, make_desc_128(st + kk * 32), make_desc_128(st + P_W_BYTES + kk * 32), it != 0 || kk != 0 ? 1u : 0u, idesc);
+            umma_commit(&ctrl->empty[s]);
+        }
+        if (ok) umma_commit(&ctrl->done);
+    }
+    __syncwarp();
+    const bool summed = __all_sync(0xffffffffu, mbar_wait(&ctrl->done, 0, wctx, 43));
+    if (!summed && lane == 0) *reinterpret_cast<volatile int*>(p.told) = 43;
+    if (!ok) {
+        // a millisecond for the copies that are in flight before the block's memory is let go
+        const long long t0 = clock64();
+        while (clock64() - t0 < 2000000) {
+        }
+    }
+    __syncwarp();
+    tc_fence_after();
+
+    const bool has_channel = channel < p.m;
+    const float w_scale = has_channel ? __ldg(p.w_scales + static_cast<size_t>(t.group) * p.m + channel) : 0.f;
+    const uint32_t taddr = tmem_base + (warp * 32 << 16);
+    auto put = [&](uint32_t r, int sum) {
+        if (t.row0 + r < t.row1 && has_channel)
+            store_result(out + static_cast<size_t>(t.row0 + r) * p.m + channel, __int2float_rn(sum) * ctrl->x_scales[r] * w_scale);
+    };
+    if (split == 1) {
+        if (summed)
+#pragma unroll 1
+            for (uint32_t c = 0; c < ROWS; c += 16) {
+                uint32_t r[16];
+                tmem_ld16(taddr + c, r);
+#pragma unroll
+                for (uint32_t j = 0; j < 16; ++j) put(c + j, static_cast<int>(r[j]));
+            }
+    } else {
+        // sums of all rows into this CTA's shared memory (the stages are through), 128 channels to a row
+        int* sums = reinterpret_cast<int*>(smem);
+        if (summed)
+#pragma unroll 1
+            for (uint32_t c = 0; c < ROWS; c += 16) {
+                uint32_t r[16];
+                tmem_ld16(taddr + c, r);
+#pragma unroll
+                for (uint32_t j = 0; j < 16; ++j) sums[(c + j) * P_CHANNELS + threadIdx.x] = static_cast<int>(r[j]);
+            }
+        cluster_sync();
+        const uint32_t share = ROWS / split;
+        if (summed)
+            for (uint32_t r = rank * share; r < (rank + 1) * share; ++r) {
+                int sum = 0;
+                for (uint32_t q = 0; q < split; ++q) sum += load_cluster(cluster_address(sums + r * P_CHANNELS + threadIdx.x, q));
+                put(r, sum);
+            }
+        cluster_sync();   // nobody reads this CTA's sums any more
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 0) tmem_dealloc(tmem_base, COLS);
+}
+
+// The tiles of `rows` rows that the groups consist of, one block.
+__global__ void __launch_bounds__(1024) row_tiles_kernel(const uint32_t* __restrict__ offsets, uint32_t groups, uint32_t n, uint32_t rows, uint32_t room, RowTile* __restrict__ tiles,
+                                                         uint32_t* __restrict__ n_tiles) {
+    __shared__ uint32_t sums[32];
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    uint32_t base = 0;
+    for (uint32_t g0 = 0; g0 < groups + 2; g0 += 1024) {
+        const uint32_t g = g0 + threadIdx.x;
+        uint32_t a = 0, b = 0;
+        if (g < groups) {
+            a = min(__ldg(offsets + g), n);
+            b = min(__ldg(offsets + g + 1), n);
+        } else if (g == groups) {
+            a = min(__ldg(offsets + groups), n);
+            b = n;
+        } else if (g == groups + 1) {
+            b = min(__ldg(offsets), n);
+        }
+        const uint32_t count = b > a ? (b - a + rows - 1) / rows : 0;
+        uint32_t upto = count;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t v = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= static_cast<uint32_t>(o)) upto += v;
+        }
+        if (lane == 31) sums[warp] = upto;
+        __syncthreads();
+        uint32_t before = base, total = 0;
+        for (uint32_t w = 0; w < 32; ++w) {
+            if (w < warp) before += sums[w];
+            total += sums[w];
+        }
+        before += upto - count;
+        for (uint32_t i = 0; i < count && before + i < room; ++i) tiles[before + i] = {a + i * rows, min(a + (i + 1) * rows, b), g};
+        base += total;
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) *n_tiles = min(base, room);
+}
+
+// Where a kernel records that a wait ran out: for the kernels in device memory, for the host in its own.
+struct Status {
+    int* device = nullptr;
+    int* host = nullptr;
+    int* host_on_device = nullptr;
+};
+constexpr int kMaxDevices = 64;
+__device__ int g_product_error;   // (in host code a handle, no address)
+
+Status& status_of_current_device() {
+    static std::mutex mutex;
+    static Status all[kMaxDevices];
+    int device = 0;
+    SKM_CUDA(cudaGetDevice(&device));
+    if (device >= kMaxDevices) throw CudaError("too many CUDA devices");
+    std::lock_guard<std::mutex> lock(mutex);
+    Status& s = all[device];
+    if (!s.host_on_device) {
+        // (also when a stream is being captured, which this is no part of)
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        SKM_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
+        void* word = nullptr;
+        cudaError_t e = cudaGetSymbolAddress(&word, g_product_error);
+        s.device = static_cast<int*>(word);
+        if (e == cudaSuccess && !s.host) e = cudaHostAlloc(&s.host, sizeof(int), cudaHostAllocMapped | cudaHostAllocPortable);
+        if (e == cudaSuccess) {
+            *s.host = 0;
+            e = cudaHostGetDevicePointer(&s.host_on_device, s.host, 0);
+        }
+        const cudaError_t back = cudaThreadExchangeStreamCaptureMode(&mode);
+        SKM_CUDA(e);
+        SKM_CUDA(back);
+        note_device_alloc();
+    }
+    return s;
+}
+
+void throw_if_told(Status& s, cudaStream_t stream) {
+    volatile int* told = s.host;
+    if (*told == 0) return;
+    const int code = *told;
+    *told = 0;
+    SKM_CUDA(cudaMemsetAsync(s.device, 0, sizeof(int), stream));
+    throw CudaError("a product in 8 bits gave up waiting on a barrier (code " + std::to_string(code) + "): its results are not valid");
+}
+
+bool tma_takes(const void* p, size_t ld, size_t d) { return (address(p) & 15) == 0 && ld % 16 == 0 && ld >= d; }
+size_t pitch_of(size_t d) { return (d + 15) / 16 * 16; }
+size_t rounded(size_t bytes) { return (bytes + 255) / 256 * 256; }
+
+struct ProductPlan {
+    uint32_t rows, split, row_tiles;   // row_tiles: with groups at most
+};
+ProductPlan make_plan(const Product& p) {
+    const size_t channel_tiles = (p.m + P_CHANNELS - 1) / P_CHANNELS, depth_blocks = (p.d + P_DEPTH - 1) / P_DEPTH;
+    const size_t typical = p.groups ? (p.n + p.groups - 1) / p.groups : p.n;
+    ProductPlan plan{};
+    plan.rows = typical <= 16 ? 16 : typical <= 32 ? 32 : typical <= 64 ? 64 : 128;
+    if (plan.rows == 128 && (p.n + 127) / 128 * channel_tiles < 148) plan.rows = 64;
+    plan.row_tiles = static_cast<uint32_t>((p.n + plan.rows - 1) / plan.rows + (p.groups ? p.groups + 1 : 0));
+    plan.split = 1;
+    if (!p.groups && plan.rows <= 64)
+        while (plan.split < 8 && plan.row_tiles * channel_tiles * plan.split * 2 <= 2 * 148 && depth_blocks >= 2 * plan.split) plan.split *= 2;
+    return plan;
+}
+
+} // namespace
+
+void launch_quantize_rows(const Rows& x, Type type, size_t n, size_t d, int8_t* q, size_t ldq, float* scales, cudaStream_t stream) {
+    if (n == 0) return;
+    const size_t t = type_bytes(type), pitch = x.ld * t;
+    with_width(type, access_bytes({address(x.p), pitch, d * t, address(q) * t, ldq * t}), [&](auto value, auto width) {
+        using T = decltype(value);
+        constexpr int B = decltype(width)::bytes;
+        const uint32_t chunks = static_cast<uint32_t>(d * t / B);
+        auto launch = [&](auto* kernel, int lanes) {
+            kernel<<<static_cast<unsigned>((n + 256 / lanes - 1) / (256 / lanes)), 256, 0, stream>>>(x.p, pitch, n, chunks, q, ldq, scales);
+        };
+        if (chunks <= 8 * 4) launch(quantize_rows_kernel<T, B, 8, 4>, 8);
+        else if (chunks <= 32 * 4) launch(quantize_rows_kernel<T, B, 32, 4>, 32);
+        else if (chunks <= 32 * 8) launch(quantize_rows_kernel<T, B, 32, 8>, 32);
+        else launch(quantize_rows_kernel<T, B, 256, 4>, 256);
+    });
+    SKM_LAUNCH_CHECK();
+}
+
+size_t product_workspace_bytes(const Product& p) {
+    const ProductPlan plan = make_plan(p);
+    size_t bytes = 0;
+    if (!tma_takes(p.x, p.ldx, p.d)) bytes += rounded(p.n * pitch_of(p.d));
+    if (!tma_takes(p.w, p.ldw, p.d)) bytes += rounded(std::max<size_t>(1, p.groups) * p.m * pitch_of(p.d));
+    if (p.groups) bytes += rounded(plan.row_tiles * sizeof(RowTile)) + 256;
+    return bytes;
+}
+
+void launch_product(const Product& p, void* workspace, cudaStream_t stream) {
+    if (p.n == 0 || p.m == 0) return;
+    Status& status = status_of_current_device();
+    throw_if_told(status, stream);
+    const ProductPlan plan = make_plan(p);
+    char* at = static_cast<char*>(workspace);
+    auto take = [&](size_t bytes) {
+        char* here = at;
+        at += rounded(bytes);
+        return here;
+    };
+    auto padded = [&](const int8_t*& rows, size_t& ld, size_t n) {
+        if (tma_takes(rows, ld, p.d)) return;
+        const size_t pitch = pitch_of(p.d);
+        int8_t* copy = reinterpret_cast<int8_t*>(take(n * pitch));
+        pad_bytes_kernel<<<static_cast<unsigned>((n + 7) / 8), 256, 0, stream>>>(rows, ld, n, static_cast<uint32_t>(p.d), static_cast<uint32_t>(pitch), copy);
+        SKM_LAUNCH_CHECK();
+        rows = copy;
+        ld = pitch;
+    };
+    const int8_t *x = p.x, *w = p.w;
+    size_t ldx = p.ldx, ldw = p.ldw;
+    const size_t w_rows = std::max<size_t>(1, p.groups) * p.m;
+    padded(x, ldx, p.n);
+    padded(w, ldw, w_rows);
+
+    ProductParams k{};
+    k.x_scales = p.x_scales;
+    k.w_scales = p.w_scales;
+    k.out = p.out;
+    k.n = static_cast<uint32_t>(p.n);
+    k.m = static_cast<uint32_t>(p.m);
+    k.depth_blocks = static_cast<uint32_t>((p.d + P_DEPTH - 1) / P_DEPTH);
+    k.channel_tiles = static_cast<uint32_t>((p.m + P_CHANNELS - 1) / P_CHANNELS);
+    k.groups = static_cast<uint32_t>(p.groups);
+    k.error = status.device;
+    k.told = status.host_on_device;
+    k.wait_limit = wait_limit();
+    k.producer_stop = producer_stop();
+    if (p.groups) {
+        RowTile* tiles = reinterpret_cast<RowTile*>(take(plan.row_tiles * sizeof(RowTile)));
+        uint32_t* n_tiles = reinterpret_cast<uint32_t*>(take(4));
+        row_tiles_kernel<<<1, 1024, 0, stream>>>(p.offsets, k.groups, k.n, plan.rows, plan.row_tiles, tiles, n_tiles);
+        SKM_LAUNCH_CHECK();
+        k.tiles = tiles;
+        k.n_tiles = n_tiles;
+    }
+    ProductMaps maps;
+    maps.w = make_byte_tmap(w, p.d, w_rows, P_CHANNELS, ldw);
+    maps.x = make_byte_tmap(x, p.d, p.n, plan.rows, ldx);
+    auto launch = [&](auto rows, auto result) {
+        constexpr int ROWS = decltype(rows)::value;
+        using O = decltype(result);
+        auto* kernel = product_kernel<ROWS, O>;
+        SKM_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kProductSmem<ROWS>)));
+        cudaLaunchConfig_t config{};
+        const size_t blocks = static_cast<size_t>(plan.row_tiles) * k.channel_tiles * plan.split;
+        if (blocks > 0x7fffffff) throw std::invalid_argument("a product of these sizes needs too many tiles");
+        config.gridDim = dim3(static_cast<unsigned>(blocks));
+        config.blockDim = dim3(P_THREADS);
+        config.dynamicSmemBytes = kProductSmem<ROWS>;
+        config.stream = stream;
+        cudaLaunchAttribute cluster{};
+        cluster.id = cudaLaunchAttributeClusterDimension;
+        cluster.val.clusterDim = {plan.split, 1, 1};
+        config.attrs = &cluster;
+        config.numAttrs = 1;
+        SKM_CUDA(cudaLaunchKernelEx(&config, kernel, maps, k));
+        SKM_LAUNCH_CHECK();
+    };
+    auto of_type = [&](auto rows) {
+        if (p.out_type == Type::f32) launch(rows, float{});
+        else if (p.out_type == Type::f16) launch(rows, __half{});
+        else launch(rows, __nv_bfloat16{});
+    };
+    if (plan.rows == 16) of_type(std::integral_constant<int, 16>{});
+    else if (plan.rows == 32) of_type(std::integral_constant<int, 32>{});
+    else if (plan.rows == 64) of_type(std::integral_constant<int, 64>{});
+    else of_type(std::integral_constant<int, 128>{});
+}
+
+void check_products(cudaStream_t stream) {
+    Status& s = status_of_current_device();
+    SKM_CUDA(cudaStreamSynchronize(stream));
+    throw_if_told(s, stream);
+}
+
+} // namespace rows
+} // namespace skmb

@@ -1,0 +1,142 @@
+// Loads and stores of a few neighbouring values of a row, and their conversion to and from fp32, shared by the operators on rows.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+
+#include "common.cuh"
+#include "rows.h"
+
+namespace skmb {
+namespace rows {
+
+// What one load or store moves.
+template <int BYTES>
+struct ChunkOf;
+template <>
+struct ChunkOf<16> {
+    using type = uint4;
+};
+template <>
+struct ChunkOf<8> {
+    using type = uint2;
+};
+template <>
+struct ChunkOf<4> {
+    using type = uint32_t;
+};
+template <>
+struct ChunkOf<2> {
+    using type = uint16_t;
+};
+template <int BYTES>
+using Chunk = typename ChunkOf<BYTES>::type;
+
+template <int BYTES>
+__device__ __forceinline__ Chunk<BYTES> zero_chunk() {
+    Chunk<BYTES> c;
+    memset(&c, 0, BYTES);
+    return c;
+}
+
+__device__ __forceinline__ float2 pair_to_float(uint32_t u, const __half*) { return __half22float2(*reinterpret_cast<const __half2*>(&u)); }
+__device__ __forceinline__ float2 pair_to_float(uint32_t u, const __nv_bfloat16*) { return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u)); }
+__device__ __forceinline__ uint32_t pair_from_float(float a, float b, const __half*) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t pair_from_float(float a, float b, const __nv_bfloat16*) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// The values of a chunk in fp32, and back (rounded to nearest).
+template <typename T, int BYTES>
+struct Values {
+    static constexpr int N = BYTES / static_cast<int>(sizeof(T));
+    float v[N];
+
+    __device__ __forceinline__ void from(const Chunk<BYTES>& c) {
+        if constexpr (sizeof(T) == 4) {
+            memcpy(v, &c, BYTES);
+        } else if constexpr (BYTES == 2) {
+            v[0] = pair_to_float(c, static_cast<const T*>(nullptr)).x;
+        } else {
+            uint32_t u[BYTES / 4];
+            memcpy(u, &c, BYTES);
+#pragma unroll
+            for (int i = 0; i < BYTES / 4; ++i) {
+                const float2 f = pair_to_float(u[i], static_cast<const T*>(nullptr));
+                v[2 * i] = f.x;
+                v[2 * i + 1] = f.y;
+            }
+        }
+    }
+    __device__ __forceinline__ Chunk<BYTES> to() const {
+        Chunk<BYTES> c;
+        if constexpr (sizeof(T) == 4) {
+            memcpy(&c, v, BYTES);
+        } else if constexpr (BYTES == 2) {
+            c = static_cast<uint16_t>(pair_from_float(v[0], 0.f, static_cast<const T*>(nullptr)));
+        } else {
+            uint32_t u[BYTES / 4];
+#pragma unroll
+            for (int i = 0; i < BYTES / 4; ++i) u[i] = pair_from_float(v[2 * i], v[2 * i + 1], static_cast<const T*>(nullptr));
+            memcpy(&c, u, BYTES);
+        }
+        return c;
+    }
+};
+
+// The cluster of pair i, or k.
+__device__ __forceinline__ uint32_t load_id(const void* ids, bool wide, size_t i, uint32_t k) {
+    if (wide) {
+        const unsigned long long v = __ldg(static_cast<const unsigned long long*>(ids) + i);   // (a negative one is large)
+        return v < k ? static_cast<uint32_t>(v) : k;
+    }
+    return min(__ldg(static_cast<const uint32_t*>(ids) + i), k);
+}
+
+// Division of small numbers by one that a launch knows: magic is 0 where multiplication would not give the quotient.
+struct Divisor {
+    uint32_t d, magic;
+};
+// for dividends below `most`: floor(a / d) = (a * ceil(2^32 / d)) >> 32 as long as a * (d * ceil(2^32 / d) - 2^32) < 2^32, and the bracket is less than d
+inline Divisor make_divisor(size_t d, size_t most) {
+    const uint64_t magic = ((uint64_t{1} << 32) + d - 1) / d;
+    return {static_cast<uint32_t>(d), d > 1 && most * d < (uint64_t{1} << 32) ? static_cast<uint32_t>(magic) : 0u};
+}
+__device__ __forceinline__ uint32_t divide(uint32_t a, const Divisor& by) { return by.magic ? __umulhi(a, by.magic) : a / by.d; }
+
+// How many bytes a load of each of these may move at once: all of them are multiples of it.
+inline int access_bytes(std::initializer_list<size_t> multiples) {
+    size_t all = 16;
+    for (const size_t m : multiples) all |= m;
+    return static_cast<int>(all & (~all + 1));
+}
+inline size_t address(const void* p) { return reinterpret_cast<uintptr_t>(p); }
+
+// f(T{}, integral_constant<BYTES>) for a type and a width of access
+template <int BYTES>
+struct Width {
+    static constexpr int bytes = BYTES;
+};
+template <class F>
+void with_width(Type type, int bytes, F&& f) {
+    auto of = [&](auto t) {
+        if (bytes >= 16) f(t, Width<16>{});
+        else if (bytes == 8) f(t, Width<8>{});
+        else if (bytes == 4) f(t, Width<4>{});
+        else if constexpr (sizeof(t) == 2) f(t, Width<2>{});
+    };
+    if (type == Type::f32) of(float{});
+    else if (type == Type::f16) of(__half{});
+    else of(__nv_bfloat16{});
+}
+
+} // namespace rows
+} // namespace skmb

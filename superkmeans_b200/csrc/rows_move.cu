@@ -1,0 +1,292 @@
+// Rows by index: lookup in a table, rows to the places of their clusters and back, and the gradients of the weights and scales.
+//
+// All of them move rows once and compute next to nothing: they are bound by HBM, or for small calls by the launch.  The rows of an
+// output (or for to_clusters of the input) are taken as one sequence of 16-byte chunks, 256 x 4 of them to a block whatever the rows'
+// width, so that narrow and odd rows fill the lanes as well as wide ones; a row whose address, pitch or width is no multiple of 16
+// bytes is taken in chunks of 8, 4 or 2.  Products and sums are in fp32 and rounded once.
+#include "rows_access.cuh"
+
+#include "device_utils.cuh"
+
+namespace skmb {
+namespace rows {
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kAhead = 4;   // chunks of a thread, all loaded before the first is stored
+
+// The chunks of n rows, `width` to a row.
+struct Spread {
+    size_t total;
+    Divisor width;
+};
+
+Spread make_spread(size_t n, size_t row_bytes, int bytes) {
+    const size_t width = row_bytes / bytes;
+    return {n * width, make_divisor(width, width + kThreads * kAhead)};
+}
+unsigned spread_blocks(const Spread& s) { return static_cast<unsigned>((s.total + kThreads * kAhead - 1) / (kThreads * kAhead)); }
+
+// This thread's chunks: row and place in the row of chunk u, and whether there is one.
+struct Mine {
+    size_t row0;
+    uint32_t off;
+    size_t left;   // chunks from this thread's first one to the end
+    Divisor width;
+
+    __device__ __forceinline__ explicit Mine(const Spread& s) : width(s.width) {
+        const size_t first = static_cast<size_t>(blockIdx.x) * (kThreads * kAhead);
+        row0 = (first >> 32) == 0 ? static_cast<uint32_t>(first) / s.width.d : first / s.width.d;
+        off = static_cast<uint32_t>(first - row0 * s.width.d) + threadIdx.x;
+        left = first + threadIdx.x < s.total ? s.total - first - threadIdx.x : 0;
+    }
+    __device__ __forceinline__ bool has(int u) const { return static_cast<size_t>(u) * kThreads < left; }
+    __device__ __forceinline__ void at(int u, size_t& row, uint32_t& col) const {
+        const uint32_t a = off + u * kThreads, q = divide(a, width);
+        row = row0 + q;
+        col = a - q * width.d;
+    }
+};
+
+template <typename C>
+__device__ __forceinline__ const C* row_at(const void* p, size_t pitch, size_t row) {
+    return reinterpret_cast<const C*>(static_cast<const char*>(p) + row * pitch);
+}
+
+template <typename T, int BYTES, bool SCALED>
+__global__ void __launch_bounds__(kThreads) lookup_kernel(const void* __restrict__ table, size_t pitch, uint32_t k, const void* __restrict__ ids, bool wide, float scale,
+                                                          const float* __restrict__ row_scales, Chunk<BYTES>* __restrict__ out, const Spread spread) {
+    const Mine mine(spread);
+    size_t row[kAhead];
+    uint32_t col[kAhead], id[kAhead];
+    Chunk<BYTES> c[kAhead];
+    float f[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+        id[u] = k;
+        if (mine.has(u)) {
+            mine.at(u, row[u], col[u]);
+            id[u] = load_id(ids, wide, row[u], k);
+            if (SCALED) f[u] = row_scales ? scale * __ldg(row_scales + row[u]) : scale;
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) c[u] = id[u] < k ? __ldg(row_at<Chunk<BYTES>>(table, pitch, id[u]) + col[u]) : zero_chunk<BYTES>();
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+        if (!mine.has(u)) continue;
+        if (SCALED && id[u] < k) {
+            Values<T, BYTES> v;
+            v.from(c[u]);
+#pragma unroll
+            for (int i = 0; i < v.N; ++i) v.v[i] *= f[u];
+            c[u] = v.to();
+        }
+        out[row[u] * spread.width.d + col[u]] = c[u];
+    }
+}
+
+template <int BYTES>
+__global__ void __launch_bounds__(kThreads) to_clusters_kernel(const void* __restrict__ x, size_t pitch, const Places at, Chunk<BYTES>* __restrict__ out, const Spread spread) {
+    const Mine mine(spread);
+    const uint32_t slots = static_cast<uint32_t>(at.n * at.m), held = min(__ldg(at.held), slots);
+    Chunk<BYTES> c[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+        if (mine.has(u)) {
+            size_t row;
+            uint32_t col;
+            mine.at(u, row, col);
+            c[u] = __ldg(row_at<Chunk<BYTES>>(x, pitch, row) + col);
+        }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+        if (mine.has(u)) {
+            size_t row;
+            uint32_t col;
+            mine.at(u, row, col);
+            for (size_t j = 0; j < at.m; ++j) {
+                const uint32_t slot = __ldg(at.position + row * at.m + j);
+                if (slot < slots) out[static_cast<size_t>(slot) * spread.width.d + col] = slot < held ? c[u] : zero_chunk<BYTES>();
+            }
+        }
+}
+
+template <typename T, int BYTES>
+__global__ void __launch_bounds__(kThreads) from_clusters_kernel(const void* __restrict__ y, size_t pitch, const Places at, const float* __restrict__ weights,
+                                                                 Chunk<BYTES>* __restrict__ out, const Spread spread) {
+    const Mine mine(spread);
+    const uint32_t slots = static_cast<uint32_t>(at.n * at.m), held = min(__ldg(at.held), slots);
+    size_t row[kAhead];
+    uint32_t col[kAhead];
+    Values<T, BYTES> sum[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+        if (mine.has(u)) mine.at(u, row[u], col[u]);
+#pragma unroll
+        for (int i = 0; i < sum[u].N; ++i) sum[u].v[i] = 0.f;
+    }
+    for (size_t j = 0; j < at.m; ++j) {
+        Chunk<BYTES> c[kAhead];
+        float w[kAhead];
+        bool there[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            there[u] = false;
+            if (mine.has(u)) {
+                const uint32_t slot = __ldg(at.position + row[u] * at.m + j);
+                there[u] = slot < held;
+                if (there[u]) {
+                    c[u] = __ldg(row_at<Chunk<BYTES>>(y, pitch, slot) + col[u]);
+                    w[u] = weights ? __ldg(weights + row[u] * at.m + j) : 1.f;
+                }
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+            if (there[u]) {
+                Values<T, BYTES> v;
+                v.from(c[u]);
+#pragma unroll
+                for (int i = 0; i < v.N; ++i) sum[u].v[i] = fmaf(w[u], v.v[i], sum[u].v[i]);
+            }
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+        if (mine.has(u)) out[row[u] * spread.width.d + col[u]] = sum[u].to();
+}
+
+// A warp per row of grad: <grad[i], y[slot]> and grad_y[slot] = w * grad[i] for its choices, y read once.
+template <typename T, int BYTES>
+__global__ void __launch_bounds__(kThreads) from_clusters_grad_kernel(const void* __restrict__ grad, size_t grad_pitch, const void* __restrict__ y, size_t y_pitch, const Places at,
+                                                                      const float* __restrict__ weights, Chunk<BYTES>* __restrict__ grad_y, float* __restrict__ grad_weights,
+                                                                      uint32_t width) {
+    const size_t row = static_cast<size_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
+    if (row >= at.n) return;
+    const uint32_t lane = threadIdx.x & 31;
+    const uint32_t slots = static_cast<uint32_t>(at.n * at.m), held = min(__ldg(at.held), slots);
+    const Chunk<BYTES>* g = row_at<Chunk<BYTES>>(grad, grad_pitch, row);
+    for (size_t j = 0; j < at.m; ++j) {
+        const uint32_t slot = __ldg(at.position + row * at.m + j);
+        const bool there = slot < held;
+        const float w = weights ? __ldg(weights + row * at.m + j) : 1.f;
+        const Chunk<BYTES>* from = row_at<Chunk<BYTES>>(y, y_pitch, slot);
+        Chunk<BYTES>* to = grad_y + static_cast<size_t>(slot) * width;
+        float dot = 0.f;
+        if (!there) {
+            if (grad_y && slot < slots)
+                for (uint32_t c = lane; c < width; c += 32) to[c] = zero_chunk<BYTES>();
+        } else {
+#pragma unroll 4
+            for (uint32_t c = lane; c < width; c += 32) {
+                Values<T, BYTES> a;
+                a.from(__ldg(g + c));
+                if (grad_weights) {
+                    Values<T, BYTES> b;
+                    b.from(__ldg(from + c));
+#pragma unroll
+                    for (int i = 0; i < a.N; ++i) dot = fmaf(a.v[i], b.v[i], dot);
+                }
+                if (grad_y) {
+#pragma unroll
+                    for (int i = 0; i < a.N; ++i) a.v[i] *= w;
+                    to[c] = a.to();
+                }
+            }
+        }
+        if (grad_weights) {
+            dot = warp_sum(dot);
+            if (lane == 0) grad_weights[row * at.m + j] = dot;
+        }
+    }
+}
+
+template <typename T, int BYTES>
+__global__ void __launch_bounds__(kThreads) lookup_scale_grad_kernel(const void* __restrict__ grad, size_t grad_pitch, const void* __restrict__ table, size_t table_pitch, uint32_t k,
+                                                                     const void* __restrict__ ids, bool wide, size_t n, float scale, float* __restrict__ out, uint32_t width) {
+    const size_t row = static_cast<size_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
+    if (row >= n) return;
+    const uint32_t lane = threadIdx.x & 31;
+    const uint32_t id = load_id(ids, wide, row, k);
+    float dot = 0.f;
+    if (id < k) {
+        const Chunk<BYTES>* g = row_at<Chunk<BYTES>>(grad, grad_pitch, row);
+        const Chunk<BYTES>* t = row_at<Chunk<BYTES>>(table, table_pitch, id);
+#pragma unroll 4
+        for (uint32_t c = lane; c < width; c += 32) {
+            Values<T, BYTES> a, b;
+            a.from(__ldg(g + c));
+            b.from(__ldg(t + c));
+#pragma unroll
+            for (int i = 0; i < a.N; ++i) dot = fmaf(a.v[i], b.v[i], dot);
+        }
+    }
+    dot = warp_sum(dot);
+    if (lane == 0) out[row] = id < k ? scale * dot : 0.f;
+}
+
+unsigned warp_blocks(size_t n) { return static_cast<unsigned>((n + kThreads / 32 - 1) / (kThreads / 32)); }
+
+} // namespace
+
+void launch_lookup(const Rows& table, Type type, size_t k, size_t d, const Ids& ids, size_t n, float scale, const float* row_scales, void* out, cudaStream_t stream) {
+    if (n == 0) return;
+    const size_t t = type_bytes(type), pitch = table.ld * t;
+    with_width(type, access_bytes({address(table.p), pitch, d * t, address(out)}), [&](auto value, auto width) {
+        using T = decltype(value);
+        constexpr int B = decltype(width)::bytes;
+        const Spread s = make_spread(n, d * t, B);
+        // (a product with one changes no value: the plain copy is for that)
+        auto* kernel = row_scales || scale != 1.0f ? lookup_kernel<T, B, true> : lookup_kernel<T, B, false>;
+        kernel<<<spread_blocks(s), kThreads, 0, stream>>>(table.p, pitch, static_cast<uint32_t>(k), ids.p, ids.wide, scale, row_scales, static_cast<Chunk<B>*>(out), s);
+    });
+    SKM_LAUNCH_CHECK();
+}
+
+void launch_lookup_scale_grad(const Rows& grad, const Rows& table, Type type, size_t k, size_t d, const Ids& ids, size_t n, float scale, float* out, cudaStream_t stream) {
+    if (n == 0) return;
+    const size_t t = type_bytes(type);
+    with_width(type, access_bytes({address(grad.p), grad.ld * t, address(table.p), table.ld * t, d * t}), [&](auto value, auto width) {
+        constexpr int B = decltype(width)::bytes;
+        lookup_scale_grad_kernel<decltype(value), B><<<warp_blocks(n), kThreads, 0, stream>>>(grad.p, grad.ld * t, table.p, table.ld * t, static_cast<uint32_t>(k), ids.p, ids.wide, n, scale, out,
+                                                                                            static_cast<uint32_t>(d * t / B));
+    });
+    SKM_LAUNCH_CHECK();
+}
+
+void launch_to_clusters(const Rows& x, Type type, size_t d, const Places& at, void* out, cudaStream_t stream) {
+    if (at.n == 0) return;
+    const size_t t = type_bytes(type), pitch = x.ld * t;
+    with_width(type, access_bytes({address(x.p), pitch, d * t, address(out)}), [&](auto, auto width) {
+        constexpr int B = decltype(width)::bytes;
+        const Spread s = make_spread(at.n, d * t, B);
+        to_clusters_kernel<B><<<spread_blocks(s), kThreads, 0, stream>>>(x.p, pitch, at, static_cast<Chunk<B>*>(out), s);
+    });
+    SKM_LAUNCH_CHECK();
+}
+
+void launch_from_clusters(const Rows& y, Type type, size_t d, const Places& at, const float* weights, void* out, cudaStream_t stream) {
+    if (at.n == 0) return;
+    const size_t t = type_bytes(type), pitch = y.ld * t;
+    with_width(type, access_bytes({address(y.p), pitch, d * t, address(out)}), [&](auto value, auto width) {
+        constexpr int B = decltype(width)::bytes;
+        const Spread s = make_spread(at.n, d * t, B);
+        from_clusters_kernel<decltype(value), B><<<spread_blocks(s), kThreads, 0, stream>>>(y.p, pitch, at, weights, static_cast<Chunk<B>*>(out), s);
+    });
+    SKM_LAUNCH_CHECK();
+}
+
+void launch_from_clusters_grad(const Rows& grad, const Rows& y, Type type, size_t d, const Places& at, const float* weights, void* grad_y, float* grad_weights, cudaStream_t stream) {
+    if (at.n == 0) return;
+    const size_t t = type_bytes(type);
+    with_width(type, access_bytes({address(grad.p), grad.ld * t, address(y.p), y.ld * t, d * t, address(grad_y)}), [&](auto value, auto width) {
+        constexpr int B = decltype(width)::bytes;
+        from_clusters_grad_kernel<decltype(value), B><<<warp_blocks(at.n), kThreads, 0, stream>>>(grad.p, grad.ld * t, y.p, y.ld * t, at, weights, static_cast<Chunk<B>*>(grad_y), grad_weights,
+                                                                                               static_cast<uint32_t>(d * t / B));
+    });
+    SKM_LAUNCH_CHECK();
+}
+
+} // namespace rows
+} // namespace skmb

@@ -1,0 +1,412 @@
+"""Operators on rows held in torch tensors on the GPU, for programs that use clusters inside a model.
+
+    lookup          vectors of a codebook by assignment, scaled; differentiable in the codebook and the scales
+    group_rows      the order of rows by cluster
+    to_clusters     rows to the places of their clusters, and
+    from_clusters   back with weights; both differentiable
+    quantize_rows   rows in 8 bits with a scale each
+    product_8bit    their product with a matrix in 8 bits, or with a matrix of each cluster's own
+
+A thin layer over the functions of the same names in include/skm_b200.h.  Every call works on the current stream of its tensors'
+device (which need not be the current device), allocates its outputs and its workspace through torch, waits for nothing and can be
+captured into a CUDA graph.  Tensors that are used on another stream than the one they were made on need `record_stream`, as with
+any operator of torch.  Rows may have any distance from one another; the values of a row lie side by side, or the rows are copied
+first.  Arguments that do not fit raise ValueError.
+"""
+from __future__ import annotations
+
+from typing import NamedTuple, Optional, Tuple
+
+import torch
+
+from ._lib import check, lib
+
+_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+_ID_BITS = {torch.int32: 32, torch.uint32: 32, torch.int64: 64}
+_MOST = 2**31 - 1
+
+
+class RowGroups(NamedTuple):
+    """Pairs (row, choice) in the order of their cluster, as `group_rows` makes them; all int32.
+
+    order[slot]: the pair (row * m + choice) in that slot;  position[row, choice]: the slot of that pair;  offsets[c]: the first slot
+    of cluster c, c = 0 .. n_clusters.  Slots from offsets[-1] on hold the pairs without a cluster."""
+
+    order: torch.Tensor
+    position: torch.Tensor
+    offsets: torch.Tensor
+
+
+class QuantizedRows(NamedTuple):
+    """Rows in 8 bits: row i stands for values[i] * scales[i]."""
+
+    values: torch.Tensor
+    scales: torch.Tensor
+
+
+# ---- checks ---------------------------------------------------------------------------------------------------------------------
+
+
+def _on_gpu(t, name: str, like=None) -> None:
+    if not isinstance(t, torch.Tensor):
+        raise ValueError(f"{name} must be a torch tensor")
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be on a CUDA device")
+    if like is not None and t.device != like.device:
+        raise ValueError(f"{name} must be on {like.device}, got {t.device}")
+
+
+def _rows(t, name: str, like=None, dtype=None) -> Tuple[torch.Tensor, int]:
+    """The rows with their values side by side, and the distance from one to the next."""
+    _on_gpu(t, name, like)
+    if t.dim() != 2:
+        raise ValueError(f"{name} must be 2-dimensional, got {t.dim()}")
+    if t.dtype not in _DTYPES:
+        raise ValueError(f"{name} must have dtype float32, float16 or bfloat16, got {t.dtype}")
+    if dtype is not None and t.dtype != dtype:
+        raise ValueError(f"{name} must have dtype {dtype}, got {t.dtype}")
+    n, d = t.shape
+    if d == 0:
+        raise ValueError(f"{name} must have at least one column")
+    if d > 1 and t.stride(1) != 1:
+        t = t.contiguous()
+    return t, t.stride(0) if n > 1 else d
+
+
+def _ids(ids, name: str, like=None) -> Tuple[torch.Tensor, int]:
+    _on_gpu(ids, name, like)
+    bits = _ID_BITS.get(ids.dtype)
+    if bits is None:
+        raise ValueError(f"{name} must have dtype int32, uint32 or int64, got {ids.dtype}")
+    if ids.numel() > _MOST:
+        raise ValueError(f"{name} must have no more than 2**31 - 1 entries")
+    return ids if ids.is_contiguous() else ids.contiguous(), bits
+
+
+def _floats(t, name: str, shape, like) -> torch.Tensor:
+    _on_gpu(t, name, like)
+    if t.dtype != torch.float32:
+        raise ValueError(f"{name} must have dtype float32, got {t.dtype}")
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _groups(groups: RowGroups, like) -> Tuple[torch.Tensor, torch.Tensor, int, int, int]:
+    """position, offsets, number of clusters, rows, choices to a row"""
+    _, position, offsets = groups
+    _on_gpu(position, "position", like)
+    _on_gpu(offsets, "offsets", like)
+    if position.dtype != torch.int32 or offsets.dtype != torch.int32:
+        raise ValueError("position and offsets must have dtype int32")
+    if position.dim() not in (1, 2) or offsets.dim() != 1 or offsets.shape[0] < 2:
+        raise ValueError("position must have one or two dimensions, offsets one with at least two entries")
+    if not (position.is_contiguous() and offsets.is_contiguous()):
+        raise ValueError("position and offsets must be contiguous")
+    m = position.shape[1] if position.dim() == 2 else 1
+    if m == 0:
+        raise ValueError("a row must have at least one choice")
+    return position, offsets, offsets.shape[0] - 1, position.shape[0], m
+
+
+def _clusters(n_clusters: int) -> int:
+    n_clusters = int(n_clusters)
+    if not 0 < n_clusters < _MOST:
+        raise ValueError("the number of clusters must be positive and below 2**31 - 1")
+    return n_clusters
+
+
+def _p(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
+
+
+def _stream(t: torch.Tensor) -> int:
+    return torch.cuda.current_stream(t.device).cuda_stream
+
+
+def _workspace(n_bytes: int, like: torch.Tensor) -> torch.Tensor:
+    return torch.empty(n_bytes, dtype=torch.uint8, device=like.device)
+
+
+# ---- lookup ---------------------------------------------------------------------------------------------------------------------
+
+
+def _lookup(table, ids, scale, row_scales):
+    rows, ld = _rows(table, "table")
+    at, bits = _ids(ids, "ids", table)
+    k, d = rows.shape
+    _clusters(k)
+    if row_scales is not None:
+        row_scales = _floats(row_scales, "row_scales", ids.shape, table)
+    out = torch.empty(*ids.shape, d, dtype=table.dtype, device=table.device)
+    check(lib.skm_op_lookup(table.device.index, _p(rows), ld, _DTYPES[table.dtype], k, d, _p(at), bits, at.numel(), scale, _p(row_scales), _p(out), _stream(table)))
+    return out
+
+
+class _Lookup(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, table, ids, scale, row_scales):
+        ctx.scale, ctx.k = scale, table.shape[0]
+        # (the table itself is needed for the scales' gradient only)
+        ctx.save_for_backward(table if row_scales is not None and ctx.needs_input_grad[3] else None, ids, row_scales)
+        return _lookup(table, ids, scale, row_scales)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        table, ids, row_scales = ctx.saved_tensors
+        grad = grad.reshape(-1, grad.shape[-1])
+        flat = ids.reshape(-1)
+        grad_table = grad_scales = None
+        if ctx.needs_input_grad[0]:
+            grad_table = lookup_grad(grad, flat, ctx.k, ctx.scale, None if row_scales is None else row_scales.reshape(-1))
+        if ctx.needs_input_grad[3]:
+            grad_scales = lookup_scale_grad(grad, table, flat, ctx.scale).reshape(ids.shape)
+        return grad_table, None, None, grad_scales
+
+
+def lookup(table: torch.Tensor, ids: torch.Tensor, scale: float = 1.0, row_scales: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """scale * row_scales * table[ids]: the vectors of `ids` (any shape; int32, uint32 or int64, as the assignments of a model), out of
+    a table of k x d values in fp32, fp16 or bf16.  `row_scales`, if given, has the shape of `ids` and dtype float32.  An id that is no
+    row of the table (-1 as padding) gives zeros and no gradient.  Differentiable in `table` (see lookup_grad) and `row_scales`."""
+    scale = float(scale)
+    if torch.is_grad_enabled() and (getattr(table, "requires_grad", False) or getattr(row_scales, "requires_grad", False)):
+        return _Lookup.apply(table, ids, scale, row_scales)
+    return _lookup(table, ids, scale, row_scales)
+
+
+def lookup_grad(grad: torch.Tensor, ids: torch.Tensor, n_rows: int, scale: float = 1.0, row_scales: Optional[torch.Tensor] = None,
+                dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """Gradient of a table of `n_rows` rows: row c is the sum of scale * row_scales[i] * grad[i] over ids[i] = c, zeros where there is no such
+    i.  Summed in fp32 in an order that depends on the ids alone, and rounded once to `dtype` (that of `grad`, or float32)."""
+    rows, ld = _rows(grad, "grad")
+    at, bits = _ids(ids, "ids", grad)
+    n, d = rows.shape
+    if at.numel() != n or at.dim() != 1:
+        raise ValueError(f"ids must have shape ({n},), got {tuple(at.shape)}")
+    k = _clusters(n_rows)
+    dtype = grad.dtype if dtype is None else dtype
+    if dtype not in (grad.dtype, torch.float32):
+        raise ValueError(f"dtype must be {grad.dtype} or float32, got {dtype}")
+    if row_scales is not None:
+        row_scales = _floats(row_scales, "row_scales", ids.shape, grad)
+    kind = _DTYPES[grad.dtype]
+    out = torch.empty(k, d, dtype=dtype, device=grad.device)
+    space = _workspace(lib.skm_op_lookup_grad_workspace(n, k, d, kind), grad)
+    check(lib.skm_op_lookup_grad(grad.device.index, _p(rows), ld, kind, k, d, _p(at), bits, n, float(scale), _p(row_scales), _p(out), _DTYPES[dtype], _p(space), space.numel(),
+                                 _stream(grad)))
+    return out
+
+
+def lookup_scale_grad(grad: torch.Tensor, table: torch.Tensor, ids: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
+    """Gradient of the row scales of a lookup, float32: scale * <grad[i], table[ids[i]]>, zero where the id is no row of the table."""
+    rows, ld = _rows(grad, "grad")
+    t, ld_t = _rows(table, "table", grad, grad.dtype)
+    at, bits = _ids(ids, "ids", grad)
+    n, d = rows.shape
+    if t.shape[1] != d:
+        raise ValueError(f"grad and table must have the same dimensionality, got {d} and {t.shape[1]}")
+    if at.numel() != n or at.dim() != 1:
+        raise ValueError(f"ids must have shape ({n},), got {tuple(at.shape)}")
+    k = _clusters(t.shape[0])
+    out = torch.empty(n, dtype=torch.float32, device=grad.device)
+    check(lib.skm_op_lookup_scale_grad(grad.device.index, _p(rows), ld, _p(t), ld_t, _DTYPES[grad.dtype], k, d, _p(at), bits, n, float(scale), _p(out), _stream(grad)))
+    return out
+
+
+# ---- rows to their clusters and back --------------------------------------------------------------------------------------------
+
+
+def group_rows(ids: torch.Tensor, n_clusters: int) -> RowGroups:
+    """The order of rows by cluster: `ids` has one entry for each row (n), or one for each of its m choices (n x m).  Pairs of the same
+    cluster keep their order; those without one (an id outside 0 .. n_clusters - 1) come last.  The offsets stay on the device."""
+    at, bits = _ids(ids, "ids")
+    if at.dim() not in (1, 2) or (at.dim() == 2 and at.shape[1] == 0):
+        raise ValueError(f"ids must have shape (n,) or (n, m) with m > 0, got {tuple(at.shape)}")
+    k, n = _clusters(n_clusters), at.numel()
+    order = torch.empty(n, dtype=torch.int32, device=ids.device)
+    position = torch.empty(at.shape, dtype=torch.int32, device=ids.device)
+    offsets = torch.empty(k + 1, dtype=torch.int32, device=ids.device)
+    space = _workspace(lib.skm_op_group_rows_workspace(n, k), ids)
+    check(lib.skm_op_group_rows(ids.device.index, _p(at), bits, n, k, _p(order), _p(position), _p(offsets), _p(space), space.numel(), _stream(ids)))
+    return RowGroups(order, position, offsets)
+
+
+def _to_clusters(x, groups):
+    rows, ld = _rows(x, "x")
+    position, offsets, k, n, m = _groups(groups, x)
+    if rows.shape[0] != n:
+        raise ValueError(f"x must have {n} rows, got {rows.shape[0]}")
+    d = rows.shape[1]
+    out = torch.empty(n * m, d, dtype=x.dtype, device=x.device)
+    check(lib.skm_op_to_clusters(x.device.index, _p(rows), ld, _DTYPES[x.dtype], d, _p(position), _p(offsets), k, n, m, _p(out), _stream(x)))
+    return out
+
+
+def _from_clusters(y, groups, weights, name="y"):
+    rows, ld = _rows(y, name)
+    position, offsets, k, n, m = _groups(groups, y)
+    if rows.shape[0] != n * m:
+        raise ValueError(f"{name} must have {n * m} rows, got {rows.shape[0]}")
+    if weights is not None:
+        weights = _floats(weights, "weights", position.shape, y)
+    d = rows.shape[1]
+    out = torch.empty(n, d, dtype=y.dtype, device=y.device)
+    check(lib.skm_op_from_clusters(y.device.index, _p(rows), ld, _DTYPES[y.dtype], d, _p(position), _p(offsets), k, n, m, _p(weights), _p(out), _stream(y)))
+    return out
+
+
+def _from_clusters_grad(grad, y, groups, weights, want_y, want_weights):
+    rows, ld = _rows(grad, "grad")
+    position, offsets, k, n, m = _groups(groups, grad)
+    d = rows.shape[1]
+    if rows.shape[0] != n:
+        raise ValueError(f"grad must have {n} rows, got {rows.shape[0]}")
+    if weights is not None:
+        weights = _floats(weights, "weights", position.shape, grad)
+    from_y, ld_y = None, 0
+    if want_weights:
+        from_y, ld_y = _rows(y, "y", grad, grad.dtype)
+        if tuple(from_y.shape) != (n * m, d):
+            raise ValueError(f"y must have shape {(n * m, d)}, got {tuple(from_y.shape)}")
+    grad_y = torch.empty(n * m, d, dtype=grad.dtype, device=grad.device) if want_y else None
+    grad_weights = torch.empty(position.shape, dtype=torch.float32, device=grad.device) if want_weights else None
+    check(lib.skm_op_from_clusters_grad(grad.device.index, _p(rows), ld, _p(from_y), ld_y, _DTYPES[grad.dtype], d, _p(position), _p(offsets), k, n, m, _p(weights), _p(grad_y),
+                                        _p(grad_weights), _stream(grad)))
+    return grad_y, grad_weights
+
+
+class _ToClusters(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, order, position, offsets):
+        ctx.save_for_backward(order, position, offsets)
+        return _to_clusters(x, RowGroups(order, position, offsets))
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        return to_clusters_grad(grad, RowGroups(*ctx.saved_tensors)), None, None, None
+
+
+class _FromClusters(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, y, weights, order, position, offsets):
+        # (y is needed for the weights' gradient only)
+        ctx.save_for_backward(y if weights is not None and ctx.needs_input_grad[1] else None, weights, order, position, offsets)
+        return _from_clusters(y, RowGroups(order, position, offsets), weights)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        y, weights, *groups = ctx.saved_tensors
+        grad_y, grad_weights = _from_clusters_grad(grad, y, RowGroups(*groups), weights, ctx.needs_input_grad[0], ctx.needs_input_grad[1])
+        return grad_y, grad_weights, None, None, None
+
+
+def to_clusters(x: torch.Tensor, groups: RowGroups) -> torch.Tensor:
+    """Rows in the order of their clusters: n x d to (n * m) x d, row i once for each of its m choices, at groups.position[i, j].  The rows of
+    cluster c are offsets[c] .. offsets[c + 1] - 1; behind the last cluster the slots of choices without one hold zeros.
+    Differentiable in x (see to_clusters_grad)."""
+    if torch.is_grad_enabled() and getattr(x, "requires_grad", False):
+        return _ToClusters.apply(x, *groups)
+    return _to_clusters(x, groups)
+
+
+def to_clusters_grad(grad: torch.Tensor, groups: RowGroups) -> torch.Tensor:
+    """Gradient of the rows of to_clusters: the sum over a row's choices of their slots' gradients (n x d), without those that have no
+    cluster."""
+    return _from_clusters(grad, groups, None, "grad")
+
+
+def from_clusters(y: torch.Tensor, groups: RowGroups, weights: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Rows back from the order of their clusters: out[i] = sum over j of weights[i, j] * y[position[i, j]], n x d.  Choices without a cluster
+    contribute nothing, whatever their slots hold.  `weights` (float32, the shape of groups.position) is 1 if not given.
+    Differentiable in y and weights (see from_clusters_grad)."""
+    if torch.is_grad_enabled() and (getattr(y, "requires_grad", False) or getattr(weights, "requires_grad", False)):
+        return _FromClusters.apply(y, weights, *groups)
+    return _from_clusters(y, groups, weights)
+
+
+def from_clusters_grad(grad: torch.Tensor, y: torch.Tensor, groups: RowGroups, weights: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """Gradients of from_clusters: of y, weights[i, j] * grad[i] at position[i, j] and zeros in the slots of choices without a cluster; and of the
+    weights (float32; None where there are none), <grad[i], y[position[i, j]]>."""
+    return _from_clusters_grad(grad, y, groups, weights, True, weights is not None)
+
+
+# ---- products in 8 bits ---------------------------------------------------------------------------------------------------------
+
+
+def quantize_rows(x: torch.Tensor) -> QuantizedRows:
+    """Rows in 8 bits: scales[i] = max |x[i]| / 127 (float32), values[i] = x[i] / scales[i] rounded to the nearest whole number, int8.  A row of
+    zeros has scale 0; a row with a value that is no finite number has scale NaN.  The rows of the result begin on 16 bytes."""
+    rows, ld = _rows(x, "x")
+    n, d = rows.shape
+    if n > _MOST:
+        raise ValueError("x must have no more than 2**31 - 1 rows")
+    pitch = (d + 15) // 16 * 16
+    q = torch.empty(n, pitch, dtype=torch.int8, device=x.device)
+    scales = torch.empty(n, dtype=torch.float32, device=x.device)
+    check(lib.skm_op_quantize_rows(x.device.index, _p(rows), ld, _DTYPES[x.dtype], n, d, _p(q), pitch, _p(scales), _stream(x)))
+    return QuantizedRows(q[:, :d] if pitch != d else q, scales)
+
+
+def _bytes(t, name: str, like=None) -> torch.Tensor:
+    _on_gpu(t, name, like)
+    if t.dtype != torch.int8:
+        raise ValueError(f"{name} must have dtype int8, got {t.dtype}")
+    return t.contiguous() if t.shape[-1] > 1 and t.stride(-1) != 1 else t
+
+
+def product_8bit(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, offsets: Optional[torch.Tensor] = None,
+                 dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """x w^T of rows in 8 bits: out[i, c] = x_scales[i] * w_scales[c] * sum_j x[i, j] * w[c, j], the sum exact.  x is n x d, w m x d (both int8), the
+    scales float32, the result n x m of `dtype`.
+
+    With `offsets` (int32, from group_rows) w is n_clusters x m x d and w_scales n_clusters x m: row i is multiplied by the matrix of the cluster c with
+    offsets[c] <= i < offsets[c + 1]; rows of no cluster come out as zeros.
+
+    Rows that do not begin on 16 bytes are copied first; quantize_rows makes rows that do.  d is at most 131071."""
+    if dtype not in _DTYPES:
+        raise ValueError(f"dtype must be float32, float16 or bfloat16, got {dtype}")
+    _on_gpu(x, "x")
+    _on_gpu(w, "w", x)
+    if x.dim() != 2:
+        raise ValueError(f"x must be 2-dimensional, got {x.dim()}")
+    if w.dim() != (2 if offsets is None else 3):
+        raise ValueError(f"w must be {2 if offsets is None else 3}-dimensional, got {w.dim()}")
+    x, w = _bytes(x, "x"), _bytes(w, "w", x)
+    n, d = x.shape
+    m, e = w.shape[-2], 0
+    if w.shape[-1] != d:
+        raise ValueError(f"x and w must have the same dimensionality, got {d} and {w.shape[-1]}")
+    if not 0 < d <= 131071:
+        raise ValueError(f"the dimensionality of a product in 8 bits must be positive and at most 131071, got {d}")
+    if offsets is not None:
+        e = _clusters(w.shape[0])
+        _on_gpu(offsets, "offsets", x)
+        if offsets.dtype != torch.int32 or tuple(offsets.shape) != (e + 1,) or not offsets.is_contiguous():
+            raise ValueError(f"offsets must be {e + 1} contiguous int32")
+        if e > 1 and m > 0 and w.stride(0) != m * (w.stride(1) if m > 1 else w.stride(0)):
+            w = w.contiguous()
+    x_scales = _floats(x_scales, "x_scales", (n,), x)
+    w_scales = _floats(w_scales, "w_scales", w.shape[:-1], x)
+    ld_x = x.stride(0) if n > 1 else d
+    ld_w = w.stride(-2) if m > 1 else w.stride(0) if e > 1 else d
+    out = torch.empty(n, m, dtype=dtype, device=x.device)
+    space = _workspace(lib.skm_op_product_8bit_workspace(_p(x), ld_x, _p(w), ld_w, n, m, d, e), x)
+    check(lib.skm_op_product_8bit(x.device.index, _p(x), ld_x, _p(x_scales), _p(w), ld_w, _p(w_scales), n, m, d, e, _p(offsets), _p(out), _DTYPES[dtype], _p(space), space.numel(),
+                                  _stream(x)))
+    return out
+
+
+def check_products(device=None) -> None:
+    """Waits for the current stream of `device` and raises RuntimeError if a product on it gave up waiting inside its kernel (the next
+    product_8bit on the device raises it too)."""
+    device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+    check(lib.skm_op_product_8bit_status(-1 if device.index is None else device.index, torch.cuda.current_stream(device).cuda_stream))
+
+
+__all__ = [
+    "RowGroups", "QuantizedRows", "lookup", "lookup_grad", "lookup_scale_grad", "group_rows", "to_clusters", "to_clusters_grad", "from_clusters", "from_clusters_grad",
+    "quantize_rows", "product_8bit", "check_products",
+]
