@@ -604,6 +604,11 @@ CUtensorMap make_byte_tmap(const void* base, size_t cols, size_t rows, uint32_t 
     return make_tmap_of(CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, CU_TENSOR_MAP_SWIZZLE_128B, base, cols, rows, pitch, 128, box_rows);
 }
 
+CUtensorMap make_result_tmap(void* base, size_t element, size_t cols, size_t rows, uint32_t box_rows) {
+    return make_tmap_of(element == 2 ? CU_TENSOR_MAP_DATA_TYPE_UINT16 : CU_TENSOR_MAP_DATA_TYPE_UINT32, element, CU_TENSOR_MAP_SWIZZLE_128B, base, cols, rows, cols,
+                        static_cast<uint32_t>(128 / element), box_rows);
+}
+
 CUtensorMap make_row_major_tmap_128(const float* base, size_t extent, size_t rows, size_t ld, uint32_t box_rows) {
     return make_tmap_of(CU_TENSOR_MAP_DATA_TYPE_FLOAT32, sizeof(float), CU_TENSOR_MAP_SWIZZLE_128B, base, extent, rows, ld, 32, box_rows);
 }

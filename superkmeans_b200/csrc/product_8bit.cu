@@ -110,6 +110,7 @@ struct RowTile {
 
 struct ProductMaps {
     CUtensorMap w, x;
+    CUtensorMap out;   // (where lanes are rows)
 };
 
 struct ProductParams {
@@ -120,7 +121,7 @@ struct ProductParams {
     uint32_t channel_tiles;
     uint32_t groups;             // 0: none
     const RowTile* tiles;        // with groups
-    const uint32_t* n_tiles;
+    const uint32_t* n_tiles;     // that belong to a group, and all
     int* error;
     int* told;                   // in host memory
     long long wait_limit;
@@ -162,7 +163,7 @@ __global__ void __launch_bounds__(P_THREADS) product_kernel(const __grid_constan
     const uint32_t tile = blockIdx.x / split, channel_tile = tile % p.channel_tiles, row_tile = tile / p.channel_tiles;
     RowTile t;
     if (p.groups) {
-        if (row_tile >= __ldg(p.n_tiles)) return;   // (the whole cluster)
+        if (row_tile >= __ldg(p.n_tiles + 1)) return;   // (the whole cluster)
         t = p.tiles[row_tile];
     } else {
         t = {row_tile * ROWS, min(row_tile * ROWS + ROWS, p.n), 0};
@@ -276,7 +277,340 @@ __global__ void __launch_bounds__(P_THREADS) product_kernel(const __grid_constan
     if (warp == 0) tmem_dealloc(tmem_base, COLS);
 }
 
-// The tiles of `rows` rows that the groups consist of, one block.
+// ---- many rows: persistent pairs of CTAs on tiles of 256 lanes x COLS columns, each CTA with its 128 lanes, half of the columns as operand
+// and all of them in its accumulator:
+//   warp 0       TMA producer
+//   warp 1       MMA issuer (the leader's)
+//   warps 4-11   epilogue: 32 lanes and half of the columns each, out of one accumulator while the other is filled
+// Where rows of the result begin on 32 bytes, the lanes are rows of x: a thread then holds 128 neighbouring results of a row and stores
+// 32 bytes at a time.  Elsewhere, and where the tile is narrow because the groups are small, the lanes are channels, and the 32 lanes of
+// a warp store 32 neighbouring results of a row.
+constexpr int Q_EPI_WARPS = 8;
+constexpr int Q_THREADS = 128 + 32 * Q_EPI_WARPS;
+constexpr uint32_t Q_TRAY_BYTES = 32 * 128;   // 32 rows of results on their way out, of each epilogue warp
+template <bool LANES_ARE_ROWS>
+constexpr int kPairStages = LANES_ARE_ROWS ? 5 : 6;
+
+template <int COLS>
+struct PairControl {
+    uint64_t full[6];            // (the leader's are used)
+    uint64_t empty[6];
+    uint64_t acc_full[2];
+    uint64_t acc_empty[2];       // (the leader's are used)
+    uint32_t tmem_base;
+    alignas(16) float scales[Q_EPI_WARPS][COLS / 2];   // of a warp's columns
+};
+template <int COLS>
+constexpr uint32_t kPairStageBytes = P_W_BYTES + COLS / 2 * P_DEPTH;
+template <int COLS, bool LANES_ARE_ROWS>
+constexpr uint32_t kPairSmem = kPairStages<LANES_ARE_ROWS> * kPairStageBytes<COLS> + (LANES_ARE_ROWS ? Q_EPI_WARPS * Q_TRAY_BYTES : 0) + sizeof(PairControl<COLS>) + 1024;
+
+__device__ __forceinline__ float low_of(uint64_t p) { return __uint_as_float(static_cast<uint32_t>(p)); }
+__device__ __forceinline__ float high_of(uint64_t p) { return __uint_as_float(static_cast<uint32_t>(p >> 32)); }
+
+// 32 sums times the scales of their columns, and the lane's.
+__device__ __forceinline__ void scale_columns(const uint32_t (&r)[32], const float* scales, uint64_t lane_scale2, uint64_t (&v)[16]) {
+#pragma unroll
+    for (int j = 0; j < 16; j += 2) {
+        const ulonglong2 s = *reinterpret_cast<const ulonglong2*>(scales + 2 * j);
+        v[j] = mul2(mul2(pack2(__int2float_rn(static_cast<int>(r[2 * j])), __int2float_rn(static_cast<int>(r[2 * j + 1]))), s.x), lane_scale2);
+        v[j + 1] = mul2(mul2(pack2(__int2float_rn(static_cast<int>(r[2 * j + 2])), __int2float_rn(static_cast<int>(r[2 * j + 3]))), s.y), lane_scale2);
+    }
+}
+
+// store(c, v) for each 32 of a lane's `count` columns in tensor memory; the next 32 are on their way meanwhile.
+template <int MOST, class F>
+__device__ __forceinline__ void each_32_columns(uint32_t taddr, uint32_t count, const float* scales, float lane_scale, F&& store) {
+    if (count == 0) return;
+    const uint64_t lane_scale2 = pack2(lane_scale, lane_scale);
+    uint32_t a[32], b[32];
+    uint64_t v[16];
+    tmem_ld32_issue(taddr, a);
+#pragma unroll
+    for (uint32_t c = 0; c < MOST; c += 64) {
+        if (c >= count) break;
+        tmem_ld_wait(a);
+        const bool second = c + 32 < MOST && c + 32 < count;
+        if (second) tmem_ld32_issue(taddr + c + 32, b);
+        scale_columns(a, scales + c, lane_scale2, v);
+        store(c, v);
+        if (second) {
+            tmem_ld_wait(b);
+            if (c + 64 < MOST && c + 64 < count) tmem_ld32_issue(taddr + c + 64, a);
+            scale_columns(b, scales + c + 32, lane_scale2, v);
+            store(c + 32, v);
+        }
+    }
+}
+
+__device__ __forceinline__ void store_32_bytes(void* p, const uint32_t (&w)[8]) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+}
+
+// 32 results of one row, of which `left` are to be stored (a multiple of 32 bytes).
+template <typename O>
+__device__ __forceinline__ void store_along_row(O* to, const uint64_t (&v)[16], uint32_t left) {
+    constexpr uint32_t PAIRS = sizeof(O) == 2 ? 8 : 4;   // in 32 bytes
+#pragma unroll
+    for (uint32_t j = 0; j < 16; j += PAIRS)
+        if (2 * j < left) {
+            uint32_t w[8];
+#pragma unroll
+            for (uint32_t e = 0; e < PAIRS; ++e) {
+                if constexpr (sizeof(O) == 2) w[e] = pair_from_float(low_of(v[j + e]), high_of(v[j + e]), static_cast<const O*>(nullptr));
+                else {
+                    w[2 * e] = static_cast<uint32_t>(v[j + e]);
+                    w[2 * e + 1] = static_cast<uint32_t>(v[j + e] >> 32);
+                }
+            }
+            store_32_bytes(to + 2 * j, w);
+        }
+}
+
+// Results of 32 rows for the channel of each lane, of which `left` rows are to be stored.
+template <typename O>
+__device__ __forceinline__ void store_across_rows(O* out, uint32_t m, uint32_t channel, bool has_channel, uint32_t lane, const uint64_t (&v)[16], uint32_t left, bool packed) {
+    auto all = [&](auto whole) {
+        if constexpr (sizeof(O) == 2) {
+            if (packed) {
+                // two lanes swap halves, so that each stores two channels of one row
+                const uint32_t odd = lane & 1, pick = odd ? 0x3276 : 0x5410;
+                O* to = out + static_cast<size_t>(odd) * m + (channel - odd);
+#pragma unroll
+                for (uint32_t j = 0; j < 16; ++j) {
+                    const uint32_t mine = pair_from_float(low_of(v[j]), high_of(v[j]), static_cast<const O*>(nullptr)), other = __shfl_xor_sync(0xffffffffu, mine, 1);
+                    if ((whole.value || 2 * j + odd < left) && has_channel) *reinterpret_cast<uint32_t*>(to + static_cast<size_t>(2 * j) * m) = __byte_perm(mine, other, pick);
+                }
+                return;
+            }
+        }
+        O* to = out + channel;
+#pragma unroll
+        for (uint32_t j = 0; j < 16; ++j) {
+            if ((whole.value || 2 * j < left) && has_channel) store_result(to + static_cast<size_t>(2 * j) * m, low_of(v[j]));
+            if ((whole.value || 2 * j + 1 < left) && has_channel) store_result(to + static_cast<size_t>(2 * j + 1) * m, high_of(v[j]));
+        }
+    };
+    if (left >= 32) all(std::true_type{});
+    else all(std::false_type{});
+}
+
+template <int COLS, typename O, bool LANES_ARE_ROWS>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Q_THREADS, 1) product_pair_kernel(const __grid_constant__ ProductMaps maps, const ProductParams p) {
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t raw_addr = smem_u32(smem_raw);
+    const uint32_t pad = (1024u - (raw_addr & 1023u)) & 1023u;
+    uint8_t* smem = smem_raw + pad;
+    const uint32_t smem_base = raw_addr + pad;
+    constexpr int STAGES = kPairStages<LANES_ARE_ROWS>;
+    constexpr uint32_t TRAYS_AT = STAGES * kPairStageBytes<COLS>;
+    auto* ctrl = reinterpret_cast<PairControl<COLS>*>(smem + TRAYS_AT + (LANES_ARE_ROWS ? Q_EPI_WARPS * Q_TRAY_BYTES : 0));
+    const WaitCtx wctx{p.error, p.wait_limit};
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_rank();
+    constexpr uint32_t ROWS = LANES_ARE_ROWS ? 256 : COLS, CHANNELS = LANES_ARE_ROWS ? COLS : 256;   // of a tile
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) {
+            mbar_init(&ctrl->full[s], 1);
+            mbar_init(&ctrl->empty[s], 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(&ctrl->acc_full[b], 1);
+            mbar_init(&ctrl->acc_empty[b], 2 * Q_EPI_WARPS);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        fence_proxy_async();
+    }
+    if (warp == 1) tmem_alloc_pair(&ctrl->tmem_base, TMEM_COLS);
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();   // the peer's barriers exist
+    tc_fence_after();
+    const uint32_t tmem_base = ctrl->tmem_base;
+
+    const uint32_t row_tiles = p.groups ? __ldg(p.n_tiles) : (p.n + ROWS - 1) / ROWS;   // that have a group
+    const uint32_t n_tiles = row_tiles * p.channel_tiles;
+    const uint32_t first = blockIdx.x >> 1, step = gridDim.x >> 1;
+    // the rows of tile t and its first channel
+    auto tile_at = [&](uint32_t t, uint32_t& channel0) {
+        const uint32_t i = t / p.channel_tiles;
+        channel0 = (t - i * p.channel_tiles) * CHANNELS;
+        if (p.groups) return p.tiles[i];
+        return RowTile{i * ROWS, min(i * ROWS + ROWS, p.n), 0};
+    };
+
+    bool ok = true;
+    if (warp == 0 && lane == 0) {
+        uint32_t it = 0, next_channel0 = 0;
+        RowTile next = first < n_tiles ? tile_at(first, next_channel0) : RowTile{};
+        const CUtensorMap* lane_map = LANES_ARE_ROWS ? &maps.x : &maps.w;
+        const CUtensorMap* column_map = LANES_ARE_ROWS ? &maps.w : &maps.x;
+        for (uint32_t t = first; t < n_tiles && ok; t += step) {
+            const uint32_t w_row = next.group * p.m + next_channel0, x_row = next.row0;
+            const int at_lanes = static_cast<int>((LANES_ARE_ROWS ? x_row : w_row) + rank * 128), at_columns = static_cast<int>((LANES_ARE_ROWS ? w_row : x_row) + rank * (COLS / 2));
+            if (t + step < n_tiles) next = tile_at(t + step, next_channel0);
+            for (uint32_t k = 0; k < p.depth_blocks; ++k, ++it) {
+                const uint32_t s = it % STAGES, ph = (it / STAGES) & 1u;
+                if ((p.producer_stop != 0 && it >= p.producer_stop) || !mbar_wait(&ctrl->empty[s], ph ^ 1u, wctx, 44)) {
+                    ok = false;
+                    break;
+                }
+                if (rank == 0) mbar_arrive_expect_tx(&ctrl->full[s], 2 * kPairStageBytes<COLS>);
+                const uint32_t bar = cluster_address(&ctrl->full[s], 0), st = smem_base + s * kPairStageBytes<COLS>;
+                tma_load_2d_pair(st, lane_map, bar, static_cast<int>(k * P_DEPTH), at_lanes);
+                tma_load_2d_pair(st + P_W_BYTES, column_map, bar, static_cast<int>(k * P_DEPTH), at_columns);
+            }
+        }
+        if (!ok) {
+            // another role gave up: a millisecond for the copies that are in flight before the block's memory is let go
+            const long long t0 = clock64();
+            while (clock64() - t0 < 2000000) {
+            }
+        }
+    } else if (warp == 1 && lane == 0 && rank == 0) {
+        constexpr uint32_t idesc = make_idesc_i8(256, COLS);
+        uint32_t it = 0, i = 0;
+        for (uint32_t t = first; t < n_tiles && ok; t += step, ++i) {
+            const uint32_t b = i & 1u, acc = tmem_base + b * 256;
+            if (!mbar_wait(&ctrl->acc_empty[b], ((i >> 1) & 1u) ^ 1u, wctx, 45)) {
+                ok = false;
+                break;
+            }
+            tc_fence_after();
+            for (uint32_t k = 0; k < p.depth_blocks; ++k, ++it) {
+                const uint32_t s = it % STAGES, ph = (it / STAGES) & 1u;
+                if (!mbar_wait(&ctrl->full[s], ph, wctx, 46)) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                const uint32_t st = smem_base + s * kPairStageBytes<COLS>;
+#pragma unroll
+                for (uint32_t kk = 0; kk < P_DEPTH / 32; ++kk) umma_i8_pair(acc, make_desc_128(st + kk * 32), make_desc_128(st + P_W_BYTES + kk * 32), k != 0 || kk != 0 ? 1u : 0u, idesc);
+                umma_commit_pair(&ctrl->empty[s]);
+            }
+            if (ok) umma_commit_pair(&ctrl->acc_full[b]);
+        }
+    } else if (warp >= 4) {
+        constexpr uint32_t MINE = COLS / 2, EACH = MINE / 32;   // columns of a warp
+        const uint32_t quarter = warp & 3u, half = (warp - 4) >> 2;
+        float* scales = ctrl->scales[warp - 4];
+        [[maybe_unused]] uint8_t* tray = smem + TRAYS_AT + (warp - 4) * Q_TRAY_BYTES;
+        O* out = static_cast<O*>(p.out);
+        const bool packed = p.m % 2 == 0 && (reinterpret_cast<uintptr_t>(out) & 3) == 0;
+        // a tile's place and scales are looked up while the one before is stored
+        uint32_t row = 0, channel = 0, count = 0;   // row and channel of this lane's first column, columns
+        bool valid = false;                         // this lane is in the matrix
+        float lane_scale = 0.f, scale[EACH];
+        auto look_up = [&](uint32_t t) {
+            uint32_t channel0;
+            const RowTile tile = tile_at(t, channel0);
+            const float* w_scales = p.w_scales + static_cast<size_t>(tile.group) * p.m;
+            const uint32_t at_lane = rank * 128 + quarter * 32 + lane;
+            uint32_t end, column;
+            const float* column_scales;
+            if constexpr (LANES_ARE_ROWS) {
+                row = tile.row0 + at_lane;
+                channel = channel0 + half * MINE;
+                valid = row < tile.row1;
+                column = channel;
+                end = p.m;
+                column_scales = w_scales;
+                lane_scale = valid ? __ldg(p.x_scales + row) : 0.f;
+            } else {
+                row = tile.row0 + half * MINE;
+                channel = channel0 + at_lane;
+                valid = channel < p.m;
+                column = row;
+                end = tile.row1;
+                column_scales = p.x_scales;
+                lane_scale = valid ? __ldg(w_scales + channel) : 0.f;
+            }
+            count = end > column ? min(end - column, MINE) : 0;
+#pragma unroll
+            for (uint32_t e = 0; e < EACH; ++e) scale[e] = e * 32 + lane < count ? __ldg(column_scales + column + e * 32 + lane) : 0.f;
+        };
+        if (first < n_tiles) look_up(first);
+        uint32_t i = 0;
+        for (uint32_t t = first; t < n_tiles; t += step, ++i) {
+            const uint32_t b = i & 1u, my_row = row, my_channel = channel, my_count = count;
+            const bool my_valid = valid;
+            const float my_scale = lane_scale;
+            __syncwarp();
+#pragma unroll
+            for (uint32_t e = 0; e < EACH; ++e) scales[e * 32 + lane] = scale[e];
+            __syncwarp();
+            if (t + step < n_tiles) look_up(t + step);
+            if (!__all_sync(0xffffffffu, mbar_wait(&ctrl->acc_full[b], (i >> 1) & 1u, wctx, 47))) {
+                if (lane == 0) *reinterpret_cast<volatile int*>(p.told) = 47;
+                break;
+            }
+            tc_fence_after();
+            const uint32_t taddr = tmem_base + (quarter * 32 << 16) + b * 256 + half * MINE;
+            O* to = out + static_cast<size_t>(my_row) * p.m;
+            [[maybe_unused]] const bool whole = __all_sync(0xffffffffu, my_valid);   // (what is behind the last column is left out by the copy)
+            each_32_columns<MINE>(taddr, my_count, scales, my_scale, [&](uint32_t c, const uint64_t (&v)[16]) {
+                if constexpr (LANES_ARE_ROWS) {
+                    if (!whole) {
+                        if (my_valid) store_along_row(to + my_channel + c, v, my_count - c);
+                        return;
+                    }
+                    // by way of shared memory, so that whole lines go out: 16-byte unit u of row r of the tray lies at unit u ^ (r & 7)
+                    constexpr uint32_t TRAY = 128 / sizeof(O), UNITS = 32 * sizeof(O) / 16;   // columns of a tray, units of 32 columns
+                    const uint32_t at = c % TRAY / 32 * UNITS;
+                    if (at == 0) {
+                        if (lane == 0) tma_stores_read();
+                        __syncwarp();
+                    }
+#pragma unroll
+                    for (uint32_t u = 0; u < UNITS; ++u) {
+                        uint4 w;
+                        if constexpr (sizeof(O) == 2) {
+                            auto two = [&](uint64_t x) { return pair_from_float(low_of(x), high_of(x), static_cast<const O*>(nullptr)); };
+                            w = make_uint4(two(v[4 * u]), two(v[4 * u + 1]), two(v[4 * u + 2]), two(v[4 * u + 3]));
+                        } else {
+                            w = make_uint4(static_cast<uint32_t>(v[2 * u]), static_cast<uint32_t>(v[2 * u] >> 32), static_cast<uint32_t>(v[2 * u + 1]), static_cast<uint32_t>(v[2 * u + 1] >> 32));
+                        }
+                        *reinterpret_cast<uint4*>(tray + lane * 128 + (((at + u) ^ (lane & 7)) << 4)) = w;
+                    }
+                    if (at + UNITS == 8 || c + 32 >= my_count) {
+                        fence_proxy_async();
+                        __syncwarp();
+                        if (lane == 0) tma_store_2d(&maps.out, smem_u32(tray), static_cast<int>(my_channel + c / TRAY * TRAY), static_cast<int>(my_row));
+                    }
+                } else {
+                    store_across_rows(to + static_cast<size_t>(c) * p.m, p.m, my_channel, my_valid, lane, v, my_count - c, packed);
+                }
+            });
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster_read(cluster_address(&ctrl->acc_empty[b], 0));
+        }
+        if (LANES_ARE_ROWS && lane == 0) tma_stores_done();
+        // rows of no group
+        if (p.groups) {
+            const uint32_t all = __ldg(p.n_tiles + 1), threads = threadIdx.x - 128;
+            for (uint32_t t = row_tiles * p.channel_tiles + first; t < all * p.channel_tiles; t += step) {
+                uint32_t channel0;
+                const RowTile tile = tile_at(t, channel0);
+                const uint32_t width = min(CHANNELS, p.m - channel0), c = threads % CHANNELS;
+                if (c < width)
+                    for (uint32_t r = tile.row0 + rank * (256 / CHANNELS) + threads / CHANNELS; r < tile.row1; r += 2 * (256 / CHANNELS))
+                        store_result(out + static_cast<size_t>(r) * p.m + channel0 + c, 0.f);
+            }
+        }
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();   // nothing of the pair is in flight towards this CTA any more
+    if (warp == 1) tmem_dealloc_pair(tmem_base, TMEM_COLS);
+}
+
+// The tiles of `rows` rows that the groups consist of, one block; those of no group come last.  n_tiles: how many belong to a group, and
+// all.
 __global__ void __launch_bounds__(1024) row_tiles_kernel(const uint32_t* __restrict__ offsets, uint32_t groups, uint32_t n, uint32_t rows, uint32_t room, RowTile* __restrict__ tiles,
                                                          uint32_t* __restrict__ n_tiles) {
     __shared__ uint32_t sums[32];
@@ -309,11 +643,12 @@ __global__ void __launch_bounds__(1024) row_tiles_kernel(const uint32_t* __restr
             total += sums[w];
         }
         before += upto - count;
+        if (g == groups) n_tiles[0] = min(before, room);
         for (uint32_t i = 0; i < count && before + i < room; ++i) tiles[before + i] = {a + i * rows, min(a + (i + 1) * rows, b), g};
         base += total;
         __syncthreads();
     }
-    if (threadIdx.x == 0) *n_tiles = min(base, room);
+    if (threadIdx.x == 0) n_tiles[1] = min(base, room);
 }
 
 // Where a kernel records that a wait ran out: for the kernels in device memory, for the host in its own.
@@ -367,16 +702,25 @@ size_t pitch_of(size_t d) { return (d + 15) / 16 * 16; }
 size_t rounded(size_t bytes) { return (bytes + 255) / 256 * 256; }
 
 struct ProductPlan {
+    bool pairs, lanes_are_rows;
     uint32_t rows, split, row_tiles;   // row_tiles: with groups at most
 };
 ProductPlan make_plan(const Product& p) {
     const size_t channel_tiles = (p.m + P_CHANNELS - 1) / P_CHANNELS, depth_blocks = (p.d + P_DEPTH - 1) / P_DEPTH;
     const size_t typical = p.groups ? (p.n + p.groups - 1) / p.groups : p.n;
     ProductPlan plan{};
+    plan.split = 1;
+    plan.pairs = typical > 64 && (p.n + 127) / 128 * ((p.m + 255) / 256) >= 64;
+    if (plan.pairs) {
+        const bool wide = typical >= 192;
+        plan.lanes_are_rows = wide && p.m * type_bytes(p.out_type) % 32 == 0 && (address(p.out) & 31) == 0;
+        plan.rows = wide ? 256 : 128;
+        plan.row_tiles = static_cast<uint32_t>((p.n + plan.rows - 1) / plan.rows + (p.groups ? p.groups + 1 : 0));
+        return plan;
+    }
     plan.rows = typical <= 16 ? 16 : typical <= 32 ? 32 : typical <= 64 ? 64 : 128;
     if (plan.rows == 128 && (p.n + 127) / 128 * channel_tiles < 148) plan.rows = 64;
     plan.row_tiles = static_cast<uint32_t>((p.n + plan.rows - 1) / plan.rows + (p.groups ? p.groups + 1 : 0));
-    plan.split = 1;
     if (!p.groups && plan.rows <= 64)
         while (plan.split < 8 && plan.row_tiles * channel_tiles * plan.split * 2 <= 2 * 148 && depth_blocks >= 2 * plan.split) plan.split *= 2;
     return plan;
@@ -444,7 +788,8 @@ void launch_product(const Product& p, void* workspace, cudaStream_t stream) {
     k.n = static_cast<uint32_t>(p.n);
     k.m = static_cast<uint32_t>(p.m);
     k.depth_blocks = static_cast<uint32_t>((p.d + P_DEPTH - 1) / P_DEPTH);
-    k.channel_tiles = static_cast<uint32_t>((p.m + P_CHANNELS - 1) / P_CHANNELS);
+    const uint32_t channels = plan.pairs ? 256 : P_CHANNELS;
+    k.channel_tiles = static_cast<uint32_t>((p.m + channels - 1) / channels);
     k.groups = static_cast<uint32_t>(p.groups);
     k.error = status.device;
     k.told = status.host_on_device;
@@ -452,24 +797,44 @@ void launch_product(const Product& p, void* workspace, cudaStream_t stream) {
     k.producer_stop = producer_stop();
     if (p.groups) {
         RowTile* tiles = reinterpret_cast<RowTile*>(take(plan.row_tiles * sizeof(RowTile)));
-        uint32_t* n_tiles = reinterpret_cast<uint32_t*>(take(4));
+        uint32_t* n_tiles = reinterpret_cast<uint32_t*>(take(8));
         row_tiles_kernel<<<1, 1024, 0, stream>>>(p.offsets, k.groups, k.n, plan.rows, plan.row_tiles, tiles, n_tiles);
         SKM_LAUNCH_CHECK();
         k.tiles = tiles;
         k.n_tiles = n_tiles;
     }
-    ProductMaps maps;
+    ProductMaps maps{};
     maps.w = make_byte_tmap(w, p.d, w_rows, P_CHANNELS, ldw);
-    maps.x = make_byte_tmap(x, p.d, p.n, plan.rows, ldx);
+    maps.x = make_byte_tmap(x, p.d, p.n, plan.pairs ? plan.rows / 2 : plan.rows, ldx);
+    const size_t all_tiles = static_cast<size_t>(plan.row_tiles) * k.channel_tiles;
+    if (all_tiles * plan.split > 0x7fffffff) throw std::invalid_argument("a product of these sizes needs too many tiles");
+    auto launch_pairs = [&](auto columns, auto result) {
+        constexpr int COLS = decltype(columns)::value;
+        using O = decltype(result);
+        const unsigned grid = 2 * static_cast<unsigned>(std::min<size_t>(all_tiles, static_cast<size_t>(sm_pairs())));
+        auto go = [&](auto* kernel, uint32_t smem) {
+            SKM_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+            kernel<<<grid, Q_THREADS, smem, stream>>>(maps, k);
+        };
+        if constexpr (COLS == 256) {
+            if (plan.lanes_are_rows) {
+                maps.out = make_result_tmap(p.out, sizeof(O), p.m, p.n, 32);
+                go(product_pair_kernel<COLS, O, true>, kPairSmem<COLS, true>);
+            } else {
+                go(product_pair_kernel<COLS, O, false>, kPairSmem<COLS, false>);
+            }
+        } else {
+            go(product_pair_kernel<COLS, O, false>, kPairSmem<COLS, false>);
+        }
+        SKM_LAUNCH_CHECK();
+    };
     auto launch = [&](auto rows, auto result) {
         constexpr int ROWS = decltype(rows)::value;
         using O = decltype(result);
         auto* kernel = product_kernel<ROWS, O>;
         SKM_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kProductSmem<ROWS>)));
         cudaLaunchConfig_t config{};
-        const size_t blocks = static_cast<size_t>(plan.row_tiles) * k.channel_tiles * plan.split;
-        if (blocks > 0x7fffffff) throw std::invalid_argument("a product of these sizes needs too many tiles");
-        config.gridDim = dim3(static_cast<unsigned>(blocks));
+        config.gridDim = dim3(static_cast<unsigned>(all_tiles * plan.split));
         config.blockDim = dim3(P_THREADS);
         config.dynamicSmemBytes = kProductSmem<ROWS>;
         config.stream = stream;
@@ -481,15 +846,17 @@ void launch_product(const Product& p, void* workspace, cudaStream_t stream) {
         SKM_CUDA(cudaLaunchKernelEx(&config, kernel, maps, k));
         SKM_LAUNCH_CHECK();
     };
-    auto of_type = [&](auto rows) {
-        if (p.out_type == Type::f32) launch(rows, float{});
-        else if (p.out_type == Type::f16) launch(rows, __half{});
-        else launch(rows, __nv_bfloat16{});
+    auto of_type = [&](auto&& go, auto rows) {
+        if (p.out_type == Type::f32) go(rows, float{});
+        else if (p.out_type == Type::f16) go(rows, __half{});
+        else go(rows, __nv_bfloat16{});
     };
-    if (plan.rows == 16) of_type(std::integral_constant<int, 16>{});
-    else if (plan.rows == 32) of_type(std::integral_constant<int, 32>{});
-    else if (plan.rows == 64) of_type(std::integral_constant<int, 64>{});
-    else of_type(std::integral_constant<int, 128>{});
+    if (plan.pairs && plan.rows == 256) of_type(launch_pairs, std::integral_constant<int, 256>{});
+    else if (plan.pairs) of_type(launch_pairs, std::integral_constant<int, 128>{});
+    else if (plan.rows == 16) of_type(launch, std::integral_constant<int, 16>{});
+    else if (plan.rows == 32) of_type(launch, std::integral_constant<int, 32>{});
+    else if (plan.rows == 64) of_type(launch, std::integral_constant<int, 64>{});
+    else of_type(launch, std::integral_constant<int, 128>{});
 }
 
 void check_products(cudaStream_t stream) {

@@ -116,6 +116,15 @@ __device__ __forceinline__ void tma_load_2d(uint32_t smem_dst, const CUtensorMap
                  : "memory");
 }
 
+// Shared memory -> global, what lies outside the matrix left out; the calling thread's stores are a group, and these wait until all its
+// groups have read their shared memory, or are complete.
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* tmap, uint32_t smem_src, int x, int y) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(reinterpret_cast<uint64_t>(tmap)), "r"(smem_src), "r"(x), "r"(y) : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+__device__ __forceinline__ void tma_stores_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void tma_stores_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+
 // Asynchronous 16-byte copy global -> shared (both 16-byte aligned), its group bookkeeping, and the wait for all but the
 // N newest groups of the calling thread.
 __device__ __forceinline__ void cp_async_16(uint32_t smem_dst, const void* gmem_src) {
@@ -236,6 +245,14 @@ __device__ __forceinline__ void umma_i8(uint32_t tmem_d, uint64_t adesc, uint64_
         "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
         : "memory");
 }
+__device__ __forceinline__ void umma_i8_pair(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t accumulate, uint32_t idesc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
 // arrives at the barrier at this place in both CTAs
 __device__ __forceinline__ void umma_commit_pair(uint64_t* bar) {
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)), "h"(static_cast<uint16_t>(3)) : "memory");
@@ -336,6 +353,8 @@ CUtensorMap make_half_tmap(const void* base, size_t cols, size_t rows, uint32_t 
 // Row-major bytes [rows][pitch] (pitch a multiple of 16) of which the first cols columns are visible; boxes of 128 columns x box_rows
 // rows, 128-byte swizzle.
 CUtensorMap make_byte_tmap(const void* base, size_t cols, size_t rows, uint32_t box_rows, size_t pitch);
+// Row-major results [rows][cols] of 2 or 4 bytes, for stores in boxes of 128 bytes x box_rows rows, 128-byte swizzle.
+CUtensorMap make_result_tmap(void* base, size_t element, size_t cols, size_t rows, uint32_t box_rows);
 
 } // namespace tc
 } // namespace skmb

@@ -392,7 +392,7 @@ def check_product(got, x, xs, w, ws, dtype):
 
 
 PRODUCTS = [(1, 1, 1), (1, 16_384, 768), (3, 5, 17), (16, 128, 128), (17, 129, 129), (33, 1000, 50), (64, 300, 4096), (128, 128, 256), (777, 1001, 130), (1000, 64, 16), (300, 4097, 640),
-            (5, 100, 40_000)]
+            (5, 100, 40_000), (300, 6000, 256), (4100, 1030, 200), (2000, 1001, 768), (70, 20_001, 33), (8197, 517, 130)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -429,7 +429,7 @@ def test_product_of_scales_that_are_zero_or_no_number(ops):
     assert not got[4, keep].any() and torch.isfinite(got[5:, keep]).all()
 
 
-GROUPED = [(1, 1, 5, 16), (40, 3, 200, 100), (1000, 300, 64, 32), (3000, 7, 768, 768), (5000, 2, 130, 257), (20_000, 64, 100, 129)]
+GROUPED = [(1, 1, 5, 16), (40, 3, 200, 100), (1000, 300, 64, 32), (3000, 7, 768, 768), (5000, 2, 130, 257), (20_000, 64, 100, 129), (30_000, 9, 301, 200), (9000, 40, 520, 96)]
 
 
 @pytest.mark.parametrize("n,e,m,d", GROUPED)
