@@ -17,6 +17,13 @@ namespace rows {
 // What one load or store moves.
 template <int BYTES>
 struct ChunkOf;
+struct alignas(32) Words8 {
+    uint32_t w[8];
+};
+template <>
+struct ChunkOf<32> {
+    using type = Words8;
+};
 template <>
 struct ChunkOf<16> {
     using type = uint4;
@@ -41,6 +48,30 @@ __device__ __forceinline__ Chunk<BYTES> zero_chunk() {
     Chunk<BYTES> c;
     memset(&c, 0, BYTES);
     return c;
+}
+
+// Global memory that nobody writes meanwhile, and stores.
+template <int BYTES>
+__device__ __forceinline__ Chunk<BYTES> load_chunk(const Chunk<BYTES>* p) {
+    if constexpr (BYTES == 32) {
+        Words8 c;
+        asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                     : "=r"(c.w[0]), "=r"(c.w[1]), "=r"(c.w[2]), "=r"(c.w[3]), "=r"(c.w[4]), "=r"(c.w[5]), "=r"(c.w[6]), "=r"(c.w[7])
+                     : "l"(p));
+        return c;
+    } else {
+        return __ldg(p);
+    }
+}
+template <int BYTES>
+__device__ __forceinline__ void store_chunk(Chunk<BYTES>* p, const Chunk<BYTES>& c) {
+    if constexpr (BYTES == 32) {
+        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(c.w[0]), "r"(c.w[1]), "r"(c.w[2]), "r"(c.w[3]), "r"(c.w[4]), "r"(c.w[5]), "r"(c.w[6]),
+                     "r"(c.w[7])
+                     : "memory");
+    } else {
+        *p = c;
+    }
 }
 
 __device__ __forceinline__ float2 pair_to_float(uint32_t u, const __half*) { return __half22float2(*reinterpret_cast<const __half2*>(&u)); }
@@ -112,23 +143,24 @@ inline Divisor make_divisor(size_t d, size_t most) {
 }
 __device__ __forceinline__ uint32_t divide(uint32_t a, const Divisor& by) { return by.magic ? __umulhi(a, by.magic) : a / by.d; }
 
-// How many bytes a load of each of these may move at once: all of them are multiples of it.
-inline int access_bytes(std::initializer_list<size_t> multiples) {
-    size_t all = 16;
+// How many bytes a load of each of these may move at once, up to `most`: all of them are multiples of it.
+inline int access_bytes(std::initializer_list<size_t> multiples, size_t most = 16) {
+    size_t all = most;
     for (const size_t m : multiples) all |= m;
     return static_cast<int>(all & (~all + 1));
 }
 inline size_t address(const void* p) { return reinterpret_cast<uintptr_t>(p); }
 
-// f(T{}, integral_constant<BYTES>) for a type and a width of access
+// f(T{}, Width<BYTES>{}) for a type and a width of access up to MOST
 template <int BYTES>
 struct Width {
     static constexpr int bytes = BYTES;
 };
-template <class F>
+template <int MOST = 16, class F>
 void with_width(Type type, int bytes, F&& f) {
     auto of = [&](auto t) {
-        if (bytes >= 16) f(t, Width<16>{});
+        if (MOST >= 32 && bytes >= 32) f(t, Width<MOST>{});
+        else if (bytes >= 16) f(t, Width<16>{});
         else if (bytes == 8) f(t, Width<8>{});
         else if (bytes == 4) f(t, Width<4>{});
         else if constexpr (sizeof(t) == 2) f(t, Width<2>{});

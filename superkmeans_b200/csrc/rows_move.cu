@@ -1,9 +1,9 @@
 // Rows by index: lookup in a table, rows to the places of their clusters and back, and the gradients of the weights and scales.
 //
 // All of them move rows once and compute next to nothing: they are bound by HBM, or for small calls by the launch.  The rows of an
-// output (or for to_clusters of the input) are taken as one sequence of 16-byte chunks, 256 x 4 of them to a block whatever the rows'
-// width, so that narrow and odd rows fill the lanes as well as wide ones; a row whose address, pitch or width is no multiple of 16
-// bytes is taken in chunks of 8, 4 or 2.  Products and sums are in fp32 and rounded once.
+// output (or for to_clusters of the input) are taken as one sequence of 32-byte chunks, 256 x 2 of them to a block whatever the rows'
+// width, so that narrow and odd rows fill the lanes as well as wide ones; a row whose address, pitch or width is no multiple of 32
+// bytes is taken in chunks of 16, 8, 4 or 2, 256 x 4 to a block.  Products and sums are in fp32 and rounded once.
 #include "rows_access.cuh"
 
 #include "device_utils.cuh"
@@ -14,7 +14,10 @@ namespace rows {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kAhead = 4;   // chunks of a thread, all loaded before the first is stored
+
+// Chunks of a thread, all loaded before the first is stored: 64 bytes, which with the 40 warps of an SM keep 80 KB on their way.
+template <int BYTES>
+constexpr int kAhead = BYTES == 32 ? 2 : 4;
 
 // The chunks of n rows, `width` to a row.
 struct Spread {
@@ -22,13 +25,21 @@ struct Spread {
     Divisor width;
 };
 
-Spread make_spread(size_t n, size_t row_bytes, int bytes) {
-    const size_t width = row_bytes / bytes;
-    return {n * width, make_divisor(width, width + kThreads * kAhead)};
+template <int BYTES>
+constexpr size_t kBlockChunks = kThreads * kAhead<BYTES>;
+
+template <int BYTES>
+Spread make_spread(size_t n, size_t row_bytes) {
+    const size_t width = row_bytes / BYTES;
+    return {n * width, make_divisor(width, width + kBlockChunks<BYTES>)};
 }
-unsigned spread_blocks(const Spread& s) { return static_cast<unsigned>((s.total + kThreads * kAhead - 1) / (kThreads * kAhead)); }
+template <int BYTES>
+unsigned spread_blocks(const Spread& s) {
+    return static_cast<unsigned>((s.total + kBlockChunks<BYTES> - 1) / kBlockChunks<BYTES>);
+}
 
 // This thread's chunks: row and place in the row of chunk u, and whether there is one.
+template <int BYTES>
 struct Mine {
     size_t row0;
     uint32_t off;
@@ -36,7 +47,7 @@ struct Mine {
     Divisor width;
 
     __device__ __forceinline__ explicit Mine(const Spread& s) : width(s.width) {
-        const size_t first = static_cast<size_t>(blockIdx.x) * (kThreads * kAhead);
+        const size_t first = static_cast<size_t>(blockIdx.x) * kBlockChunks<BYTES>;
         row0 = (first >> 32) == 0 ? static_cast<uint32_t>(first) / s.width.d : first / s.width.d;
         off = static_cast<uint32_t>(first - row0 * s.width.d) + threadIdx.x;
         left = first + threadIdx.x < s.total ? s.total - first - threadIdx.x : 0;
@@ -57,13 +68,14 @@ __device__ __forceinline__ const C* row_at(const void* p, size_t pitch, size_t r
 template <typename T, int BYTES, bool SCALED>
 __global__ void __launch_bounds__(kThreads) lookup_kernel(const void* __restrict__ table, size_t pitch, uint32_t k, const void* __restrict__ ids, bool wide, float scale,
                                                           const float* __restrict__ row_scales, Chunk<BYTES>* __restrict__ out, const Spread spread) {
-    const Mine mine(spread);
-    size_t row[kAhead];
-    uint32_t col[kAhead], id[kAhead];
-    Chunk<BYTES> c[kAhead];
-    float f[kAhead];
+    constexpr int AHEAD = kAhead<BYTES>;
+    const Mine<BYTES> mine(spread);
+    size_t row[AHEAD];
+    uint32_t col[AHEAD], id[AHEAD];
+    Chunk<BYTES> c[AHEAD];
+    float f[AHEAD];
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
+    for (int u = 0; u < AHEAD; ++u) {
         id[u] = k;
         if (mine.has(u)) {
             mine.at(u, row[u], col[u]);
@@ -72,9 +84,9 @@ __global__ void __launch_bounds__(kThreads) lookup_kernel(const void* __restrict
         }
     }
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) c[u] = id[u] < k ? __ldg(row_at<Chunk<BYTES>>(table, pitch, id[u]) + col[u]) : zero_chunk<BYTES>();
+    for (int u = 0; u < AHEAD; ++u) c[u] = id[u] < k ? load_chunk<BYTES>(row_at<Chunk<BYTES>>(table, pitch, id[u]) + col[u]) : zero_chunk<BYTES>();
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
+    for (int u = 0; u < AHEAD; ++u) {
         if (!mine.has(u)) continue;
         if (SCALED && id[u] < k) {
             Values<T, BYTES> v;
@@ -83,78 +95,84 @@ __global__ void __launch_bounds__(kThreads) lookup_kernel(const void* __restrict
             for (int i = 0; i < v.N; ++i) v.v[i] *= f[u];
             c[u] = v.to();
         }
-        out[row[u] * spread.width.d + col[u]] = c[u];
+        store_chunk<BYTES>(out + row[u] * spread.width.d + col[u], c[u]);
     }
 }
 
 template <int BYTES>
 __global__ void __launch_bounds__(kThreads) to_clusters_kernel(const void* __restrict__ x, size_t pitch, const Places at, Chunk<BYTES>* __restrict__ out, const Spread spread) {
-    const Mine mine(spread);
+    constexpr int AHEAD = kAhead<BYTES>;
+    const Mine<BYTES> mine(spread);
     const uint32_t slots = static_cast<uint32_t>(at.n * at.m), held = min(__ldg(at.held), slots);
-    Chunk<BYTES> c[kAhead];
+    Chunk<BYTES> c[AHEAD];
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u)
+    for (int u = 0; u < AHEAD; ++u)
         if (mine.has(u)) {
             size_t row;
             uint32_t col;
             mine.at(u, row, col);
-            c[u] = __ldg(row_at<Chunk<BYTES>>(x, pitch, row) + col);
+            c[u] = load_chunk<BYTES>(row_at<Chunk<BYTES>>(x, pitch, row) + col);
         }
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u)
+    for (int u = 0; u < AHEAD; ++u)
         if (mine.has(u)) {
             size_t row;
             uint32_t col;
             mine.at(u, row, col);
             for (size_t j = 0; j < at.m; ++j) {
                 const uint32_t slot = __ldg(at.position + row * at.m + j);
-                if (slot < slots) out[static_cast<size_t>(slot) * spread.width.d + col] = slot < held ? c[u] : zero_chunk<BYTES>();
+                if (slot < slots) store_chunk<BYTES>(out + static_cast<size_t>(slot) * spread.width.d + col, slot < held ? c[u] : zero_chunk<BYTES>());
             }
         }
 }
 
+// Two choices of each chunk are on their way at a time.
 template <typename T, int BYTES>
 __global__ void __launch_bounds__(kThreads) from_clusters_kernel(const void* __restrict__ y, size_t pitch, const Places at, const float* __restrict__ weights,
                                                                  Chunk<BYTES>* __restrict__ out, const Spread spread) {
-    const Mine mine(spread);
+    constexpr int AHEAD = kAhead<BYTES>;
+    const Mine<BYTES> mine(spread);
     const uint32_t slots = static_cast<uint32_t>(at.n * at.m), held = min(__ldg(at.held), slots);
-    size_t row[kAhead];
-    uint32_t col[kAhead];
-    Values<T, BYTES> sum[kAhead];
+    size_t row[AHEAD];
+    uint32_t col[AHEAD];
+    Values<T, BYTES> sum[AHEAD];
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
+    for (int u = 0; u < AHEAD; ++u) {
         if (mine.has(u)) mine.at(u, row[u], col[u]);
 #pragma unroll
         for (int i = 0; i < sum[u].N; ++i) sum[u].v[i] = 0.f;
     }
-    for (size_t j = 0; j < at.m; ++j) {
-        Chunk<BYTES> c[kAhead];
-        float w[kAhead];
-        bool there[kAhead];
+    for (size_t j = 0; j < at.m; j += 2) {
+        Chunk<BYTES> c[AHEAD][2];
+        float w[AHEAD][2];
+        uint32_t slot[AHEAD][2];
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u) {
-            there[u] = false;
-            if (mine.has(u)) {
-                const uint32_t slot = __ldg(at.position + row[u] * at.m + j);
-                there[u] = slot < held;
-                if (there[u]) {
-                    c[u] = __ldg(row_at<Chunk<BYTES>>(y, pitch, slot) + col[u]);
-                    w[u] = weights ? __ldg(weights + row[u] * at.m + j) : 1.f;
+        for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const bool there = mine.has(u) && j + e < at.m;
+                slot[u][e] = there ? __ldg(at.position + row[u] * at.m + j + e) : 0xffffffffu;
+                w[u][e] = there && weights ? __ldg(weights + row[u] * at.m + j + e) : 1.f;
+            }
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+                if (slot[u][e] < held) c[u][e] = load_chunk<BYTES>(row_at<Chunk<BYTES>>(y, pitch, slot[u][e]) + col[u]);
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+                if (slot[u][e] < held) {
+                    Values<T, BYTES> v;
+                    v.from(c[u][e]);
+#pragma unroll
+                    for (int i = 0; i < v.N; ++i) sum[u].v[i] = fmaf(w[u][e], v.v[i], sum[u].v[i]);
                 }
-            }
-        }
-#pragma unroll
-        for (int u = 0; u < kAhead; ++u)
-            if (there[u]) {
-                Values<T, BYTES> v;
-                v.from(c[u]);
-#pragma unroll
-                for (int i = 0; i < v.N; ++i) sum[u].v[i] = fmaf(w[u], v.v[i], sum[u].v[i]);
-            }
     }
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u)
-        if (mine.has(u)) out[row[u] * spread.width.d + col[u]] = sum[u].to();
+    for (int u = 0; u < AHEAD; ++u)
+        if (mine.has(u)) store_chunk<BYTES>(out + row[u] * spread.width.d + col[u], sum[u].to());
 }
 
 // A warp per row of grad: <grad[i], y[slot]> and grad_y[slot] = w * grad[i] for its choices, y read once.
@@ -176,22 +194,22 @@ __global__ void __launch_bounds__(kThreads) from_clusters_grad_kernel(const void
         float dot = 0.f;
         if (!there) {
             if (grad_y && slot < slots)
-                for (uint32_t c = lane; c < width; c += 32) to[c] = zero_chunk<BYTES>();
+                for (uint32_t c = lane; c < width; c += 32) store_chunk<BYTES>(to + c, zero_chunk<BYTES>());
         } else {
 #pragma unroll 4
             for (uint32_t c = lane; c < width; c += 32) {
                 Values<T, BYTES> a;
-                a.from(__ldg(g + c));
+                a.from(load_chunk<BYTES>(g + c));
                 if (grad_weights) {
                     Values<T, BYTES> b;
-                    b.from(__ldg(from + c));
+                    b.from(load_chunk<BYTES>(from + c));
 #pragma unroll
                     for (int i = 0; i < a.N; ++i) dot = fmaf(a.v[i], b.v[i], dot);
                 }
                 if (grad_y) {
 #pragma unroll
                     for (int i = 0; i < a.N; ++i) a.v[i] *= w;
-                    to[c] = a.to();
+                    store_chunk<BYTES>(to + c, a.to());
                 }
             }
         }
@@ -216,8 +234,8 @@ __global__ void __launch_bounds__(kThreads) lookup_scale_grad_kernel(const void*
 #pragma unroll 4
         for (uint32_t c = lane; c < width; c += 32) {
             Values<T, BYTES> a, b;
-            a.from(__ldg(g + c));
-            b.from(__ldg(t + c));
+            a.from(load_chunk<BYTES>(g + c));
+            b.from(load_chunk<BYTES>(t + c));
 #pragma unroll
             for (int i = 0; i < a.N; ++i) dot = fmaf(a.v[i], b.v[i], dot);
         }
@@ -233,13 +251,13 @@ unsigned warp_blocks(size_t n) { return static_cast<unsigned>((n + kThreads / 32
 void launch_lookup(const Rows& table, Type type, size_t k, size_t d, const Ids& ids, size_t n, float scale, const float* row_scales, void* out, cudaStream_t stream) {
     if (n == 0) return;
     const size_t t = type_bytes(type), pitch = table.ld * t;
-    with_width(type, access_bytes({address(table.p), pitch, d * t, address(out)}), [&](auto value, auto width) {
+    with_width<32>(type, access_bytes({address(table.p), pitch, d * t, address(out)}, 32), [&](auto value, auto width) {
         using T = decltype(value);
         constexpr int B = decltype(width)::bytes;
-        const Spread s = make_spread(n, d * t, B);
+        const Spread s = make_spread<B>(n, d * t);
         // (a product with one changes no value: the plain copy is for that)
         auto* kernel = row_scales || scale != 1.0f ? lookup_kernel<T, B, true> : lookup_kernel<T, B, false>;
-        kernel<<<spread_blocks(s), kThreads, 0, stream>>>(table.p, pitch, static_cast<uint32_t>(k), ids.p, ids.wide, scale, row_scales, static_cast<Chunk<B>*>(out), s);
+        kernel<<<spread_blocks<B>(s), kThreads, 0, stream>>>(table.p, pitch, static_cast<uint32_t>(k), ids.p, ids.wide, scale, row_scales, static_cast<Chunk<B>*>(out), s);
     });
     SKM_LAUNCH_CHECK();
 }
@@ -258,10 +276,10 @@ void launch_lookup_scale_grad(const Rows& grad, const Rows& table, Type type, si
 void launch_to_clusters(const Rows& x, Type type, size_t d, const Places& at, void* out, cudaStream_t stream) {
     if (at.n == 0) return;
     const size_t t = type_bytes(type), pitch = x.ld * t;
-    with_width(type, access_bytes({address(x.p), pitch, d * t, address(out)}), [&](auto, auto width) {
+    with_width<32>(type, access_bytes({address(x.p), pitch, d * t, address(out)}, 32), [&](auto, auto width) {
         constexpr int B = decltype(width)::bytes;
-        const Spread s = make_spread(at.n, d * t, B);
-        to_clusters_kernel<B><<<spread_blocks(s), kThreads, 0, stream>>>(x.p, pitch, at, static_cast<Chunk<B>*>(out), s);
+        const Spread s = make_spread<B>(at.n, d * t);
+        to_clusters_kernel<B><<<spread_blocks<B>(s), kThreads, 0, stream>>>(x.p, pitch, at, static_cast<Chunk<B>*>(out), s);
     });
     SKM_LAUNCH_CHECK();
 }
@@ -269,10 +287,10 @@ void launch_to_clusters(const Rows& x, Type type, size_t d, const Places& at, vo
 void launch_from_clusters(const Rows& y, Type type, size_t d, const Places& at, const float* weights, void* out, cudaStream_t stream) {
     if (at.n == 0) return;
     const size_t t = type_bytes(type), pitch = y.ld * t;
-    with_width(type, access_bytes({address(y.p), pitch, d * t, address(out)}), [&](auto value, auto width) {
+    with_width<32>(type, access_bytes({address(y.p), pitch, d * t, address(out)}, 32), [&](auto value, auto width) {
         constexpr int B = decltype(width)::bytes;
-        const Spread s = make_spread(at.n, d * t, B);
-        from_clusters_kernel<decltype(value), B><<<spread_blocks(s), kThreads, 0, stream>>>(y.p, pitch, at, weights, static_cast<Chunk<B>*>(out), s);
+        const Spread s = make_spread<B>(at.n, d * t);
+        from_clusters_kernel<decltype(value), B><<<spread_blocks<B>(s), kThreads, 0, stream>>>(y.p, pitch, at, weights, static_cast<Chunk<B>*>(out), s);
     });
     SKM_LAUNCH_CHECK();
 }

@@ -68,9 +68,11 @@ def _rows(t, name: str, like=None, dtype=None) -> Tuple[torch.Tensor, int]:
     n, d = t.shape
     if d == 0:
         raise ValueError(f"{name} must have at least one column")
-    if d > 1 and t.stride(1) != 1:
+    ld, step = t.stride()
+    if step != 1 and d > 1:
         t = t.contiguous()
-    return t, t.stride(0) if n > 1 else d
+        ld = d
+    return t, ld if n > 1 else d
 
 
 def _ids(ids, name: str, like=None) -> Tuple[torch.Tensor, int]:
@@ -116,16 +118,33 @@ def _clusters(n_clusters: int) -> int:
     return n_clusters
 
 
+# A call on a few rows takes as long as the host takes to make it: the handle of a stream without the Stream around it (4 us less where
+# a call took 24), outputs from `new_empty`, no workspace where none is needed.
+try:
+    from torch._C import _cuda_getCurrentRawStream as _raw_stream
+except ImportError:   # (a torch without CUDA, or another torch)
+
+    def _raw_stream(index: int) -> int:
+        return torch.cuda.current_stream(index).cuda_stream
+
+
 def _p(t: Optional[torch.Tensor]):
     return None if t is None else t.data_ptr()
 
 
-def _stream(t: torch.Tensor) -> int:
-    return torch.cuda.current_stream(t.device).cuda_stream
+def _workspace(n_bytes: int, like: torch.Tensor) -> Tuple[Optional[torch.Tensor], Optional[int], int]:
+    """The workspace, its address and its size."""
+    if n_bytes == 0:
+        return None, None, 0
+    space = like.new_empty(n_bytes, dtype=torch.uint8)
+    return space, space.data_ptr(), n_bytes
 
 
-def _workspace(n_bytes: int, like: torch.Tensor) -> torch.Tensor:
-    return torch.empty(n_bytes, dtype=torch.uint8, device=like.device)
+def _wants_grad(*tensors) -> bool:
+    for t in tensors:
+        if isinstance(t, torch.Tensor) and t.requires_grad:
+            return torch.is_grad_enabled()
+    return False
 
 
 # ---- lookup ---------------------------------------------------------------------------------------------------------------------
@@ -138,8 +157,11 @@ def _lookup(table, ids, scale, row_scales):
     _clusters(k)
     if row_scales is not None:
         row_scales = _floats(row_scales, "row_scales", ids.shape, table)
-    out = torch.empty(*ids.shape, d, dtype=table.dtype, device=table.device)
-    check(lib.skm_op_lookup(table.device.index, _p(rows), ld, _DTYPES[table.dtype], k, d, _p(at), bits, at.numel(), scale, _p(row_scales), _p(out), _stream(table)))
+    out = rows.new_empty((*at.shape, d))
+    index = rows.device.index
+    status = lib.skm_op_lookup(index, rows.data_ptr(), ld, _DTYPES[rows.dtype], k, d, at.data_ptr(), bits, at.numel(), scale, _p(row_scales), out.data_ptr(), _raw_stream(index))
+    if status:
+        check(status)
     return out
 
 
@@ -170,7 +192,7 @@ def lookup(table: torch.Tensor, ids: torch.Tensor, scale: float = 1.0, row_scale
     a table of k x d values in fp32, fp16 or bf16.  `row_scales`, if given, has the shape of `ids` and dtype float32.  An id that is no
     row of the table (-1 as padding) gives zeros and no gradient.  Differentiable in `table` (see lookup_grad) and `row_scales`."""
     scale = float(scale)
-    if torch.is_grad_enabled() and (getattr(table, "requires_grad", False) or getattr(row_scales, "requires_grad", False)):
+    if _wants_grad(table, row_scales):
         return _Lookup.apply(table, ids, scale, row_scales)
     return _lookup(table, ids, scale, row_scales)
 
@@ -191,10 +213,11 @@ def lookup_grad(grad: torch.Tensor, ids: torch.Tensor, n_rows: int, scale: float
     if row_scales is not None:
         row_scales = _floats(row_scales, "row_scales", ids.shape, grad)
     kind = _DTYPES[grad.dtype]
-    out = torch.empty(k, d, dtype=dtype, device=grad.device)
-    space = _workspace(lib.skm_op_lookup_grad_workspace(n, k, d, kind), grad)
-    check(lib.skm_op_lookup_grad(grad.device.index, _p(rows), ld, kind, k, d, _p(at), bits, n, float(scale), _p(row_scales), _p(out), _DTYPES[dtype], _p(space), space.numel(),
-                                 _stream(grad)))
+    out = rows.new_empty((k, d), dtype=dtype)
+    space, address, size = _workspace(lib.skm_op_lookup_grad_workspace(n, k, d, kind), rows)
+    index = rows.device.index
+    check(lib.skm_op_lookup_grad(index, rows.data_ptr(), ld, kind, k, d, at.data_ptr(), bits, n, float(scale), _p(row_scales), out.data_ptr(), _DTYPES[dtype], address, size,
+                                 _raw_stream(index)))
     return out
 
 
@@ -209,8 +232,10 @@ def lookup_scale_grad(grad: torch.Tensor, table: torch.Tensor, ids: torch.Tensor
     if at.numel() != n or at.dim() != 1:
         raise ValueError(f"ids must have shape ({n},), got {tuple(at.shape)}")
     k = _clusters(t.shape[0])
-    out = torch.empty(n, dtype=torch.float32, device=grad.device)
-    check(lib.skm_op_lookup_scale_grad(grad.device.index, _p(rows), ld, _p(t), ld_t, _DTYPES[grad.dtype], k, d, _p(at), bits, n, float(scale), _p(out), _stream(grad)))
+    out = rows.new_empty(n, dtype=torch.float32)
+    index = rows.device.index
+    check(lib.skm_op_lookup_scale_grad(index, rows.data_ptr(), ld, t.data_ptr(), ld_t, _DTYPES[rows.dtype], k, d, at.data_ptr(), bits, n, float(scale), out.data_ptr(),
+                                       _raw_stream(index)))
     return out
 
 
@@ -224,12 +249,13 @@ def group_rows(ids: torch.Tensor, n_clusters: int) -> RowGroups:
     if at.dim() not in (1, 2) or (at.dim() == 2 and at.shape[1] == 0):
         raise ValueError(f"ids must have shape (n,) or (n, m) with m > 0, got {tuple(at.shape)}")
     k, n = _clusters(n_clusters), at.numel()
-    order = torch.empty(n, dtype=torch.int32, device=ids.device)
-    position = torch.empty(at.shape, dtype=torch.int32, device=ids.device)
-    offsets = torch.empty(k + 1, dtype=torch.int32, device=ids.device)
-    space = _workspace(lib.skm_op_group_rows_workspace(n, k), ids)
-    check(lib.skm_op_group_rows(ids.device.index, _p(at), bits, n, k, _p(order), _p(position), _p(offsets), _p(space), space.numel(), _stream(ids)))
-    return RowGroups(order, position, offsets)
+    whole = at.new_empty(2 * n + k + 1, dtype=torch.int32)
+    order, position, offsets = whole.split((n, n, k + 1))
+    space, address, size = _workspace(lib.skm_op_group_rows_workspace(n, k), at)
+    index = at.device.index
+    first = whole.data_ptr()
+    check(lib.skm_op_group_rows(index, at.data_ptr(), bits, n, k, first, first + 4 * n, first + 8 * n, address, size, _raw_stream(index)))
+    return RowGroups(order, position if at.dim() == 1 else position.view(at.shape), offsets)
 
 
 def _to_clusters(x, groups):
@@ -238,8 +264,9 @@ def _to_clusters(x, groups):
     if rows.shape[0] != n:
         raise ValueError(f"x must have {n} rows, got {rows.shape[0]}")
     d = rows.shape[1]
-    out = torch.empty(n * m, d, dtype=x.dtype, device=x.device)
-    check(lib.skm_op_to_clusters(x.device.index, _p(rows), ld, _DTYPES[x.dtype], d, _p(position), _p(offsets), k, n, m, _p(out), _stream(x)))
+    out = rows.new_empty((n * m, d))
+    index = rows.device.index
+    check(lib.skm_op_to_clusters(index, rows.data_ptr(), ld, _DTYPES[rows.dtype], d, position.data_ptr(), offsets.data_ptr(), k, n, m, out.data_ptr(), _raw_stream(index)))
     return out
 
 
@@ -251,8 +278,9 @@ def _from_clusters(y, groups, weights, name="y"):
     if weights is not None:
         weights = _floats(weights, "weights", position.shape, y)
     d = rows.shape[1]
-    out = torch.empty(n, d, dtype=y.dtype, device=y.device)
-    check(lib.skm_op_from_clusters(y.device.index, _p(rows), ld, _DTYPES[y.dtype], d, _p(position), _p(offsets), k, n, m, _p(weights), _p(out), _stream(y)))
+    out = rows.new_empty((n, d))
+    index = rows.device.index
+    check(lib.skm_op_from_clusters(index, rows.data_ptr(), ld, _DTYPES[rows.dtype], d, position.data_ptr(), offsets.data_ptr(), k, n, m, _p(weights), out.data_ptr(), _raw_stream(index)))
     return out
 
 
@@ -269,10 +297,11 @@ def _from_clusters_grad(grad, y, groups, weights, want_y, want_weights):
         from_y, ld_y = _rows(y, "y", grad, grad.dtype)
         if tuple(from_y.shape) != (n * m, d):
             raise ValueError(f"y must have shape {(n * m, d)}, got {tuple(from_y.shape)}")
-    grad_y = torch.empty(n * m, d, dtype=grad.dtype, device=grad.device) if want_y else None
-    grad_weights = torch.empty(position.shape, dtype=torch.float32, device=grad.device) if want_weights else None
-    check(lib.skm_op_from_clusters_grad(grad.device.index, _p(rows), ld, _p(from_y), ld_y, _DTYPES[grad.dtype], d, _p(position), _p(offsets), k, n, m, _p(weights), _p(grad_y),
-                                        _p(grad_weights), _stream(grad)))
+    grad_y = rows.new_empty((n * m, d)) if want_y else None
+    grad_weights = rows.new_empty(position.shape, dtype=torch.float32) if want_weights else None
+    index = rows.device.index
+    check(lib.skm_op_from_clusters_grad(index, rows.data_ptr(), ld, _p(from_y), ld_y, _DTYPES[rows.dtype], d, position.data_ptr(), offsets.data_ptr(), k, n, m, _p(weights), _p(grad_y),
+                                        _p(grad_weights), _raw_stream(index)))
     return grad_y, grad_weights
 
 
@@ -307,7 +336,7 @@ def to_clusters(x: torch.Tensor, groups: RowGroups) -> torch.Tensor:
     """Rows in the order of their clusters: n x d to (n * m) x d, row i once for each of its m choices, at groups.position[i, j].  The rows of
     cluster c are offsets[c] .. offsets[c + 1] - 1; behind the last cluster the slots of choices without one hold zeros.
     Differentiable in x (see to_clusters_grad)."""
-    if torch.is_grad_enabled() and getattr(x, "requires_grad", False):
+    if _wants_grad(x):
         return _ToClusters.apply(x, *groups)
     return _to_clusters(x, groups)
 
@@ -322,7 +351,7 @@ def from_clusters(y: torch.Tensor, groups: RowGroups, weights: Optional[torch.Te
     """Rows back from the order of their clusters: out[i] = sum over j of weights[i, j] * y[position[i, j]], n x d.  Choices without a cluster
     contribute nothing, whatever their slots hold.  `weights` (float32, the shape of groups.position) is 1 if not given.
     Differentiable in y and weights (see from_clusters_grad)."""
-    if torch.is_grad_enabled() and (getattr(y, "requires_grad", False) or getattr(weights, "requires_grad", False)):
+    if _wants_grad(y, weights):
         return _FromClusters.apply(y, weights, *groups)
     return _from_clusters(y, groups, weights)
 
@@ -344,9 +373,10 @@ def quantize_rows(x: torch.Tensor) -> QuantizedRows:
     if n > _MOST:
         raise ValueError("x must have no more than 2**31 - 1 rows")
     pitch = (d + 15) // 16 * 16
-    q = torch.empty(n, pitch, dtype=torch.int8, device=x.device)
-    scales = torch.empty(n, dtype=torch.float32, device=x.device)
-    check(lib.skm_op_quantize_rows(x.device.index, _p(rows), ld, _DTYPES[x.dtype], n, d, _p(q), pitch, _p(scales), _stream(x)))
+    q = rows.new_empty((n, pitch), dtype=torch.int8)
+    scales = rows.new_empty(n, dtype=torch.float32)
+    index = rows.device.index
+    check(lib.skm_op_quantize_rows(index, rows.data_ptr(), ld, _DTYPES[rows.dtype], n, d, q.data_ptr(), pitch, scales.data_ptr(), _raw_stream(index)))
     return QuantizedRows(q[:, :d] if pitch != d else q, scales)
 
 
@@ -392,10 +422,12 @@ def product_8bit(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_sca
     w_scales = _floats(w_scales, "w_scales", w.shape[:-1], x)
     ld_x = x.stride(0) if n > 1 else d
     ld_w = w.stride(-2) if m > 1 else w.stride(0) if e > 1 else d
-    out = torch.empty(n, m, dtype=dtype, device=x.device)
-    space = _workspace(lib.skm_op_product_8bit_workspace(_p(x), ld_x, _p(w), ld_w, n, m, d, e), x)
-    check(lib.skm_op_product_8bit(x.device.index, _p(x), ld_x, _p(x_scales), _p(w), ld_w, _p(w_scales), n, m, d, e, _p(offsets), _p(out), _DTYPES[dtype], _p(space), space.numel(),
-                                  _stream(x)))
+    out = x_scales.new_empty((n, m), dtype=dtype)
+    x_at, w_at = x.data_ptr(), w.data_ptr()
+    space, address, size = _workspace(lib.skm_op_product_8bit_workspace(x_at, ld_x, w_at, ld_w, n, m, d, e), x)
+    index = x.device.index
+    check(lib.skm_op_product_8bit(index, x_at, ld_x, x_scales.data_ptr(), w_at, ld_w, w_scales.data_ptr(), n, m, d, e, _p(offsets), out.data_ptr(), _DTYPES[dtype], address, size,
+                                  _raw_stream(index)))
     return out
 
 
