@@ -4,9 +4,8 @@
 // whole chip, and a launch is what the time of a small call consists of.
 //
 // More: a radix sort, up to 11 bits at a time.  A unit of a few hundred pairs belongs to a warp, which counts its digits in shared
-// memory; a warp for each digit turns the units' counts into the places where each unit's pairs of that digit begin; and the units,
-// read again, rank equal digits among 32 neighbours by __match_any_sync, in order, so that the sort is stable and nothing depends on
-// the order of atomics (those add whole numbers).  Up to 2047 clusters need one pass.
+// memory; a block for each digit turns the units' counts into places; and the units, read again, rank equal digits among 32 neighbours by
+// __match_any_sync, in order, so that the sort is stable; no order of atomics matters.  Up to 2047 clusters need one pass.
 #include <algorithm>
 
 #include "rows_access.cuh"
@@ -18,43 +17,67 @@ namespace {
 
 constexpr size_t kFewPairs = 4096;
 constexpr int kMaxBits = 11;
-constexpr int kUnitWarps = 4;
+// Units of a block, whose tables are in shared memory: 16, where that leaves a block for each SM.
+int unit_warps(int bits, size_t n_units) { return bits <= 9 && n_units >= 148 * 16 ? 16 : 4; }
 
 // ---------------------------------------------------------------------------------------------- few pairs
-// A block ranks 32 pairs (one to a lane) against all: each of its eight warps compares them with an eighth of the keys.
-__global__ void __launch_bounds__(256) rank_kernel(const void* __restrict__ ids, bool wide, uint32_t n, uint32_t k, uint32_t* __restrict__ order, uint32_t* __restrict__ position,
+// A block ranks 32 pairs (one to a lane) against all: each of its warps compares them with a part of the keys.
+constexpr uint32_t kRankWarps = 16;
+
+__global__ void __launch_bounds__(32 * kRankWarps) rank_kernel(const void* __restrict__ ids, bool wide, uint32_t n, uint32_t k, uint32_t* __restrict__ order, uint32_t* __restrict__ position,
                                                    uint32_t* __restrict__ keys_out, uint32_t* __restrict__ offsets) {
     __shared__ uint4 key4[kFewPairs / 4];
-    __shared__ uint32_t parts[3][8][32];
+    __shared__ uint32_t parts[3][kRankWarps][32];
     uint32_t* key = reinterpret_cast<uint32_t*>(key4);
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t n4 = (n + 3) / 4;
-    for (uint32_t i = threadIdx.x; i < 4 * n4; i += 256) key[i] = i < n ? load_id(ids, wide, i, k) : 0xffffffffu;
+    constexpr int AHEAD = 4;
+    constexpr uint32_t THREADS = 32 * kRankWarps;
+    for (uint32_t i0 = 0; i0 < 4 * n4; i0 += THREADS * AHEAD) {
+        uint32_t v[AHEAD];
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            const uint32_t i = i0 + u * THREADS + threadIdx.x;
+            v[u] = i < n ? load_id(ids, wide, i, k) : 0xffffffffu;
+        }
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            const uint32_t i = i0 + u * THREADS + threadIdx.x;
+            if (i < 4 * n4) key[i] = v[u];
+        }
+    }
     __syncthreads();
     const uint32_t mine = blockIdx.x * 32 + lane;
     const uint32_t c = mine < n ? key[mine] : 0u;
     // keys less than c, equal ones of earlier pairs, and 1 + the largest of the lesser ones
     uint32_t less = 0, earlier = 0, below = 0;
-    const uint32_t a = warp * n4 / 8, b = (warp + 1) * n4 / 8;
-    for (uint32_t i = a; i < b; ++i) {
-        const uint4 q = key4[i];
-        const uint32_t v[4] = {q.x, q.y, q.z, q.w};
+    auto compare = [&](uint32_t from, uint32_t to, auto&& is_earlier) {
+#pragma unroll 4
+        for (uint32_t i = from; i < to; ++i) {
+            const uint4 q = key4[i];
+            const uint32_t v[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-        for (uint32_t e = 0; e < 4; ++e) {
-            if (v[e] < c) {
-                ++less;
-                below = max(below, v[e] + 1);
+            for (uint32_t e = 0; e < 4; ++e) {
+                // (selections, no branches)
+                const uint32_t lower = v[e] < c ? 1u : 0u;
+                less += lower;
+                below = max(below, lower ? v[e] + 1 : 0u);
+                earlier += v[e] == c && is_earlier(4 * i + e) ? 1u : 0u;
             }
-            if (v[e] == c && 4 * i + e < mine) ++earlier;
         }
-    }
+    };
+    // the keys before the block's own 32, those, and the ones behind them
+    const uint32_t a = warp * n4 / kRankWarps, b = (warp + 1) * n4 / kRankWarps, own0 = min(max(blockIdx.x * 8, a), b), own1 = min(max(blockIdx.x * 8 + 8, a), b);
+    compare(a, own0, [](uint32_t) { return true; });
+    compare(own0, own1, [&](uint32_t j) { return j < mine; });
+    compare(own1, b, [](uint32_t) { return false; });
     parts[0][warp][lane] = less;
     parts[1][warp][lane] = earlier;
     parts[2][warp][lane] = below;
     __syncthreads();
     if (warp != 0) return;
 #pragma unroll
-    for (int w = 1; w < 8; ++w) {
+    for (uint32_t w = 1; w < kRankWarps; ++w) {
         less += parts[0][w][lane];
         earlier += parts[1][w][lane];
         below = max(below, parts[2][w][lane]);
@@ -77,11 +100,15 @@ __global__ void __launch_bounds__(256) rank_kernel(const void* __restrict__ ids,
         rest_from = c + 1;
         rest_upto = k;
     }
-    for (uint32_t l = 0; l < 32; ++l) {
+    for (uint32_t left = __ballot_sync(0xffffffffu, from <= upto); left; left &= left - 1) {
+        const int l = __ffs(left) - 1;
         const uint32_t f = __shfl_sync(0xffffffffu, from, l), t = __shfl_sync(0xffffffffu, upto, l), v = __shfl_sync(0xffffffffu, value, l);
         for (uint32_t i = f + lane; i <= t; i += 32) offsets[i] = v;
-        const uint32_t rf = __shfl_sync(0xffffffffu, rest_from, l), rt = __shfl_sync(0xffffffffu, rest_upto, l);
-        for (uint32_t i = rf + lane; i <= rt; i += 32) offsets[i] = n;
+    }
+    const uint32_t last = __ballot_sync(0xffffffffu, rest_from <= rest_upto);
+    if (last) {
+        const uint32_t f = __shfl_sync(0xffffffffu, rest_from, __ffs(last) - 1);
+        for (uint32_t i = f + lane; i <= k; i += 32) offsets[i] = n;
     }
 }
 
@@ -91,6 +118,7 @@ struct Pass {
     uint32_t k;
     int shift, bits;
     uint32_t n_units, unit;   // a unit has this many pairs, a multiple of 32
+    uint32_t pitch;           // of the table: units, rounded up to a multiple of 4
 };
 
 // What a pass sorts: the caller's ids (the first), or the pass before's keys and pairs.
@@ -105,13 +133,14 @@ __device__ __forceinline__ uint32_t key_of(const PassInput& in, size_t i, uint32
 
 constexpr int kSortAhead = 4;
 
-// table[digit][unit] = the unit's pairs with that digit; totals[digit] += them
-__global__ void __launch_bounds__(32 * kUnitWarps) count_kernel(const PassInput in, const Pass p, uint32_t* __restrict__ table, uint32_t* __restrict__ totals) {
-    extern __shared__ uint32_t counts[];   // [digit][warp]
-    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, digits = 1u << p.bits;
-    for (uint32_t i = threadIdx.x; i < digits * kUnitWarps; i += 32 * kUnitWarps) counts[i] = 0;
+// table[digit][unit] = the unit's pairs with that digit
+template <int WARPS>
+__global__ void __launch_bounds__(32 * WARPS) count_kernel(const PassInput in, const Pass p, uint32_t* __restrict__ table) {
+    extern __shared__ uint32_t counts[];   // a row for each warp
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, digits = 1u << p.bits, apart = digits + 1;
+    for (uint32_t i = threadIdx.x; i < apart * WARPS; i += 32 * WARPS) counts[i] = 0;
     __syncthreads();
-    const uint32_t unit0 = blockIdx.x * kUnitWarps, unit = unit0 + warp;
+    const uint32_t unit0 = blockIdx.x * WARPS, unit = unit0 + warp;
     const size_t begin = static_cast<size_t>(unit) * p.unit, end = min(begin + p.unit, p.n);
     for (size_t s = begin; s < end; s += 32 * kSortAhead) {
         uint32_t key[kSortAhead];
@@ -122,65 +151,81 @@ __global__ void __launch_bounds__(32 * kUnitWarps) count_kernel(const PassInput 
         }
 #pragma unroll
         for (int u = 0; u < kSortAhead; ++u)
-            if (s + u * 32 + lane < end) atomicAdd(&counts[((key[u] >> p.shift) & (digits - 1)) * kUnitWarps + warp], 1u);
+            if (s + u * 32 + lane < end) atomicAdd(&counts[warp * apart + ((key[u] >> p.shift) & (digits - 1))], 1u);
     }
     __syncthreads();
-    const uint32_t here = min(static_cast<uint32_t>(kUnitWarps), p.n_units - unit0);
-    for (uint32_t i = threadIdx.x; i < digits; i += 32 * kUnitWarps) {
-        uint32_t sum = 0;
-        for (uint32_t w = 0; w < here; ++w) {
-            const uint32_t c = counts[i * kUnitWarps + w];
-            table[static_cast<size_t>(i) * p.n_units + unit0 + w] = c;
-            sum += c;
-        }
-        if (sum) atomicAdd(totals + i, sum);
+    // WARPS neighbouring lanes have a digit (past the last unit, up to the pitch, its counts are zero)
+    for (uint32_t i = threadIdx.x; i < digits * WARPS; i += 32 * WARPS) {
+        const uint32_t digit = i / WARPS, w = i % WARPS;
+        if (unit0 + w < p.pitch) table[static_cast<size_t>(digit) * p.pitch + unit0 + w] = counts[w * apart + digit];
     }
 }
 
-// table[digit][unit] = the slot of the unit's first pair with that digit; a warp for each digit.  offsets (may be null): of the
-// digits up to k.
-__global__ void __launch_bounds__(256) place_kernel(const Pass p, uint32_t* __restrict__ table, const uint32_t* __restrict__ totals, uint32_t* __restrict__ offsets) {
-    __shared__ uint32_t sums[8];
-    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, digits = 1u << p.bits, digit0 = blockIdx.x * 8, digit = digit0 + warp;
+// table[digit][unit] = how many pairs of that digit the units before have, totals[digit] all; a block for each digit.
+__global__ void __launch_bounds__(256) place_kernel(const Pass p, uint32_t* __restrict__ table, uint32_t* __restrict__ totals) {
+    __shared__ uint32_t sums[2][8];
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    uint4* row = reinterpret_cast<uint4*>(table + static_cast<size_t>(blockIdx.x) * p.pitch);
+    const uint32_t n4 = p.pitch / 4;
+    uint4 v = threadIdx.x < n4 ? row[threadIdx.x] : make_uint4(0, 0, 0, 0);
     uint32_t before = 0;
-    for (uint32_t i = threadIdx.x; i < digit0; i += 256) before += __ldg(totals + i);
-    before = __reduce_add_sync(0xffffffffu, before);
-    if (lane == 0) sums[warp] = before;
-    __syncthreads();
-    uint32_t slot = 0;
+    for (uint32_t s = 0; s < n4; s += 256) {
+        const uint32_t i = s + threadIdx.x;
+        const uint4 c = v;
+        v = i + 256 < n4 ? row[i + 256] : make_uint4(0, 0, 0, 0);
+        const uint32_t four = c.x + c.y + c.z + c.w;
+        uint32_t upto = four;
 #pragma unroll
-    for (int w = 0; w < 8; ++w) slot += sums[w];
-    for (uint32_t i = digit0; i < digit; ++i) slot += __ldg(totals + i);
-    if (digit >= digits) return;
-    if (offsets && lane == 0 && digit <= p.k) offsets[digit] = slot;
-    uint32_t* row = table + static_cast<size_t>(digit) * p.n_units;
-    constexpr int AHEAD = 8;
-    for (uint32_t s = 0; s < p.n_units; s += 32 * AHEAD) {
-        uint32_t v[AHEAD];
-#pragma unroll
-        for (int u = 0; u < AHEAD; ++u) v[u] = s + u * 32 + lane < p.n_units ? row[s + u * 32 + lane] : 0u;
-#pragma unroll
-        for (int u = 0; u < AHEAD; ++u) {
-            uint32_t upto = v[u];
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const uint32_t t = __shfl_up_sync(0xffffffffu, upto, o);
-                if (lane >= o) upto += t;
-            }
-            if (s + u * 32 + lane < p.n_units) row[s + u * 32 + lane] = slot + upto - v[u];
-            slot += __shfl_sync(0xffffffffu, upto, 31);
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t t = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= static_cast<uint32_t>(o)) upto += t;
         }
+        if (lane == 31) sums[s / 256 & 1][warp] = upto;   // (the other half may still be read)
+        __syncthreads();
+        uint32_t here = before + upto - four;
+#pragma unroll
+        for (uint32_t w = 0; w < 8; ++w) {
+            const uint32_t t = sums[s / 256 & 1][w];
+            if (w < warp) here += t;
+            before += t;
+        }
+        if (i < n4) row[i] = make_uint4(here, here + c.x, here + c.x + c.y, here + c.x + c.y + c.z);
     }
+    if (threadIdx.x == 0) totals[blockIdx.x] = before;
 }
 
-__global__ void __launch_bounds__(32 * kUnitWarps) scatter_kernel(const PassInput in, const Pass p, const uint32_t* __restrict__ table, uint32_t* __restrict__ pairs_out,
-                                                                  uint32_t* __restrict__ keys_out, uint32_t* __restrict__ position) {
-    extern __shared__ uint32_t next[];   // [digit][warp]
-    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, digits = 1u << p.bits;
-    const uint32_t unit0 = blockIdx.x * kUnitWarps, unit = unit0 + warp;
-    for (uint32_t i = threadIdx.x; i < digits * kUnitWarps; i += 32 * kUnitWarps) {
-        const uint32_t w = i % kUnitWarps;
-        if (unit0 + w < p.n_units) next[i] = __ldg(table + static_cast<size_t>(i / kUnitWarps) * p.n_units + unit0 + w);
+template <int WARPS>
+__global__ void __launch_bounds__(32 * WARPS) scatter_kernel(const PassInput in, const Pass p, const uint32_t* __restrict__ table, const uint32_t* __restrict__ totals,
+                                                             uint32_t* __restrict__ pairs_out, uint32_t* __restrict__ keys_out, uint32_t* __restrict__ position,
+                                                             uint32_t* __restrict__ offsets) {
+    extern __shared__ uint32_t next[];   // a row for each warp
+    __shared__ uint32_t sums[WARPS];
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, digits = 1u << p.bits, apart = digits + 1;
+    const uint32_t unit0 = blockIdx.x * WARPS, unit = unit0 + warp;
+    // where each digit begins: the totals before it, `each` neighbouring digits to a thread (offsets, if given: of the digits up to k)
+    uint32_t* base = next + apart * WARPS;
+    const uint32_t each = (digits + 32 * WARPS - 1) / (32 * WARPS), digit0 = threadIdx.x * each;
+    uint32_t mine = 0;
+    for (uint32_t e = 0; e < each && digit0 + e < digits; ++e) mine += __ldg(totals + digit0 + e);
+    uint32_t upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t t = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= static_cast<uint32_t>(o)) upto += t;
+    }
+    if (lane == 31) sums[warp] = upto;
+    __syncthreads();
+    uint32_t slot0 = upto - mine;
+    for (uint32_t w = 0; w < warp; ++w) slot0 += sums[w];
+    for (uint32_t e = 0; e < each && digit0 + e < digits; ++e) {
+        base[digit0 + e] = slot0;
+        if (offsets && blockIdx.x == 0 && digit0 + e <= p.k) offsets[digit0 + e] = slot0;
+        slot0 += __ldg(totals + digit0 + e);
+    }
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < digits * WARPS; i += 32 * WARPS) {
+        const uint32_t w = i % WARPS, digit = i / WARPS;
+        if (unit0 + w < p.n_units) next[w * apart + digit] = base[digit] + __ldg(table + static_cast<size_t>(digit) * p.pitch + unit0 + w);
     }
     __syncthreads();
     const size_t begin = static_cast<size_t>(unit) * p.unit, end = min(begin + p.unit, p.n);
@@ -199,29 +244,29 @@ __global__ void __launch_bounds__(32 * kUnitWarps) scatter_kernel(const PassInpu
             const uint32_t digit = valid ? (key[u] >> p.shift) & (digits - 1) : 0xffffffffu;
             const uint32_t same = __match_any_sync(0xffffffffu, digit), rank = __popc(same & ((1u << lane) - 1u));
             if (valid) {
-                const uint32_t slot = next[digit * kUnitWarps + warp] + rank;
+                const uint32_t slot = next[warp * apart + digit] + rank;
                 pairs_out[slot] = pair[u];
                 if (keys_out) keys_out[slot] = key[u];
                 if (position) position[pair[u]] = slot;
             }
             __syncwarp();
-            if (valid && rank == 0) next[digit * kUnitWarps + warp] += __popc(same);
+            if (valid && rank == 0) next[warp * apart + digit] += __popc(same);
             __syncwarp();
         }
     }
 }
 
-// offsets[c] = first slot whose key is c or more
+// offsets[c] = first slot whose key is c or more: where a key begins it sets those of the keys behind the one before, 32 lanes together
 __global__ void __launch_bounds__(256) offsets_kernel(const uint32_t* __restrict__ keys, uint32_t n, uint32_t k, uint32_t* __restrict__ offsets) {
-    const uint32_t c = blockIdx.x * 256 + threadIdx.x;
-    if (c > k) return;
-    uint32_t lo = 0, hi = n;
-    while (lo < hi) {
-        const uint32_t mid = lo + (hi - lo) / 2;
-        if (__ldg(keys + mid) < c) lo = mid + 1;
-        else hi = mid;
+    const uint32_t lane = threadIdx.x & 31, slot = blockIdx.x * 256 + threadIdx.x;
+    const uint32_t key = slot < n ? __ldg(keys + slot) : 0u, from = slot == 0 ? 0u : slot < n ? __ldg(keys + slot - 1) + 1 : 1u;
+    for (uint32_t left = __ballot_sync(0xffffffffu, slot < n && from <= key); left; left &= left - 1) {
+        const int l = __ffs(left) - 1;
+        const uint32_t f = __shfl_sync(0xffffffffu, from, l), t = __shfl_sync(0xffffffffu, key, l), v = __shfl_sync(0xffffffffu, slot, l);
+        for (uint32_t c = f + lane; c <= t; c += 32) offsets[c] = v;
     }
-    offsets[c] = lo;
+    // behind the last key, by the grid
+    for (uint32_t c = __ldg(keys + n - 1) + 1 + slot; c <= k; c += gridDim.x * 256) offsets[c] = n;
 }
 
 struct Plan {
@@ -232,9 +277,14 @@ Plan make_plan(size_t n, size_t k) {
     int all = 1;
     while ((k >> all) != 0) ++all;   // keys are 0 .. k
     const int passes = (all + kMaxBits - 1) / kMaxBits;
-    const uint32_t unit = n < (size_t{1} << 17) ? 128 : n < (size_t{1} << 20) ? 512 : n < (size_t{1} << 23) ? 2048 : 16384;
-    return {passes, (all + passes - 1) / passes, unit, static_cast<uint32_t>((n + unit - 1) / unit)};
+    const int bits = (all + passes - 1) / passes;
+    // about 4096 units (so many warps hide the latency of what they read), but no table that is larger than the lists by far
+    const size_t most = std::min<size_t>(4096, (size_t{1} << 20) >> bits);
+    const size_t unit = std::max<size_t>(128, (n + most - 1) / most);
+    const uint32_t rounded = static_cast<uint32_t>((unit + 127) / 128 * 128);
+    return {passes, bits, rounded, static_cast<uint32_t>((n + rounded - 1) / rounded)};
 }
+size_t pitch_of(const Plan& plan) { return (plan.n_units + 3) / 4 * 4; }
 size_t rounded(size_t words) { return (words + 63) / 64 * 64; }
 
 } // namespace
@@ -244,7 +294,7 @@ size_t group_workspace_bytes(size_t n, size_t k) {
     const Plan plan = make_plan(n, k);
     // digits' totals, the units' table, and between passes two copies of keys and pairs
     const size_t lists = plan.passes == 1 ? 0 : 4;
-    return 4 * (rounded(size_t{1} << plan.bits) * plan.passes + rounded(static_cast<size_t>(plan.n_units) << plan.bits) + lists * rounded(n));
+    return 4 * (rounded(size_t{1} << plan.bits) + rounded(pitch_of(plan) << plan.bits) + lists * rounded(n));
 }
 
 void launch_group(const Ids& ids, size_t n, size_t k, uint32_t* order, uint32_t* position, uint32_t* keys, uint32_t* offsets, void* workspace, cudaStream_t stream) {
@@ -253,35 +303,35 @@ void launch_group(const Ids& ids, size_t n, size_t k, uint32_t* order, uint32_t*
         return;
     }
     if (n <= kFewPairs) {
-        rank_kernel<<<static_cast<unsigned>((n + 31) / 32), 256, 0, stream>>>(ids.p, ids.wide, static_cast<uint32_t>(n), static_cast<uint32_t>(k), order, position, keys, offsets);
+        rank_kernel<<<static_cast<unsigned>((n + 31) / 32), 32 * kRankWarps, 0, stream>>>(ids.p, ids.wide, static_cast<uint32_t>(n), static_cast<uint32_t>(k), order, position, keys, offsets);
         SKM_LAUNCH_CHECK();
         return;
     }
     const Plan plan = make_plan(n, k);
     const size_t digits = size_t{1} << plan.bits;
     uint32_t* totals = static_cast<uint32_t*>(workspace);
-    uint32_t* table = totals + rounded(digits) * plan.passes;
-    uint32_t* lists = table + rounded(static_cast<size_t>(plan.n_units) << plan.bits);
-    const unsigned blocks = (plan.n_units + kUnitWarps - 1) / kUnitWarps, shared = static_cast<unsigned>(digits * kUnitWarps * 4);
-    SKM_CUDA(cudaMemsetAsync(totals, 0, rounded(digits) * plan.passes * 4, stream));
+    uint32_t* table = totals + rounded(digits);
+    uint32_t* lists = table + rounded(pitch_of(plan) << plan.bits);
+    const unsigned warps = static_cast<unsigned>(unit_warps(plan.bits, plan.n_units)), blocks = (plan.n_units + warps - 1) / warps, shared = static_cast<unsigned>((digits + 1) * warps * 4);
     PassInput in{ids.p, ids.wide, nullptr, nullptr};
     for (int pass = 0; pass < plan.passes; ++pass) {
         const bool last = pass == plan.passes - 1;
-        const Pass p{n, static_cast<uint32_t>(k), pass * plan.bits, plan.bits, plan.n_units, plan.unit};
+        const Pass p{n, static_cast<uint32_t>(k), pass * plan.bits, plan.bits, plan.n_units, plan.unit, static_cast<uint32_t>(pitch_of(plan))};
         uint32_t* keys_here = plan.passes == 1 ? keys : (last && keys) ? keys : lists + rounded(n) * 2 * (pass & 1);
         uint32_t* pairs_here = last ? order : lists + rounded(n) * (2 * (pass & 1) + 1);
-        uint32_t* total = totals + rounded(digits) * pass;
-        count_kernel<<<blocks, 32 * kUnitWarps, shared, stream>>>(in, p, table, total);
+        if (warps == 16) count_kernel<16><<<blocks, 512, shared, stream>>>(in, p, table);
+        else count_kernel<4><<<blocks, 128, shared, stream>>>(in, p, table);
         SKM_LAUNCH_CHECK();
-        place_kernel<<<static_cast<unsigned>((digits + 7) / 8), 256, 0, stream>>>(p, table, total, plan.passes == 1 ? offsets : nullptr);
+        place_kernel<<<static_cast<unsigned>(digits), 256, 0, stream>>>(p, table, totals);
         SKM_LAUNCH_CHECK();
-        scatter_kernel<<<blocks, 32 * kUnitWarps, shared, stream>>>(in, p, table, pairs_here, keys_here, last ? position : nullptr);
+        if (warps == 16) scatter_kernel<16><<<blocks, 512, shared + digits * 4, stream>>>(in, p, table, totals, pairs_here, keys_here, last ? position : nullptr, plan.passes == 1 ? offsets : nullptr);
+        else scatter_kernel<4><<<blocks, 128, shared + digits * 4, stream>>>(in, p, table, totals, pairs_here, keys_here, last ? position : nullptr, plan.passes == 1 ? offsets : nullptr);
         SKM_LAUNCH_CHECK();
         in.keys = keys_here;
         in.pairs = pairs_here;
     }
     if (plan.passes > 1) {
-        offsets_kernel<<<static_cast<unsigned>(k / 256 + 1), 256, 0, stream>>>(in.keys, static_cast<uint32_t>(n), static_cast<uint32_t>(k), offsets);
+        offsets_kernel<<<static_cast<unsigned>((n + 255) / 256), 256, 0, stream>>>(in.keys, static_cast<uint32_t>(n), static_cast<uint32_t>(k), offsets);
         SKM_LAUNCH_CHECK();
     }
 }

@@ -1,9 +1,9 @@
 // Rows by index: lookup in a table, rows to the places of their clusters and back, and the gradients of the weights and scales.
 //
 // All of them move rows once and compute next to nothing: they are bound by HBM, or for small calls by the launch.  The rows of an
-// output (or for to_clusters of the input) are taken as one sequence of 32-byte chunks, 256 x 2 of them to a block whatever the rows'
+// output (or for to_clusters of the input) are taken as one sequence of 32-byte chunks, 128 x 2 of them to a block whatever the rows'
 // width, so that narrow and odd rows fill the lanes as well as wide ones; a row whose address, pitch or width is no multiple of 32
-// bytes is taken in chunks of 16, 8, 4 or 2, 256 x 4 to a block.  Products and sums are in fp32 and rounded once.
+// bytes is taken in chunks of 16, 8, 4 or 2, 128 x 4 to a block.  Products and sums are in fp32 and rounded once.
 #include "rows_access.cuh"
 
 #include "device_utils.cuh"
@@ -13,7 +13,7 @@ namespace rows {
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;
 
 // Chunks of a thread, all loaded before the first is stored: 64 bytes, which with the 40 warps of an SM keep 80 KB on their way.
 template <int BYTES>
@@ -26,20 +26,14 @@ struct Spread {
 };
 
 template <int BYTES>
-constexpr size_t kBlockChunks = kThreads * kAhead<BYTES>;
-
-template <int BYTES>
 Spread make_spread(size_t n, size_t row_bytes) {
     const size_t width = row_bytes / BYTES;
-    return {n * width, make_divisor(width, width + kBlockChunks<BYTES>)};
+    return {n * width, make_divisor(width, width + kThreads * kAhead<BYTES>)};
 }
-template <int BYTES>
-unsigned spread_blocks(const Spread& s) {
-    return static_cast<unsigned>((s.total + kBlockChunks<BYTES> - 1) / kBlockChunks<BYTES>);
-}
+unsigned spread_blocks(const Spread& s, int ahead) { return static_cast<unsigned>((s.total + kThreads * ahead - 1) / (kThreads * ahead)); }
 
 // This thread's chunks: row and place in the row of chunk u, and whether there is one.
-template <int BYTES>
+template <int BYTES, int AHEAD = kAhead<BYTES>>
 struct Mine {
     size_t row0;
     uint32_t off;
@@ -47,7 +41,7 @@ struct Mine {
     Divisor width;
 
     __device__ __forceinline__ explicit Mine(const Spread& s) : width(s.width) {
-        const size_t first = static_cast<size_t>(blockIdx.x) * kBlockChunks<BYTES>;
+        const size_t first = static_cast<size_t>(blockIdx.x) * (kThreads * AHEAD);
         row0 = (first >> 32) == 0 ? static_cast<uint32_t>(first) / s.width.d : first / s.width.d;
         off = static_cast<uint32_t>(first - row0 * s.width.d) + threadIdx.x;
         left = first + threadIdx.x < s.total ? s.total - first - threadIdx.x : 0;
@@ -130,8 +124,8 @@ __global__ void __launch_bounds__(kThreads) to_clusters_kernel(const void* __res
 template <typename T, int BYTES>
 __global__ void __launch_bounds__(kThreads) from_clusters_kernel(const void* __restrict__ y, size_t pitch, const Places at, const float* __restrict__ weights,
                                                                  Chunk<BYTES>* __restrict__ out, const Spread spread) {
-    constexpr int AHEAD = kAhead<BYTES>;
-    const Mine<BYTES> mine(spread);
+    constexpr int AHEAD = kAhead<BYTES> / 2;
+    const Mine<BYTES, AHEAD> mine(spread);
     const uint32_t slots = static_cast<uint32_t>(at.n * at.m), held = min(__ldg(at.held), slots);
     size_t row[AHEAD];
     uint32_t col[AHEAD];
@@ -257,7 +251,7 @@ void launch_lookup(const Rows& table, Type type, size_t k, size_t d, const Ids& 
         const Spread s = make_spread<B>(n, d * t);
         // (a product with one changes no value: the plain copy is for that)
         auto* kernel = row_scales || scale != 1.0f ? lookup_kernel<T, B, true> : lookup_kernel<T, B, false>;
-        kernel<<<spread_blocks<B>(s), kThreads, 0, stream>>>(table.p, pitch, static_cast<uint32_t>(k), ids.p, ids.wide, scale, row_scales, static_cast<Chunk<B>*>(out), s);
+        kernel<<<spread_blocks(s, kAhead<B>), kThreads, 0, stream>>>(table.p, pitch, static_cast<uint32_t>(k), ids.p, ids.wide, scale, row_scales, static_cast<Chunk<B>*>(out), s);
     });
     SKM_LAUNCH_CHECK();
 }
@@ -279,7 +273,7 @@ void launch_to_clusters(const Rows& x, Type type, size_t d, const Places& at, vo
     with_width<32>(type, access_bytes({address(x.p), pitch, d * t, address(out)}, 32), [&](auto, auto width) {
         constexpr int B = decltype(width)::bytes;
         const Spread s = make_spread<B>(at.n, d * t);
-        to_clusters_kernel<B><<<spread_blocks<B>(s), kThreads, 0, stream>>>(x.p, pitch, at, static_cast<Chunk<B>*>(out), s);
+        to_clusters_kernel<B><<<spread_blocks(s, kAhead<B>), kThreads, 0, stream>>>(x.p, pitch, at, static_cast<Chunk<B>*>(out), s);
     });
     SKM_LAUNCH_CHECK();
 }
@@ -290,7 +284,7 @@ void launch_from_clusters(const Rows& y, Type type, size_t d, const Places& at, 
     with_width<32>(type, access_bytes({address(y.p), pitch, d * t, address(out)}, 32), [&](auto value, auto width) {
         constexpr int B = decltype(width)::bytes;
         const Spread s = make_spread<B>(at.n, d * t);
-        from_clusters_kernel<decltype(value), B><<<spread_blocks<B>(s), kThreads, 0, stream>>>(y.p, pitch, at, weights, static_cast<Chunk<B>*>(out), s);
+        from_clusters_kernel<decltype(value), B><<<spread_blocks(s, kAhead<B> / 2), kThreads, 0, stream>>>(y.p, pitch, at, weights, static_cast<Chunk<B>*>(out), s);
     });
     SKM_LAUNCH_CHECK();
 }

@@ -13,7 +13,7 @@ namespace rows {
 namespace {
 
 constexpr int kWarps = 4;
-constexpr int kAhead = 8;
+constexpr uint32_t kAhead = 8;
 
 struct SumParams {
     const void* grad;
@@ -27,32 +27,51 @@ struct SumParams {
     uint32_t width;            // chunks to a row
     uint32_t slabs;            // of 32 chunks
     uint32_t tile;             // pairs to a tile
+    uint32_t join_ids;         // ids to a warp of the second launch
     float* partials;           // per tile two rows of d: the first run, and the last if it is another
     void* out;
 };
 
-template <typename T, typename O, int BYTES>
-__device__ __forceinline__ void store_sum(const Values<T, BYTES>& sum, O* to) {
-    constexpr int N = Values<T, BYTES>::N, OUT = N * static_cast<int>(sizeof(O));
-    if constexpr (OUT <= 16) {
-        Values<O, OUT> v;
+// Sums of a chunk's values, and their stores: at `to` as they are or as the output's type.
+template <typename T, int BYTES>
+struct Sums {
+    static constexpr int N = Values<T, BYTES>::N;
+    float v[N];
+
+    __device__ __forceinline__ void clear() {
 #pragma unroll
-        for (int i = 0; i < N; ++i) v.v[i] = sum.v[i];
-        *reinterpret_cast<Chunk<OUT>*>(to) = v.to();
-    } else {   // eight sums of halves in fp32
-        Values<O, 16> v;
+        for (int i = 0; i < N; ++i) v[i] = 0.f;
+    }
+    __device__ __forceinline__ void add(const Chunk<BYTES>& c) {
+        Values<T, BYTES> x;
+        x.from(c);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int i = 0; i < N; ++i) v[i] += x.v[i];
+    }
+    __device__ __forceinline__ void add(const Chunk<BYTES>& c, float f) {
+        Values<T, BYTES> x;
+        x.from(c);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v.v[i] = sum.v[4 * h + i];
-            reinterpret_cast<Chunk<16>*>(to)[h] = v.to();
+        for (int i = 0; i < N; ++i) v[i] = fmaf(f, x.v[i], v[i]);
+    }
+    template <typename O>
+    __device__ __forceinline__ void store(O* to, float scale) const {
+        constexpr int ALL = N * static_cast<int>(sizeof(O)), EACH = ALL < 16 ? ALL : 16, PART = EACH / static_cast<int>(sizeof(O));
+#pragma unroll
+        for (int h = 0; h < ALL / EACH; ++h) {
+            Values<O, EACH> x;
+#pragma unroll
+            for (int i = 0; i < PART; ++i) x.v[i] = v[h * PART + i] * scale;
+            reinterpret_cast<Chunk<EACH>*>(to)[h] = x.to();
         }
     }
-}
+};
 
-template <typename T, typename O, int BYTES>
+// SCALED: each pair with a factor of its own; otherwise the sums are scaled.
+template <typename T, typename O, int BYTES, bool SCALED>
 __global__ void __launch_bounds__(32 * kWarps) sum_tiles_kernel(const SumParams p) {
-    using V = Values<T, BYTES>;
+    constexpr uint32_t AHEAD = kAhead;
+    using S = Sums<T, BYTES>;
     const uint32_t lane = threadIdx.x & 31;
     const size_t unit = static_cast<size_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
     const size_t tile = unit / p.slabs, begin = tile * p.tile;
@@ -61,127 +80,135 @@ __global__ void __launch_bounds__(32 * kWarps) sum_tiles_kernel(const SumParams 
     const uint32_t col = static_cast<uint32_t>(unit - tile * p.slabs) * 32 + lane;
     const bool mine = col < p.width;
     const uint32_t s0 = static_cast<uint32_t>(begin), s1 = min(s0 + p.tile, held);
-    const size_t at = static_cast<size_t>(col) * V::N;
+    const size_t at = static_cast<size_t>(col) * S::N;
     float* first_part = p.partials + tile * 2 * p.d + at;
-    V sum;
-    auto clear = [&] {
-#pragma unroll
-        for (int i = 0; i < V::N; ++i) sum.v[i] = 0.f;
-    };
-    clear();
+    const char* grad = static_cast<const char*>(p.grad) + static_cast<size_t>(mine ? col : 0) * BYTES;
+    const float scale = SCALED ? 1.f : p.scale;
+    S sum;
+    sum.clear();
     uint32_t now = __ldg(p.keys + s0);
     bool first = true;
     for (uint32_t s = s0; s < s1; s += 32) {
-        // a lane's pair of the next 32
+        // a lane's pair of the next 32, and where runs of equal ids begin
         const uint32_t my = s + lane;
         const uint32_t my_pair = my < s1 ? __ldg(p.order + my) : 0u, my_key = my < s1 ? __ldg(p.keys + my) : 0u;
-        const float my_factor = p.row_scales ? p.scale * (my < s1 ? __ldg(p.row_scales + my_pair) : 0.f) : p.scale;
+        float my_factor = 0.f;
+        if (SCALED && my < s1) my_factor = p.scale * __ldg(p.row_scales + my_pair);
+        const uint32_t above = __shfl_up_sync(0xffffffffu, my_key, 1);
+        const uint32_t begins = __ballot_sync(0xffffffffu, my < s1 && my_key != (lane == 0 ? now : above));
         const uint32_t count = min(32u, s1 - s);
-        for (uint32_t u0 = 0; u0 < count; u0 += kAhead) {
-            Chunk<BYTES> c[kAhead];
+        for (uint32_t u0 = 0; u0 < count; u0 += AHEAD) {
+            Chunk<BYTES> c[AHEAD];
 #pragma unroll
-            for (uint32_t u = 0; u < kAhead; ++u) {
-                const uint32_t pair = __shfl_sync(0xffffffffu, my_pair, u0 + u);
-                if (u0 + u < count && mine) c[u] = __ldg(reinterpret_cast<const Chunk<BYTES>*>(static_cast<const char*>(p.grad) + pair * p.pitch) + col);
+            for (uint32_t u = 0; u < AHEAD; ++u) {
+                const uint32_t pair = __shfl_sync(0xffffffffu, my_pair, u0 + u);   // (behind the last: row 0, which is not added)
+                c[u] = load_chunk<BYTES>(reinterpret_cast<const Chunk<BYTES>*>(grad + pair * p.pitch));
+            }
+            const uint32_t here = begins >> u0 & ((1u << AHEAD) - 1);
+            if (here == 0 && u0 + AHEAD <= count) {
+#pragma unroll
+                for (uint32_t u = 0; u < AHEAD; ++u) {
+                    if (SCALED) sum.add(c[u], __shfl_sync(0xffffffffu, my_factor, u0 + u));
+                    else sum.add(c[u]);
+                }
+                continue;
             }
 #pragma unroll
-            for (uint32_t u = 0; u < kAhead; ++u) {
-                const uint32_t key = __shfl_sync(0xffffffffu, my_key, u0 + u);
-                const float f = __shfl_sync(0xffffffffu, my_factor, u0 + u);
-                if (u0 + u < count) {
-                    if (key != now) {
-                        if (mine) {
-                            if (first) store_sum<T, float, BYTES>(sum, first_part);
-                            else store_sum<T, O, BYTES>(sum, static_cast<O*>(p.out) + static_cast<size_t>(now) * p.d + at);
-                        }
-                        clear();
-                        first = false;
-                        now = key;
-                    }
+            for (uint32_t u = 0; u < AHEAD; ++u) {
+                const float f = SCALED ? __shfl_sync(0xffffffffu, my_factor, u0 + u) : 1.f;
+                if (here >> u & 1) {
                     if (mine) {
-                        V v;
-                        v.from(c[u]);
-#pragma unroll
-                        for (int i = 0; i < V::N; ++i) sum.v[i] = fmaf(f, v.v[i], sum.v[i]);
+                        if (first) sum.template store<float>(first_part, scale);
+                        else sum.template store<O>(static_cast<O*>(p.out) + static_cast<size_t>(now) * p.d + at, scale);
                     }
+                    sum.clear();
+                    first = false;
+                    now = __shfl_sync(0xffffffffu, my_key, u0 + u);
+                }
+                if (u0 + u < count) {
+                    if (SCALED) sum.add(c[u], f);
+                    else sum.add(c[u]);
                 }
             }
         }
     }
-    if (mine) store_sum<T, float, BYTES>(sum, first ? first_part : first_part + p.d);
+    if (mine) sum.template store<float>(first ? first_part : first_part + p.d, scale);
 }
 
-// Eight ids to a block, a warp and 32 chunks each; ids whose pairs fill many tiles are taken by all eight warps together.
+// Up to 32 ids and 32 chunks to a warp; ids whose pairs fill many tiles are taken by all eight warps of a block together.
 constexpr int kJoinWarps = 8;
-constexpr uint32_t kLongRun = 32;   // tiles
+constexpr uint32_t kLongRun = 8;   // tiles
 
 template <typename T, typename O, int BYTES>
 __global__ void __launch_bounds__(32 * kJoinWarps) join_tiles_kernel(const SumParams p) {
-    using V = Values<T, BYTES>;
-    __shared__ float parts[kJoinWarps][32][V::N + 1];
+    using S = Sums<T, BYTES>;
+    __shared__ float parts[kJoinWarps][32][S::N + 1];
+    __shared__ uint32_t long_ids[kJoinWarps];
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t id0 = blockIdx.x * kJoinWarps, col = blockIdx.y * 32 + lane;
+    const uint32_t block0 = blockIdx.x * (p.join_ids * kJoinWarps), id0 = block0 + warp * p.join_ids, col = blockIdx.y * 32 + lane;
     const bool mine = col < p.width;
-    const size_t at = static_cast<size_t>(col) * V::N;
-    // tiles of an id, and whether its sum is in the output already
-    auto tiles_of = [&](uint32_t id, uint32_t& t0, uint32_t& t1, uint32_t& begin) {
-        begin = __ldg(p.offsets + id);
-        const uint32_t end = __ldg(p.offsets + id + 1);
+    const size_t at = static_cast<size_t>(col) * S::N;
+    O* out = static_cast<O*>(p.out) + at;
+    // the tiles t0 .. t1 - 1 of this lane's id, and whether there is something to do: its sum is in the output already if its pairs
+    // lie inside their tile, which ends where the pairs with an id end
+    uint32_t begin = 0, t0 = 0, t1 = 0;
+    bool todo = false;
+    if (lane < p.join_ids && id0 + lane < p.k) {
+        begin = __ldg(p.offsets + id0 + lane);
+        const uint32_t end = __ldg(p.offsets + id0 + lane + 1), held = __ldg(p.offsets + p.k);
         t0 = begin / p.tile;
         t1 = end > begin ? (end - 1) / p.tile + 1 : t0;
-        if (t1 == t0 + 1) {
-            // inside its tile, which ends where the pairs with an id end
-            const uint32_t tile_end = min(static_cast<size_t>(t0 + 1) * p.tile, static_cast<size_t>(__ldg(p.offsets + p.k)));
-            if (begin > t0 * p.tile && end < tile_end) return false;
-        }
-        return true;
-    };
-    auto add_tiles = [&](V& sum, uint32_t from, uint32_t to, uint32_t begin) {
+        todo = !(t1 == t0 + 1 && begin > t0 * p.tile && end < min(static_cast<size_t>(t1) * p.tile, static_cast<size_t>(held)));
+    }
+    auto add_tiles = [&](S& sum, uint32_t from, uint32_t to, uint32_t first) {
         constexpr uint32_t AHEAD = 4;
         for (uint32_t t = from; t < to; t += AHEAD) {
-            float v[AHEAD][V::N];
+            constexpr int EACH = S::N < 4 ? S::N : 4;   // floats of a load
+            Values<float, EACH * 4> v[AHEAD][S::N / EACH];
 #pragma unroll
             for (uint32_t u = 0; u < AHEAD; ++u) {
                 const size_t tile = t + u;
-                const float* src = p.partials + (tile * 2 + (begin > tile * p.tile ? 1 : 0)) * p.d + at;
+                const float* src = p.partials + (tile * 2 + (first > tile * p.tile ? 1 : 0)) * p.d + at;
 #pragma unroll
-                for (int i = 0; i < V::N; ++i) v[u][i] = t + u < to && mine ? __ldg(src + i) : 0.f;
+                for (int i = 0; i < S::N / EACH; ++i)
+                    v[u][i].from(t + u < to && mine ? __ldg(reinterpret_cast<const Chunk<EACH * 4>*>(src) + i) : zero_chunk<EACH * 4>());
             }
 #pragma unroll
             for (uint32_t u = 0; u < AHEAD; ++u)
 #pragma unroll
-                for (int i = 0; i < V::N; ++i) sum.v[i] += v[u][i];
+                for (int i = 0; i < S::N; ++i) sum.v[i] += v[u][i / EACH].v[i % EACH];
         }
     };
-    uint32_t t0 = 0, t1 = 0, begin = 0;
-    const bool own = id0 + warp < p.k && tiles_of(id0 + warp, t0, t1, begin);
-    if (own && t1 - t0 <= kLongRun) {
-        V sum;
-#pragma unroll
-        for (int i = 0; i < V::N; ++i) sum.v[i] = 0.f;
-        add_tiles(sum, t0, t1, begin);
-        if (mine) store_sum<T, O, BYTES>(sum, static_cast<O*>(p.out) + static_cast<size_t>(id0 + warp) * p.d + at);
+    const uint32_t long_here = __ballot_sync(0xffffffffu, todo && t1 - t0 > kLongRun);
+    for (uint32_t left = __ballot_sync(0xffffffffu, todo) & ~long_here; left; left &= left - 1) {
+        const int l = __ffs(left) - 1;
+        S sum;
+        sum.clear();
+        add_tiles(sum, __shfl_sync(0xffffffffu, t0, l), __shfl_sync(0xffffffffu, t1, l), __shfl_sync(0xffffffffu, begin, l));
+        if (mine) sum.template store<O>(out + static_cast<size_t>(id0 + l) * p.d, 1.f);
     }
-    if (!__syncthreads_or(own && t1 - t0 > kLongRun)) return;
-    for (uint32_t i = 0; i < kJoinWarps && id0 + i < p.k; ++i) {
-        if (!tiles_of(id0 + i, t0, t1, begin) || t1 - t0 <= kLongRun) continue;   // (the same for the whole block)
-        const uint32_t share = (t1 - t0 + kJoinWarps - 1) / kJoinWarps, from = min(t0 + warp * share, t1);
-        V sum;
+    if (lane == 0) long_ids[warp] = long_here;
+    if (!__syncthreads_or(long_here != 0)) return;
+    for (uint32_t w = 0; w < kJoinWarps; ++w)
+        for (uint32_t left = long_ids[w]; left; left &= left - 1) {   // (the same for the whole block)
+            const uint32_t id = block0 + w * p.join_ids + __ffs(left) - 1;
+            const uint32_t first = __ldg(p.offsets + id), from0 = first / p.tile, to0 = (__ldg(p.offsets + id + 1) - 1) / p.tile + 1;
+            const uint32_t share = (to0 - from0 + kJoinWarps - 1) / kJoinWarps, from = min(from0 + warp * share, to0);
+            S sum;
+            sum.clear();
+            add_tiles(sum, from, min(from + share, to0), first);
 #pragma unroll
-        for (int e = 0; e < V::N; ++e) sum.v[e] = 0.f;
-        add_tiles(sum, from, min(from + share, t1), begin);
+            for (int e = 0; e < S::N; ++e) parts[warp][lane][e] = sum.v[e];
+            __syncthreads();
+            if (warp == 0) {
 #pragma unroll
-        for (int e = 0; e < V::N; ++e) parts[warp][lane][e] = sum.v[e];
-        __syncthreads();
-        if (warp == 0) {
+                for (int q = 1; q < kJoinWarps; ++q)
 #pragma unroll
-            for (int w = 1; w < kJoinWarps; ++w)
-#pragma unroll
-                for (int e = 0; e < V::N; ++e) sum.v[e] += parts[w][lane][e];
-            if (mine) store_sum<T, O, BYTES>(sum, static_cast<O*>(p.out) + static_cast<size_t>(id0 + i) * p.d + at);
+                    for (int e = 0; e < S::N; ++e) sum.v[e] += parts[q][lane][e];
+                if (mine) sum.template store<O>(out + static_cast<size_t>(id) * p.d, 1.f);
+            }
+            __syncthreads();
         }
-        __syncthreads();
-    }
 }
 
 // Pairs to a tile: enough tiles to fill the chip several times over (148 SMs, 16 warps each), and no shorter than it takes to keep the
@@ -236,9 +263,9 @@ void launch_lookup_grad(const Rows& grad, Type type, size_t k, size_t d, const I
     p.k = static_cast<uint32_t>(k);
     p.d = static_cast<uint32_t>(d);
     p.out = out;
-    // the output's chunks have as many values as the input's: of the same bytes, or in fp32 up to twice 16
+    // (the output's chunks have as many values as the input's, and are stored 16 bytes at a time)
     const size_t ot = type_bytes(out_type);
-    const int bytes = access_bytes({address(grad.p), p.pitch, d * t, ot == t ? address(out) : address(out) / 2});
+    const int bytes = access_bytes({address(grad.p), p.pitch, d * t, address(out) * t / ot});
     auto launch = [&](auto value, auto result, auto width) {
         using T = decltype(value);
         using O = decltype(result);
@@ -246,9 +273,14 @@ void launch_lookup_grad(const Rows& grad, Type type, size_t k, size_t d, const I
         p.width = static_cast<uint32_t>(d * t / B);
         p.slabs = (p.width + 31) / 32;
         const size_t units = tiles * p.slabs;
-        sum_tiles_kernel<T, O, B><<<static_cast<unsigned>((units + kWarps - 1) / kWarps), 32 * kWarps, 0, stream>>>(p);
+        auto* kernel = row_scales ? sum_tiles_kernel<T, O, B, true> : sum_tiles_kernel<T, O, B, false>;
+        kernel<<<static_cast<unsigned>((units + kWarps - 1) / kWarps), 32 * kWarps, 0, stream>>>(p);
         SKM_LAUNCH_CHECK();
-        join_tiles_kernel<T, O, B><<<dim3(static_cast<unsigned>((k + kJoinWarps - 1) / kJoinWarps), p.slabs), 32 * kJoinWarps, 0, stream>>>(p);
+        // a warp takes its ids one after the other: few, as long as there are warps for them
+        p.join_ids = 1;
+        while (p.join_ids < 32 && k * p.slabs > static_cast<size_t>(p.join_ids) * 148 * 32) p.join_ids *= 2;
+        const size_t ids_of_block = static_cast<size_t>(p.join_ids) * kJoinWarps;
+        join_tiles_kernel<T, O, B><<<dim3(static_cast<unsigned>((k + ids_of_block - 1) / ids_of_block), p.slabs), 32 * kJoinWarps, 0, stream>>>(p);
         SKM_LAUNCH_CHECK();
     };
     with_width(type, bytes, [&](auto value, auto width) {
