@@ -320,7 +320,7 @@ skm_status skm_op_find_nearest_noalloc(int device, const float* x_dev, const flo
  *
  * Values of rows have one of the types below; sums and products are in fp32 and rounded once.  `ld_*` is the number of elements from
  * one row to the next; outputs are contiguous.  Cluster numbers (ids) are int32, uint32 (ids_bits 32) or int64 (64); one outside
- * [0, k) stands for no cluster.  k and the number of ids stay below 2^31. */
+ * [0, k) stands for no cluster.  k and the number of ids stay below 2^31, d is at most 2^20. */
 typedef enum skm_dtype { SKM_F32 = 0, SKM_F16 = 1, SKM_BF16 = 2 } skm_dtype;
 
 /* out[i] = scale * row_scales[i] * table[ids[i]] for i < n: table k x d, row_scales n (fp32) or NULL, out n x d.  An id that is no row of

@@ -74,7 +74,7 @@ void check_sizes(uint64_t n, uint64_t k) {
     need(n <= 0x7fffffff, "no more than 2^31 - 1 ids");
 }
 
-void check_width(uint64_t d) { need(d > 0 && d <= 0x1fffffff, "the dimensionality must be positive and below 2^29"); }
+void check_width(uint64_t d) { need(d > 0 && d <= (1u << 20), "the dimensionality must be positive and at most 2^20"); }
 
 void check_workspace(const void* workspace, uint64_t given, uint64_t needed) {
     need(given >= needed, "the workspace is too small");

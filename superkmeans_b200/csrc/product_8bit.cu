@@ -7,6 +7,7 @@
 // 32 neighbouring results of a row.
 #include <cmath>
 #include <mutex>
+#include <set>
 #include <string>
 
 #include "rows_access.cuh"
@@ -697,6 +698,18 @@ void throw_if_told(Status& s, cudaStream_t stream) {
     throw CudaError("a product in 8 bits gave up waiting on a barrier (code " + std::to_string(code) + "): its results are not valid");
 }
 
+// Lets a kernel have as much shared memory as it needs, once per kernel and device.
+template <typename... A>
+void allow_shared(void (*kernel)(A...), uint32_t bytes) {
+    static std::mutex mutex;
+    static std::set<std::pair<int, const void*>> done;
+    int device = 0;
+    SKM_CUDA(cudaGetDevice(&device));
+    std::lock_guard<std::mutex> lock(mutex);
+    if (!done.insert({device, reinterpret_cast<const void*>(kernel)}).second) return;
+    SKM_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)));
+}
+
 bool tma_takes(const void* p, size_t ld, size_t d) { return (address(p) & 15) == 0 && ld % 16 == 0 && ld >= d; }
 size_t pitch_of(size_t d) { return (d + 15) / 16 * 16; }
 size_t rounded(size_t bytes) { return (bytes + 255) / 256 * 256; }
@@ -813,7 +826,7 @@ void launch_product(const Product& p, void* workspace, cudaStream_t stream) {
         using O = decltype(result);
         const unsigned grid = 2 * static_cast<unsigned>(std::min<size_t>(all_tiles, static_cast<size_t>(sm_pairs())));
         auto go = [&](auto* kernel, uint32_t smem) {
-            SKM_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+            allow_shared(kernel, smem);
             kernel<<<grid, Q_THREADS, smem, stream>>>(maps, k);
         };
         if constexpr (COLS == 256) {
@@ -832,7 +845,7 @@ void launch_product(const Product& p, void* workspace, cudaStream_t stream) {
         constexpr int ROWS = decltype(rows)::value;
         using O = decltype(result);
         auto* kernel = product_kernel<ROWS, O>;
-        SKM_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kProductSmem<ROWS>)));
+        allow_shared(kernel, kProductSmem<ROWS>);
         cudaLaunchConfig_t config{};
         config.gridDim = dim3(static_cast<unsigned>(all_tiles * plan.split));
         config.blockDim = dim3(P_THREADS);

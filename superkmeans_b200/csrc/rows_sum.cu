@@ -211,6 +211,69 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_tiles_kernel(const SumPa
         }
 }
 
+// Few pairs and few ids: one launch, a block for an id and 32 chunks.  Each of its warps looks for the id in its part of the pairs and adds
+// the rows that it finds; their sums are added in the order of the warps.  Against sort, tiles and join (three launches, 16 us on the
+// GPU and as much on the host) 2001 pairs of 130 halves with 300 ids take 4 us.
+constexpr int kFewWarps = 8;
+constexpr uint32_t kFewSumPairs = 4096;
+
+template <typename T, typename O, int BYTES>
+__global__ void __launch_bounds__(32 * kFewWarps) sum_few_kernel(const SumParams p, const void* __restrict__ ids, bool wide) {
+    using S = Sums<T, BYTES>;
+    constexpr uint32_t MOST = kFewSumPairs / kFewWarps;   // pairs of a warp
+    __shared__ uint16_t found[kFewWarps][MOST];
+    __shared__ float parts[kFewWarps][32][S::N + 1];
+    __shared__ uint32_t counts[kFewWarps];
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, id = blockIdx.x, col = blockIdx.y * 32 + lane;
+    const bool mine = col < p.width;
+    const uint32_t share = (p.n + 32 * kFewWarps - 1) / (32 * kFewWarps) * 32, begin = min(warp * share, p.n), end = min(begin + share, p.n);
+    uint32_t count = 0;
+    constexpr int LOOK = 8;
+    for (uint32_t s = begin; s < end; s += 32 * LOOK) {
+        uint32_t v[LOOK];
+#pragma unroll
+        for (int u = 0; u < LOOK; ++u) v[u] = s + u * 32 + lane < end ? load_id(ids, wide, s + u * 32 + lane, p.k) : p.k;
+#pragma unroll
+        for (int u = 0; u < LOOK; ++u) {
+            const uint32_t same = __ballot_sync(0xffffffffu, v[u] == id);
+            if (v[u] == id) found[warp][count + __popc(same & ((1u << lane) - 1u))] = static_cast<uint16_t>(s + u * 32 + lane);
+            count += __popc(same);
+        }
+    }
+    __syncwarp();
+    S sum;
+    sum.clear();
+    const char* grad = static_cast<const char*>(p.grad) + static_cast<size_t>(mine ? col : 0) * BYTES;
+    for (uint32_t s = 0; s < count; s += kAhead) {
+        Chunk<BYTES> c[kAhead];
+        float f[kAhead];
+#pragma unroll
+        for (uint32_t u = 0; u < kAhead; ++u)
+            if (s + u < count) {
+                const uint32_t pair = found[warp][s + u];
+                c[u] = load_chunk<BYTES>(reinterpret_cast<const Chunk<BYTES>*>(grad + pair * p.pitch));
+                f[u] = p.row_scales ? p.scale * __ldg(p.row_scales + pair) : p.scale;
+            }
+#pragma unroll
+        for (uint32_t u = 0; u < kAhead; ++u)
+            if (s + u < count) sum.add(c[u], f[u]);
+    }
+    if (lane == 0) counts[warp] = count;
+    if (count != 0)
+#pragma unroll
+        for (int e = 0; e < S::N; ++e) parts[warp][lane][e] = sum.v[e];
+    __syncthreads();
+    if (warp != 0) return;
+    for (int w = 1; w < kFewWarps; ++w)
+        if (counts[w] != 0)
+#pragma unroll
+            for (int e = 0; e < S::N; ++e) sum.v[e] += parts[w][lane][e];
+    if (mine) sum.template store<O>(static_cast<O*>(p.out) + static_cast<size_t>(id) * p.d + static_cast<size_t>(col) * S::N, 1.f);
+}
+
+// (the width of an access is not known where the workspace is sized: it is taken for 16 bytes, and a few more blocks do no harm)
+bool few(size_t n, size_t k, size_t d, Type type) { return n <= kFewSumPairs && k * ((d * type_bytes(type) + 511) / 512) <= 4096; }
+
 // Pairs to a tile: enough tiles to fill the chip several times over (148 SMs, 16 warps each), and no shorter than it takes to keep the
 // partial sums' traffic below the rows'.
 uint32_t tile_pairs(size_t n, size_t slabs) {
@@ -227,6 +290,7 @@ size_t rounded(size_t bytes) { return (bytes + 255) / 256 * 256; }
 } // namespace
 
 size_t lookup_grad_workspace_bytes(size_t n, size_t k, size_t d, Type type) {
+    if (few(n, k, d, type)) return 0;
     const size_t tile = tile_pairs(n, slabs_of(d, type, 16)), tiles = (n + tile - 1) / tile;
     return rounded(n * 4) * 2 + rounded((k + 1) * 4) + rounded(tiles * 2 * d * 4) + rounded(group_workspace_bytes(n, k));
 }
@@ -245,18 +309,22 @@ void launch_lookup_grad(const Rows& grad, Type type, size_t k, size_t d, const I
         at += rounded(bytes);
         return here;
     };
-    uint32_t* order = reinterpret_cast<uint32_t*>(take(n * 4));
-    uint32_t* keys = reinterpret_cast<uint32_t*>(take(n * 4));
-    uint32_t* offsets = reinterpret_cast<uint32_t*>(take((k + 1) * 4));
-    p.tile = tile_pairs(n, slabs_of(d, type, 16));
-    const size_t tiles = (n + p.tile - 1) / p.tile;
-    p.partials = reinterpret_cast<float*>(take(tiles * 2 * d * 4));
-    launch_group(ids, n, k, order, nullptr, keys, offsets, at, stream);
+    const bool is_few = few(n, k, d, type);
+    size_t tiles = 0;
+    if (!is_few) {
+        uint32_t* order = reinterpret_cast<uint32_t*>(take(n * 4));
+        uint32_t* keys = reinterpret_cast<uint32_t*>(take(n * 4));
+        uint32_t* offsets = reinterpret_cast<uint32_t*>(take((k + 1) * 4));
+        p.tile = tile_pairs(n, slabs_of(d, type, 16));
+        tiles = (n + p.tile - 1) / p.tile;
+        p.partials = reinterpret_cast<float*>(take(tiles * 2 * d * 4));
+        launch_group(ids, n, k, order, nullptr, keys, offsets, at, stream);
+        p.order = order;
+        p.keys = keys;
+        p.offsets = offsets;
+    }
     p.grad = grad.p;
     p.pitch = grad.ld * t;
-    p.order = order;
-    p.keys = keys;
-    p.offsets = offsets;
     p.row_scales = row_scales;
     p.scale = scale;
     p.n = static_cast<uint32_t>(n);
@@ -272,6 +340,11 @@ void launch_lookup_grad(const Rows& grad, Type type, size_t k, size_t d, const I
         constexpr int B = decltype(width)::bytes;
         p.width = static_cast<uint32_t>(d * t / B);
         p.slabs = (p.width + 31) / 32;
+        if (is_few) {
+            sum_few_kernel<T, O, B><<<dim3(static_cast<unsigned>(k), p.slabs), 32 * kFewWarps, 0, stream>>>(p, ids.p, ids.wide);
+            SKM_LAUNCH_CHECK();
+            return;
+        }
         const size_t units = tiles * p.slabs;
         auto* kernel = row_scales ? sum_tiles_kernel<T, O, B, true> : sum_tiles_kernel<T, O, B, false>;
         kernel<<<static_cast<unsigned>((units + kWarps - 1) / kWarps), 32 * kWarps, 0, stream>>>(p);

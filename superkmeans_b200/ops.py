@@ -21,6 +21,11 @@ import torch
 
 from ._lib import check, lib
 
+# (looked up once: a call on a few rows takes as long as the host takes to make it)
+_op_lookup, _op_lookup_grad, _op_lookup_scale_grad = lib.skm_op_lookup, lib.skm_op_lookup_grad, lib.skm_op_lookup_scale_grad
+_op_group_rows, _op_to_clusters, _op_from_clusters = lib.skm_op_group_rows, lib.skm_op_to_clusters, lib.skm_op_from_clusters
+_op_from_clusters_grad, _op_quantize_rows, _op_product_8bit = lib.skm_op_from_clusters_grad, lib.skm_op_quantize_rows, lib.skm_op_product_8bit
+
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _ID_BITS = {torch.int32: 32, torch.uint32: 32, torch.int64: 64}
 _MOST = 2**31 - 1
@@ -52,27 +57,29 @@ def _on_gpu(t, name: str, like=None) -> None:
         raise ValueError(f"{name} must be a torch tensor")
     if not t.is_cuda:
         raise ValueError(f"{name} must be on a CUDA device")
-    if like is not None and t.device != like.device:
+    if like is not None and t.get_device() != like.get_device():
         raise ValueError(f"{name} must be on {like.device}, got {t.device}")
 
 
-def _rows(t, name: str, like=None, dtype=None) -> Tuple[torch.Tensor, int]:
-    """The rows with their values side by side, and the distance from one to the next."""
+def _rows(t, name: str, like=None, dtype=None) -> Tuple[torch.Tensor, int, int, int, int]:
+    """The rows with their values side by side, how many they are and how wide, the distance from one to the next, and their type."""
     _on_gpu(t, name, like)
-    if t.dim() != 2:
+    shape = t.shape
+    if len(shape) != 2:
         raise ValueError(f"{name} must be 2-dimensional, got {t.dim()}")
-    if t.dtype not in _DTYPES:
+    kind = _DTYPES.get(t.dtype)
+    if kind is None:
         raise ValueError(f"{name} must have dtype float32, float16 or bfloat16, got {t.dtype}")
     if dtype is not None and t.dtype != dtype:
         raise ValueError(f"{name} must have dtype {dtype}, got {t.dtype}")
-    n, d = t.shape
+    n, d = shape
     if d == 0:
         raise ValueError(f"{name} must have at least one column")
     ld, step = t.stride()
     if step != 1 and d > 1:
         t = t.contiguous()
         ld = d
-    return t, ld if n > 1 else d
+    return t, n, d, ld if n > 1 else d, kind
 
 
 def _ids(ids, name: str, like=None) -> Tuple[torch.Tensor, int]:
@@ -118,14 +125,19 @@ def _clusters(n_clusters: int) -> int:
     return n_clusters
 
 
-# A call on a few rows takes as long as the host takes to make it: the handle of a stream without the Stream around it (4 us less where
-# a call took 24), outputs from `new_empty`, no workspace where none is needed.
+# The handle of a stream without the Stream around it (2 us less where a call took 13), outputs from `new_empty`, no workspace where
+# none is needed.
 try:
     from torch._C import _cuda_getCurrentRawStream as _raw_stream
 except ImportError:   # (a torch without CUDA, or another torch)
 
     def _raw_stream(index: int) -> int:
         return torch.cuda.current_stream(index).cuda_stream
+
+
+def _check(status: int) -> None:
+    if status:
+        check(status)
 
 
 def _p(t: Optional[torch.Tensor]):
@@ -151,17 +163,14 @@ def _wants_grad(*tensors) -> bool:
 
 
 def _lookup(table, ids, scale, row_scales):
-    rows, ld = _rows(table, "table")
+    rows, k, d, ld, kind = _rows(table, "table")
     at, bits = _ids(ids, "ids", table)
-    k, d = rows.shape
     _clusters(k)
     if row_scales is not None:
         row_scales = _floats(row_scales, "row_scales", ids.shape, table)
     out = rows.new_empty((*at.shape, d))
-    index = rows.device.index
-    status = lib.skm_op_lookup(index, rows.data_ptr(), ld, _DTYPES[rows.dtype], k, d, at.data_ptr(), bits, at.numel(), scale, _p(row_scales), out.data_ptr(), _raw_stream(index))
-    if status:
-        check(status)
+    index = rows.get_device()
+    _check(_op_lookup(index, rows.data_ptr(), ld, kind, k, d, at.data_ptr(), bits, at.numel(), scale, _p(row_scales), out.data_ptr(), _raw_stream(index)))
     return out
 
 
@@ -201,40 +210,39 @@ def lookup_grad(grad: torch.Tensor, ids: torch.Tensor, n_rows: int, scale: float
                 dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """Gradient of a table of `n_rows` rows: row c is the sum of scale * row_scales[i] * grad[i] over ids[i] = c, zeros where there is no such
     i.  Summed in fp32 in an order that depends on the ids alone, and rounded once to `dtype` (that of `grad`, or float32)."""
-    rows, ld = _rows(grad, "grad")
+    rows, n, d, ld, kind = _rows(grad, "grad")
     at, bits = _ids(ids, "ids", grad)
-    n, d = rows.shape
-    if at.numel() != n or at.dim() != 1:
+    if at.shape != (n,):
         raise ValueError(f"ids must have shape ({n},), got {tuple(at.shape)}")
     k = _clusters(n_rows)
-    dtype = grad.dtype if dtype is None else dtype
-    if dtype not in (grad.dtype, torch.float32):
-        raise ValueError(f"dtype must be {grad.dtype} or float32, got {dtype}")
     if row_scales is not None:
         row_scales = _floats(row_scales, "row_scales", ids.shape, grad)
-    kind = _DTYPES[grad.dtype]
-    out = rows.new_empty((k, d), dtype=dtype)
+    if dtype is None or dtype == rows.dtype:
+        out, out_kind = rows.new_empty((k, d)), kind
+    elif dtype == torch.float32:
+        out, out_kind = rows.new_empty((k, d), dtype=dtype), 0
+    else:
+        raise ValueError(f"dtype must be {grad.dtype} or float32, got {dtype}")
     space, address, size = _workspace(lib.skm_op_lookup_grad_workspace(n, k, d, kind), rows)
-    index = rows.device.index
-    check(lib.skm_op_lookup_grad(index, rows.data_ptr(), ld, kind, k, d, at.data_ptr(), bits, n, float(scale), _p(row_scales), out.data_ptr(), _DTYPES[dtype], address, size,
-                                 _raw_stream(index)))
+    index = rows.get_device()
+    _check(_op_lookup_grad(index, rows.data_ptr(), ld, kind, k, d, at.data_ptr(), bits, n, float(scale), _p(row_scales), out.data_ptr(), out_kind, address, size,
+                               _raw_stream(index)))
     return out
 
 
 def lookup_scale_grad(grad: torch.Tensor, table: torch.Tensor, ids: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
     """Gradient of the row scales of a lookup, float32: scale * <grad[i], table[ids[i]]>, zero where the id is no row of the table."""
-    rows, ld = _rows(grad, "grad")
-    t, ld_t = _rows(table, "table", grad, grad.dtype)
+    rows, n, d, ld, kind = _rows(grad, "grad")
+    t, k, d_t, ld_t, _ = _rows(table, "table", grad, grad.dtype)
     at, bits = _ids(ids, "ids", grad)
-    n, d = rows.shape
-    if t.shape[1] != d:
-        raise ValueError(f"grad and table must have the same dimensionality, got {d} and {t.shape[1]}")
-    if at.numel() != n or at.dim() != 1:
+    if d_t != d:
+        raise ValueError(f"grad and table must have the same dimensionality, got {d} and {d_t}")
+    if at.shape != (n,):
         raise ValueError(f"ids must have shape ({n},), got {tuple(at.shape)}")
-    k = _clusters(t.shape[0])
+    _clusters(k)
     out = rows.new_empty(n, dtype=torch.float32)
-    index = rows.device.index
-    check(lib.skm_op_lookup_scale_grad(index, rows.data_ptr(), ld, t.data_ptr(), ld_t, _DTYPES[rows.dtype], k, d, at.data_ptr(), bits, n, float(scale), out.data_ptr(),
+    index = rows.get_device()
+    _check(_op_lookup_scale_grad(index, rows.data_ptr(), ld, t.data_ptr(), ld_t, kind, k, d, at.data_ptr(), bits, n, float(scale), out.data_ptr(),
                                        _raw_stream(index)))
     return out
 
@@ -252,55 +260,52 @@ def group_rows(ids: torch.Tensor, n_clusters: int) -> RowGroups:
     whole = at.new_empty(2 * n + k + 1, dtype=torch.int32)
     order, position, offsets = whole.split((n, n, k + 1))
     space, address, size = _workspace(lib.skm_op_group_rows_workspace(n, k), at)
-    index = at.device.index
+    index = at.get_device()
     first = whole.data_ptr()
-    check(lib.skm_op_group_rows(index, at.data_ptr(), bits, n, k, first, first + 4 * n, first + 8 * n, address, size, _raw_stream(index)))
+    _check(_op_group_rows(index, at.data_ptr(), bits, n, k, first, first + 4 * n, first + 8 * n, address, size, _raw_stream(index)))
     return RowGroups(order, position if at.dim() == 1 else position.view(at.shape), offsets)
 
 
 def _to_clusters(x, groups):
-    rows, ld = _rows(x, "x")
+    rows, n_x, d, ld, kind = _rows(x, "x")
     position, offsets, k, n, m = _groups(groups, x)
-    if rows.shape[0] != n:
-        raise ValueError(f"x must have {n} rows, got {rows.shape[0]}")
-    d = rows.shape[1]
+    if n_x != n:
+        raise ValueError(f"x must have {n} rows, got {n_x}")
     out = rows.new_empty((n * m, d))
-    index = rows.device.index
-    check(lib.skm_op_to_clusters(index, rows.data_ptr(), ld, _DTYPES[rows.dtype], d, position.data_ptr(), offsets.data_ptr(), k, n, m, out.data_ptr(), _raw_stream(index)))
+    index = rows.get_device()
+    _check(_op_to_clusters(index, rows.data_ptr(), ld, kind, d, position.data_ptr(), offsets.data_ptr(), k, n, m, out.data_ptr(), _raw_stream(index)))
     return out
 
 
 def _from_clusters(y, groups, weights, name="y"):
-    rows, ld = _rows(y, name)
+    rows, n_y, d, ld, kind = _rows(y, name)
     position, offsets, k, n, m = _groups(groups, y)
-    if rows.shape[0] != n * m:
-        raise ValueError(f"{name} must have {n * m} rows, got {rows.shape[0]}")
+    if n_y != n * m:
+        raise ValueError(f"{name} must have {n * m} rows, got {n_y}")
     if weights is not None:
         weights = _floats(weights, "weights", position.shape, y)
-    d = rows.shape[1]
     out = rows.new_empty((n, d))
-    index = rows.device.index
-    check(lib.skm_op_from_clusters(index, rows.data_ptr(), ld, _DTYPES[rows.dtype], d, position.data_ptr(), offsets.data_ptr(), k, n, m, _p(weights), out.data_ptr(), _raw_stream(index)))
+    index = rows.get_device()
+    _check(_op_from_clusters(index, rows.data_ptr(), ld, kind, d, position.data_ptr(), offsets.data_ptr(), k, n, m, _p(weights), out.data_ptr(), _raw_stream(index)))
     return out
 
 
 def _from_clusters_grad(grad, y, groups, weights, want_y, want_weights):
-    rows, ld = _rows(grad, "grad")
+    rows, n_grad, d, ld, kind = _rows(grad, "grad")
     position, offsets, k, n, m = _groups(groups, grad)
-    d = rows.shape[1]
-    if rows.shape[0] != n:
-        raise ValueError(f"grad must have {n} rows, got {rows.shape[0]}")
+    if n_grad != n:
+        raise ValueError(f"grad must have {n} rows, got {n_grad}")
     if weights is not None:
         weights = _floats(weights, "weights", position.shape, grad)
     from_y, ld_y = None, 0
     if want_weights:
-        from_y, ld_y = _rows(y, "y", grad, grad.dtype)
-        if tuple(from_y.shape) != (n * m, d):
-            raise ValueError(f"y must have shape {(n * m, d)}, got {tuple(from_y.shape)}")
+        from_y, n_y, d_y, ld_y, _ = _rows(y, "y", grad, grad.dtype)
+        if (n_y, d_y) != (n * m, d):
+            raise ValueError(f"y must have shape {(n * m, d)}, got {(n_y, d_y)}")
     grad_y = rows.new_empty((n * m, d)) if want_y else None
     grad_weights = rows.new_empty(position.shape, dtype=torch.float32) if want_weights else None
-    index = rows.device.index
-    check(lib.skm_op_from_clusters_grad(index, rows.data_ptr(), ld, _p(from_y), ld_y, _DTYPES[rows.dtype], d, position.data_ptr(), offsets.data_ptr(), k, n, m, _p(weights), _p(grad_y),
+    index = rows.get_device()
+    _check(_op_from_clusters_grad(index, rows.data_ptr(), ld, _p(from_y), ld_y, kind, d, position.data_ptr(), offsets.data_ptr(), k, n, m, _p(weights), _p(grad_y),
                                         _p(grad_weights), _raw_stream(index)))
     return grad_y, grad_weights
 
@@ -368,15 +373,14 @@ def from_clusters_grad(grad: torch.Tensor, y: torch.Tensor, groups: RowGroups, w
 def quantize_rows(x: torch.Tensor) -> QuantizedRows:
     """Rows in 8 bits: scales[i] = max |x[i]| / 127 (float32), values[i] = x[i] / scales[i] rounded to the nearest whole number, int8.  A row of
     zeros has scale 0; a row with a value that is no finite number has scale NaN.  The rows of the result begin on 16 bytes."""
-    rows, ld = _rows(x, "x")
-    n, d = rows.shape
+    rows, n, d, ld, kind = _rows(x, "x")
     if n > _MOST:
         raise ValueError("x must have no more than 2**31 - 1 rows")
     pitch = (d + 15) // 16 * 16
     q = rows.new_empty((n, pitch), dtype=torch.int8)
     scales = rows.new_empty(n, dtype=torch.float32)
-    index = rows.device.index
-    check(lib.skm_op_quantize_rows(index, rows.data_ptr(), ld, _DTYPES[rows.dtype], n, d, q.data_ptr(), pitch, scales.data_ptr(), _raw_stream(index)))
+    index = rows.get_device()
+    _check(_op_quantize_rows(index, rows.data_ptr(), ld, kind, n, d, q.data_ptr(), pitch, scales.data_ptr(), _raw_stream(index)))
     return QuantizedRows(q[:, :d] if pitch != d else q, scales)
 
 
@@ -425,8 +429,8 @@ def product_8bit(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_sca
     out = x_scales.new_empty((n, m), dtype=dtype)
     x_at, w_at = x.data_ptr(), w.data_ptr()
     space, address, size = _workspace(lib.skm_op_product_8bit_workspace(x_at, ld_x, w_at, ld_w, n, m, d, e), x)
-    index = x.device.index
-    check(lib.skm_op_product_8bit(index, x_at, ld_x, x_scales.data_ptr(), w_at, ld_w, w_scales.data_ptr(), n, m, d, e, _p(offsets), out.data_ptr(), _DTYPES[dtype], address, size,
+    index = x.get_device()
+    _check(_op_product_8bit(index, x_at, ld_x, x_scales.data_ptr(), w_at, ld_w, w_scales.data_ptr(), n, m, d, e, _p(offsets), out.data_ptr(), _DTYPES[dtype], address, size,
                                   _raw_stream(index)))
     return out
 

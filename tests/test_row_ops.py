@@ -38,6 +38,7 @@ def test_lookup_refusals():
     refused(call(k=0), "clusters")
     refused(call(k=2**31), "clusters")
     refused(call(d=0), "dimensionality")
+    refused(call(d=2**20 + 1), "dimensionality")
     refused(call(dtype=3), "dtype")
     refused(call(bits=16), "ids_bits")
     refused(call(n=2**31), "2^31")
@@ -48,10 +49,11 @@ def test_lookup_refusals():
 
 
 def test_lookup_grad_refusals():
-    need = lib.skm_op_lookup_grad_workspace(100, 10, 8, 2)
+    need = lib.skm_op_lookup_grad_workspace(5000, 10, 8, 2)
+    assert lib.skm_op_lookup_grad_workspace(100, 10, 8, 2) == 0   # (few pairs need none)
 
     def call(dtype=2, out_dtype=2, grad=AT, out=AT, workspace=AT, size=need, k=10):
-        return lib.skm_op_lookup_grad(-1, grad, 8, dtype, k, 8, AT, 32, 100, 1.0, None, out, out_dtype, workspace, size, None)
+        return lib.skm_op_lookup_grad(-1, grad, 8, dtype, k, 8, AT, 32, 5000, 1.0, None, out, out_dtype, workspace, size, None)
 
     refused(call(out_dtype=1), "fp32")
     refused(call(dtype=0, out_dtype=2), "fp32")
@@ -127,7 +129,7 @@ def test_workspaces_grow_with_what_they_hold():
     assert lib.skm_op_product_8bit_workspace(AT, 16, AT, 18, 5, 7, 17, 3) >= 3 * 7 * 32
     small, large = (lib.skm_op_group_rows_workspace(n, 100) for n in (5_000, 5_000_000))
     assert 0 < small < large
-    assert lib.skm_op_lookup_grad_workspace(1000, 10, 64, 0) >= 1000 * 8 + 11 * 4
+    assert lib.skm_op_lookup_grad_workspace(10_000, 10, 64, 0) >= 10_000 * 8 + 11 * 4
 
 
 def test_signatures_take_64_bit_sizes():
