@@ -23,65 +23,97 @@ namespace {
 
 // ---------------------------------------------------------------------------------------------- rows to 8 bits
 
-// LANES threads to a row, of which each keeps HELD chunks in registers between finding the largest value and dividing by it; rows that
-// are longer are read twice.
+// LANES threads to a row, of which each keeps HELD chunks in registers between finding the largest value and dividing by it (the rest of
+// longer rows is read twice), while the next row's are on their way: as many blocks as are resident, in turn over the rows.
+// Rounding is an addition to 1.5 * 2^23, which leaves the whole number in the low bits (its low byte is q).
 template <typename T, int BYTES, int LANES, int HELD>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(const void* __restrict__ x, size_t pitch, size_t n, uint32_t width, int8_t* __restrict__ q, size_t ldq,
                                                             float* __restrict__ scales) {
     using V = Values<T, BYTES>;
-    const size_t row = static_cast<size_t>(blockIdx.x) * (256 / LANES) + threadIdx.x / LANES;
+    const size_t step = static_cast<size_t>(gridDim.x) * (256 / LANES);
     const uint32_t lane = threadIdx.x % LANES;
-    const bool valid = row < n;
-    const Chunk<BYTES>* from = reinterpret_cast<const Chunk<BYTES>*>(static_cast<const char*>(x) + (valid ? row : 0) * pitch);
+    auto chunks_of = [&](size_t row) { return reinterpret_cast<const Chunk<BYTES>*>(static_cast<const char*>(x) + row * pitch); };
     Chunk<BYTES> held[HELD];
+    auto fetch = [&](size_t row) {
+        const Chunk<BYTES>* from = chunks_of(row < n ? row : 0);   // (behind the last row: the first, for nothing)
 #pragma unroll
-    for (int h = 0; h < HELD; ++h) held[h] = valid && lane + h * LANES < width ? __ldg(from + lane + h * LANES) : zero_chunk<BYTES>();
-    // magnitudes as whole numbers: a NaN is above infinity
-    uint32_t most = 0;
-    auto look = [&](const Chunk<BYTES>& c) {
-        V v;
-        v.from(c);
-#pragma unroll
-        for (int i = 0; i < V::N; ++i) most = max(most, __float_as_uint(v.v[i]) & 0x7fffffffu);
+        for (int h = 0; h < HELD; ++h) held[h] = lane + h * LANES < width ? __ldg(from + lane + h * LANES) : zero_chunk<BYTES>();
     };
+    size_t row = static_cast<size_t>(blockIdx.x) * (256 / LANES) + threadIdx.x / LANES;
+    fetch(row);
+    // (whole blocks, and with them the warps of the shuffles, take the same number of turns)
+    for (size_t turn = static_cast<size_t>(blockIdx.x) * (256 / LANES); turn < n; turn += step, row += step) {
+        V v[HELD];
 #pragma unroll
-    for (int h = 0; h < HELD; ++h) look(held[h]);
-    if (valid)
-        for (uint32_t c = lane + HELD * LANES; c < width; c += LANES) look(__ldg(from + c));
+        for (int h = 0; h < HELD; ++h) v[h].from(held[h]);
+        fetch(row + step);
+        const bool valid = row < n;
+        const Chunk<BYTES>* from = chunks_of(valid ? row : 0);
+        // magnitudes as whole numbers: a NaN is above infinity
+        uint32_t most = 0;
+        auto look = [&](const V& w) {
 #pragma unroll
-    for (int o = (LANES < 32 ? LANES : 32) / 2; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
-    if constexpr (LANES > 32) {
-        __shared__ uint32_t of_warp[8];
-        if ((threadIdx.x & 31) == 0) of_warp[threadIdx.x >> 5] = most;
-        __syncthreads();
+            for (int i = 0; i < V::N; ++i) most = max(most, __float_as_uint(w.v[i]) & 0x7fffffffu);
+        };
 #pragma unroll
-        for (int w = 0; w < 8; ++w) most = max(most, of_warp[w]);
-    }
-    if (!valid) return;
-    const bool finite = most < 0x7f800000u, some = finite && most != 0;
-    const float largest = __uint_as_float(most);
-    // 127 / largest is a float for all but the smallest, which are taken 2^100 times as large
-    const float up = largest < 0x1p-100f ? 0x1p100f : 1.0f;
-    const float inverse = some ? __fdiv_rn(127.0f, largest * up) : 0.0f;
-    if (lane == 0) scales[row] = finite ? __fdiv_rn(largest, 127.0f) : __uint_as_float(0x7fc00000u);
-    int8_t* to = q + row * ldq;
-    auto put = [&](const Chunk<BYTES>& c, uint32_t at) {
-        V v;
-        v.from(c);
-        int8_t b[V::N];
-#pragma unroll
-        for (int i = 0; i < V::N; ++i) b[i] = some ? static_cast<int8_t>(__float2int_rn(__fmul_rn(v.v[i] * up, inverse))) : int8_t{0};
-        if constexpr (V::N == 1) to[at] = b[0];
-        else {
-            Chunk<V::N> packed;
-            memcpy(&packed, b, V::N);
-            *reinterpret_cast<Chunk<V::N>*>(to + at * V::N) = packed;
+        for (int h = 0; h < HELD; ++h) look(v[h]);
+        for (uint32_t c = lane + HELD * LANES; c < width; c += LANES) {
+            V w;
+            w.from(__ldg(from + c));
+            look(w);
         }
-    };
 #pragma unroll
-    for (int h = 0; h < HELD; ++h)
-        if (lane + h * LANES < width) put(held[h], lane + h * LANES);
-    for (uint32_t c = lane + HELD * LANES; c < width; c += LANES) put(__ldg(from + c), c);
+        for (int o = (LANES < 32 ? LANES : 32) / 2; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+        if constexpr (LANES > 32) {
+            __shared__ uint32_t of_warp[8];
+            __syncthreads();   // (the turn before has read them)
+            if ((threadIdx.x & 31) == 0) of_warp[threadIdx.x >> 5] = most;
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < 8; ++w) most = max(most, of_warp[w]);
+        }
+        if (!valid) continue;
+        const bool finite = most < 0x7f800000u, some = finite && most != 0;
+        const float largest = __uint_as_float(most);
+        // 127 / largest is a float for all but the smallest, which are taken 2^100 times as large
+        const float up = largest < 0x1p-100f ? 0x1p100f : 1.0f;
+        const float inverse = some ? __fdiv_rn(127.0f, largest * up) : 0.0f;
+        if (lane == 0) scales[row] = finite ? __fdiv_rn(largest, 127.0f) : __uint_as_float(0x7fc00000u);
+        int8_t* to = q + row * ldq;
+        constexpr float kWhole = 12582912.0f;
+        // (the product is rounded before the sum: as one operation on pairs, mul2 and add2, it was not, and values at a half went the other way)
+        auto whole_of = [&](float w) { return __float_as_uint(__fadd_rn(__fmul_rn(w, inverse), kWhole)); };
+        auto put = [&](V w, uint32_t at) {
+            if (up != 1.0f || !some) {
+#pragma unroll
+                for (int i = 0; i < V::N; ++i) w.v[i] = some ? w.v[i] * up : 0.0f;   // (no number times zero is none)
+            }
+            if constexpr (V::N == 1) {
+                to[at] = static_cast<int8_t>(whole_of(w.v[0]));
+            } else {
+                uint32_t b[V::N];
+#pragma unroll
+                for (int i = 0; i < V::N; ++i) b[i] = whole_of(w.v[i]);
+                Chunk<V::N> packed;
+                if constexpr (V::N == 2) packed = static_cast<uint16_t>(__byte_perm(b[0], b[1], 0x0040));
+                else {
+                    uint32_t words[V::N / 4];
+#pragma unroll
+                    for (int i = 0; i < V::N / 4; ++i) words[i] = __byte_perm(__byte_perm(b[4 * i], b[4 * i + 1], 0x0040), __byte_perm(b[4 * i + 2], b[4 * i + 3], 0x0040), 0x5410);
+                    memcpy(&packed, words, V::N);
+                }
+                *reinterpret_cast<Chunk<V::N>*>(to + at * V::N) = packed;
+            }
+        };
+#pragma unroll
+        for (int h = 0; h < HELD; ++h)
+            if (lane + h * LANES < width) put(v[h], lane + h * LANES);
+        for (uint32_t c = lane + HELD * LANES; c < width; c += LANES) {
+            V w;
+            w.from(__ldg(from + c));
+            put(w, c);
+        }
+    }
 }
 
 // Rows with a pitch that TMA takes (zeros behind d).
@@ -145,166 +177,6 @@ constexpr uint32_t kProductSmem = P_STAGES * kStageBytes<ROWS> + sizeof(ProductC
 __device__ __forceinline__ void store_result(float* p, float v) { *p = v; }
 __device__ __forceinline__ void store_result(__half* p, float v) { *p = __float2half_rn(v); }
 __device__ __forceinline__ void store_result(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
-
-// One tile of 128 channels x ROWS rows per cluster; the CTAs of a cluster share the depth and add their sums at the end, each for its
-// part of the rows, out of one another's shared memory.
-template <int ROWS, typename O>
-__global__ void __launch_bounds__(P_THREADS) product_kernel(const __grid_constant__ ProductMaps maps, const ProductParams p) {
-    extern __shared__ uint8_t smem_raw[];
-    const uint32_t raw_addr = smem_u32(smem_raw);
-    const uint32_t pad = (1024u - (raw_addr & 1023u)) & 1023u;
-    uint8_t* smem = smem_raw + pad;
-    const uint32_t smem_base = raw_addr + pad;
-    auto* ctrl = reinterpret_cast<ProductControl<ROWS>*>(smem + P_STAGES * kStageBytes<ROWS>);
-    constexpr uint32_t COLS = ROWS < 32 ? 32 : ROWS;
-    const WaitCtx wctx{p.error, p.wait_limit};
-    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t split = cluster_size(), rank = cluster_rank();
-
-    const uint32_t tile = blockIdx.x / split, channel_tile = tile % p.channel_tiles, row_tile = tile / p.channel_tiles;
-    RowTile t;
-    if (p.groups) {
-        if (row_tile >= __ldg(p.n_tiles + 1)) return;   // (the whole cluster)
-        t = p.tiles[row_tile];
-    } else {
-        t = {row_tile * ROWS, min(row_tile * ROWS + ROWS, p.n), 0};
-    }
-    const uint32_t channel = channel_tile * P_CHANNELS + threadIdx.x;
-    O* out = static_cast<O*>(p.out);
-    if (p.groups && t.group >= p.groups) {   // rows of no group
-        if (rank == 0 && channel < p.m)
-            for (uint32_t r = t.row0; r < t.row1; ++r) store_result(out + static_cast<size_t>(r) * p.m + channel, 0.f);
-        return;
-    }
-
-    if (threadIdx.x == 0) {
-        for (int s = 0; s < P_STAGES; ++s) {
-            mbar_init(&ctrl->full[s], 1);
-            mbar_init(&ctrl->empty[s], 1);
-        }
-        mbar_init(&ctrl->done, 1);
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        fence_proxy_async();
-    }
-    if (warp == 0) tmem_alloc(&ctrl->tmem_base, COLS);
-    for (uint32_t r = threadIdx.x; r < ROWS; r += P_THREADS) ctrl->x_scales[r] = t.row0 + r < t.row1 ? __ldg(p.x_scales + t.row0 + r) : 0.f;
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    const uint32_t tmem_base = ctrl->tmem_base;
-    const uint32_t k0 = p.depth_blocks * rank / split, k1 = p.depth_blocks * (rank + 1) / split;
-
-    bool ok = true;
-    if (threadIdx.x == 0) {
-        const int w_row = static_cast<int>(t.group * p.m + channel_tile * P_CHANNELS), x_row = static_cast<int>(t.row0);
-        for (uint32_t k = k0, it = 0; k < k1; ++k, ++it) {
-            const uint32_t s = it % P_STAGES, ph = (it / P_STAGES) & 1u;
-            if ((p.producer_stop != 0 && it >= p.producer_stop) || !mbar_wait(&ctrl->empty[s], ph ^ 1u, wctx, 41)) {
-                ok = false;
-                break;
-            }
-            const uint32_t st = smem_base + s * kStageBytes<ROWS>;
-            mbar_arrive_expect_tx(&ctrl->full[s], kStageBytes<ROWS>);
-            tma_load_2d(st, &maps.w, &ctrl->full[s], static_cast<int>(k * P_DEPTH), w_row);
-            tma_load_2d(st + P_W_BYTES, &maps.x, &ctrl->full[s], static_cast<int>(k * P_DEPTH), x_row);
-        }
-    } else if (threadIdx.x == 32) {
-        constexpr uint32_t idesc = make_idesc_i8(P_CHANNELS, ROWS);
-        for (uint32_t k = k0, it = 0; k < k1; ++k, ++it) {
-            const uint32_t s = it % P_STAGES, ph = (it / P_STAGES) & 1u;
-            if (!mbar_wait(&ctrl->full[s], ph, wctx, 42)) {
-                ok = false;
-                break;
-            }
-            tc_fence_after();
-            const uint32_t st = smem_base + s * kStageBytes<ROWS>;
-#pragma unroll
-            for (uint32_t kk = 0; kk < P_DEPTH / 32; ++kk) umma_i8(tmem_base, make_desc_128(st + kk * 32), make_desc_128(st + P_W_BYTES + kk * 32), it != 0 || kk != 0 ? 1u : 0u, idesc);
-            umma_commit(&ctrl->empty[s]);
-        }
-        if (ok) umma_commit(&ctrl->done);
-    }
-    __syncwarp();
-    const bool summed = __all_sync(0xffffffffu, mbar_wait(&ctrl->done, 0, wctx, 43));
-    if (!summed && lane == 0) *reinterpret_cast<volatile int*>(p.told) = 43;
-    if (!ok) {
-        // a millisecond for the copies that are in flight before the block's memory is let go
-        const long long t0 = clock64();
-        while (clock64() - t0 < 2000000) {
-        }
-    }
-    __syncwarp();
-    tc_fence_after();
-
-    const bool has_channel = channel < p.m;
-    const float w_scale = has_channel ? __ldg(p.w_scales + static_cast<size_t>(t.group) * p.m + channel) : 0.f;
-    const uint32_t taddr = tmem_base + (warp * 32 << 16);
-    auto put = [&](uint32_t r, int sum) {
-        if (t.row0 + r < t.row1 && has_channel)
-            store_result(out + static_cast<size_t>(t.row0 + r) * p.m + channel, __int2float_rn(sum) * ctrl->x_scales[r] * w_scale);
-    };
-    if (split == 1) {
-        if (summed)
-#pragma unroll 1
-            for (uint32_t c = 0; c < ROWS; c += 16) {
-                uint32_t r[16];
-                tmem_ld16(taddr + c, r);
-#pragma unroll
-                for (uint32_t j = 0; j < 16; ++j) put(c + j, static_cast<int>(r[j]));
-            }
-    } else {
-        // sums of all rows into this CTA's shared memory (the stages are through), 128 channels to a row
-        int* sums = reinterpret_cast<int*>(smem);
-        if (summed)
-#pragma unroll 1
-            for (uint32_t c = 0; c < ROWS; c += 16) {
-                uint32_t r[16];
-                tmem_ld16(taddr + c, r);
-#pragma unroll
-                for (uint32_t j = 0; j < 16; ++j) sums[(c + j) * P_CHANNELS + threadIdx.x] = static_cast<int>(r[j]);
-            }
-        cluster_sync();
-        const uint32_t share = ROWS / split;
-        if (summed)
-            for (uint32_t r = rank * share; r < (rank + 1) * share; ++r) {
-                int sum = 0;
-                for (uint32_t q = 0; q < split; ++q) sum += load_cluster(cluster_address(sums + r * P_CHANNELS + threadIdx.x, q));
-                put(r, sum);
-            }
-        cluster_sync();   // nobody reads this CTA's sums any more
-    }
-    tc_fence_before();
-    __syncthreads();
-    if (warp == 0) tmem_dealloc(tmem_base, COLS);
-}
-
-// ---- many rows: persistent pairs of CTAs on tiles of 256 lanes x COLS columns, each CTA with its 128 lanes, half of the columns as operand
-// and all of them in its accumulator:
-//   warp 0       TMA producer
-//   warp 1       MMA issuer (the leader's)
-//   warps 4-11   epilogue: 32 lanes and half of the columns each, out of one accumulator while the other is filled
-// Where rows of the result begin on 32 bytes, the lanes are rows of x: a thread then holds 128 neighbouring results of a row and stores
-// 32 bytes at a time.  Elsewhere, and where the tile is narrow because the groups are small, the lanes are channels, and the 32 lanes of
-// a warp store 32 neighbouring results of a row.
-constexpr int Q_EPI_WARPS = 8;
-constexpr int Q_THREADS = 128 + 32 * Q_EPI_WARPS;
-constexpr uint32_t Q_TRAY_BYTES = 32 * 128;   // 32 rows of results on their way out, of each epilogue warp
-template <bool LANES_ARE_ROWS>
-constexpr int kPairStages = LANES_ARE_ROWS ? 5 : 6;
-
-template <int COLS>
-struct PairControl {
-    uint64_t full[6];            // (the leader's are used)
-    uint64_t empty[6];
-    uint64_t acc_full[2];
-    uint64_t acc_empty[2];       // (the leader's are used)
-    uint32_t tmem_base;
-    alignas(16) float scales[Q_EPI_WARPS][COLS / 2];   // of a warp's columns
-};
-template <int COLS>
-constexpr uint32_t kPairStageBytes = P_W_BYTES + COLS / 2 * P_DEPTH;
-template <int COLS, bool LANES_ARE_ROWS>
-constexpr uint32_t kPairSmem = kPairStages<LANES_ARE_ROWS> * kPairStageBytes<COLS> + (LANES_ARE_ROWS ? Q_EPI_WARPS * Q_TRAY_BYTES : 0) + sizeof(PairControl<COLS>) + 1024;
 
 __device__ __forceinline__ float low_of(uint64_t p) { return __uint_as_float(static_cast<uint32_t>(p)); }
 __device__ __forceinline__ float high_of(uint64_t p) { return __uint_as_float(static_cast<uint32_t>(p >> 32)); }
@@ -397,6 +269,182 @@ __device__ __forceinline__ void store_across_rows(O* out, uint32_t m, uint32_t c
     else all(std::false_type{});
 }
 
+// One tile of 128 channels x ROWS rows per cluster; the CTAs of a cluster share the depth and add their sums at the end, each for its
+// part of the rows, out of one another's shared memory.
+template <int ROWS, typename O>
+__global__ void __launch_bounds__(P_THREADS) product_kernel(const __grid_constant__ ProductMaps maps, const ProductParams p) {
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t raw_addr = smem_u32(smem_raw);
+    const uint32_t pad = (1024u - (raw_addr & 1023u)) & 1023u;
+    uint8_t* smem = smem_raw + pad;
+    const uint32_t smem_base = raw_addr + pad;
+    auto* ctrl = reinterpret_cast<ProductControl<ROWS>*>(smem + P_STAGES * kStageBytes<ROWS>);
+    constexpr uint32_t COLS = ROWS < 32 ? 32 : ROWS;
+    const WaitCtx wctx{p.error, p.wait_limit};
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t split = cluster_size(), rank = cluster_rank();
+
+    const uint32_t tile = blockIdx.x / split, channel_tile = tile % p.channel_tiles, row_tile = tile / p.channel_tiles;
+    RowTile t;
+    if (p.groups) {
+        if (row_tile >= __ldg(p.n_tiles + 1)) return;   // (the whole cluster)
+        t = p.tiles[row_tile];
+    } else {
+        t = {row_tile * ROWS, min(row_tile * ROWS + ROWS, p.n), 0};
+    }
+    const uint32_t channel = channel_tile * P_CHANNELS + threadIdx.x;
+    O* out = static_cast<O*>(p.out);
+    if (p.groups && t.group >= p.groups) {   // rows of no group
+        if (rank == 0 && channel < p.m)
+            for (uint32_t r = t.row0; r < t.row1; ++r) store_result(out + static_cast<size_t>(r) * p.m + channel, 0.f);
+        return;
+    }
+
+    if (threadIdx.x == 0) {
+        tma_prefetch_map(&maps.w);
+        tma_prefetch_map(&maps.x);
+        for (int s = 0; s < P_STAGES; ++s) {
+            mbar_init(&ctrl->full[s], 1);
+            mbar_init(&ctrl->empty[s], 1);
+        }
+        mbar_init(&ctrl->done, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        fence_proxy_async();
+    }
+    if (warp == 0) tmem_alloc(&ctrl->tmem_base, COLS);
+    for (uint32_t r = threadIdx.x; r < ROWS; r += P_THREADS) ctrl->x_scales[r] = t.row0 + r < t.row1 ? __ldg(p.x_scales + t.row0 + r) : 0.f;
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = ctrl->tmem_base;
+    const uint32_t k0 = p.depth_blocks * rank / split, k1 = p.depth_blocks * (rank + 1) / split;
+
+    bool ok = true;
+    if (threadIdx.x == 0) {
+        const int w_row = static_cast<int>(t.group * p.m + channel_tile * P_CHANNELS), x_row = static_cast<int>(t.row0);
+        for (uint32_t k = k0, it = 0; k < k1; ++k, ++it) {
+            const uint32_t s = it % P_STAGES, ph = (it / P_STAGES) & 1u;
+            if ((p.producer_stop != 0 && it >= p.producer_stop) || !mbar_wait(&ctrl->empty[s], ph ^ 1u, wctx, 41)) {
+                ok = false;
+                break;
+            }
+            const uint32_t st = smem_base + s * kStageBytes<ROWS>;
+            mbar_arrive_expect_tx(&ctrl->full[s], kStageBytes<ROWS>);
+            tma_load_2d(st, &maps.w, &ctrl->full[s], static_cast<int>(k * P_DEPTH), w_row);
+            tma_load_2d(st + P_W_BYTES, &maps.x, &ctrl->full[s], static_cast<int>(k * P_DEPTH), x_row);
+        }
+    } else if (threadIdx.x == 32) {
+        constexpr uint32_t idesc = make_idesc_i8(P_CHANNELS, ROWS);
+        for (uint32_t k = k0, it = 0; k < k1; ++k, ++it) {
+            const uint32_t s = it % P_STAGES, ph = (it / P_STAGES) & 1u;
+            if (!mbar_wait(&ctrl->full[s], ph, wctx, 42)) {
+                ok = false;
+                break;
+            }
+            tc_fence_after();
+            const uint32_t st = smem_base + s * kStageBytes<ROWS>;
+#pragma unroll
+            for (uint32_t kk = 0; kk < P_DEPTH / 32; ++kk) umma_i8(tmem_base, make_desc_128(st + kk * 32), make_desc_128(st + P_W_BYTES + kk * 32), it != 0 || kk != 0 ? 1u : 0u, idesc);
+            umma_commit(&ctrl->empty[s]);
+        }
+        if (ok) umma_commit(&ctrl->done);
+    }
+    __syncwarp();
+    const bool summed = __all_sync(0xffffffffu, mbar_wait(&ctrl->done, 0, wctx, 43));
+    if (!summed && lane == 0) *reinterpret_cast<volatile int*>(p.told) = 43;
+    if (!ok) {
+        // a millisecond for the copies that are in flight before the block's memory is let go
+        const long long t0 = clock64();
+        while (clock64() - t0 < 2000000) {
+        }
+    }
+    __syncwarp();
+    tc_fence_after();
+
+    const bool has_channel = channel < p.m;
+    const float w_scale = has_channel ? __ldg(p.w_scales + static_cast<size_t>(t.group) * p.m + channel) : 0.f;
+    const uint32_t taddr = tmem_base + (warp * 32 << 16), count = t.row1 - t.row0;
+    out += static_cast<size_t>(t.row0) * p.m;
+    if (split == 1) {
+        if (summed) {
+            if constexpr (ROWS >= 32) {
+                const bool packed = p.m % 2 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 3) == 0;
+                each_32_columns<ROWS>(taddr, count, ctrl->x_scales, w_scale,
+                                      [&](uint32_t c, const uint64_t (&v)[16]) { store_across_rows(out + static_cast<size_t>(c) * p.m, p.m, channel, has_channel, lane, v, count - c, packed); });
+            } else {
+                uint32_t r[16];
+                tmem_ld16(taddr, r);
+#pragma unroll
+                for (uint32_t j = 0; j < 16; ++j)
+                    if (j < count && has_channel) store_result(out + static_cast<size_t>(j) * p.m + channel, __int2float_rn(static_cast<int>(r[j])) * ctrl->x_scales[j] * w_scale);
+            }
+        }
+    } else {
+        // the rows' sums into this CTA's shared memory (the stages are through), 128 channels to a row
+        int* sums = reinterpret_cast<int*>(smem);
+        if (summed)
+#pragma unroll 1
+            for (uint32_t c = 0; c < count; c += 16) {
+                uint32_t r[16];
+                tmem_ld16(taddr + c, r);
+#pragma unroll
+                for (uint32_t j = 0; j < 16; ++j) sums[(c + j) * P_CHANNELS + threadIdx.x] = static_cast<int>(r[j]);
+            }
+        cluster_sync();
+        if (summed) {
+            constexpr uint32_t AHEAD = 4;
+            for (uint32_t r0 = rank; r0 < count; r0 += AHEAD * split) {
+                int sum[AHEAD] = {};
+                for (uint32_t q = 0; q < split; ++q) {
+                    const uint32_t from = cluster_address(sums + threadIdx.x, q);
+                    int v[AHEAD];
+#pragma unroll
+                    for (uint32_t e = 0; e < AHEAD; ++e) v[e] = load_cluster(from + min(r0 + e * split, count - 1) * (P_CHANNELS * 4));
+#pragma unroll
+                    for (uint32_t e = 0; e < AHEAD; ++e) sum[e] += v[e];
+                }
+#pragma unroll
+                for (uint32_t e = 0; e < AHEAD; ++e) {
+                    const uint32_t r = r0 + e * split;
+                    if (r < count && has_channel) store_result(out + static_cast<size_t>(r) * p.m + channel, __int2float_rn(sum[e]) * ctrl->x_scales[r] * w_scale);
+                }
+            }
+        }
+        cluster_sync();   // nobody reads this CTA's sums any more
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 0) tmem_dealloc(tmem_base, COLS);
+}
+
+// ---- many rows: persistent pairs of CTAs on tiles of 256 lanes x COLS columns, each CTA with its 128 lanes, half of the columns as operand
+// and all of them in its accumulator:
+//   warp 0       TMA producer
+//   warp 1       MMA issuer (the leader's)
+//   warps 4-11   epilogue: 32 lanes and half of the columns each, out of one accumulator while the other is filled
+// Where rows of the result begin on 32 bytes, the lanes are rows of x: a thread then holds 128 neighbouring results of a row and stores
+// 32 bytes at a time.  Elsewhere, and where the tile is narrow because the groups are small, the lanes are channels, and the 32 lanes of
+// a warp store 32 neighbouring results of a row.
+constexpr int Q_EPI_WARPS = 8;
+constexpr int Q_THREADS = 128 + 32 * Q_EPI_WARPS;
+constexpr uint32_t Q_TRAY_BYTES = 32 * 128;   // 32 rows of results on their way out, of each epilogue warp
+template <bool LANES_ARE_ROWS>
+constexpr int kPairStages = LANES_ARE_ROWS ? 5 : 6;
+
+template <int COLS>
+struct PairControl {
+    uint64_t full[6];            // (the leader's are used)
+    uint64_t empty[6];
+    uint64_t acc_full[2];
+    uint64_t acc_empty[2];       // (the leader's are used)
+    uint32_t tmem_base;
+    alignas(16) float scales[Q_EPI_WARPS][COLS / 2];   // of a warp's columns
+};
+template <int COLS>
+constexpr uint32_t kPairStageBytes = P_W_BYTES + COLS / 2 * P_DEPTH;
+template <int COLS, bool LANES_ARE_ROWS>
+constexpr uint32_t kPairSmem = kPairStages<LANES_ARE_ROWS> * kPairStageBytes<COLS> + (LANES_ARE_ROWS ? Q_EPI_WARPS * Q_TRAY_BYTES : 0) + sizeof(PairControl<COLS>) + 1024;
+
 template <int COLS, typename O, bool LANES_ARE_ROWS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Q_THREADS, 1) product_pair_kernel(const __grid_constant__ ProductMaps maps, const ProductParams p) {
     extern __shared__ uint8_t smem_raw[];
@@ -413,6 +461,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Q_THREADS, 1) produc
     constexpr uint32_t ROWS = LANES_ARE_ROWS ? 256 : COLS, CHANNELS = LANES_ARE_ROWS ? COLS : 256;   // of a tile
 
     if (threadIdx.x == 0) {
+        tma_prefetch_map(&maps.w);
+        tma_prefetch_map(&maps.x);
         for (int s = 0; s < STAGES; ++s) {
             mbar_init(&ctrl->full[s], 1);
             mbar_init(&ctrl->empty[s], 1);
@@ -731,11 +781,11 @@ ProductPlan make_plan(const Product& p) {
         plan.row_tiles = static_cast<uint32_t>((p.n + plan.rows - 1) / plan.rows + (p.groups ? p.groups + 1 : 0));
         return plan;
     }
-    plan.rows = typical <= 16 ? 16 : typical <= 32 ? 32 : typical <= 64 ? 64 : 128;
-    if (plan.rows == 128 && (p.n + 127) / 128 * channel_tiles < 148) plan.rows = 64;
+    plan.rows = typical <= 16 ? 16 : typical <= 32 ? 32 : 64;
     plan.row_tiles = static_cast<uint32_t>((p.n + plan.rows - 1) / plan.rows + (p.groups ? p.groups + 1 : 0));
-    if (!p.groups && plan.rows <= 64)
-        while (plan.split < 8 && plan.row_tiles * channel_tiles * plan.split * 2 <= 2 * 148 && depth_blocks >= 2 * plan.split) plan.split *= 2;
+    // (adding the sums up costs two barriers of the cluster and 2 us: no block gets fewer than four steps)
+    if (!p.groups)
+        while (plan.split < 8 && plan.row_tiles * channel_tiles * plan.split * 2 <= 148 && depth_blocks >= 8 * plan.split) plan.split *= 2;
     return plan;
 }
 
@@ -749,7 +799,8 @@ void launch_quantize_rows(const Rows& x, Type type, size_t n, size_t d, int8_t* 
         constexpr int B = decltype(width)::bytes;
         const uint32_t chunks = static_cast<uint32_t>(d * t / B);
         auto launch = [&](auto* kernel, int lanes) {
-            kernel<<<static_cast<unsigned>((n + 256 / lanes - 1) / (256 / lanes)), 256, 0, stream>>>(x.p, pitch, n, chunks, q, ldq, scales);
+            const size_t blocks = (n + 256 / lanes - 1) / (256 / lanes);
+            kernel<<<static_cast<unsigned>(std::min<size_t>(blocks, static_cast<size_t>(sm_count()) * 8)), 256, 0, stream>>>(x.p, pitch, n, chunks, q, ldq, scales);
         };
         if (chunks <= 8 * 4) launch(quantize_rows_kernel<T, B, 8, 4>, 8);
         else if (chunks <= 32 * 4) launch(quantize_rows_kernel<T, B, 32, 4>, 32);
@@ -868,8 +919,7 @@ void launch_product(const Product& p, void* workspace, cudaStream_t stream) {
     else if (plan.pairs) of_type(launch_pairs, std::integral_constant<int, 128>{});
     else if (plan.rows == 16) of_type(launch, std::integral_constant<int, 16>{});
     else if (plan.rows == 32) of_type(launch, std::integral_constant<int, 32>{});
-    else if (plan.rows == 64) of_type(launch, std::integral_constant<int, 64>{});
-    else of_type(launch, std::integral_constant<int, 128>{});
+    else of_type(launch, std::integral_constant<int, 64>{});
 }
 
 void check_products(cudaStream_t stream) {

@@ -116,6 +116,8 @@ __device__ __forceinline__ void tma_load_2d(uint32_t smem_dst, const CUtensorMap
                  : "memory");
 }
 
+__device__ __forceinline__ void tma_prefetch_map(const CUtensorMap* tmap) { asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(tmap)) : "memory"); }
+
 // Shared memory -> global, what lies outside the matrix left out; the calling thread's stores are a group, and these wait until all its
 // groups have read their shared memory, or are complete.
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap* tmap, uint32_t smem_src, int x, int y) {

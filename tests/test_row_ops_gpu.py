@@ -392,7 +392,7 @@ def check_product(got, x, xs, w, ws, dtype):
 
 
 PRODUCTS = [(1, 1, 1), (1, 16_384, 768), (3, 5, 17), (16, 128, 128), (17, 129, 129), (33, 1000, 50), (64, 300, 4096), (128, 128, 256), (777, 1001, 130), (1000, 64, 16), (300, 4097, 640),
-            (5, 100, 40_000), (300, 6000, 256), (4100, 1030, 200), (2000, 1001, 768), (70, 20_001, 33), (8197, 517, 130)]
+            (5, 100, 40_000), (300, 6000, 256), (4100, 1030, 200), (2000, 1001, 768), (70, 20_001, 33), (8197, 517, 130), (1000, 2048, 1100), (6000, 2000, 700), (20_000, 4112, 64)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
