@@ -1,13 +1,18 @@
 """Builds libskm_b200.so in-tree with nvcc for sm_100a.  Run as `python superkmeans_b200/build.py` (by path: importing the package needs the library).
 
+`_ops_calls.so`, the short cuts of ops.py into that library, is built beside it where torch and Python's headers are there; ops.py
+works without.
+
 Every source file is compiled to an object of its own (in parallel, and only when it or a header changed), then the
 objects are linked into the shared library.  `-v` prints what ptxas reports (registers, spills, shared memory)."""
 from __future__ import annotations
 
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -18,6 +23,8 @@ SOURCES = ["memory.cu", "host_copy.cu", "phase_timers.cu", "kernels.cu", "kernel
 HEADERS = ["common.cuh", "device_utils.cuh", "gemm_simt.cuh", "tc_ptx.cuh", "kernels_tc.cuh", "rows.h", "rows_access.cuh", "noalloc.h", "engine.h", "engine_buffers.h", "host_copy.h", "phase_timers.h", "exact_assign.h", "host_logic.h", "comm_nccl.h",
            os.path.join("..", "..", "include", "skm_b200.h")]
 OUTPUT = os.path.join(HERE, "libskm_b200.so")
+CALLS_SOURCE = os.path.join(CSRC, "ops_calls.cpp")
+CALLS_OUTPUT = os.path.join(HERE, "_ops_calls.so")
 
 
 def _nvcc() -> str:
@@ -60,9 +67,41 @@ def _compile_one(nvcc: str, src: str, verbose: bool):
     return src, obj, res
 
 
+def _stale_calls() -> bool:
+    if not os.path.exists(CALLS_OUTPUT):
+        return True
+    header = os.path.join(CSRC, "..", "..", "include", "skm_b200.h")
+    return max(os.path.getmtime(CALLS_SOURCE), os.path.getmtime(header)) > os.path.getmtime(CALLS_OUTPUT)
+
+
+def build_calls(force: bool = False) -> None:
+    """The short cuts between torch tensors and the library (needs the library)."""
+    if not force and not _stale_calls():
+        return
+    include = sysconfig.get_paths()["include"]
+    found = importlib.util.find_spec("torch")
+    if found is None or not os.path.exists(os.path.join(include, "Python.h")):
+        sys.stderr.write("torch or Python.h is missing: ops.py goes without its short cuts\n")
+        return
+    torch_dir = os.path.dirname(found.origin)
+    cuda = os.path.dirname(os.path.dirname(os.path.realpath(_nvcc())))
+    cmd = ["/usr/bin/g++", "-std=c++17", "-O2", "-fPIC", "-shared", "-Wall", f"-I{include}", f"-I{torch_dir}/include", f"-I{torch_dir}/include/torch/csrc/api/include",
+           f"-I{cuda}/include", CALLS_SOURCE, "-o", CALLS_OUTPUT, f"-L{torch_dir}/lib", "-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10", "-lc10_cuda", f"-L{HERE}", "-lskm_b200",
+           "-Wl,-rpath,$ORIGIN"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        sys.stderr.write(res.stdout + res.stderr)
+        raise RuntimeError("compiling ops_calls.cpp failed")
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
-    if not force and not verbose and not needs_build():
-        return OUTPUT
+    if force or verbose or needs_build():
+        build_library(force, verbose)
+    build_calls(force)
+    return OUTPUT
+
+
+def build_library(force: bool, verbose: bool) -> None:
     nvcc = _nvcc()
     os.makedirs(OBJDIR, exist_ok=True)
     hdr_t = _newest_header()
@@ -88,7 +127,6 @@ def build(force: bool = False, verbose: bool = False) -> str:
     if res.returncode != 0:
         sys.stderr.write(res.stdout + res.stderr)
         raise RuntimeError("link failed")
-    return OUTPUT
 
 
 if __name__ == "__main__":

@@ -9,7 +9,8 @@
 
 A thin layer over the functions of the same names in include/skm_b200.h.  Every call works on the current stream of its tensors'
 device (which need not be the current device), allocates its outputs and its workspace through torch, waits for nothing and can be
-captured into a CUDA graph.  Tensors that are used on another stream than the one they were made on need `record_stream`, as with
+captured into a CUDA graph.  Calls with tensors that need no conversion take a short cut in C++ (csrc/ops_calls.cpp), which answers None
+where there is something to refuse, copy or record; those are made here.  Tensors that are used on another stream than the one they were made on need `record_stream`, as with
 any operator of torch.  Rows may have any distance from one another; the values of a row lie side by side, or the rows are copied
 first.  Arguments that do not fit raise ValueError.
 """
@@ -20,6 +21,14 @@ from typing import NamedTuple, Optional, Tuple
 import torch
 
 from ._lib import check, lib
+
+try:
+    from . import _ops_calls as _calls
+except ImportError:   # (not built, or for another torch: every call takes the way through ctypes)
+
+    class _calls:   # noqa: N801
+        lookup = lookup_grad = lookup_scale_grad = group_rows = to_clusters = from_clusters = from_clusters_grad = quantize_rows = product_8bit = staticmethod(lambda *_: None)
+
 
 # (looked up once: a call on a few rows takes as long as the host takes to make it)
 _op_lookup, _op_lookup_grad, _op_lookup_scale_grad = lib.skm_op_lookup, lib.skm_op_lookup_grad, lib.skm_op_lookup_scale_grad
@@ -201,6 +210,9 @@ def lookup(table: torch.Tensor, ids: torch.Tensor, scale: float = 1.0, row_scale
     a table of k x d values in fp32, fp16 or bf16.  `row_scales`, if given, has the shape of `ids` and dtype float32.  An id that is no
     row of the table (-1 as padding) gives zeros and no gradient.  Differentiable in `table` (see lookup_grad) and `row_scales`."""
     scale = float(scale)
+    out = _calls.lookup(table, ids, scale, row_scales)
+    if out is not None:
+        return out
     if _wants_grad(table, row_scales):
         return _Lookup.apply(table, ids, scale, row_scales)
     return _lookup(table, ids, scale, row_scales)
@@ -210,6 +222,10 @@ def lookup_grad(grad: torch.Tensor, ids: torch.Tensor, n_rows: int, scale: float
                 dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """Gradient of a table of `n_rows` rows: row c is the sum of scale * row_scales[i] * grad[i] over ids[i] = c, zeros where there is no such
     i.  Summed in fp32 in an order that depends on the ids alone, and rounded once to `dtype` (that of `grad`, or float32)."""
+    if dtype is None:
+        out = _calls.lookup_grad(grad, ids, n_rows, float(scale), row_scales)
+        if out is not None:
+            return out
     rows, n, d, ld, kind = _rows(grad, "grad")
     at, bits = _ids(ids, "ids", grad)
     if at.shape != (n,):
@@ -232,6 +248,9 @@ def lookup_grad(grad: torch.Tensor, ids: torch.Tensor, n_rows: int, scale: float
 
 def lookup_scale_grad(grad: torch.Tensor, table: torch.Tensor, ids: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
     """Gradient of the row scales of a lookup, float32: scale * <grad[i], table[ids[i]]>, zero where the id is no row of the table."""
+    out = _calls.lookup_scale_grad(grad, table, ids, float(scale))
+    if out is not None:
+        return out
     rows, n, d, ld, kind = _rows(grad, "grad")
     t, k, d_t, ld_t, _ = _rows(table, "table", grad, grad.dtype)
     at, bits = _ids(ids, "ids", grad)
@@ -253,6 +272,9 @@ def lookup_scale_grad(grad: torch.Tensor, table: torch.Tensor, ids: torch.Tensor
 def group_rows(ids: torch.Tensor, n_clusters: int) -> RowGroups:
     """The order of rows by cluster: `ids` has one entry for each row (n), or one for each of its m choices (n x m).  Pairs of the same
     cluster keep their order; those without one (an id outside 0 .. n_clusters - 1) come last.  The offsets stay on the device."""
+    out = _calls.group_rows(ids, n_clusters)
+    if out is not None:
+        return RowGroups(*out)
     at, bits = _ids(ids, "ids")
     if at.dim() not in (1, 2) or (at.dim() == 2 and at.shape[1] == 0):
         raise ValueError(f"ids must have shape (n,) or (n, m) with m > 0, got {tuple(at.shape)}")
@@ -341,6 +363,9 @@ def to_clusters(x: torch.Tensor, groups: RowGroups) -> torch.Tensor:
     """Rows in the order of their clusters: n x d to (n * m) x d, row i once for each of its m choices, at groups.position[i, j].  The rows of
     cluster c are offsets[c] .. offsets[c + 1] - 1; behind the last cluster the slots of choices without one hold zeros.
     Differentiable in x (see to_clusters_grad)."""
+    out = _calls.to_clusters(x, groups[1], groups[2])
+    if out is not None:
+        return out
     if _wants_grad(x):
         return _ToClusters.apply(x, *groups)
     return _to_clusters(x, groups)
@@ -349,13 +374,17 @@ def to_clusters(x: torch.Tensor, groups: RowGroups) -> torch.Tensor:
 def to_clusters_grad(grad: torch.Tensor, groups: RowGroups) -> torch.Tensor:
     """Gradient of the rows of to_clusters: the sum over a row's choices of their slots' gradients (n x d), without those that have no
     cluster."""
-    return _from_clusters(grad, groups, None, "grad")
+    out = _calls.from_clusters(grad, groups[1], groups[2], None)
+    return _from_clusters(grad, groups, None, "grad") if out is None else out
 
 
 def from_clusters(y: torch.Tensor, groups: RowGroups, weights: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Rows back from the order of their clusters: out[i] = sum over j of weights[i, j] * y[position[i, j]], n x d.  Choices without a cluster
     contribute nothing, whatever their slots hold.  `weights` (float32, the shape of groups.position) is 1 if not given.
     Differentiable in y and weights (see from_clusters_grad)."""
+    out = _calls.from_clusters(y, groups[1], groups[2], weights)
+    if out is not None:
+        return out
     if _wants_grad(y, weights):
         return _FromClusters.apply(y, weights, *groups)
     return _from_clusters(y, groups, weights)
@@ -364,7 +393,8 @@ def from_clusters(y: torch.Tensor, groups: RowGroups, weights: Optional[torch.Te
 def from_clusters_grad(grad: torch.Tensor, y: torch.Tensor, groups: RowGroups, weights: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """Gradients of from_clusters: of y, weights[i, j] * grad[i] at position[i, j] and zeros in the slots of choices without a cluster; and of the
     weights (float32; None where there are none), <grad[i], y[position[i, j]]>."""
-    return _from_clusters_grad(grad, y, groups, weights, True, weights is not None)
+    out = _calls.from_clusters_grad(grad, y, groups[1], groups[2], weights)
+    return _from_clusters_grad(grad, y, groups, weights, True, weights is not None) if out is None else out
 
 
 # ---- products in 8 bits ---------------------------------------------------------------------------------------------------------
@@ -373,6 +403,9 @@ def from_clusters_grad(grad: torch.Tensor, y: torch.Tensor, groups: RowGroups, w
 def quantize_rows(x: torch.Tensor) -> QuantizedRows:
     """Rows in 8 bits: scales[i] = max |x[i]| / 127 (float32), values[i] = x[i] / scales[i] rounded to the nearest whole number, int8.  A row of
     zeros has scale 0; a row with a value that is no finite number has scale NaN.  The rows of the result begin on 16 bytes."""
+    out = _calls.quantize_rows(x)
+    if out is not None:
+        return QuantizedRows(*out)
     rows, n, d, ld, kind = _rows(x, "x")
     if n > _MOST:
         raise ValueError("x must have no more than 2**31 - 1 rows")
@@ -400,8 +433,12 @@ def product_8bit(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_sca
     offsets[c] <= i < offsets[c + 1]; rows of no cluster come out as zeros.
 
     Rows that do not begin on 16 bytes are copied first; quantize_rows makes rows that do.  d is at most 131071."""
-    if dtype not in _DTYPES:
+    kind = _DTYPES.get(dtype)
+    if kind is None:
         raise ValueError(f"dtype must be float32, float16 or bfloat16, got {dtype}")
+    out = _calls.product_8bit(x, x_scales, w, w_scales, offsets, kind)
+    if out is not None:
+        return out
     _on_gpu(x, "x")
     _on_gpu(w, "w", x)
     if x.dim() != 2:
@@ -430,7 +467,7 @@ def product_8bit(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_sca
     x_at, w_at = x.data_ptr(), w.data_ptr()
     space, address, size = _workspace(lib.skm_op_product_8bit_workspace(x_at, ld_x, w_at, ld_w, n, m, d, e), x)
     index = x.get_device()
-    _check(_op_product_8bit(index, x_at, ld_x, x_scales.data_ptr(), w_at, ld_w, w_scales.data_ptr(), n, m, d, e, _p(offsets), out.data_ptr(), _DTYPES[dtype], address, size,
+    _check(_op_product_8bit(index, x_at, ld_x, x_scales.data_ptr(), w_at, ld_w, w_scales.data_ptr(), n, m, d, e, _p(offsets), out.data_ptr(), kind, address, size,
                                   _raw_stream(index)))
     return out
 

@@ -15,11 +15,21 @@ STEP = {torch.float32: 2.0**-149, torch.float16: 2.0**-24, torch.bfloat16: 2.0**
 TYPES = [torch.float32, torch.float16, torch.bfloat16]
 
 
-@pytest.fixture(scope="module")
-def ops():
+@pytest.fixture(scope="module", params=["short cuts", "ctypes"])
+def ops(request):
+    """Every test runs twice: with the short cuts of plain calls, and with all calls on the way through ctypes."""
     from superkmeans_b200 import ops
 
-    return ops
+    class Nothing:
+        def __getattr__(self, _):
+            return lambda *_: None
+
+    calls = ops._calls
+    assert type(calls).__name__ == "module", "_ops_calls.so is not built"
+    if request.param == "ctypes":
+        ops._calls = Nothing()
+    yield ops
+    ops._calls = calls
 
 
 def rng(seed):
