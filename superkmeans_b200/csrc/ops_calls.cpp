@@ -1,10 +1,11 @@
 // Short cuts for the calls of superkmeans_b200/ops.py that need no conversion: plain CUDA tensors of the right types, shapes and strides,
 // no gradient to be recorded.  Such a call goes from its tensors to the C ABI without Python in between (a lookup of a few rows: 9.5 us
-// through ctypes, XX here; the kernel launch alone is 3).  Everything else - refusals, copies, gradients - is
+// through ctypes, 5 here; the kernel launch alone is 3).  Everything else - refusals, copies, gradients - is
 // answered with None, and ops.py makes the call itself (a failure on the GPU is raised).
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/core/LegacyTypeDispatch.h>
 #include <ATen/core/grad_mode.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -119,6 +120,8 @@ PyObject* failed(skm_status status) {
 // An exception of torch's (no memory) is the caller's to meet again.
 template <class F>
 PyObject* shortcut(F&& f) {
+    // (no gradient is recorded here: allocations and views go straight to what makes them)
+    const at::AutoDispatchBelowADInplaceOrView direct;
     try {
         return f();
     } catch (const std::exception&) {

@@ -1,7 +1,7 @@
 // Pairs (row, choice) in the order of their cluster: a stable sort of small numbers by counting.
 //
-// A few pairs: every pair counts, against all others, how many come before it.  That is n^2 comparisons, but in one launch over the
-// whole chip, and a launch is what the time of a small call consists of.
+// A few pairs: every pair's place is looked for among all others, in one launch over the whole chip; a launch is what the time of a small
+// call consists of.
 //
 // More: a radix sort, up to 11 bits at a time.  A unit of a few hundred pairs belongs to a warp, which counts its digits in shared
 // memory; a block for each digit turns the units' counts into places; and the units, read again, rank equal digits among 32 neighbours by
@@ -21,96 +21,99 @@ constexpr int kMaxBits = 11;
 int unit_warps(int bits, size_t n_units) { return bits <= 9 && n_units >= 148 * 16 ? 16 : 4; }
 
 // ---------------------------------------------------------------------------------------------- few pairs
-// A block ranks 32 pairs (one to a lane) against all: each of its warps compares them with a part of the keys.
+// A key is the cluster and behind it the pair's number, so that no two are equal: a pair's slot is how many keys are less, and the
+// largest of those says which cluster comes before.  Every block sorts all keys in groups of 32 (a warp a group, by exchanges between
+// lanes) and then looks for the place of one group's keys, one to a lane, in all groups by halving.  (4096 pairs with 1000 clusters:
+// YY us; comparing every pair with every key, 13.)
 constexpr uint32_t kRankWarps = 16;
+constexpr uint32_t kRankAhead = 4;   // groups of a warp at a time
+constexpr int kPairBits = 12;
+static_assert(kFewPairs <= size_t{1} << kPairBits, "pairs' numbers fit their bits");
 
 __global__ void __launch_bounds__(32 * kRankWarps) rank_kernel(const void* __restrict__ ids, bool wide, uint32_t n, uint32_t k, uint32_t* __restrict__ order, uint32_t* __restrict__ position,
-                                                   uint32_t* __restrict__ keys_out, uint32_t* __restrict__ offsets) {
-    __shared__ uint4 key4[kFewPairs / 4];
-    __shared__ uint32_t parts[3][kRankWarps][32];
-    uint32_t* key = reinterpret_cast<uint32_t*>(key4);
-    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t n4 = (n + 3) / 4;
-    constexpr int AHEAD = 4;
-    constexpr uint32_t THREADS = 32 * kRankWarps;
-    for (uint32_t i0 = 0; i0 < 4 * n4; i0 += THREADS * AHEAD) {
-        uint32_t v[AHEAD];
+                                                               uint32_t* __restrict__ keys_out, uint32_t* __restrict__ offsets) {
+    __shared__ uint32_t key[kFewPairs];
+    __shared__ uint32_t parts[2][kRankWarps][32];
+    __shared__ uint32_t fill[3][32];   // of each lane's pair: offsets fill[0] .. fill[1] become fill[2]
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, groups = (n + 31) / 32;
+    for (uint32_t g0 = warp; g0 < groups; g0 += kRankWarps * kRankAhead) {
+        uint32_t v[kRankAhead];
 #pragma unroll
-        for (int u = 0; u < AHEAD; ++u) {
-            const uint32_t i = i0 + u * THREADS + threadIdx.x;
-            v[u] = i < n ? load_id(ids, wide, i, k) : 0xffffffffu;
+        for (uint32_t u = 0; u < kRankAhead; ++u) {
+            const uint32_t i = (g0 + u * kRankWarps) * 32 + lane;
+            v[u] = i < n ? load_id(ids, wide, i, k) << kPairBits | i : 0xffffffffu;
         }
 #pragma unroll
-        for (int u = 0; u < AHEAD; ++u) {
-            const uint32_t i = i0 + u * THREADS + threadIdx.x;
-            if (i < 4 * n4) key[i] = v[u];
-        }
+        for (uint32_t size = 2; size <= 32; size *= 2)
+#pragma unroll
+            for (uint32_t apart = size / 2; apart > 0; apart /= 2) {
+                const bool lower = ((lane & apart) == 0) == ((lane & size) == 0);
+#pragma unroll
+                for (uint32_t u = 0; u < kRankAhead; ++u) {
+                    const uint32_t other = __shfl_xor_sync(0xffffffffu, v[u], apart);
+                    v[u] = lower ? min(v[u], other) : max(v[u], other);
+                }
+            }
+#pragma unroll
+        for (uint32_t u = 0; u < kRankAhead; ++u)
+            if (g0 + u * kRankWarps < groups) key[(g0 + u * kRankWarps) * 32 + lane] = v[u];
     }
     __syncthreads();
-    const uint32_t mine = blockIdx.x * 32 + lane;
-    const uint32_t c = mine < n ? key[mine] : 0u;
-    // keys less than c, equal ones of earlier pairs, and 1 + the largest of the lesser ones
-    uint32_t less = 0, earlier = 0, below = 0;
-    auto compare = [&](uint32_t from, uint32_t to, auto&& is_earlier) {
-#pragma unroll 4
-        for (uint32_t i = from; i < to; ++i) {
-            const uint4 q = key4[i];
-            const uint32_t v[4] = {q.x, q.y, q.z, q.w};
+    const uint32_t own = key[blockIdx.x * 32 + lane];
+    const bool mine = own != 0xffffffffu || blockIdx.x * 32 + lane < n;   // (the last group's gaps come last in it)
+    uint32_t slot = 0, before = 0;   // keys that are less, and the largest of them
+    for (uint32_t g0 = warp; g0 < groups; g0 += kRankWarps * kRankAhead) {
+        uint32_t less[kRankAhead];
 #pragma unroll
-            for (uint32_t e = 0; e < 4; ++e) {
-                // (selections, no branches)
-                const uint32_t lower = v[e] < c ? 1u : 0u;
-                less += lower;
-                below = max(below, lower ? v[e] + 1 : 0u);
-                earlier += v[e] == c && is_earlier(4 * i + e) ? 1u : 0u;
+        for (uint32_t u = 0; u < kRankAhead; ++u) less[u] = 0;
+#pragma unroll
+        for (uint32_t half = 16; half > 0; half /= 2)
+#pragma unroll
+            for (uint32_t u = 0; u < kRankAhead; ++u) {
+                const uint32_t g = g0 + u * kRankWarps;
+                if (g < groups && key[g * 32 + less[u] + half - 1] < own) less[u] += half;
+            }
+#pragma unroll
+        for (uint32_t u = 0; u < kRankAhead; ++u) {
+            const uint32_t g = g0 + u * kRankWarps;
+            if (g < groups) {
+                if (key[g * 32 + less[u]] < own) ++less[u];   // (31 at most until here)
+                if (less[u] > 0) before = max(before, key[g * 32 + less[u] - 1]);
+                slot += less[u];
             }
         }
-    };
-    // the keys before the block's own 32, those, and the ones behind them
-    const uint32_t a = warp * n4 / kRankWarps, b = (warp + 1) * n4 / kRankWarps, own0 = min(max(blockIdx.x * 8, a), b), own1 = min(max(blockIdx.x * 8 + 8, a), b);
-    compare(a, own0, [](uint32_t) { return true; });
-    compare(own0, own1, [&](uint32_t j) { return j < mine; });
-    compare(own1, b, [](uint32_t) { return false; });
-    parts[0][warp][lane] = less;
-    parts[1][warp][lane] = earlier;
-    parts[2][warp][lane] = below;
+    }
+    parts[0][warp][lane] = slot;
+    parts[1][warp][lane] = before;
     __syncthreads();
-    if (warp != 0) return;
+    if (warp == 0) {
 #pragma unroll
-    for (uint32_t w = 1; w < kRankWarps; ++w) {
-        less += parts[0][w][lane];
-        earlier += parts[1][w][lane];
-        below = max(below, parts[2][w][lane]);
-    }
-    const uint32_t slot = less + earlier;
-    // the first pair of a cluster sets where the clusters behind the one before it begin, the last pair of all the rest
-    uint32_t from = 1, upto = 0, value = 0;
-    if (mine < n) {
-        order[slot] = mine;
-        if (position) position[mine] = slot;
-        if (keys_out) keys_out[slot] = c;
-        if (earlier == 0) {
-            from = below;
-            upto = c;
-            value = slot;
+        for (uint32_t w = 1; w < kRankWarps; ++w) {
+            slot += parts[0][w][lane];
+            before = max(before, parts[1][w][lane]);
         }
+        const uint32_t cluster = own >> kPairBits, pair = own & (kFewPairs - 1);
+        if (mine) {
+            order[slot] = pair;
+            if (position) position[pair] = slot;
+            if (keys_out) keys_out[slot] = cluster;
+        }
+        // the first pair of a cluster sets where the clusters behind the one before it begin
+        fill[0][lane] = !mine ? 1u : slot == 0 ? 0u : (before >> kPairBits) + 1;
+        fill[1][lane] = mine ? cluster : 0u;
+        fill[2][lane] = slot;
     }
-    uint32_t rest_from = 1, rest_upto = 0;
-    if (mine < n && slot == n - 1) {
-        rest_from = c + 1;
-        rest_upto = k;
-    }
-    for (uint32_t left = __ballot_sync(0xffffffffu, from <= upto); left; left &= left - 1) {
-        const int l = __ffs(left) - 1;
-        const uint32_t f = __shfl_sync(0xffffffffu, from, l), t = __shfl_sync(0xffffffffu, upto, l), v = __shfl_sync(0xffffffffu, value, l);
-        for (uint32_t i = f + lane; i <= t; i += 32) offsets[i] = v;
-    }
-    const uint32_t last = __ballot_sync(0xffffffffu, rest_from <= rest_upto);
-    if (last) {
-        const uint32_t f = __shfl_sync(0xffffffffu, rest_from, __ffs(last) - 1);
-        for (uint32_t i = f + lane; i <= k; i += 32) offsets[i] = n;
+    __syncthreads();
+    for (uint32_t l = warp; l < 32; l += kRankWarps) {
+        const uint32_t from = fill[0][l], upto = fill[1][l], value = fill[2][l];
+        for (uint32_t i = from + lane; i <= upto; i += 32) offsets[i] = value;
+        // the last pair of all sets the rest
+        if (value == n - 1 && blockIdx.x * 32 + l < n)
+            for (uint32_t i = upto + 1 + lane; i <= k; i += 32) offsets[i] = n;
     }
 }
+
+bool few(size_t n, size_t k) { return n <= kFewPairs && k < (size_t{1} << (32 - kPairBits)); }
 
 // ---------------------------------------------------------------------------------------------- many pairs
 struct Pass {
@@ -290,7 +293,7 @@ size_t rounded(size_t words) { return (words + 63) / 64 * 64; }
 } // namespace
 
 size_t group_workspace_bytes(size_t n, size_t k) {
-    if (n <= kFewPairs) return 0;
+    if (n == 0 || few(n, k)) return 0;
     const Plan plan = make_plan(n, k);
     // digits' totals, the units' table, and between passes two copies of keys and pairs
     const size_t lists = plan.passes == 1 ? 0 : 4;
@@ -302,7 +305,7 @@ void launch_group(const Ids& ids, size_t n, size_t k, uint32_t* order, uint32_t*
         SKM_CUDA(cudaMemsetAsync(offsets, 0, (k + 1) * sizeof(uint32_t), stream));
         return;
     }
-    if (n <= kFewPairs) {
+    if (few(n, k)) {
         rank_kernel<<<static_cast<unsigned>((n + 31) / 32), 32 * kRankWarps, 0, stream>>>(ids.p, ids.wide, static_cast<uint32_t>(n), static_cast<uint32_t>(k), order, position, keys, offsets);
         SKM_LAUNCH_CHECK();
         return;

@@ -229,7 +229,7 @@ def plain_groups(ids, k):
     return order, position.reshape(ids.shape), torch.cat([torch.zeros(1, dtype=torch.int64), counts.cumsum(0)])
 
 
-SORTS = [(1, 1), (2, 1), (33, 5), (1000, 65_536), (4095, 300), (4096, 1), (4097, 1), (5000, 2047), (5000, 2048), (70_000, 255), (140_001, 10_000), (300_000, 5_000_000), (1_100_000, 37)]
+SORTS = [(1, 1), (2, 1), (33, 5), (1000, 65_536), (4095, 300), (4096, 1), (4097, 1), (5000, 2047), (5000, 2048), (70_000, 255), (140_001, 10_000), (300_000, 5_000_000), (1_100_000, 37), (700, 2**20 - 1), (700, 2**20), (4000, 3_000_000)]
 
 
 @pytest.mark.parametrize("n,k", SORTS)
