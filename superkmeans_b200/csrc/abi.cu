@@ -69,12 +69,14 @@ rows::Ids ids_of(const void* ids, int bits, uint64_t n) {
     return {ids, bits == 64};
 }
 
+bool sizes_are_fine(uint64_t n, uint64_t k) { return k > 0 && k < 0x7fffffff && n <= 0x7fffffff; }
 void check_sizes(uint64_t n, uint64_t k) {
     need(k > 0 && k < 0x7fffffff, "the number of clusters must be positive and below 2^31 - 1");
-    need(n <= 0x7fffffff, "no more than 2^31 - 1 ids");
+    need(sizes_are_fine(n, k), "no more than 2^31 - 1 ids");
 }
 
-void check_width(uint64_t d) { need(d > 0 && d <= (1u << 20), "the dimensionality must be positive and at most 2^20"); }
+bool width_is_fine(uint64_t d) { return d > 0 && d <= (1u << 20); }
+void check_width(uint64_t d) { need(width_is_fine(d), "the dimensionality must be positive and at most 2^20"); }
 
 void check_workspace(const void* workspace, uint64_t given, uint64_t needed) {
     need(given >= needed, "the workspace is too small");
@@ -431,6 +433,7 @@ skm_status skm_op_lookup(int device, const void* table, uint64_t ld_table, int d
 }
 
 uint64_t skm_op_lookup_grad_workspace(uint64_t n, uint64_t k, uint64_t d, int dtype) {
+    if (!sizes_are_fine(n, k) || !width_is_fine(d)) return 0;   // (skm_op_lookup_grad refuses them)
     return rows::lookup_grad_workspace_bytes(n, k, d, dtype == SKM_F32 ? rows::Type::f32 : rows::Type::f16);
 }
 
@@ -462,7 +465,7 @@ skm_status skm_op_lookup_scale_grad(int device, const void* grad, uint64_t ld_gr
     });
 }
 
-uint64_t skm_op_group_rows_workspace(uint64_t n, uint64_t k) { return rows::group_workspace_bytes(n, k); }
+uint64_t skm_op_group_rows_workspace(uint64_t n, uint64_t k) { return sizes_are_fine(n, k) ? rows::group_workspace_bytes(n, k) : 0; }
 
 skm_status skm_op_group_rows(int device, const void* ids, int ids_bits, uint64_t n, uint64_t k, uint32_t* order, uint32_t* position, uint32_t* offsets, void* workspace,
                              uint64_t workspace_bytes, void* cuda_stream) {

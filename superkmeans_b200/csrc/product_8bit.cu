@@ -29,6 +29,7 @@ namespace {
 template <typename T, int BYTES, int LANES, int HELD>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(const void* __restrict__ x, size_t pitch, size_t n, uint32_t width, int8_t* __restrict__ q, size_t ldq,
                                                             float* __restrict__ scales) {
+    wait_for_the_one_before();
     using V = Values<T, BYTES>;
     const size_t step = static_cast<size_t>(gridDim.x) * (256 / LANES);
     const uint32_t lane = threadIdx.x % LANES;
@@ -118,6 +119,7 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const void* __restri
 
 // Rows with a pitch that TMA takes (zeros behind d).
 __global__ void __launch_bounds__(256) pad_bytes_kernel(const int8_t* __restrict__ in, size_t ld, size_t n, uint32_t d, uint32_t pitch, int8_t* __restrict__ out) {
+    wait_for_the_one_before();
     const size_t row = static_cast<size_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
     if (row >= n) return;
     for (uint32_t j = threadIdx.x & 31; j < pitch / 4; j += 32) {
@@ -140,6 +142,8 @@ constexpr uint32_t P_W_BYTES = P_CHANNELS * P_DEPTH;
 struct RowTile {
     uint32_t row0, row1, group;
 };
+
+__device__ __forceinline__ RowTile load_tile(const RowTile* p) { return {__ldcg(&p->row0), __ldcg(&p->row1), __ldcg(&p->group)}; }
 
 struct ProductMaps {
     CUtensorMap w, x;
@@ -273,6 +277,7 @@ __device__ __forceinline__ void store_across_rows(O* out, uint32_t m, uint32_t c
 // part of the rows, out of one another's shared memory.
 template <int ROWS, typename O>
 __global__ void __launch_bounds__(P_THREADS) product_kernel(const __grid_constant__ ProductMaps maps, const ProductParams p) {
+    wait_for_the_one_before();
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw_addr = smem_u32(smem_raw);
     const uint32_t pad = (1024u - (raw_addr & 1023u)) & 1023u;
@@ -287,8 +292,8 @@ __global__ void __launch_bounds__(P_THREADS) product_kernel(const __grid_constan
     const uint32_t tile = blockIdx.x / split, channel_tile = tile % p.channel_tiles, row_tile = tile / p.channel_tiles;
     RowTile t;
     if (p.groups) {
-        if (row_tile >= __ldg(p.n_tiles + 1)) return;   // (the whole cluster)
-        t = p.tiles[row_tile];
+        if (row_tile >= __ldcg(p.n_tiles + 1)) return;   // (the whole cluster)
+        t = load_tile(p.tiles + row_tile);
     } else {
         t = {row_tile * ROWS, min(row_tile * ROWS + ROWS, p.n), 0};
     }
@@ -312,7 +317,7 @@ __global__ void __launch_bounds__(P_THREADS) product_kernel(const __grid_constan
         fence_proxy_async();
     }
     if (warp == 0) tmem_alloc(&ctrl->tmem_base, COLS);
-    for (uint32_t r = threadIdx.x; r < ROWS; r += P_THREADS) ctrl->x_scales[r] = t.row0 + r < t.row1 ? __ldg(p.x_scales + t.row0 + r) : 0.f;
+    for (uint32_t r = threadIdx.x; r < ROWS; r += P_THREADS) ctrl->x_scales[r] = t.row0 + r < t.row1 ? __ldcg(p.x_scales + t.row0 + r) : 0.f;
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -447,6 +452,7 @@ constexpr uint32_t kPairSmem = kPairStages<LANES_ARE_ROWS> * kPairStageBytes<COL
 
 template <int COLS, typename O, bool LANES_ARE_ROWS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Q_THREADS, 1) product_pair_kernel(const __grid_constant__ ProductMaps maps, const ProductParams p) {
+    wait_for_the_one_before();
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw_addr = smem_u32(smem_raw);
     const uint32_t pad = (1024u - (raw_addr & 1023u)) & 1023u;
@@ -481,14 +487,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Q_THREADS, 1) produc
     tc_fence_after();
     const uint32_t tmem_base = ctrl->tmem_base;
 
-    const uint32_t row_tiles = p.groups ? __ldg(p.n_tiles) : (p.n + ROWS - 1) / ROWS;   // that have a group
+    const uint32_t row_tiles = p.groups ? __ldcg(p.n_tiles) : (p.n + ROWS - 1) / ROWS;   // that have a group
     const uint32_t n_tiles = row_tiles * p.channel_tiles;
     const uint32_t first = blockIdx.x >> 1, step = gridDim.x >> 1;
     // the rows of tile t and its first channel
     auto tile_at = [&](uint32_t t, uint32_t& channel0) {
         const uint32_t i = t / p.channel_tiles;
         channel0 = (t - i * p.channel_tiles) * CHANNELS;
-        if (p.groups) return p.tiles[i];
+        if (p.groups) return load_tile(p.tiles + i);
         return RowTile{i * ROWS, min(i * ROWS + ROWS, p.n), 0};
     };
 
@@ -569,7 +575,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Q_THREADS, 1) produc
                 column = channel;
                 end = p.m;
                 column_scales = w_scales;
-                lane_scale = valid ? __ldg(p.x_scales + row) : 0.f;
+                lane_scale = valid ? __ldcg(p.x_scales + row) : 0.f;
             } else {
                 row = tile.row0 + half * MINE;
                 channel = channel0 + at_lane;
@@ -581,7 +587,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Q_THREADS, 1) produc
             }
             count = end > column ? min(end - column, MINE) : 0;
 #pragma unroll
-            for (uint32_t e = 0; e < EACH; ++e) scale[e] = e * 32 + lane < count ? __ldg(column_scales + column + e * 32 + lane) : 0.f;
+            for (uint32_t e = 0; e < EACH; ++e) scale[e] = e * 32 + lane < count ? __ldcg(column_scales + column + e * 32 + lane) : 0.f;
         };
         if (first < n_tiles) look_up(first);
         uint32_t i = 0;
@@ -642,7 +648,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Q_THREADS, 1) produc
         if (LANES_ARE_ROWS && lane == 0) tma_stores_done();
         // rows of no group
         if (p.groups) {
-            const uint32_t all = __ldg(p.n_tiles + 1), threads = threadIdx.x - 128;
+            const uint32_t all = __ldcg(p.n_tiles + 1), threads = threadIdx.x - 128;
             for (uint32_t t = row_tiles * p.channel_tiles + first; t < all * p.channel_tiles; t += step) {
                 uint32_t channel0;
                 const RowTile tile = tile_at(t, channel0);
@@ -664,6 +670,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Q_THREADS, 1) produc
 // all.
 __global__ void __launch_bounds__(1024) row_tiles_kernel(const uint32_t* __restrict__ offsets, uint32_t groups, uint32_t n, uint32_t rows, uint32_t room, RowTile* __restrict__ tiles,
                                                          uint32_t* __restrict__ n_tiles) {
+    wait_for_the_one_before();
     __shared__ uint32_t sums[32];
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     uint32_t base = 0;
@@ -671,13 +678,13 @@ __global__ void __launch_bounds__(1024) row_tiles_kernel(const uint32_t* __restr
         const uint32_t g = g0 + threadIdx.x;
         uint32_t a = 0, b = 0;
         if (g < groups) {
-            a = min(__ldg(offsets + g), n);
-            b = min(__ldg(offsets + g + 1), n);
+            a = min(__ldcg(offsets + g), n);
+            b = min(__ldcg(offsets + g + 1), n);
         } else if (g == groups) {
-            a = min(__ldg(offsets + groups), n);
+            a = min(__ldcg(offsets + groups), n);
             b = n;
         } else if (g == groups + 1) {
-            b = min(__ldg(offsets), n);
+            b = min(__ldcg(offsets), n);
         }
         const uint32_t count = b > a ? (b - a + rows - 1) / rows : 0;
         uint32_t upto = count;
@@ -800,14 +807,13 @@ void launch_quantize_rows(const Rows& x, Type type, size_t n, size_t d, int8_t* 
         const uint32_t chunks = static_cast<uint32_t>(d * t / B);
         auto launch = [&](auto* kernel, int lanes) {
             const size_t blocks = (n + 256 / lanes - 1) / (256 / lanes);
-            kernel<<<static_cast<unsigned>(std::min<size_t>(blocks, static_cast<size_t>(sm_count()) * 8)), 256, 0, stream>>>(x.p, pitch, n, chunks, q, ldq, scales);
+            launch_after(kernel, dim3(static_cast<unsigned>(std::min<size_t>(blocks, static_cast<size_t>(sm_count()) * 8))), 256, 0, stream, x.p, pitch, n, chunks, q, ldq, scales);
         };
         if (chunks <= 8 * 4) launch(quantize_rows_kernel<T, B, 8, 4>, 8);
         else if (chunks <= 32 * 4) launch(quantize_rows_kernel<T, B, 32, 4>, 32);
         else if (chunks <= 32 * 8) launch(quantize_rows_kernel<T, B, 32, 8>, 32);
         else launch(quantize_rows_kernel<T, B, 256, 4>, 256);
     });
-    SKM_LAUNCH_CHECK();
 }
 
 size_t product_workspace_bytes(const Product& p) {
@@ -834,8 +840,7 @@ void launch_product(const Product& p, void* workspace, cudaStream_t stream) {
         if (tma_takes(rows, ld, p.d)) return;
         const size_t pitch = pitch_of(p.d);
         int8_t* copy = reinterpret_cast<int8_t*>(take(n * pitch));
-        pad_bytes_kernel<<<static_cast<unsigned>((n + 7) / 8), 256, 0, stream>>>(rows, ld, n, static_cast<uint32_t>(p.d), static_cast<uint32_t>(pitch), copy);
-        SKM_LAUNCH_CHECK();
+        launch_after(pad_bytes_kernel, dim3(static_cast<unsigned>((n + 7) / 8)), 256, 0, stream, rows, ld, n, static_cast<uint32_t>(p.d), static_cast<uint32_t>(pitch), copy);
         rows = copy;
         ld = pitch;
     };
@@ -862,8 +867,7 @@ void launch_product(const Product& p, void* workspace, cudaStream_t stream) {
     if (p.groups) {
         RowTile* tiles = reinterpret_cast<RowTile*>(take(plan.row_tiles * sizeof(RowTile)));
         uint32_t* n_tiles = reinterpret_cast<uint32_t*>(take(8));
-        row_tiles_kernel<<<1, 1024, 0, stream>>>(p.offsets, k.groups, k.n, plan.rows, plan.row_tiles, tiles, n_tiles);
-        SKM_LAUNCH_CHECK();
+        launch_after(row_tiles_kernel, dim3(1), 1024, 0, stream, p.offsets, k.groups, k.n, plan.rows, plan.row_tiles, tiles, n_tiles);
         k.tiles = tiles;
         k.n_tiles = n_tiles;
     }
@@ -878,7 +882,7 @@ void launch_product(const Product& p, void* workspace, cudaStream_t stream) {
         const unsigned grid = 2 * static_cast<unsigned>(std::min<size_t>(all_tiles, static_cast<size_t>(sm_pairs())));
         auto go = [&](auto* kernel, uint32_t smem) {
             allow_shared(kernel, smem);
-            kernel<<<grid, Q_THREADS, smem, stream>>>(maps, k);
+            launch_after(kernel, dim3(grid), Q_THREADS, smem, stream, maps, k);
         };
         if constexpr (COLS == 256) {
             if (plan.lanes_are_rows) {
@@ -890,25 +894,13 @@ void launch_product(const Product& p, void* workspace, cudaStream_t stream) {
         } else {
             go(product_pair_kernel<COLS, O, false>, kPairSmem<COLS, false>);
         }
-        SKM_LAUNCH_CHECK();
     };
     auto launch = [&](auto rows, auto result) {
         constexpr int ROWS = decltype(rows)::value;
         using O = decltype(result);
         auto* kernel = product_kernel<ROWS, O>;
         allow_shared(kernel, kProductSmem<ROWS>);
-        cudaLaunchConfig_t config{};
-        config.gridDim = dim3(static_cast<unsigned>(all_tiles * plan.split));
-        config.blockDim = dim3(P_THREADS);
-        config.dynamicSmemBytes = kProductSmem<ROWS>;
-        config.stream = stream;
-        cudaLaunchAttribute cluster{};
-        cluster.id = cudaLaunchAttributeClusterDimension;
-        cluster.val.clusterDim = {plan.split, 1, 1};
-        config.attrs = &cluster;
-        config.numAttrs = 1;
-        SKM_CUDA(cudaLaunchKernelEx(&config, kernel, maps, k));
-        SKM_LAUNCH_CHECK();
+        launch_clusters_after(kernel, dim3(static_cast<unsigned>(all_tiles * plan.split)), plan.split, P_THREADS, kProductSmem<ROWS>, stream, maps, k);
     };
     auto of_type = [&](auto&& go, auto rows) {
         if (p.out_type == Type::f32) go(rows, float{});

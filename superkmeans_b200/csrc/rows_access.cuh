@@ -7,6 +7,7 @@
 
 #include <algorithm>
 #include <cstdint>
+#include <utility>
 
 #include "common.cuh"
 #include "rows.h"
@@ -122,6 +123,37 @@ struct Values {
         return c;
     }
 };
+
+// Kernels that follow one another (launch_after) start before the one ahead has ended and wait for it here, before they touch memory: what
+// that one wrote is visible then.  It is read past the first-level cache (__ldcg), which may hold older lines: a kernel's start, which
+// empties that cache, is no longer behind the end of the one ahead.  (Sort and sums of 500 000 pairs, eight launches: 227 -> 219 us;
+// routing of 30 001 x 4 rows: 118 -> 108.)
+__device__ __forceinline__ void wait_for_the_one_before() {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+// (cluster: blocks to a cluster, 0 where the kernel says itself)
+template <typename... P, typename... A>
+void launch_clusters_after(void (*kernel)(P...), dim3 grid, unsigned cluster, unsigned threads, size_t shared, cudaStream_t stream, A&&... args) {
+    cudaLaunchAttribute attributes[2]{};
+    attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attributes[0].val.programmaticStreamSerializationAllowed = 1;
+    attributes[1].id = cudaLaunchAttributeClusterDimension;
+    attributes[1].val.clusterDim = {cluster, 1, 1};
+    cudaLaunchConfig_t config{};
+    config.gridDim = grid;
+    config.blockDim = dim3(threads);
+    config.dynamicSmemBytes = shared;
+    config.stream = stream;
+    config.attrs = attributes;
+    config.numAttrs = cluster == 0 ? 1 : 2;
+    SKM_CUDA(cudaLaunchKernelEx(&config, kernel, static_cast<P>(args)...));
+    SKM_LAUNCH_CHECK();
+}
+template <typename... P, typename... A>
+void launch_after(void (*kernel)(P...), dim3 grid, unsigned threads, size_t shared, cudaStream_t stream, A&&... args) {
+    launch_clusters_after(kernel, grid, 0, threads, shared, stream, std::forward<A>(args)...);
+}
 
 // The cluster of pair i, or k.
 __device__ __forceinline__ uint32_t load_id(const void* ids, bool wide, size_t i, uint32_t k) {

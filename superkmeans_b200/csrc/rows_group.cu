@@ -32,6 +32,7 @@ static_assert(kFewPairs <= size_t{1} << kPairBits, "pairs' numbers fit their bit
 
 __global__ void __launch_bounds__(32 * kRankWarps) rank_kernel(const void* __restrict__ ids, bool wide, uint32_t n, uint32_t k, uint32_t* __restrict__ order, uint32_t* __restrict__ position,
                                                                uint32_t* __restrict__ keys_out, uint32_t* __restrict__ offsets) {
+    wait_for_the_one_before();
     __shared__ uint32_t key[kFewPairs];
     __shared__ uint32_t parts[2][kRankWarps][32];
     __shared__ uint32_t fill[3][32];   // of each lane's pair: offsets fill[0] .. fill[1] become fill[2]
@@ -132,13 +133,14 @@ struct PassInput {
     const uint32_t* pairs;
 };
 
-__device__ __forceinline__ uint32_t key_of(const PassInput& in, size_t i, uint32_t k) { return in.keys ? __ldg(in.keys + i) : load_id(in.ids, in.wide, i, k); }
+__device__ __forceinline__ uint32_t key_of(const PassInput& in, size_t i, uint32_t k) { return in.keys ? __ldcg(in.keys + i) : load_id(in.ids, in.wide, i, k); }
 
 constexpr int kSortAhead = 4;
 
 // table[digit][unit] = the unit's pairs with that digit
 template <int WARPS>
 __global__ void __launch_bounds__(32 * WARPS) count_kernel(const PassInput in, const Pass p, uint32_t* __restrict__ table) {
+    wait_for_the_one_before();
     extern __shared__ uint32_t counts[];   // a row for each warp
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, digits = 1u << p.bits, apart = digits + 1;
     for (uint32_t i = threadIdx.x; i < apart * WARPS; i += 32 * WARPS) counts[i] = 0;
@@ -166,16 +168,17 @@ __global__ void __launch_bounds__(32 * WARPS) count_kernel(const PassInput in, c
 
 // table[digit][unit] = how many pairs of that digit the units before have, totals[digit] all; a block for each digit.
 __global__ void __launch_bounds__(256) place_kernel(const Pass p, uint32_t* __restrict__ table, uint32_t* __restrict__ totals) {
+    wait_for_the_one_before();
     __shared__ uint32_t sums[2][8];
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     uint4* row = reinterpret_cast<uint4*>(table + static_cast<size_t>(blockIdx.x) * p.pitch);
     const uint32_t n4 = p.pitch / 4;
-    uint4 v = threadIdx.x < n4 ? row[threadIdx.x] : make_uint4(0, 0, 0, 0);
+    uint4 v = threadIdx.x < n4 ? __ldcg(row + threadIdx.x) : make_uint4(0, 0, 0, 0);
     uint32_t before = 0;
     for (uint32_t s = 0; s < n4; s += 256) {
         const uint32_t i = s + threadIdx.x;
         const uint4 c = v;
-        v = i + 256 < n4 ? row[i + 256] : make_uint4(0, 0, 0, 0);
+        v = i + 256 < n4 ? __ldcg(row + i + 256) : make_uint4(0, 0, 0, 0);
         const uint32_t four = c.x + c.y + c.z + c.w;
         uint32_t upto = four;
 #pragma unroll
@@ -201,6 +204,7 @@ template <int WARPS>
 __global__ void __launch_bounds__(32 * WARPS) scatter_kernel(const PassInput in, const Pass p, const uint32_t* __restrict__ table, const uint32_t* __restrict__ totals,
                                                              uint32_t* __restrict__ pairs_out, uint32_t* __restrict__ keys_out, uint32_t* __restrict__ position,
                                                              uint32_t* __restrict__ offsets) {
+    wait_for_the_one_before();
     extern __shared__ uint32_t next[];   // a row for each warp
     __shared__ uint32_t sums[WARPS];
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, digits = 1u << p.bits, apart = digits + 1;
@@ -209,7 +213,7 @@ __global__ void __launch_bounds__(32 * WARPS) scatter_kernel(const PassInput in,
     uint32_t* base = next + apart * WARPS;
     const uint32_t each = (digits + 32 * WARPS - 1) / (32 * WARPS), digit0 = threadIdx.x * each;
     uint32_t mine = 0;
-    for (uint32_t e = 0; e < each && digit0 + e < digits; ++e) mine += __ldg(totals + digit0 + e);
+    for (uint32_t e = 0; e < each && digit0 + e < digits; ++e) mine += __ldcg(totals + digit0 + e);
     uint32_t upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -223,12 +227,12 @@ __global__ void __launch_bounds__(32 * WARPS) scatter_kernel(const PassInput in,
     for (uint32_t e = 0; e < each && digit0 + e < digits; ++e) {
         base[digit0 + e] = slot0;
         if (offsets && blockIdx.x == 0 && digit0 + e <= p.k) offsets[digit0 + e] = slot0;
-        slot0 += __ldg(totals + digit0 + e);
+        slot0 += __ldcg(totals + digit0 + e);
     }
     __syncthreads();
     for (uint32_t i = threadIdx.x; i < digits * WARPS; i += 32 * WARPS) {
         const uint32_t w = i % WARPS, digit = i / WARPS;
-        if (unit0 + w < p.n_units) next[w * apart + digit] = base[digit] + __ldg(table + static_cast<size_t>(digit) * p.pitch + unit0 + w);
+        if (unit0 + w < p.n_units) next[w * apart + digit] = base[digit] + __ldcg(table + static_cast<size_t>(digit) * p.pitch + unit0 + w);
     }
     __syncthreads();
     const size_t begin = static_cast<size_t>(unit) * p.unit, end = min(begin + p.unit, p.n);
@@ -239,7 +243,7 @@ __global__ void __launch_bounds__(32 * WARPS) scatter_kernel(const PassInput in,
             const size_t i = s + u * 32 + lane;
             const bool valid = i < end;
             key[u] = valid ? key_of(in, i, p.k) : 0u;
-            pair[u] = valid && in.pairs ? __ldg(in.pairs + i) : static_cast<uint32_t>(i);
+            pair[u] = valid && in.pairs ? __ldcg(in.pairs + i) : static_cast<uint32_t>(i);
         }
 #pragma unroll
         for (int u = 0; u < kSortAhead; ++u) {
@@ -261,15 +265,16 @@ __global__ void __launch_bounds__(32 * WARPS) scatter_kernel(const PassInput in,
 
 // offsets[c] = first slot whose key is c or more: where a key begins it sets those of the keys behind the one before, 32 lanes together
 __global__ void __launch_bounds__(256) offsets_kernel(const uint32_t* __restrict__ keys, uint32_t n, uint32_t k, uint32_t* __restrict__ offsets) {
+    wait_for_the_one_before();
     const uint32_t lane = threadIdx.x & 31, slot = blockIdx.x * 256 + threadIdx.x;
-    const uint32_t key = slot < n ? __ldg(keys + slot) : 0u, from = slot == 0 ? 0u : slot < n ? __ldg(keys + slot - 1) + 1 : 1u;
+    const uint32_t key = slot < n ? __ldcg(keys + slot) : 0u, from = slot == 0 ? 0u : slot < n ? __ldcg(keys + slot - 1) + 1 : 1u;
     for (uint32_t left = __ballot_sync(0xffffffffu, slot < n && from <= key); left; left &= left - 1) {
         const int l = __ffs(left) - 1;
         const uint32_t f = __shfl_sync(0xffffffffu, from, l), t = __shfl_sync(0xffffffffu, key, l), v = __shfl_sync(0xffffffffu, slot, l);
         for (uint32_t c = f + lane; c <= t; c += 32) offsets[c] = v;
     }
     // behind the last key, by the grid
-    for (uint32_t c = __ldg(keys + n - 1) + 1 + slot; c <= k; c += gridDim.x * 256) offsets[c] = n;
+    for (uint32_t c = __ldcg(keys + n - 1) + 1 + slot; c <= k; c += gridDim.x * 256) offsets[c] = n;
 }
 
 struct Plan {
@@ -306,8 +311,8 @@ void launch_group(const Ids& ids, size_t n, size_t k, uint32_t* order, uint32_t*
         return;
     }
     if (few(n, k)) {
-        rank_kernel<<<static_cast<unsigned>((n + 31) / 32), 32 * kRankWarps, 0, stream>>>(ids.p, ids.wide, static_cast<uint32_t>(n), static_cast<uint32_t>(k), order, position, keys, offsets);
-        SKM_LAUNCH_CHECK();
+        launch_after(rank_kernel, dim3(static_cast<unsigned>((n + 31) / 32)), 32 * kRankWarps, 0, stream, ids.p, ids.wide, static_cast<uint32_t>(n), static_cast<uint32_t>(k), order,
+                     position, keys, offsets);
         return;
     }
     const Plan plan = make_plan(n, k);
@@ -322,20 +327,15 @@ void launch_group(const Ids& ids, size_t n, size_t k, uint32_t* order, uint32_t*
         const Pass p{n, static_cast<uint32_t>(k), pass * plan.bits, plan.bits, plan.n_units, plan.unit, static_cast<uint32_t>(pitch_of(plan))};
         uint32_t* keys_here = plan.passes == 1 ? keys : (last && keys) ? keys : lists + rounded(n) * 2 * (pass & 1);
         uint32_t* pairs_here = last ? order : lists + rounded(n) * (2 * (pass & 1) + 1);
-        if (warps == 16) count_kernel<16><<<blocks, 512, shared, stream>>>(in, p, table);
-        else count_kernel<4><<<blocks, 128, shared, stream>>>(in, p, table);
-        SKM_LAUNCH_CHECK();
-        place_kernel<<<static_cast<unsigned>(digits), 256, 0, stream>>>(p, table, totals);
-        SKM_LAUNCH_CHECK();
-        if (warps == 16) scatter_kernel<16><<<blocks, 512, shared + digits * 4, stream>>>(in, p, table, totals, pairs_here, keys_here, last ? position : nullptr, plan.passes == 1 ? offsets : nullptr);
-        else scatter_kernel<4><<<blocks, 128, shared + digits * 4, stream>>>(in, p, table, totals, pairs_here, keys_here, last ? position : nullptr, plan.passes == 1 ? offsets : nullptr);
-        SKM_LAUNCH_CHECK();
+        launch_after(warps == 16 ? count_kernel<16> : count_kernel<4>, dim3(blocks), 32 * warps, shared, stream, in, p, table);
+        launch_after(place_kernel, dim3(static_cast<unsigned>(digits)), 256, 0, stream, p, table, totals);
+        launch_after(warps == 16 ? scatter_kernel<16> : scatter_kernel<4>, dim3(blocks), 32 * warps, shared + digits * 4, stream, in, p, table, totals, pairs_here, keys_here,
+                     last ? position : nullptr, plan.passes == 1 ? offsets : nullptr);
         in.keys = keys_here;
         in.pairs = pairs_here;
     }
     if (plan.passes > 1) {
-        offsets_kernel<<<static_cast<unsigned>((n + 255) / 256), 256, 0, stream>>>(in.keys, static_cast<uint32_t>(n), static_cast<uint32_t>(k), offsets);
-        SKM_LAUNCH_CHECK();
+        launch_after(offsets_kernel, dim3(static_cast<unsigned>((n + 255) / 256)), 256, 0, stream, in.keys, static_cast<uint32_t>(n), static_cast<uint32_t>(k), offsets);
     }
 }
 

@@ -70,12 +70,13 @@ struct Sums {
 // SCALED: each pair with a factor of its own; otherwise the sums are scaled.
 template <typename T, typename O, int BYTES, bool SCALED>
 __global__ void __launch_bounds__(32 * kWarps) sum_tiles_kernel(const SumParams p) {
+    wait_for_the_one_before();
     constexpr uint32_t AHEAD = kAhead;
     using S = Sums<T, BYTES>;
     const uint32_t lane = threadIdx.x & 31;
     const size_t unit = static_cast<size_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
     const size_t tile = unit / p.slabs, begin = tile * p.tile;
-    const uint32_t held = __ldg(p.offsets + p.k);
+    const uint32_t held = __ldcg(p.offsets + p.k);
     if (begin >= held) return;   // (pairs without an id come last)
     const uint32_t col = static_cast<uint32_t>(unit - tile * p.slabs) * 32 + lane;
     const bool mine = col < p.width;
@@ -86,12 +87,12 @@ __global__ void __launch_bounds__(32 * kWarps) sum_tiles_kernel(const SumParams 
     const float scale = SCALED ? 1.f : p.scale;
     S sum;
     sum.clear();
-    uint32_t now = __ldg(p.keys + s0);
+    uint32_t now = __ldcg(p.keys + s0);
     bool first = true;
     for (uint32_t s = s0; s < s1; s += 32) {
         // a lane's pair of the next 32, and where runs of equal ids begin
         const uint32_t my = s + lane;
-        const uint32_t my_pair = my < s1 ? __ldg(p.order + my) : 0u, my_key = my < s1 ? __ldg(p.keys + my) : 0u;
+        const uint32_t my_pair = my < s1 ? __ldcg(p.order + my) : 0u, my_key = my < s1 ? __ldcg(p.keys + my) : 0u;
         float my_factor = 0.f;
         if (SCALED && my < s1) my_factor = p.scale * __ldg(p.row_scales + my_pair);
         const uint32_t above = __shfl_up_sync(0xffffffffu, my_key, 1);
@@ -141,6 +142,7 @@ constexpr uint32_t kLongRun = 8;   // tiles
 
 template <typename T, typename O, int BYTES>
 __global__ void __launch_bounds__(32 * kJoinWarps) join_tiles_kernel(const SumParams p) {
+    wait_for_the_one_before();
     using S = Sums<T, BYTES>;
     __shared__ float parts[kJoinWarps][32][S::N + 1];
     __shared__ uint32_t long_ids[kJoinWarps];
@@ -154,8 +156,8 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_tiles_kernel(const SumPa
     uint32_t begin = 0, t0 = 0, t1 = 0;
     bool todo = false;
     if (lane < p.join_ids && id0 + lane < p.k) {
-        begin = __ldg(p.offsets + id0 + lane);
-        const uint32_t end = __ldg(p.offsets + id0 + lane + 1), held = __ldg(p.offsets + p.k);
+        begin = __ldcg(p.offsets + id0 + lane);
+        const uint32_t end = __ldcg(p.offsets + id0 + lane + 1), held = __ldcg(p.offsets + p.k);
         t0 = begin / p.tile;
         t1 = end > begin ? (end - 1) / p.tile + 1 : t0;
         todo = !(t1 == t0 + 1 && begin > t0 * p.tile && end < min(static_cast<size_t>(t1) * p.tile, static_cast<size_t>(held)));
@@ -171,7 +173,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_tiles_kernel(const SumPa
                 const float* src = p.partials + (tile * 2 + (first > tile * p.tile ? 1 : 0)) * p.d + at;
 #pragma unroll
                 for (int i = 0; i < S::N / EACH; ++i)
-                    v[u][i].from(t + u < to && mine ? __ldg(reinterpret_cast<const Chunk<EACH * 4>*>(src) + i) : zero_chunk<EACH * 4>());
+                    v[u][i].from(t + u < to && mine ? __ldcg(reinterpret_cast<const Chunk<EACH * 4>*>(src) + i) : zero_chunk<EACH * 4>());
             }
 #pragma unroll
             for (uint32_t u = 0; u < AHEAD; ++u)
@@ -192,7 +194,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_tiles_kernel(const SumPa
     for (uint32_t w = 0; w < kJoinWarps; ++w)
         for (uint32_t left = long_ids[w]; left; left &= left - 1) {   // (the same for the whole block)
             const uint32_t id = block0 + w * p.join_ids + __ffs(left) - 1;
-            const uint32_t first = __ldg(p.offsets + id), from0 = first / p.tile, to0 = (__ldg(p.offsets + id + 1) - 1) / p.tile + 1;
+            const uint32_t first = __ldcg(p.offsets + id), from0 = first / p.tile, to0 = (__ldcg(p.offsets + id + 1) - 1) / p.tile + 1;
             const uint32_t share = (to0 - from0 + kJoinWarps - 1) / kJoinWarps, from = min(from0 + warp * share, to0);
             S sum;
             sum.clear();
@@ -219,6 +221,7 @@ constexpr uint32_t kFewSumPairs = 4096;
 
 template <typename T, typename O, int BYTES>
 __global__ void __launch_bounds__(32 * kFewWarps) sum_few_kernel(const SumParams p, const void* __restrict__ ids, bool wide) {
+    wait_for_the_one_before();
     using S = Sums<T, BYTES>;
     constexpr uint32_t MOST = kFewSumPairs / kFewWarps;   // pairs of a warp
     __shared__ uint16_t found[kFewWarps][MOST];
@@ -341,20 +344,17 @@ void launch_lookup_grad(const Rows& grad, Type type, size_t k, size_t d, const I
         p.width = static_cast<uint32_t>(d * t / B);
         p.slabs = (p.width + 31) / 32;
         if (is_few) {
-            sum_few_kernel<T, O, B><<<dim3(static_cast<unsigned>(k), p.slabs), 32 * kFewWarps, 0, stream>>>(p, ids.p, ids.wide);
-            SKM_LAUNCH_CHECK();
+            launch_after(sum_few_kernel<T, O, B>, dim3(static_cast<unsigned>(k), p.slabs), 32 * kFewWarps, 0, stream, p, ids.p, ids.wide);
             return;
         }
         const size_t units = tiles * p.slabs;
         auto* kernel = row_scales ? sum_tiles_kernel<T, O, B, true> : sum_tiles_kernel<T, O, B, false>;
-        kernel<<<static_cast<unsigned>((units + kWarps - 1) / kWarps), 32 * kWarps, 0, stream>>>(p);
-        SKM_LAUNCH_CHECK();
+        launch_after(kernel, dim3(static_cast<unsigned>((units + kWarps - 1) / kWarps)), 32 * kWarps, 0, stream, p);
         // a warp takes its ids one after the other: few, as long as there are warps for them
         p.join_ids = 1;
         while (p.join_ids < 32 && k * p.slabs > static_cast<size_t>(p.join_ids) * 148 * 32) p.join_ids *= 2;
         const size_t ids_of_block = static_cast<size_t>(p.join_ids) * kJoinWarps;
-        join_tiles_kernel<T, O, B><<<dim3(static_cast<unsigned>((k + ids_of_block - 1) / ids_of_block), p.slabs), 32 * kJoinWarps, 0, stream>>>(p);
-        SKM_LAUNCH_CHECK();
+        launch_after(join_tiles_kernel<T, O, B>, dim3(static_cast<unsigned>((k + ids_of_block - 1) / ids_of_block), p.slabs), 32 * kJoinWarps, 0, stream, p);
     };
     with_width(type, bytes, [&](auto value, auto width) {
         if (out_type == Type::f32) launch(value, float{}, width);

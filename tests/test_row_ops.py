@@ -127,6 +127,9 @@ def test_workspaces_grow_with_what_they_hold():
     assert lib.skm_op_product_8bit_workspace(AT, 17, AT, 16, 5, 7, 16, 0) >= 5 * 16
     assert lib.skm_op_product_8bit_workspace(AT + 1, 16, AT, 16, 5, 7, 16, 0) >= 5 * 16
     assert lib.skm_op_product_8bit_workspace(AT, 16, AT, 18, 5, 7, 17, 3) >= 3 * 7 * 32
+    for n, k in ((2**40, 5), (5000, 0), (5000, 2**63), (2**64 - 1, 2**64 - 1)):   # (refused sizes need nothing)
+        assert lib.skm_op_group_rows_workspace(n, k) == 0 and lib.skm_op_lookup_grad_workspace(n, k, 8, 0) == 0
+    assert lib.skm_op_product_8bit_workspace(AT, 17, AT, 17, 2**40, 2**40, 2**40, 2**63) == 0
     small, large = (lib.skm_op_group_rows_workspace(n, 100) for n in (5_000, 5_000_000))
     assert 0 < small < large
     assert lib.skm_op_lookup_grad_workspace(10_000, 10, 64, 0) >= 10_000 * 8 + 11 * 4
