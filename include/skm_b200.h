@@ -342,18 +342,19 @@ skm_status skm_op_lookup_scale_grad(int device, const void* grad, uint64_t ld_gr
 uint64_t skm_op_group_rows_workspace(uint64_t n, uint64_t k);
 skm_status skm_op_group_rows(int device, const void* ids, int ids_bits, uint64_t n, uint64_t k, uint32_t* order, uint32_t* position, uint32_t* offsets, void* workspace,
                              uint64_t workspace_bytes, void* cuda_stream);
-/* Rows to the slots of their clusters, m choices to a row: out[position[i * m + j]] = x[i]; x n x d, out n * m x d.  Slots of choices without a
+/* Rows to the slots of their clusters, m choices to a row (order, position and offsets as skm_op_group_rows made them of the n * m ids):
+ * out[position[i * m + j]] = x[i]; x n x d, out n * m x d.  Slots of choices without a
  * cluster get zeros. */
-skm_status skm_op_to_clusters(int device, const void* x, uint64_t ld_x, int dtype, uint64_t d, const uint32_t* position, const uint32_t* offsets, uint64_t k, uint64_t n, uint64_t m,
-                              void* out, void* cuda_stream);
+skm_status skm_op_to_clusters(int device, const void* x, uint64_t ld_x, int dtype, uint64_t d, const uint32_t* order, const uint32_t* position, const uint32_t* offsets, uint64_t k,
+                              uint64_t n, uint64_t m, void* out, void* cuda_stream);
 /* ... and back: out[i] = sum over j of weights[i * m + j] * y[position[i * m + j]], without the choices that have no cluster; weights n x m
  * (fp32) or NULL for ones, y n * m x d, out n x d.  With weights NULL it is also the gradient of skm_op_to_clusters. */
-skm_status skm_op_from_clusters(int device, const void* y, uint64_t ld_y, int dtype, uint64_t d, const uint32_t* position, const uint32_t* offsets, uint64_t k, uint64_t n, uint64_t m,
-                                const float* weights, void* out, void* cuda_stream);
+skm_status skm_op_from_clusters(int device, const void* y, uint64_t ld_y, int dtype, uint64_t d, const uint32_t* order, const uint32_t* position, const uint32_t* offsets, uint64_t k,
+                                uint64_t n, uint64_t m, const float* weights, void* out, void* cuda_stream);
 /* Its gradients: grad_y[position[i * m + j]] = weights[i * m + j] * grad[i] (zeros in the slots of choices without a cluster) and
  * grad_weights[i * m + j] = <grad[i], y[position[i * m + j]]> (fp32; 0 without a cluster).  Either may be NULL; y is read for grad_weights. */
-skm_status skm_op_from_clusters_grad(int device, const void* grad, uint64_t ld_grad, const void* y, uint64_t ld_y, int dtype, uint64_t d, const uint32_t* position,
-                                     const uint32_t* offsets, uint64_t k, uint64_t n, uint64_t m, const float* weights, void* grad_y, float* grad_weights, void* cuda_stream);
+skm_status skm_op_from_clusters_grad(int device, const void* grad, uint64_t ld_grad, const void* y, uint64_t ld_y, int dtype, uint64_t d, const uint32_t* order,
+                                     const uint32_t* position, const uint32_t* offsets, uint64_t k, uint64_t n, uint64_t m, const float* weights, void* grad_y, float* grad_weights, void* cuda_stream);
 
 /* Rows in 8 bits with a scale each: scales[i] = max_j |x[i][j]| / 127, q[i][j] = x[i][j] * (127 / max) rounded to the nearest whole number (both
  * steps in fp32).  A row of zeros has scale 0; a row with a value that is no finite number has scale NaN and zeros.  ld_q in bytes: a

@@ -83,12 +83,12 @@ void check_workspace(const void* workspace, uint64_t given, uint64_t needed) {
     need(needed == 0 || (workspace && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0), "the workspace must be 256-byte aligned device memory");
 }
 
-rows::Places places_of(const uint32_t* position, const uint32_t* offsets, uint64_t k, uint64_t n, uint64_t m) {
+rows::Places places_of(const uint32_t* order, const uint32_t* position, const uint32_t* offsets, uint64_t k, uint64_t n, uint64_t m) {
     need(m > 0, "a row must have at least one choice");
     need(n <= 0x7fffffff / m, "no more than 2^31 - 1 choices");
     check_sizes(n * m, k);
-    need(n == 0 || (position && offsets), "position and offsets must not be NULL");
-    return {position, offsets ? offsets + k : nullptr, n, m};
+    need(n == 0 || (order && position && offsets), "order, position and offsets must not be NULL");
+    return {order, position, offsets ? offsets + k : nullptr, n, m};
 }
 
 rows::Product product_of(const int8_t* x, uint64_t ld_x, const int8_t* w, uint64_t ld_w, uint64_t n, uint64_t m, uint64_t d, uint64_t groups) {
@@ -479,36 +479,36 @@ skm_status skm_op_group_rows(int device, const void* ids, int ids_bits, uint64_t
     });
 }
 
-skm_status skm_op_to_clusters(int device, const void* x, uint64_t ld_x, int dtype, uint64_t d, const uint32_t* position, const uint32_t* offsets, uint64_t k, uint64_t n, uint64_t m,
-                              void* out, void* cuda_stream) {
+skm_status skm_op_to_clusters(int device, const void* x, uint64_t ld_x, int dtype, uint64_t d, const uint32_t* order, const uint32_t* position, const uint32_t* offsets, uint64_t k,
+                              uint64_t n, uint64_t m, void* out, void* cuda_stream) {
     return row_op([&] {
         const rows::Type type = type_of(dtype);
         check_width(d);
-        const rows::Places at = places_of(position, offsets, k, n, m);
+        const rows::Places at = places_of(order, position, offsets, k, n, m);
         need(n == 0 || (x && out), "x and out must not be NULL");
         const Here here(device);
         rows::launch_to_clusters({x, ld_x}, type, d, at, out, stream_of(cuda_stream));
     });
 }
 
-skm_status skm_op_from_clusters(int device, const void* y, uint64_t ld_y, int dtype, uint64_t d, const uint32_t* position, const uint32_t* offsets, uint64_t k, uint64_t n, uint64_t m,
-                                const float* weights, void* out, void* cuda_stream) {
+skm_status skm_op_from_clusters(int device, const void* y, uint64_t ld_y, int dtype, uint64_t d, const uint32_t* order, const uint32_t* position, const uint32_t* offsets, uint64_t k,
+                              uint64_t n, uint64_t m, const float* weights, void* out, void* cuda_stream) {
     return row_op([&] {
         const rows::Type type = type_of(dtype);
         check_width(d);
-        const rows::Places at = places_of(position, offsets, k, n, m);
+        const rows::Places at = places_of(order, position, offsets, k, n, m);
         need(n == 0 || (y && out), "y and out must not be NULL");
         const Here here(device);
         rows::launch_from_clusters({y, ld_y}, type, d, at, weights, out, stream_of(cuda_stream));
     });
 }
 
-skm_status skm_op_from_clusters_grad(int device, const void* grad, uint64_t ld_grad, const void* y, uint64_t ld_y, int dtype, uint64_t d, const uint32_t* position,
-                                     const uint32_t* offsets, uint64_t k, uint64_t n, uint64_t m, const float* weights, void* grad_y, float* grad_weights, void* cuda_stream) {
+skm_status skm_op_from_clusters_grad(int device, const void* grad, uint64_t ld_grad, const void* y, uint64_t ld_y, int dtype, uint64_t d, const uint32_t* order,
+                                     const uint32_t* position, const uint32_t* offsets, uint64_t k, uint64_t n, uint64_t m, const float* weights, void* grad_y, float* grad_weights, void* cuda_stream) {
     return row_op([&] {
         const rows::Type type = type_of(dtype);
         check_width(d);
-        const rows::Places at = places_of(position, offsets, k, n, m);
+        const rows::Places at = places_of(order, position, offsets, k, n, m);
         need(n == 0 || grad, "grad must not be NULL");
         need(n == 0 || grad_y || grad_weights, "one of grad_y and grad_weights must not be NULL");
         need(n == 0 || y || !grad_weights, "y must not be NULL where grad_weights is asked for");

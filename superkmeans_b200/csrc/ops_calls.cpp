@@ -75,21 +75,23 @@ struct Floats {
 
 // Where a grouping has its rows.
 struct Places {
-    at::Tensor position, offsets;
+    at::Tensor order, position, offsets;
     uint64_t n = 0, m = 1, k = 0;
 
-    bool take(PyObject* at_position, PyObject* at_offsets, const at::Tensor& like) {
-        if (!plain(at_position) || !plain(at_offsets)) return false;
-        position = THPVariable_Unpack(at_position);
-        offsets = THPVariable_Unpack(at_offsets);
-        if (position.scalar_type() != at::kInt || offsets.scalar_type() != at::kInt || !position.is_contiguous() || !offsets.is_contiguous()) return false;
-        if (position.dim() < 1 || position.dim() > 2 || offsets.dim() != 1 || offsets.size(0) < 2) return false;
-        if (position.get_device() != like.get_device() || offsets.get_device() != like.get_device()) return false;
+    static bool take_one(PyObject* o, const at::Tensor& like, at::Tensor& t) {
+        if (!plain(o)) return false;
+        t = THPVariable_Unpack(o);
+        return t.scalar_type() == at::kInt && t.is_contiguous() && t.get_device() == like.get_device();
+    }
+    bool take(PyObject* const* of, const at::Tensor& like) {   // order, position, offsets
+        if (!take_one(of[0], like, order) || !take_one(of[1], like, position) || !take_one(of[2], like, offsets)) return false;
+        if (position.dim() < 1 || position.dim() > 2 || offsets.dim() != 1 || offsets.size(0) < 2 || order.dim() != 1 || order.size(0) != position.numel()) return false;
         n = position.size(0);
         if (position.dim() == 2) m = position.size(1);
         k = offsets.size(0) - 1;
         return m > 0;
     }
+    const uint32_t* pairs() const { return static_cast<const uint32_t*>(order.const_data_ptr()); }
     const uint32_t* positions() const { return static_cast<const uint32_t*>(position.const_data_ptr()); }
     const uint32_t* starts() const { return static_cast<const uint32_t*>(offsets.const_data_ptr()); }
 };
@@ -212,44 +214,44 @@ PyObject* group_rows(PyObject*, PyObject* const* a, Py_ssize_t count) {
     });
 }
 
-// x, position, offsets
+// x, order, position, offsets
 PyObject* to_clusters(PyObject*, PyObject* const* a, Py_ssize_t count) {
     return shortcut([&]() -> PyObject* {
         Rows x;
         Places at;
-        if (count != 3 || !x.take(a[0]) || !at.take(a[1], a[2], x.t) || x.n != at.n) return none();
+        if (count != 4 || !x.take(a[0]) || !at.take(a + 1, x.t) || x.n != at.n) return none();
         const at::Tensor out = make({static_cast<int64_t>(at.n * at.m), static_cast<int64_t>(x.d)}, x.t.scalar_type(), x.t);
-        const skm_status status = skm_op_to_clusters(x.t.get_device(), x.t.const_data_ptr(), x.ld, x.kind, x.d, at.positions(), at.starts(), at.k, at.n, at.m, out.data_ptr(), stream(x.t));
+        const skm_status status = skm_op_to_clusters(x.t.get_device(), x.t.const_data_ptr(), x.ld, x.kind, x.d, at.pairs(), at.positions(), at.starts(), at.k, at.n, at.m, out.data_ptr(), stream(x.t));
         if (status != SKM_OK) return failed(status);
         return wrap(out);
     });
 }
 
-// y, position, offsets, weights
+// y, order, position, offsets, weights
 PyObject* from_clusters(PyObject*, PyObject* const* a, Py_ssize_t count) {
     return shortcut([&]() -> PyObject* {
         Rows y;
         Places at;
         Floats weights;
-        if (count != 4 || !y.take(a[0]) || !at.take(a[1], a[2], y.t) || !weights.take(a[3], at.position.sizes(), y.t) || y.n != at.n * at.m) return none();
+        if (count != 5 || !y.take(a[0]) || !at.take(a + 1, y.t) || !weights.take(a[4], at.position.sizes(), y.t) || y.n != at.n * at.m) return none();
         const at::Tensor out = make({static_cast<int64_t>(at.n), static_cast<int64_t>(y.d)}, y.t.scalar_type(), y.t);
-        const skm_status status = skm_op_from_clusters(y.t.get_device(), y.t.const_data_ptr(), y.ld, y.kind, y.d, at.positions(), at.starts(), at.k, at.n, at.m, weights.p(), out.data_ptr(), stream(y.t));
+        const skm_status status = skm_op_from_clusters(y.t.get_device(), y.t.const_data_ptr(), y.ld, y.kind, y.d, at.pairs(), at.positions(), at.starts(), at.k, at.n, at.m, weights.p(), out.data_ptr(), stream(y.t));
         if (status != SKM_OK) return failed(status);
         return wrap(out);
     });
 }
 
-// grad, y, position, offsets, weights (both gradients)
+// grad, y, order, position, offsets, weights (both gradients)
 PyObject* from_clusters_grad(PyObject*, PyObject* const* a, Py_ssize_t count) {
     return shortcut([&]() -> PyObject* {
         Rows grad, y;
         Places at;
         Floats weights;
-        if (count != 5 || a[4] == Py_None || !grad.take(a[0]) || !y.take(a[1], &grad.t) || !at.take(a[2], a[3], grad.t) || !weights.take(a[4], at.position.sizes(), grad.t)) return none();
+        if (count != 6 || a[5] == Py_None || !grad.take(a[0]) || !y.take(a[1], &grad.t) || !at.take(a + 2, grad.t) || !weights.take(a[5], at.position.sizes(), grad.t)) return none();
         if (grad.n != at.n || y.n != at.n * at.m || y.d != grad.d || y.kind != grad.kind) return none();
         const at::Tensor grad_y = make({static_cast<int64_t>(y.n), static_cast<int64_t>(y.d)}, grad.t.scalar_type(), grad.t);
         const at::Tensor grad_weights = make(at.position.sizes(), at::kFloat, grad.t);
-        const skm_status status = skm_op_from_clusters_grad(grad.t.get_device(), grad.t.const_data_ptr(), grad.ld, y.t.const_data_ptr(), y.ld, grad.kind, grad.d, at.positions(), at.starts(), at.k, at.n, at.m,
+        const skm_status status = skm_op_from_clusters_grad(grad.t.get_device(), grad.t.const_data_ptr(), grad.ld, y.t.const_data_ptr(), y.ld, grad.kind, grad.d, at.pairs(), at.positions(), at.starts(), at.k, at.n, at.m,
                                       weights.p(), grad_y.data_ptr(), grad_weights.data_ptr<float>(), stream(grad.t));
         if (status != SKM_OK) return failed(status);
         return wrap(grad_y, grad_weights);

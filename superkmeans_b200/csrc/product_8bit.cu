@@ -26,19 +26,35 @@ namespace {
 // LANES threads to a row, of which each keeps HELD chunks in registers between finding the largest value and dividing by it (the rest of
 // longer rows is read twice), while the next row's are on their way: as many blocks as are resident, in turn over the rows.
 // Rounding is an addition to 1.5 * 2^23, which leaves the whole number in the low bits (its low byte is q).
-template <typename T, int BYTES, int LANES, int HELD>
-__global__ void __launch_bounds__(256) quantize_rows_kernel(const void* __restrict__ x, size_t pitch, size_t n, uint32_t width, int8_t* __restrict__ q, size_t ldq,
+template <typename T, int BYTES, bool WINDOWS, int LANES, int HELD>
+__global__ void __launch_bounds__(256) quantize_rows_kernel(const void* __restrict__ x, size_t pitch, size_t n, uint32_t row_bytes, int8_t* __restrict__ q, size_t ldq,
                                                             float* __restrict__ scales) {
     wait_for_the_one_before();
     using V = Values<T, BYTES>;
     const size_t step = static_cast<size_t>(gridDim.x) * (256 / LANES);
     const uint32_t lane = threadIdx.x % LANES;
-    auto chunks_of = [&](size_t row) { return reinterpret_cast<const Chunk<BYTES>*>(static_cast<const char*>(x) + row * pitch); };
+    const uint32_t width = (row_bytes + BYTES - 1) / BYTES;
+    auto load = [&](size_t row, uint32_t c) {
+        const char* p = static_cast<const char*>(x) + row * pitch + static_cast<size_t>(c) * BYTES;
+        if constexpr (WINDOWS) return load_window<T>(p, 0, min(16u, row_bytes - c * 16));
+        else return load_chunk<BYTES>(reinterpret_cast<const Chunk<BYTES>*>(p));
+    };
+    // the values of chunk c: zeros behind the row
+    auto values_of = [&](const Chunk<BYTES>& chunk, uint32_t c) {
+        V v;
+        v.from(chunk);
+        if constexpr (WINDOWS) {
+#pragma unroll
+            for (uint32_t i = 0; i < V::N; ++i)
+                if (c * 16 + (i + 1) * sizeof(T) > row_bytes) v.v[i] = 0.f;
+        }
+        return v;
+    };
     Chunk<BYTES> held[HELD];
     auto fetch = [&](size_t row) {
-        const Chunk<BYTES>* from = chunks_of(row < n ? row : 0);   // (behind the last row: the first, for nothing)
+        const size_t from = row < n ? row : 0;   // (behind the last row: the first, for nothing)
 #pragma unroll
-        for (int h = 0; h < HELD; ++h) held[h] = lane + h * LANES < width ? __ldg(from + lane + h * LANES) : zero_chunk<BYTES>();
+        for (int h = 0; h < HELD; ++h) held[h] = lane + h * LANES < width ? load(from, lane + h * LANES) : zero_chunk<BYTES>();
     };
     size_t row = static_cast<size_t>(blockIdx.x) * (256 / LANES) + threadIdx.x / LANES;
     fetch(row);
@@ -46,10 +62,10 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const void* __restri
     for (size_t turn = static_cast<size_t>(blockIdx.x) * (256 / LANES); turn < n; turn += step, row += step) {
         V v[HELD];
 #pragma unroll
-        for (int h = 0; h < HELD; ++h) v[h].from(held[h]);
+        for (int h = 0; h < HELD; ++h) v[h] = values_of(held[h], lane + h * LANES);
         fetch(row + step);
         const bool valid = row < n;
-        const Chunk<BYTES>* from = chunks_of(valid ? row : 0);
+        const size_t from = valid ? row : 0;
         // magnitudes as whole numbers: a NaN is above infinity
         uint32_t most = 0;
         auto look = [&](const V& w) {
@@ -58,11 +74,7 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const void* __restri
         };
 #pragma unroll
         for (int h = 0; h < HELD; ++h) look(v[h]);
-        for (uint32_t c = lane + HELD * LANES; c < width; c += LANES) {
-            V w;
-            w.from(__ldg(from + c));
-            look(w);
-        }
+        for (uint32_t c = lane + HELD * LANES; c < width; c += LANES) look(values_of(load(from, c), c));
 #pragma unroll
         for (int o = (LANES < 32 ? LANES : 32) / 2; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
         if constexpr (LANES > 32) {
@@ -103,17 +115,19 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const void* __restri
                     for (int i = 0; i < V::N / 4; ++i) words[i] = __byte_perm(__byte_perm(b[4 * i], b[4 * i + 1], 0x0040), __byte_perm(b[4 * i + 2], b[4 * i + 3], 0x0040), 0x5410);
                     memcpy(&packed, words, V::N);
                 }
-                *reinterpret_cast<Chunk<V::N>*>(to + at * V::N) = packed;
+                if (WINDOWS && (at + 1) * 16 > row_bytes) {   // (what is behind the row is not written)
+#pragma unroll
+                    for (uint32_t i = 0; i < V::N; ++i)
+                        if (at * 16 + (i + 1) * sizeof(T) <= row_bytes) to[at * V::N + i] = static_cast<int8_t>(b[i]);
+                } else {
+                    *reinterpret_cast<Chunk<V::N>*>(to + at * V::N) = packed;
+                }
             }
         };
 #pragma unroll
         for (int h = 0; h < HELD; ++h)
             if (lane + h * LANES < width) put(v[h], lane + h * LANES);
-        for (uint32_t c = lane + HELD * LANES; c < width; c += LANES) {
-            V w;
-            w.from(__ldg(from + c));
-            put(w, c);
-        }
+        for (uint32_t c = lane + HELD * LANES; c < width; c += LANES) put(values_of(load(from, c), c), c);
     }
 }
 
@@ -800,19 +814,28 @@ ProductPlan make_plan(const Product& p) {
 
 void launch_quantize_rows(const Rows& x, Type type, size_t n, size_t d, int8_t* q, size_t ldq, float* scales, cudaStream_t stream) {
     if (n == 0) return;
-    const size_t t = type_bytes(type), pitch = x.ld * t;
-    with_width(type, access_bytes({address(x.p), pitch, d * t, address(q) * t, ldq * t}), [&](auto value, auto width) {
+    const size_t t = type_bytes(type), pitch = x.ld * t, each = 16 / t;   // (values, and bytes of q, of a 16-byte chunk)
+    const int access = access_bytes({address(x.p), pitch, d * t, address(q) * t, ldq * t});
+    const bool windows = use_windows(access, d * t) && address(q) % each == 0 && ldq % each == 0;
+    with_width(type, windows ? 16 : access, [&](auto value, auto width) {
         using T = decltype(value);
         constexpr int B = decltype(width)::bytes;
-        const uint32_t chunks = static_cast<uint32_t>(d * t / B);
+        const size_t chunks = (d * t + B - 1) / B;
         auto launch = [&](auto* kernel, int lanes) {
             const size_t blocks = (n + 256 / lanes - 1) / (256 / lanes);
-            launch_after(kernel, dim3(static_cast<unsigned>(std::min<size_t>(blocks, static_cast<size_t>(sm_count()) * 8))), 256, 0, stream, x.p, pitch, n, chunks, q, ldq, scales);
+            launch_after(kernel, dim3(static_cast<unsigned>(std::min<size_t>(blocks, static_cast<size_t>(sm_count()) * 8))), 256, 0, stream, x.p, pitch, n, d * t, q, ldq, scales);
         };
-        if (chunks <= 8 * 4) launch(quantize_rows_kernel<T, B, 8, 4>, 8);
-        else if (chunks <= 32 * 4) launch(quantize_rows_kernel<T, B, 32, 4>, 32);
-        else if (chunks <= 32 * 8) launch(quantize_rows_kernel<T, B, 32, 8>, 32);
-        else launch(quantize_rows_kernel<T, B, 256, 4>, 256);
+        auto of_width = [&](auto in_windows) {
+            constexpr bool W = decltype(in_windows)::value;
+            if (chunks <= 8 * 4) launch(quantize_rows_kernel<T, B, W, 8, 4>, 8);
+            else if (chunks <= 32 * 4) launch(quantize_rows_kernel<T, B, W, 32, 4>, 32);
+            else if (chunks <= 32 * 8) launch(quantize_rows_kernel<T, B, W, 32, 8>, 32);
+            else launch(quantize_rows_kernel<T, B, W, 256, 4>, 256);
+        };
+        if constexpr (B == 16) {
+            if (windows) return of_width(std::true_type{});
+        }
+        of_width(std::false_type{});
     });
 }
 

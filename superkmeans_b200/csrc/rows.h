@@ -40,7 +40,8 @@ void launch_lookup(const Rows& table, Type type, size_t k, size_t d, const Ids& 
 void launch_lookup_scale_grad(const Rows& grad, const Rows& table, Type type, size_t k, size_t d, const Ids& ids, size_t n, float scale, float* out, cudaStream_t stream);
 // A grouping of n rows with m choices each, as launch_group leaves it: *held slots (= offsets[k]) have a cluster.
 struct Places {
-    const uint32_t* position;   // n x m
+    const uint32_t* order;      // n x m: which pair is in a slot
+    const uint32_t* position;   // n x m: which slot a pair has
     const uint32_t* held;
     size_t n, m;                // n * m below 2^31; a slot of n * m or more is passed over
 };
@@ -51,6 +52,14 @@ void launch_from_clusters(const Rows& y, Type type, size_t d, const Places& at, 
 // grad_y[position[i][j]] = weights[i][j] * grad[i], zeros behind *held; grad_weights[i][j] = <grad[i], y[position[i][j]]>, zero without a
 // cluster.  Either output may be null; y is read for grad_weights only.
 void launch_from_clusters_grad(const Rows& grad, const Rows& y, Type type, size_t d, const Places& at, const float* weights, void* grad_y, float* grad_weights, cudaStream_t stream);
+
+// ---- rows_unaligned.cu: the same for rows whose address, pitch or length is no multiple of 16 bytes (of 32 bytes or more; outputs begin
+// on 16 bytes)
+void launch_lookup_unaligned(const Rows& table, Type type, size_t k, size_t d, const Ids& ids, size_t n, float scale, const float* row_scales, void* out, cudaStream_t stream);
+void launch_lookup_scale_grad_unaligned(const Rows& grad, const Rows& table, Type type, size_t k, size_t d, const Ids& ids, size_t n, float scale, float* out, cudaStream_t stream);
+void launch_to_clusters_unaligned(const Rows& x, Type type, size_t d, const Places& at, const float* weights, void* out, cudaStream_t stream);   // (scaled by the pair's weight, if given)
+void launch_from_clusters_unaligned(const Rows& y, Type type, size_t d, const Places& at, const float* weights, void* out, cudaStream_t stream);
+void launch_weights_grad_unaligned(const Rows& grad, const Rows& y, Type type, size_t d, const Places& at, float* grad_weights, cudaStream_t stream);
 
 // ---- rows_sum.cu
 // out[c] = sum over ids[i] = c of scale * row_scales[i] * grad[i] for c in [0, k), added in a fixed order

@@ -124,6 +124,29 @@ struct Values {
     }
 };
 
+// The 16 bytes at p, an address of values of T that need not be a multiple of 16, of which bytes from .. to - 1 are wanted: the one or two
+// aligned blocks that hold some of them, shifted.  (A block that holds a byte of the rows is memory of theirs or of the same 16 bytes:
+// nothing beyond is touched.  The bytes that are not wanted are of no meaning.)
+template <typename T>
+__device__ __forceinline__ uint4 load_window(const char* p, uint32_t from, uint32_t to) {
+    const uint32_t s = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p)) & 15u;
+    const uint4* block = reinterpret_cast<const uint4*>(p - s);
+    const uint4 lo = from < 16 - s ? __ldg(block) : make_uint4(0, 0, 0, 0), hi = to > 16 - s ? __ldg(block + 1) : make_uint4(0, 0, 0, 0);
+    uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+    for (int i = 0; i < 6; ++i) w[i] = s & 8 ? w[i + 2] : w[i];
+#pragma unroll
+    for (int i = 0; i < 5; ++i) w[i] = s & 4 ? w[i + 1] : w[i];
+    if constexpr (sizeof(T) == 2) {
+        const uint32_t bits = (s & 2) * 8;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], bits);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+// Rows that 16-byte accesses do not fit, but that are long enough for windows.
+inline bool use_windows(int bytes, size_t row_bytes) { return bytes < 16 && row_bytes >= 32; }
+
 // Kernels that follow one another (launch_after) start before the one ahead has ended and wait for it here, before they touch memory: what
 // that one wrote is visible then.  It is read past the first-level cache (__ldcg), which may hold older lines: a kernel's start, which
 // empties that cache, is no longer behind the end of the one ahead.  (Sort and sums of 500 000 pairs, eight launches: 227 -> 219 us;

@@ -24,7 +24,7 @@ int unit_warps(int bits, size_t n_units) { return bits <= 9 && n_units >= 148 * 
 // A key is the cluster and behind it the pair's number, so that no two are equal: a pair's slot is how many keys are less, and the
 // largest of those says which cluster comes before.  Every block sorts all keys in groups of 32 (a warp a group, by exchanges between
 // lanes) and then looks for the place of one group's keys, one to a lane, in all groups by halving.  (4096 pairs with 1000 clusters:
-// YY us; comparing every pair with every key, 13.)
+// 8 us a call; comparing every pair with every key, 13.)
 constexpr uint32_t kRankWarps = 16;
 constexpr uint32_t kRankAhead = 4;   // groups of a warp at a time
 constexpr int kPairBits = 12;

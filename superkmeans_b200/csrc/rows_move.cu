@@ -3,7 +3,8 @@
 // All of them move rows once and compute next to nothing: they are bound by HBM, or for small calls by the launch.  The rows of an
 // output (or for to_clusters of the input) are taken as one sequence of 32-byte chunks, 128 x 2 of them to a block whatever the rows'
 // width, so that narrow and odd rows fill the lanes as well as wide ones; a row whose address, pitch or width is no multiple of 32
-// bytes is taken in chunks of 16, 8, 4 or 2, 128 x 4 to a block.  Products and sums are in fp32 and rounded once.
+// bytes is taken in chunks of 16, 128 x 4 to a block, and one that these do not fit is left to rows_unaligned.cu, or, if it has less than
+// 32 bytes, taken in chunks of 8, 4 or 2.  Products and sums are in fp32 and rounded once.
 #include "rows_access.cuh"
 
 #include "device_utils.cuh"
@@ -245,7 +246,9 @@ unsigned warp_blocks(size_t n) { return static_cast<unsigned>((n + kThreads / 32
 void launch_lookup(const Rows& table, Type type, size_t k, size_t d, const Ids& ids, size_t n, float scale, const float* row_scales, void* out, cudaStream_t stream) {
     if (n == 0) return;
     const size_t t = type_bytes(type), pitch = table.ld * t;
-    with_width<32>(type, access_bytes({address(table.p), pitch, d * t, address(out)}, 32), [&](auto value, auto width) {
+    const int access = access_bytes({address(table.p), pitch, d * t, address(out)}, 32);
+    if (use_windows(access, d * t) && address(out) % 16 == 0) return launch_lookup_unaligned(table, type, k, d, ids, n, scale, row_scales, out, stream);
+    with_width<32>(type, access, [&](auto value, auto width) {
         using T = decltype(value);
         constexpr int B = decltype(width)::bytes;
         const Spread s = make_spread<B>(n, d * t);
@@ -259,7 +262,9 @@ void launch_lookup(const Rows& table, Type type, size_t k, size_t d, const Ids& 
 void launch_lookup_scale_grad(const Rows& grad, const Rows& table, Type type, size_t k, size_t d, const Ids& ids, size_t n, float scale, float* out, cudaStream_t stream) {
     if (n == 0) return;
     const size_t t = type_bytes(type);
-    with_width(type, access_bytes({address(grad.p), grad.ld * t, address(table.p), table.ld * t, d * t}), [&](auto value, auto width) {
+    const int access = access_bytes({address(grad.p), grad.ld * t, address(table.p), table.ld * t, d * t});
+    if (use_windows(access, d * t)) return launch_lookup_scale_grad_unaligned(grad, table, type, k, d, ids, n, scale, out, stream);
+    with_width(type, access, [&](auto value, auto width) {
         constexpr int B = decltype(width)::bytes;
         lookup_scale_grad_kernel<decltype(value), B><<<warp_blocks(n), kThreads, 0, stream>>>(grad.p, grad.ld * t, table.p, table.ld * t, static_cast<uint32_t>(k), ids.p, ids.wide, n, scale, out,
                                                                                             static_cast<uint32_t>(d * t / B));
@@ -270,7 +275,9 @@ void launch_lookup_scale_grad(const Rows& grad, const Rows& table, Type type, si
 void launch_to_clusters(const Rows& x, Type type, size_t d, const Places& at, void* out, cudaStream_t stream) {
     if (at.n == 0) return;
     const size_t t = type_bytes(type), pitch = x.ld * t;
-    with_width<32>(type, access_bytes({address(x.p), pitch, d * t, address(out)}, 32), [&](auto, auto width) {
+    const int access = access_bytes({address(x.p), pitch, d * t, address(out)}, 32);
+    if (use_windows(access, d * t) && address(out) % 16 == 0) return launch_to_clusters_unaligned(x, type, d, at, nullptr, out, stream);
+    with_width<32>(type, access, [&](auto, auto width) {
         constexpr int B = decltype(width)::bytes;
         const Spread s = make_spread<B>(at.n, d * t);
         to_clusters_kernel<B><<<spread_blocks(s, kAhead<B>), kThreads, 0, stream>>>(x.p, pitch, at, static_cast<Chunk<B>*>(out), s);
@@ -281,7 +288,9 @@ void launch_to_clusters(const Rows& x, Type type, size_t d, const Places& at, vo
 void launch_from_clusters(const Rows& y, Type type, size_t d, const Places& at, const float* weights, void* out, cudaStream_t stream) {
     if (at.n == 0) return;
     const size_t t = type_bytes(type), pitch = y.ld * t;
-    with_width<32>(type, access_bytes({address(y.p), pitch, d * t, address(out)}, 32), [&](auto value, auto width) {
+    const int access = access_bytes({address(y.p), pitch, d * t, address(out)}, 32);
+    if (use_windows(access, d * t) && address(out) % 16 == 0) return launch_from_clusters_unaligned(y, type, d, at, weights, out, stream);
+    with_width<32>(type, access, [&](auto value, auto width) {
         constexpr int B = decltype(width)::bytes;
         const Spread s = make_spread<B>(at.n, d * t);
         from_clusters_kernel<decltype(value), B><<<spread_blocks(s, kAhead<B> / 2), kThreads, 0, stream>>>(y.p, pitch, at, weights, static_cast<Chunk<B>*>(out), s);
@@ -292,7 +301,13 @@ void launch_from_clusters(const Rows& y, Type type, size_t d, const Places& at, 
 void launch_from_clusters_grad(const Rows& grad, const Rows& y, Type type, size_t d, const Places& at, const float* weights, void* grad_y, float* grad_weights, cudaStream_t stream) {
     if (at.n == 0) return;
     const size_t t = type_bytes(type);
-    with_width(type, access_bytes({address(grad.p), grad.ld * t, address(y.p), y.ld * t, d * t, address(grad_y)}), [&](auto value, auto width) {
+    const int access = access_bytes({address(grad.p), grad.ld * t, address(y.p), y.ld * t, d * t, address(grad_y)});
+    if (use_windows(access, d * t) && address(grad_y) % 16 == 0) {
+        if (grad_y) launch_to_clusters_unaligned(grad, type, d, at, weights, grad_y, stream);
+        if (grad_weights) launch_weights_grad_unaligned(grad, y, type, d, at, grad_weights, stream);
+        return;
+    }
+    with_width(type, access, [&](auto value, auto width) {
         constexpr int B = decltype(width)::bytes;
         from_clusters_grad_kernel<decltype(value), B><<<warp_blocks(at.n), kThreads, 0, stream>>>(grad.p, grad.ld * t, y.p, y.ld * t, at, weights, static_cast<Chunk<B>*>(grad_y), grad_weights,
                                                                                                static_cast<uint32_t>(d * t / B));

@@ -24,11 +24,13 @@ struct SumParams {
     const float* row_scales;
     float scale;
     uint32_t n, k, d;
+    uint32_t row_bytes;
     uint32_t width;            // chunks to a row
     uint32_t slabs;            // of 32 chunks
     uint32_t tile;             // pairs to a tile
     uint32_t join_ids;         // ids to a warp of the second launch
-    float* partials;           // per tile two rows of d: the first run, and the last if it is another
+    uint32_t apart;            // d, rounded up to whole chunks
+    float* partials;           // per tile two rows `apart` from one another: the first run, and the last if it is another
     void* out;
 };
 
@@ -54,6 +56,16 @@ struct Sums {
 #pragma unroll
         for (int i = 0; i < N; ++i) v[i] = fmaf(f, x.v[i], v[i]);
     }
+    // the first `count` of them
+    template <typename O>
+    __device__ __forceinline__ void store_some(O* to, float scale, uint32_t count) const {
+#pragma unroll
+        for (uint32_t i = 0; i < N; ++i)
+            if (i < count) {
+                if constexpr (sizeof(O) == 4) to[i] = v[i] * scale;
+                else reinterpret_cast<uint16_t*>(to)[i] = static_cast<uint16_t>(pair_from_float(v[i] * scale, 0.f, static_cast<const O*>(nullptr)));
+            }
+    }
     template <typename O>
     __device__ __forceinline__ void store(O* to, float scale) const {
         constexpr int ALL = N * static_cast<int>(sizeof(O)), EACH = ALL < 16 ? ALL : 16, PART = EACH / static_cast<int>(sizeof(O));
@@ -67,8 +79,25 @@ struct Sums {
     }
 };
 
+// A chunk of a row of the gradient, and the output's values that belong to it.  WINDOWS: rows that 16-byte accesses do not fit.
+template <typename T, int BYTES, bool WINDOWS>
+struct Lane {
+    uint32_t bytes;   // of the chunk that are the row's
+
+    __device__ __forceinline__ Lane(uint32_t row_bytes, uint32_t col) : bytes(WINDOWS ? min(16u, row_bytes - col * 16) : BYTES) {}
+    __device__ __forceinline__ Chunk<BYTES> load(const char* p) const {
+        if constexpr (WINDOWS) return load_window<T>(p, 0, bytes);
+        else return load_chunk<BYTES>(reinterpret_cast<const Chunk<BYTES>*>(p));
+    }
+    template <typename O>
+    __device__ __forceinline__ void store(const Sums<T, BYTES>& sum, O* to, float scale) const {
+        if constexpr (WINDOWS) sum.template store_some<O>(to, scale, bytes / sizeof(T));
+        else sum.template store<O>(to, scale);
+    }
+};
+
 // SCALED: each pair with a factor of its own; otherwise the sums are scaled.
-template <typename T, typename O, int BYTES, bool SCALED>
+template <typename T, typename O, int BYTES, bool WINDOWS, bool SCALED>
 __global__ void __launch_bounds__(32 * kWarps) sum_tiles_kernel(const SumParams p) {
     wait_for_the_one_before();
     constexpr uint32_t AHEAD = kAhead;
@@ -82,7 +111,8 @@ __global__ void __launch_bounds__(32 * kWarps) sum_tiles_kernel(const SumParams 
     const bool mine = col < p.width;
     const uint32_t s0 = static_cast<uint32_t>(begin), s1 = min(s0 + p.tile, held);
     const size_t at = static_cast<size_t>(col) * S::N;
-    float* first_part = p.partials + tile * 2 * p.d + at;
+    float* first_part = p.partials + tile * 2 * p.apart + at;
+    const Lane<T, BYTES, WINDOWS> chunk(p.row_bytes, mine ? col : 0);
     const char* grad = static_cast<const char*>(p.grad) + static_cast<size_t>(mine ? col : 0) * BYTES;
     const float scale = SCALED ? 1.f : p.scale;
     S sum;
@@ -103,7 +133,7 @@ __global__ void __launch_bounds__(32 * kWarps) sum_tiles_kernel(const SumParams 
 #pragma unroll
             for (uint32_t u = 0; u < AHEAD; ++u) {
                 const uint32_t pair = __shfl_sync(0xffffffffu, my_pair, u0 + u);   // (behind the last: row 0, which is not added)
-                c[u] = load_chunk<BYTES>(reinterpret_cast<const Chunk<BYTES>*>(grad + pair * p.pitch));
+                c[u] = chunk.load(grad + pair * p.pitch);
             }
             const uint32_t here = begins >> u0 & ((1u << AHEAD) - 1);
             if (here == 0 && u0 + AHEAD <= count) {
@@ -120,7 +150,7 @@ __global__ void __launch_bounds__(32 * kWarps) sum_tiles_kernel(const SumParams 
                 if (here >> u & 1) {
                     if (mine) {
                         if (first) sum.template store<float>(first_part, scale);
-                        else sum.template store<O>(static_cast<O*>(p.out) + static_cast<size_t>(now) * p.d + at, scale);
+                        else chunk.store(sum, static_cast<O*>(p.out) + static_cast<size_t>(now) * p.d + at, scale);
                     }
                     sum.clear();
                     first = false;
@@ -133,14 +163,14 @@ __global__ void __launch_bounds__(32 * kWarps) sum_tiles_kernel(const SumParams 
             }
         }
     }
-    if (mine) sum.template store<float>(first ? first_part : first_part + p.d, scale);
+    if (mine) sum.template store<float>(first ? first_part : first_part + p.apart, scale);
 }
 
 // Up to 32 ids and 32 chunks to a warp; ids whose pairs fill many tiles are taken by all eight warps of a block together.
 constexpr int kJoinWarps = 8;
 constexpr uint32_t kLongRun = 8;   // tiles
 
-template <typename T, typename O, int BYTES>
+template <typename T, typename O, int BYTES, bool WINDOWS>
 __global__ void __launch_bounds__(32 * kJoinWarps) join_tiles_kernel(const SumParams p) {
     wait_for_the_one_before();
     using S = Sums<T, BYTES>;
@@ -151,6 +181,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_tiles_kernel(const SumPa
     const bool mine = col < p.width;
     const size_t at = static_cast<size_t>(col) * S::N;
     O* out = static_cast<O*>(p.out) + at;
+    const Lane<T, BYTES, WINDOWS> chunk(p.row_bytes, mine ? col : 0);
     // the tiles t0 .. t1 - 1 of this lane's id, and whether there is something to do: its sum is in the output already if its pairs
     // lie inside their tile, which ends where the pairs with an id end
     uint32_t begin = 0, t0 = 0, t1 = 0;
@@ -170,7 +201,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_tiles_kernel(const SumPa
 #pragma unroll
             for (uint32_t u = 0; u < AHEAD; ++u) {
                 const size_t tile = t + u;
-                const float* src = p.partials + (tile * 2 + (first > tile * p.tile ? 1 : 0)) * p.d + at;
+                const float* src = p.partials + (tile * 2 + (first > tile * p.tile ? 1 : 0)) * p.apart + at;
 #pragma unroll
                 for (int i = 0; i < S::N / EACH; ++i)
                     v[u][i].from(t + u < to && mine ? __ldcg(reinterpret_cast<const Chunk<EACH * 4>*>(src) + i) : zero_chunk<EACH * 4>());
@@ -187,7 +218,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_tiles_kernel(const SumPa
         S sum;
         sum.clear();
         add_tiles(sum, __shfl_sync(0xffffffffu, t0, l), __shfl_sync(0xffffffffu, t1, l), __shfl_sync(0xffffffffu, begin, l));
-        if (mine) sum.template store<O>(out + static_cast<size_t>(id0 + l) * p.d, 1.f);
+        if (mine) chunk.store(sum, out + static_cast<size_t>(id0 + l) * p.d, 1.f);
     }
     if (lane == 0) long_ids[warp] = long_here;
     if (!__syncthreads_or(long_here != 0)) return;
@@ -207,7 +238,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_tiles_kernel(const SumPa
                 for (int q = 1; q < kJoinWarps; ++q)
 #pragma unroll
                     for (int e = 0; e < S::N; ++e) sum.v[e] += parts[q][lane][e];
-                if (mine) sum.template store<O>(out + static_cast<size_t>(id) * p.d, 1.f);
+                if (mine) chunk.store(sum, out + static_cast<size_t>(id) * p.d, 1.f);
             }
             __syncthreads();
         }
@@ -219,7 +250,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_tiles_kernel(const SumPa
 constexpr int kFewWarps = 8;
 constexpr uint32_t kFewSumPairs = 4096;
 
-template <typename T, typename O, int BYTES>
+template <typename T, typename O, int BYTES, bool WINDOWS>
 __global__ void __launch_bounds__(32 * kFewWarps) sum_few_kernel(const SumParams p, const void* __restrict__ ids, bool wide) {
     wait_for_the_one_before();
     using S = Sums<T, BYTES>;
@@ -247,6 +278,7 @@ __global__ void __launch_bounds__(32 * kFewWarps) sum_few_kernel(const SumParams
     S sum;
     sum.clear();
     const char* grad = static_cast<const char*>(p.grad) + static_cast<size_t>(mine ? col : 0) * BYTES;
+    const Lane<T, BYTES, WINDOWS> chunk(p.row_bytes, mine ? col : 0);
     for (uint32_t s = 0; s < count; s += kAhead) {
         Chunk<BYTES> c[kAhead];
         float f[kAhead];
@@ -254,7 +286,7 @@ __global__ void __launch_bounds__(32 * kFewWarps) sum_few_kernel(const SumParams
         for (uint32_t u = 0; u < kAhead; ++u)
             if (s + u < count) {
                 const uint32_t pair = found[warp][s + u];
-                c[u] = load_chunk<BYTES>(reinterpret_cast<const Chunk<BYTES>*>(grad + pair * p.pitch));
+                c[u] = chunk.load(grad + pair * p.pitch);
                 f[u] = p.row_scales ? p.scale * __ldg(p.row_scales + pair) : p.scale;
             }
 #pragma unroll
@@ -271,7 +303,7 @@ __global__ void __launch_bounds__(32 * kFewWarps) sum_few_kernel(const SumParams
         if (counts[w] != 0)
 #pragma unroll
             for (int e = 0; e < S::N; ++e) sum.v[e] += parts[w][lane][e];
-    if (mine) sum.template store<O>(static_cast<O*>(p.out) + static_cast<size_t>(id) * p.d + static_cast<size_t>(col) * S::N, 1.f);
+    if (mine) chunk.store(sum, static_cast<O*>(p.out) + static_cast<size_t>(id) * p.d + static_cast<size_t>(col) * S::N, 1.f);
 }
 
 // (the width of an access is not known where the workspace is sized: it is taken for 16 bytes, and a few more blocks do no harm)
@@ -289,13 +321,14 @@ uint32_t tile_pairs(size_t n, size_t slabs) {
 size_t slabs_of(size_t d, Type type, int bytes) { return (d * type_bytes(type) / bytes + 31) / 32; }
 
 size_t rounded(size_t bytes) { return (bytes + 255) / 256 * 256; }
+size_t whole_chunks(size_t d) { return (d + 7) / 8 * 8; }
 
 } // namespace
 
 size_t lookup_grad_workspace_bytes(size_t n, size_t k, size_t d, Type type) {
     if (few(n, k, d, type)) return 0;
     const size_t tile = tile_pairs(n, slabs_of(d, type, 16)), tiles = (n + tile - 1) / tile;
-    return rounded(n * 4) * 2 + rounded((k + 1) * 4) + rounded(tiles * 2 * d * 4) + rounded(group_workspace_bytes(n, k));
+    return rounded(n * 4) * 2 + rounded((k + 1) * 4) + rounded(tiles * 2 * whole_chunks(d) * 4) + rounded(group_workspace_bytes(n, k));
 }
 
 void launch_lookup_grad(const Rows& grad, Type type, size_t k, size_t d, const Ids& ids, size_t n, float scale, const float* row_scales, void* out, Type out_type, void* workspace,
@@ -320,7 +353,7 @@ void launch_lookup_grad(const Rows& grad, Type type, size_t k, size_t d, const I
         uint32_t* offsets = reinterpret_cast<uint32_t*>(take((k + 1) * 4));
         p.tile = tile_pairs(n, slabs_of(d, type, 16));
         tiles = (n + p.tile - 1) / p.tile;
-        p.partials = reinterpret_cast<float*>(take(tiles * 2 * d * 4));
+        p.partials = reinterpret_cast<float*>(take(tiles * 2 * whole_chunks(d) * 4));
         launch_group(ids, n, k, order, nullptr, keys, offsets, at, stream);
         p.order = order;
         p.keys = keys;
@@ -333,32 +366,42 @@ void launch_lookup_grad(const Rows& grad, Type type, size_t k, size_t d, const I
     p.n = static_cast<uint32_t>(n);
     p.k = static_cast<uint32_t>(k);
     p.d = static_cast<uint32_t>(d);
+    p.row_bytes = static_cast<uint32_t>(d * t);
+    p.apart = static_cast<uint32_t>(whole_chunks(d));
     p.out = out;
     // (the output's chunks have as many values as the input's, and are stored 16 bytes at a time)
     const size_t ot = type_bytes(out_type);
     const int bytes = access_bytes({address(grad.p), p.pitch, d * t, address(out) * t / ot});
-    auto launch = [&](auto value, auto result, auto width) {
+    const bool windows = use_windows(bytes, d * t);
+    auto launch = [&](auto value, auto result, auto width, auto in_windows) {
         using T = decltype(value);
         using O = decltype(result);
         constexpr int B = decltype(width)::bytes;
-        p.width = static_cast<uint32_t>(d * t / B);
+        constexpr bool W = decltype(in_windows)::value;
+        p.width = static_cast<uint32_t>((d * t + B - 1) / B);
         p.slabs = (p.width + 31) / 32;
         if (is_few) {
-            launch_after(sum_few_kernel<T, O, B>, dim3(static_cast<unsigned>(k), p.slabs), 32 * kFewWarps, 0, stream, p, ids.p, ids.wide);
+            launch_after(sum_few_kernel<T, O, B, W>, dim3(static_cast<unsigned>(k), p.slabs), 32 * kFewWarps, 0, stream, p, ids.p, ids.wide);
             return;
         }
         const size_t units = tiles * p.slabs;
-        auto* kernel = row_scales ? sum_tiles_kernel<T, O, B, true> : sum_tiles_kernel<T, O, B, false>;
+        auto* kernel = row_scales ? sum_tiles_kernel<T, O, B, W, true> : sum_tiles_kernel<T, O, B, W, false>;
         launch_after(kernel, dim3(static_cast<unsigned>((units + kWarps - 1) / kWarps)), 32 * kWarps, 0, stream, p);
         // a warp takes its ids one after the other: few, as long as there are warps for them
         p.join_ids = 1;
         while (p.join_ids < 32 && k * p.slabs > static_cast<size_t>(p.join_ids) * 148 * 32) p.join_ids *= 2;
         const size_t ids_of_block = static_cast<size_t>(p.join_ids) * kJoinWarps;
-        launch_after(join_tiles_kernel<T, O, B>, dim3(static_cast<unsigned>((k + ids_of_block - 1) / ids_of_block), p.slabs), 32 * kJoinWarps, 0, stream, p);
+        launch_after(join_tiles_kernel<T, O, B, W>, dim3(static_cast<unsigned>((k + ids_of_block - 1) / ids_of_block), p.slabs), 32 * kJoinWarps, 0, stream, p);
     };
-    with_width(type, bytes, [&](auto value, auto width) {
-        if (out_type == Type::f32) launch(value, float{}, width);
-        else launch(value, value, width);   // (the gradient's own type)
+    auto of_type = [&](auto value, auto width, auto in_windows) {
+        if (out_type == Type::f32) launch(value, float{}, width, in_windows);
+        else launch(value, value, width, in_windows);   // (the gradient's own type)
+    };
+    with_width(type, windows ? 16 : bytes, [&](auto value, auto width) {
+        if constexpr (decltype(width)::bytes == 16) {
+            if (windows) return of_type(value, width, std::true_type{});
+        }
+        of_type(value, width, std::false_type{});
     });
 }
 

@@ -110,21 +110,21 @@ def _floats(t, name: str, shape, like) -> torch.Tensor:
     return t if t.is_contiguous() else t.contiguous()
 
 
-def _groups(groups: RowGroups, like) -> Tuple[torch.Tensor, torch.Tensor, int, int, int]:
-    """position, offsets, number of clusters, rows, choices to a row"""
-    _, position, offsets = groups
-    _on_gpu(position, "position", like)
-    _on_gpu(offsets, "offsets", like)
-    if position.dtype != torch.int32 or offsets.dtype != torch.int32:
-        raise ValueError("position and offsets must have dtype int32")
+def _groups(groups: RowGroups, like) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, int, int, int]:
+    """order, position, offsets, number of clusters, rows, choices to a row"""
+    order, position, offsets = groups
+    for t, name in ((order, "order"), (position, "position"), (offsets, "offsets")):
+        _on_gpu(t, name, like)
+        if t.dtype != torch.int32 or not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous and have dtype int32")
     if position.dim() not in (1, 2) or offsets.dim() != 1 or offsets.shape[0] < 2:
         raise ValueError("position must have one or two dimensions, offsets one with at least two entries")
-    if not (position.is_contiguous() and offsets.is_contiguous()):
-        raise ValueError("position and offsets must be contiguous")
+    if tuple(order.shape) != (position.numel(),):
+        raise ValueError(f"order must have shape ({position.numel()},), got {tuple(order.shape)}")
     m = position.shape[1] if position.dim() == 2 else 1
     if m == 0:
         raise ValueError("a row must have at least one choice")
-    return position, offsets, offsets.shape[0] - 1, position.shape[0], m
+    return order, position, offsets, offsets.shape[0] - 1, position.shape[0], m
 
 
 def _clusters(n_clusters: int) -> int:
@@ -290,31 +290,31 @@ def group_rows(ids: torch.Tensor, n_clusters: int) -> RowGroups:
 
 def _to_clusters(x, groups):
     rows, n_x, d, ld, kind = _rows(x, "x")
-    position, offsets, k, n, m = _groups(groups, x)
+    order, position, offsets, k, n, m = _groups(groups, x)
     if n_x != n:
         raise ValueError(f"x must have {n} rows, got {n_x}")
     out = rows.new_empty((n * m, d))
     index = rows.get_device()
-    _check(_op_to_clusters(index, rows.data_ptr(), ld, kind, d, position.data_ptr(), offsets.data_ptr(), k, n, m, out.data_ptr(), _raw_stream(index)))
+    _check(_op_to_clusters(index, rows.data_ptr(), ld, kind, d, order.data_ptr(), position.data_ptr(), offsets.data_ptr(), k, n, m, out.data_ptr(), _raw_stream(index)))
     return out
 
 
 def _from_clusters(y, groups, weights, name="y"):
     rows, n_y, d, ld, kind = _rows(y, name)
-    position, offsets, k, n, m = _groups(groups, y)
+    order, position, offsets, k, n, m = _groups(groups, y)
     if n_y != n * m:
         raise ValueError(f"{name} must have {n * m} rows, got {n_y}")
     if weights is not None:
         weights = _floats(weights, "weights", position.shape, y)
     out = rows.new_empty((n, d))
     index = rows.get_device()
-    _check(_op_from_clusters(index, rows.data_ptr(), ld, kind, d, position.data_ptr(), offsets.data_ptr(), k, n, m, _p(weights), out.data_ptr(), _raw_stream(index)))
+    _check(_op_from_clusters(index, rows.data_ptr(), ld, kind, d, order.data_ptr(), position.data_ptr(), offsets.data_ptr(), k, n, m, _p(weights), out.data_ptr(), _raw_stream(index)))
     return out
 
 
 def _from_clusters_grad(grad, y, groups, weights, want_y, want_weights):
     rows, n_grad, d, ld, kind = _rows(grad, "grad")
-    position, offsets, k, n, m = _groups(groups, grad)
+    order, position, offsets, k, n, m = _groups(groups, grad)
     if n_grad != n:
         raise ValueError(f"grad must have {n} rows, got {n_grad}")
     if weights is not None:
@@ -327,7 +327,7 @@ def _from_clusters_grad(grad, y, groups, weights, want_y, want_weights):
     grad_y = rows.new_empty((n * m, d)) if want_y else None
     grad_weights = rows.new_empty(position.shape, dtype=torch.float32) if want_weights else None
     index = rows.get_device()
-    _check(_op_from_clusters_grad(index, rows.data_ptr(), ld, _p(from_y), ld_y, kind, d, position.data_ptr(), offsets.data_ptr(), k, n, m, _p(weights), _p(grad_y),
+    _check(_op_from_clusters_grad(index, rows.data_ptr(), ld, _p(from_y), ld_y, kind, d, order.data_ptr(), position.data_ptr(), offsets.data_ptr(), k, n, m, _p(weights), _p(grad_y),
                                         _p(grad_weights), _raw_stream(index)))
     return grad_y, grad_weights
 
@@ -363,7 +363,7 @@ def to_clusters(x: torch.Tensor, groups: RowGroups) -> torch.Tensor:
     """Rows in the order of their clusters: n x d to (n * m) x d, row i once for each of its m choices, at groups.position[i, j].  The rows of
     cluster c are offsets[c] .. offsets[c + 1] - 1; behind the last cluster the slots of choices without one hold zeros.
     Differentiable in x (see to_clusters_grad)."""
-    out = _calls.to_clusters(x, groups[1], groups[2])
+    out = _calls.to_clusters(x, *groups)
     if out is not None:
         return out
     if _wants_grad(x):
@@ -374,7 +374,7 @@ def to_clusters(x: torch.Tensor, groups: RowGroups) -> torch.Tensor:
 def to_clusters_grad(grad: torch.Tensor, groups: RowGroups) -> torch.Tensor:
     """Gradient of the rows of to_clusters: the sum over a row's choices of their slots' gradients (n x d), without those that have no
     cluster."""
-    out = _calls.from_clusters(grad, groups[1], groups[2], None)
+    out = _calls.from_clusters(grad, *groups, None)
     return _from_clusters(grad, groups, None, "grad") if out is None else out
 
 
@@ -382,7 +382,7 @@ def from_clusters(y: torch.Tensor, groups: RowGroups, weights: Optional[torch.Te
     """Rows back from the order of their clusters: out[i] = sum over j of weights[i, j] * y[position[i, j]], n x d.  Choices without a cluster
     contribute nothing, whatever their slots hold.  `weights` (float32, the shape of groups.position) is 1 if not given.
     Differentiable in y and weights (see from_clusters_grad)."""
-    out = _calls.from_clusters(y, groups[1], groups[2], weights)
+    out = _calls.from_clusters(y, *groups, weights)
     if out is not None:
         return out
     if _wants_grad(y, weights):
@@ -393,7 +393,7 @@ def from_clusters(y: torch.Tensor, groups: RowGroups, weights: Optional[torch.Te
 def from_clusters_grad(grad: torch.Tensor, y: torch.Tensor, groups: RowGroups, weights: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """Gradients of from_clusters: of y, weights[i, j] * grad[i] at position[i, j] and zeros in the slots of choices without a cluster; and of the
     weights (float32; None where there are none), <grad[i], y[position[i, j]]>."""
-    out = _calls.from_clusters_grad(grad, y, groups[1], groups[2], weights)
+    out = _calls.from_clusters_grad(grad, y, *groups, weights)
     return _from_clusters_grad(grad, y, groups, weights, True, weights is not None) if out is None else out
 
 

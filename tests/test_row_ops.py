@@ -83,10 +83,11 @@ def test_grouping_refusals():
 
 
 def test_moving_refusals():
-    def to(x=AT, position=AT, offsets=AT, k=4, n=3, m=2, d=8, dtype=0, out=AT):
-        return lib.skm_op_to_clusters(-1, x, 8, dtype, d, position, offsets, k, n, m, out, None)
+    def to(x=AT, order=AT, position=AT, offsets=AT, k=4, n=3, m=2, d=8, dtype=0, out=AT):
+        return lib.skm_op_to_clusters(-1, x, 8, dtype, d, order, position, offsets, k, n, m, out, None)
 
     refused(to(x=None), "NULL")
+    refused(to(order=None), "NULL")
     refused(to(position=None), "NULL")
     refused(to(offsets=None), "NULL")
     refused(to(out=None), "NULL")
@@ -94,10 +95,10 @@ def test_moving_refusals():
     refused(to(n=2**30, m=2), "2^31")
     refused(to(d=0), "dimensionality")
     refused(to(dtype=-1), "dtype")
-    refused(lib.skm_op_from_clusters(-1, None, 8, 0, 8, AT, AT, 4, 3, 2, None, AT, None), "NULL")
+    refused(lib.skm_op_from_clusters(-1, None, 8, 0, 8, AT, AT, AT, 4, 3, 2, None, AT, None), "NULL")
 
     def grad(grad=AT, y=AT, grad_y=AT, grad_weights=AT):
-        return lib.skm_op_from_clusters_grad(-1, grad, 8, y, 8, 0, 8, AT, AT, 4, 3, 2, None, grad_y, grad_weights, None)
+        return lib.skm_op_from_clusters_grad(-1, grad, 8, y, 8, 0, 8, AT, AT, AT, 4, 3, 2, None, grad_y, grad_weights, None)
 
     refused(grad(grad=None), "NULL")
     refused(grad(y=None), "NULL")

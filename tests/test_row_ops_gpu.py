@@ -83,7 +83,7 @@ def plain_lookup(table, ids, scale, row_scales):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("n,k,d", [(1, 1, 1), (2, 7, 3), (31, 10, 50), (257, 1000, 768), (1000, 33, 130), (5000, 4097, 129), (64, 5, 10_001)])
+@pytest.mark.parametrize("n,k,d", [(1, 1, 1), (2, 7, 3), (31, 10, 50), (257, 1000, 768), (1000, 33, 130), (5000, 4097, 129), (64, 5, 10_001), (999, 8, 17), (333, 50, 9), (2, 2, 33)])
 @pytest.mark.parametrize("scale,scaled", [(1.0, False), (11.4, False), (0.5, True)])
 def test_lookup(ops, dtype, n, k, d, scale, scaled):
     g = rng(n + d)
@@ -124,6 +124,46 @@ def test_lookup_of_spread_out_and_narrowed_tables(ops):
     assert torch.equal(ops.lookup(wide, every_other), plain_lookup(wide, every_other, 1.0, None).to(torch.bfloat16))
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("cut", [slice(1, 40), slice(3, 100), slice(7, 136), slice(5, 38)])
+def test_slices_between_values_that_are_no_numbers(ops, dtype, cut):
+    """Rows of odd places and lengths, cut out of larger ones: what lies beside them is neither read into results nor written over."""
+    g = rng(40)
+    d = cut.stop - cut.start
+
+    def beside(n):
+        room = torch.full((n, 150), float("nan"), device="cuda", dtype=dtype)
+        room[:, cut] = randn(g, n, d, dtype=dtype)
+        return room[:, cut]
+
+    table, grad, ids = beside(30), beside(500), some_ids(g, 500, 30)
+    s = torch.exp(randn(g, 500))
+    plain = table.contiguous(), grad.contiguous()
+    assert torch.equal(ops.lookup(table, ids), ops.lookup(plain[0], ids))
+    assert torch.equal(ops.lookup(table, ids, 2.0, s), ops.lookup(plain[0], ids, 2.0, s))
+    for k in (30, 5000):
+        got, want = ops.lookup_grad(grad, ids, k, 1.0, s), ops.lookup_grad(plain[1], ids, k, 1.0, s)
+        close(got, want.double(), rounding(want.double(), dtype, 1e-4) + want.double().abs() * torch.finfo(dtype).eps)
+    close(ops.lookup_scale_grad(grad, table, ids), ops.lookup_scale_grad(*plain[::-1], ids).double(), 1e-4)
+    groups = ops.group_rows(ids.reshape(250, 2), 30)
+    x, w = beside(250), randn(g, 250, 2)
+    assert torch.equal(ops.to_clusters(x, groups), ops.to_clusters(x.contiguous(), groups))
+    assert torch.equal(ops.from_clusters(grad, groups, w), ops.from_clusters(plain[1], groups, w))
+    for a, b in zip(ops.from_clusters_grad(x, grad, groups, w), ops.from_clusters_grad(x.contiguous(), plain[1], groups, w)):
+        close(a, b.double(), 1e-4)
+    for a, b in zip(ops.quantize_rows(x), ops.quantize_rows(x.contiguous())):
+        assert torch.equal(a, b)
+
+
+def test_rows_in_8_bits_leave_what_is_behind_them(ops):
+    from superkmeans_b200 import _lib
+
+    x = torch.randn(20, 39, device="cuda", dtype=torch.bfloat16)
+    room, scales = torch.full((20, 48), 77, dtype=torch.int8, device="cuda"), torch.empty(20, device="cuda")
+    _lib.check(_lib.lib.skm_op_quantize_rows(0, x.data_ptr(), 39, 2, 20, 39, room.data_ptr(), 48, scales.data_ptr(), torch.cuda.current_stream().cuda_stream))
+    assert (room[:, 39:] == 77).all() and torch.equal(room[:, :39], ops.quantize_rows(x).values)
+
+
 def test_values_that_are_no_numbers_stay_in_their_rows(ops):
     table = torch.ones(4, 32, device="cuda")
     table[1] = float("nan")
@@ -139,7 +179,7 @@ def test_values_that_are_no_numbers_stay_in_their_rows(ops):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("n,k,d", [(1, 1, 1), (5, 9, 3), (300, 7, 50), (2001, 300, 130), (4096, 1000, 64), (4097, 1000, 64), (9000, 20, 768), (20_011, 4097, 129), (100, 65_536, 32)])
+@pytest.mark.parametrize("n,k,d", [(1, 1, 1), (5, 9, 3), (300, 7, 50), (2001, 300, 130), (4096, 1000, 64), (4097, 1000, 64), (9000, 20, 768), (20_011, 4097, 129), (100, 65_536, 32), (6000, 50, 17), (5001, 4000, 1003)])
 @pytest.mark.parametrize("skew", [False, True])
 def test_lookup_grad(ops, dtype, n, k, d, skew):
     g = rng(n + k)
@@ -249,7 +289,7 @@ def test_group_rows_of_nothing_and_of_choices(ops):
     assert torch.equal(ops.group_rows(ids.t(), 7).order.cpu().long(), plain_groups(ids.t().contiguous(), 7)[0])
 
 
-MOVES = [(1, 1, 1, 1), (3, 2, 4, 5), (64, 2, 16, 1024), (100, 3, 7, 129), (2000, 8, 300, 50), (5001, 2, 256, 768), (10, 70, 9, 2049)]
+MOVES = [(1, 1, 1, 1), (3, 2, 4, 5), (64, 2, 16, 1024), (100, 3, 7, 129), (2000, 8, 300, 50), (5001, 2, 256, 768), (10, 70, 9, 2049), (1, 1, 3, 17), (777, 3, 20, 39)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -358,7 +398,7 @@ def plain_quantize(x):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("n,d", [(1, 1), (5, 3), (1000, 16), (77, 50), (300, 130), (129, 768), (64, 1025), (33, 2048), (9, 5001), (3, 20_000)])
+@pytest.mark.parametrize("n,d", [(1, 1), (5, 3), (1000, 16), (77, 50), (300, 130), (129, 768), (64, 1025), (33, 2048), (9, 5001), (3, 20_000), (1000, 17), (500, 39), (64, 259)])
 def test_quantize_rows(ops, dtype, n, d):
     g = rng(d)
     x = (randn(g, n, d) * torch.exp(2 * randn(g, n, 1))).to(dtype)
