@@ -6,6 +6,7 @@
 // way round one kernel serves a single row as well as many: the accumulator is as narrow as there are rows, and a warp's 32 lanes write
 // 32 neighbouring results of a row.
 #include <cmath>
+#include <map>
 #include <mutex>
 #include <set>
 #include <string>
@@ -23,6 +24,29 @@ namespace {
 
 // ---------------------------------------------------------------------------------------------- rows to 8 bits
 
+// Magnitudes as whole numbers (a NaN is above infinity): the largest of a chunk's values and `most`.  Halves are compared two at a time,
+// as what they are stored as.
+template <typename T, int BYTES>
+struct Largest {
+    uint32_t most = 0;   // halves: two of them
+
+    __device__ __forceinline__ void look(const Chunk<BYTES>& c) {
+        if constexpr (BYTES == 2) {
+            most = max(most, static_cast<uint32_t>(c) & 0x7fffu);
+        } else {
+            uint32_t w[BYTES / 4];
+            memcpy(w, &c, BYTES);
+#pragma unroll
+            for (int i = 0; i < BYTES / 4; ++i) most = sizeof(T) == 4 ? max(most, w[i] & 0x7fffffffu) : __vmaxu2(most, w[i] & 0x7fff7fffu);
+        }
+    }
+    // as a float's bits
+    __device__ __forceinline__ uint32_t bits() const {
+        if constexpr (sizeof(T) == 4) return most;
+        else return __float_as_uint(pair_to_float(max(most & 0xffffu, most >> 16), static_cast<const T*>(nullptr)).x);
+    }
+};
+
 // LANES threads to a row, of which each keeps HELD chunks in registers between finding the largest value and dividing by it (the rest of
 // longer rows is read twice), while the next row's are on their way: as many blocks as are resident, in turn over the rows.
 // Rounding is an addition to 1.5 * 2^23, which leaves the whole number in the low bits (its low byte is q).
@@ -34,47 +58,42 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const void* __restri
     const size_t step = static_cast<size_t>(gridDim.x) * (256 / LANES);
     const uint32_t lane = threadIdx.x % LANES;
     const uint32_t width = (row_bytes + BYTES - 1) / BYTES;
+    // chunk c of a row: zeros behind the row
     auto load = [&](size_t row, uint32_t c) {
         const char* p = static_cast<const char*>(x) + row * pitch + static_cast<size_t>(c) * BYTES;
-        if constexpr (WINDOWS) return load_window<T>(p, 0, min(16u, row_bytes - c * 16));
-        else return load_chunk<BYTES>(reinterpret_cast<const Chunk<BYTES>*>(p));
-    };
-    // the values of chunk c: zeros behind the row
-    auto values_of = [&](const Chunk<BYTES>& chunk, uint32_t c) {
-        V v;
-        v.from(chunk);
         if constexpr (WINDOWS) {
+            const uint32_t valid = min(16u, row_bytes - c * 16);
+            const uint4 w = load_window<T>(p, 0, valid);
+            uint32_t r[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-            for (uint32_t i = 0; i < V::N; ++i)
-                if (c * 16 + (i + 1) * sizeof(T) > row_bytes) v.v[i] = 0.f;
+            for (uint32_t i = 0; i < 4; ++i) r[i] = valid >= 4 * i + 4 ? r[i] : valid <= 4 * i ? 0u : r[i] & 0xffffu;
+            return make_uint4(r[0], r[1], r[2], r[3]);
+        } else {
+            return load_chunk<BYTES>(reinterpret_cast<const Chunk<BYTES>*>(p));
         }
-        return v;
     };
-    Chunk<BYTES> held[HELD];
+    Chunk<BYTES> held[HELD], next[HELD];
     auto fetch = [&](size_t row) {
         const size_t from = row < n ? row : 0;   // (behind the last row: the first, for nothing)
 #pragma unroll
-        for (int h = 0; h < HELD; ++h) held[h] = lane + h * LANES < width ? load(from, lane + h * LANES) : zero_chunk<BYTES>();
+        for (int h = 0; h < HELD; ++h)
+            if (h * LANES < width) next[h] = lane + h * LANES < width ? load(from, lane + h * LANES) : zero_chunk<BYTES>();
     };
     size_t row = static_cast<size_t>(blockIdx.x) * (256 / LANES) + threadIdx.x / LANES;
     fetch(row);
     // (whole blocks, and with them the warps of the shuffles, take the same number of turns)
     for (size_t turn = static_cast<size_t>(blockIdx.x) * (256 / LANES); turn < n; turn += step, row += step) {
-        V v[HELD];
 #pragma unroll
-        for (int h = 0; h < HELD; ++h) v[h] = values_of(held[h], lane + h * LANES);
+        for (int h = 0; h < HELD; ++h) held[h] = next[h];
         fetch(row + step);
         const bool valid = row < n;
         const size_t from = valid ? row : 0;
-        // magnitudes as whole numbers: a NaN is above infinity
-        uint32_t most = 0;
-        auto look = [&](const V& w) {
+        Largest<T, BYTES> largest_of;
 #pragma unroll
-            for (int i = 0; i < V::N; ++i) most = max(most, __float_as_uint(w.v[i]) & 0x7fffffffu);
-        };
-#pragma unroll
-        for (int h = 0; h < HELD; ++h) look(v[h]);
-        for (uint32_t c = lane + HELD * LANES; c < width; c += LANES) look(values_of(load(from, c), c));
+        for (int h = 0; h < HELD; ++h)
+            if (h * LANES < width) largest_of.look(held[h]);
+        for (uint32_t c = lane + HELD * LANES; c < width; c += LANES) largest_of.look(load(from, c));
+        uint32_t most = largest_of.bits();
 #pragma unroll
         for (int o = (LANES < 32 ? LANES : 32) / 2; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
         if constexpr (LANES > 32) {
@@ -91,13 +110,15 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const void* __restri
         // 127 / largest is a float for all but the smallest, which are taken 2^100 times as large
         const float up = largest < 0x1p-100f ? 0x1p100f : 1.0f;
         const float inverse = some ? __fdiv_rn(127.0f, largest * up) : 0.0f;
+        const bool plain = some && up == 1.0f;
         if (lane == 0) scales[row] = finite ? __fdiv_rn(largest, 127.0f) : __uint_as_float(0x7fc00000u);
         int8_t* to = q + row * ldq;
-        constexpr float kWhole = 12582912.0f;
-        // (the product is rounded before the sum: as one operation on pairs, mul2 and add2, it was not, and values at a half went the other way)
-        auto whole_of = [&](float w) { return __float_as_uint(__fadd_rn(__fmul_rn(w, inverse), kWhole)); };
-        auto put = [&](V w, uint32_t at) {
-            if (up != 1.0f || !some) {
+        // (the product is rounded before the sum: as operations on pairs, mul2 and add2, it was not, and values at a half went the other way)
+        auto whole_of = [&](float w) { return __float_as_uint(__fadd_rn(__fmul_rn(w, inverse), 12582912.0f)); };
+        auto put = [&](const Chunk<BYTES>& chunk, uint32_t at) {
+            V w;
+            w.from(chunk);
+            if (!plain) {
 #pragma unroll
                 for (int i = 0; i < V::N; ++i) w.v[i] = some ? w.v[i] * up : 0.0f;   // (no number times zero is none)
             }
@@ -126,8 +147,8 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const void* __restri
         };
 #pragma unroll
         for (int h = 0; h < HELD; ++h)
-            if (lane + h * LANES < width) put(v[h], lane + h * LANES);
-        for (uint32_t c = lane + HELD * LANES; c < width; c += LANES) put(values_of(load(from, c), c), c);
+            if (lane + h * LANES < width) put(held[h], lane + h * LANES);
+        for (uint32_t c = lane + HELD * LANES; c < width; c += LANES) put(load(from, c), c);
     }
 }
 
@@ -781,6 +802,24 @@ void allow_shared(void (*kernel)(A...), uint32_t bytes) {
     SKM_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)));
 }
 
+// Blocks of a kernel that are resident at a time, looked up once per kernel and device.
+template <typename... A>
+size_t resident_blocks(void (*kernel)(A...), int threads) {
+    static std::mutex mutex;
+    static std::map<std::pair<int, const void*>, size_t> known;
+    int device = 0;
+    SKM_CUDA(cudaGetDevice(&device));
+    std::lock_guard<std::mutex> lock(mutex);
+    size_t& blocks = known[{device, reinterpret_cast<const void*>(kernel)}];
+    if (blocks == 0) {
+        int of_sm = 0, sms = 0;
+        SKM_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&of_sm, kernel, threads, 0));
+        SKM_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device));
+        blocks = static_cast<size_t>(std::max(of_sm, 1)) * sms;
+    }
+    return blocks;
+}
+
 bool tma_takes(const void* p, size_t ld, size_t d) { return (address(p) & 15) == 0 && ld % 16 == 0 && ld >= d; }
 size_t pitch_of(size_t d) { return (d + 15) / 16 * 16; }
 size_t rounded(size_t bytes) { return (bytes + 255) / 256 * 256; }
@@ -822,13 +861,18 @@ void launch_quantize_rows(const Rows& x, Type type, size_t n, size_t d, int8_t* 
         constexpr int B = decltype(width)::bytes;
         const size_t chunks = (d * t + B - 1) / B;
         auto launch = [&](auto* kernel, int lanes) {
-            const size_t blocks = (n + 256 / lanes - 1) / (256 / lanes);
-            launch_after(kernel, dim3(static_cast<unsigned>(std::min<size_t>(blocks, static_cast<size_t>(sm_count()) * 8))), 256, 0, stream, x.p, pitch, n, d * t, q, ldq, scales);
+            // as many blocks as are resident, and the same number of turns for each
+            const size_t blocks = (n + 256 / lanes - 1) / (256 / lanes), resident = resident_blocks(kernel, 256), turns = (blocks + resident - 1) / resident;
+            launch_after(kernel, dim3(static_cast<unsigned>((blocks + turns - 1) / turns)), 256, 0, stream, x.p, pitch, n, d * t, q, ldq, scales);
         };
         auto of_width = [&](auto in_windows) {
             constexpr bool W = decltype(in_windows)::value;
-            if (chunks <= 8 * 4) launch(quantize_rows_kernel<T, B, W, 8, 4>, 8);
-            else if (chunks <= 32 * 4) launch(quantize_rows_kernel<T, B, W, 32, 4>, 32);
+            // as few lanes to a row as hold it: what a warp does once for its rows (shuffles, divisions, addresses) is half of its instructions
+            // (65 536 x 768 bf16: 24 us with 16 lanes, 29 with 32; 500 000 x 64: 20 with 2, 27 with 8)
+            if (chunks <= 2 * 6) launch(quantize_rows_kernel<T, B, W, 2, 6>, 2);
+            else if (chunks <= 4 * 6) launch(quantize_rows_kernel<T, B, W, 4, 6>, 4);
+            else if (chunks <= 8 * 6) launch(quantize_rows_kernel<T, B, W, 8, 6>, 8);
+            else if (chunks <= 16 * 6) launch(quantize_rows_kernel<T, B, W, 16, 6>, 16);
             else if (chunks <= 32 * 8) launch(quantize_rows_kernel<T, B, W, 32, 8>, 32);
             else launch(quantize_rows_kernel<T, B, W, 256, 4>, 256);
         };

@@ -144,8 +144,9 @@ __device__ __forceinline__ uint4 load_window(const char* p, uint32_t from, uint3
     }
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
-// Rows that 16-byte accesses do not fit, but that are long enough for windows.
-inline bool use_windows(int bytes, size_t row_bytes) { return bytes < 16 && row_bytes >= 32; }
+// Where a row's own chunks are read one after the other: by windows if neighbouring lanes could take two bytes each otherwise (100 000
+// rows of 181 fp16 to 8 bits: 31 us against 42), but not if four or eight (50 000 of 1001 fp32: 169 against 101).
+inline bool use_windows(int bytes, size_t row_bytes) { return bytes < 4 && row_bytes >= 32; }
 
 // Kernels that follow one another (launch_after) start before the one ahead has ended and wait for it here, before they touch memory: what
 // that one wrote is visible then.  It is read past the first-level cache (__ldcg), which may hold older lines: a kernel's start, which
@@ -177,6 +178,23 @@ template <typename... P, typename... A>
 void launch_after(void (*kernel)(P...), dim3 grid, unsigned threads, size_t shared, cudaStream_t stream, A&&... args) {
     launch_clusters_after(kernel, grid, 0, threads, shared, stream, std::forward<A>(args)...);
 }
+
+// Some neighbouring lanes of a warp, which may have a row of their own.
+template <int LANES>
+struct Lanes {
+    uint32_t lane, mask;
+    __device__ __forceinline__ Lanes() : lane(threadIdx.x % LANES), mask(LANES == 32 ? 0xffffffffu : ((1u << (LANES & 31)) - 1u) << ((threadIdx.x & 31) / LANES * LANES)) {}
+    template <typename V>
+    __device__ __forceinline__ V from(V v, uint32_t lane_) const {
+        return __shfl_sync(mask, v, lane_, LANES);
+    }
+    __device__ __forceinline__ uint32_t ballot(bool b) const { return __ballot_sync(mask, b) >> (LANES == 32 ? 0 : (threadIdx.x & 31) / LANES * LANES); }
+    __device__ __forceinline__ float sum(float v) const {
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) v += __shfl_xor_sync(mask, v, o, LANES);
+        return v;
+    }
+};
 
 // The cluster of pair i, or k.
 __device__ __forceinline__ uint32_t load_id(const void* ids, bool wide, size_t i, uint32_t k) {

@@ -7,8 +7,6 @@
 // 32 bytes, taken in chunks of 8, 4 or 2.  Products and sums are in fp32 and rounded once.
 #include "rows_access.cuh"
 
-#include "device_utils.cuh"
-
 namespace skmb {
 namespace rows {
 
@@ -170,14 +168,15 @@ __global__ void __launch_bounds__(kThreads) from_clusters_kernel(const void* __r
         if (mine.has(u)) store_chunk<BYTES>(out + row[u] * spread.width.d + col[u], sum[u].to());
 }
 
-// A warp per row of grad: <grad[i], y[slot]> and grad_y[slot] = w * grad[i] for its choices, y read once.
-template <typename T, int BYTES>
+// LANES lanes per row of grad: <grad[i], y[slot]> and grad_y[slot] = w * grad[i] for its choices, y read once.
+template <typename T, int BYTES, int LANES>
 __global__ void __launch_bounds__(kThreads) from_clusters_grad_kernel(const void* __restrict__ grad, size_t grad_pitch, const void* __restrict__ y, size_t y_pitch, const Places at,
                                                                       const float* __restrict__ weights, Chunk<BYTES>* __restrict__ grad_y, float* __restrict__ grad_weights,
                                                                       uint32_t width) {
-    const size_t row = static_cast<size_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
+    const Lanes<LANES> lanes;
+    const size_t row = static_cast<size_t>(blockIdx.x) * (kThreads / LANES) + threadIdx.x / LANES;
     if (row >= at.n) return;
-    const uint32_t lane = threadIdx.x & 31;
+    const uint32_t lane = lanes.lane;
     const uint32_t slots = static_cast<uint32_t>(at.n * at.m), held = min(__ldg(at.held), slots);
     const Chunk<BYTES>* g = row_at<Chunk<BYTES>>(grad, grad_pitch, row);
     for (size_t j = 0; j < at.m; ++j) {
@@ -189,10 +188,10 @@ __global__ void __launch_bounds__(kThreads) from_clusters_grad_kernel(const void
         float dot = 0.f;
         if (!there) {
             if (grad_y && slot < slots)
-                for (uint32_t c = lane; c < width; c += 32) store_chunk<BYTES>(to + c, zero_chunk<BYTES>());
+                for (uint32_t c = lane; c < width; c += LANES) store_chunk<BYTES>(to + c, zero_chunk<BYTES>());
         } else {
 #pragma unroll 4
-            for (uint32_t c = lane; c < width; c += 32) {
+            for (uint32_t c = lane; c < width; c += LANES) {
                 Values<T, BYTES> a;
                 a.from(load_chunk<BYTES>(g + c));
                 if (grad_weights) {
@@ -209,25 +208,26 @@ __global__ void __launch_bounds__(kThreads) from_clusters_grad_kernel(const void
             }
         }
         if (grad_weights) {
-            dot = warp_sum(dot);
+            dot = lanes.sum(dot);
             if (lane == 0) grad_weights[row * at.m + j] = dot;
         }
     }
 }
 
-template <typename T, int BYTES>
+template <typename T, int BYTES, int LANES>
 __global__ void __launch_bounds__(kThreads) lookup_scale_grad_kernel(const void* __restrict__ grad, size_t grad_pitch, const void* __restrict__ table, size_t table_pitch, uint32_t k,
                                                                      const void* __restrict__ ids, bool wide, size_t n, float scale, float* __restrict__ out, uint32_t width) {
-    const size_t row = static_cast<size_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
+    const Lanes<LANES> lanes;
+    const size_t row = static_cast<size_t>(blockIdx.x) * (kThreads / LANES) + threadIdx.x / LANES;
     if (row >= n) return;
-    const uint32_t lane = threadIdx.x & 31;
+    const uint32_t lane = lanes.lane;
     const uint32_t id = load_id(ids, wide, row, k);
     float dot = 0.f;
     if (id < k) {
         const Chunk<BYTES>* g = row_at<Chunk<BYTES>>(grad, grad_pitch, row);
         const Chunk<BYTES>* t = row_at<Chunk<BYTES>>(table, table_pitch, id);
 #pragma unroll 4
-        for (uint32_t c = lane; c < width; c += 32) {
+        for (uint32_t c = lane; c < width; c += LANES) {
             Values<T, BYTES> a, b;
             a.from(load_chunk<BYTES>(g + c));
             b.from(load_chunk<BYTES>(t + c));
@@ -235,11 +235,13 @@ __global__ void __launch_bounds__(kThreads) lookup_scale_grad_kernel(const void*
             for (int i = 0; i < a.N; ++i) dot = fmaf(a.v[i], b.v[i], dot);
         }
     }
-    dot = warp_sum(dot);
+    dot = lanes.sum(dot);
     if (lane == 0) out[row] = id < k ? scale * dot : 0.f;
 }
 
-unsigned warp_blocks(size_t n) { return static_cast<unsigned>((n + kThreads / 32 - 1) / (kThreads / 32)); }
+// Lanes to a row: eight where it has no more than 16 chunks (200 000 x 64 bf16: ZZ).
+bool few_chunks(size_t chunks) { return chunks <= 16; }
+unsigned row_blocks(size_t n, int lanes) { return static_cast<unsigned>((n + kThreads / lanes - 1) / (kThreads / lanes)); }
 
 } // namespace
 
@@ -247,7 +249,7 @@ void launch_lookup(const Rows& table, Type type, size_t k, size_t d, const Ids& 
     if (n == 0) return;
     const size_t t = type_bytes(type), pitch = table.ld * t;
     const int access = access_bytes({address(table.p), pitch, d * t, address(out)}, 32);
-    if (use_windows(access, d * t) && address(out) % 16 == 0) return launch_lookup_unaligned(table, type, k, d, ids, n, scale, row_scales, out, stream);
+    if (access < 16 && d * t >= 32 && address(out) % 16 == 0) return launch_lookup_unaligned(table, type, k, d, ids, n, scale, row_scales, out, stream);
     with_width<32>(type, access, [&](auto value, auto width) {
         using T = decltype(value);
         constexpr int B = decltype(width)::bytes;
@@ -266,7 +268,9 @@ void launch_lookup_scale_grad(const Rows& grad, const Rows& table, Type type, si
     if (use_windows(access, d * t)) return launch_lookup_scale_grad_unaligned(grad, table, type, k, d, ids, n, scale, out, stream);
     with_width(type, access, [&](auto value, auto width) {
         constexpr int B = decltype(width)::bytes;
-        lookup_scale_grad_kernel<decltype(value), B><<<warp_blocks(n), kThreads, 0, stream>>>(grad.p, grad.ld * t, table.p, table.ld * t, static_cast<uint32_t>(k), ids.p, ids.wide, n, scale, out,
+        const bool narrow = few_chunks(d * t / B);
+        auto* kernel = narrow ? lookup_scale_grad_kernel<decltype(value), B, 8> : lookup_scale_grad_kernel<decltype(value), B, 32>;
+        kernel<<<row_blocks(n, narrow ? 8 : 32), kThreads, 0, stream>>>(grad.p, grad.ld * t, table.p, table.ld * t, static_cast<uint32_t>(k), ids.p, ids.wide, n, scale, out,
                                                                                             static_cast<uint32_t>(d * t / B));
     });
     SKM_LAUNCH_CHECK();
@@ -276,7 +280,7 @@ void launch_to_clusters(const Rows& x, Type type, size_t d, const Places& at, vo
     if (at.n == 0) return;
     const size_t t = type_bytes(type), pitch = x.ld * t;
     const int access = access_bytes({address(x.p), pitch, d * t, address(out)}, 32);
-    if (use_windows(access, d * t) && address(out) % 16 == 0) return launch_to_clusters_unaligned(x, type, d, at, nullptr, out, stream);
+    if (access < 16 && d * t >= 32 && address(out) % 16 == 0) return launch_to_clusters_unaligned(x, type, d, at, nullptr, out, stream);
     with_width<32>(type, access, [&](auto, auto width) {
         constexpr int B = decltype(width)::bytes;
         const Spread s = make_spread<B>(at.n, d * t);
@@ -289,7 +293,7 @@ void launch_from_clusters(const Rows& y, Type type, size_t d, const Places& at, 
     if (at.n == 0) return;
     const size_t t = type_bytes(type), pitch = y.ld * t;
     const int access = access_bytes({address(y.p), pitch, d * t, address(out)}, 32);
-    if (use_windows(access, d * t) && address(out) % 16 == 0) return launch_from_clusters_unaligned(y, type, d, at, weights, out, stream);
+    if (access < 16 && d * t >= 32 && address(out) % 16 == 0) return launch_from_clusters_unaligned(y, type, d, at, weights, out, stream);
     with_width<32>(type, access, [&](auto value, auto width) {
         constexpr int B = decltype(width)::bytes;
         const Spread s = make_spread<B>(at.n, d * t);
@@ -309,7 +313,9 @@ void launch_from_clusters_grad(const Rows& grad, const Rows& y, Type type, size_
     }
     with_width(type, access, [&](auto value, auto width) {
         constexpr int B = decltype(width)::bytes;
-        from_clusters_grad_kernel<decltype(value), B><<<warp_blocks(at.n), kThreads, 0, stream>>>(grad.p, grad.ld * t, y.p, y.ld * t, at, weights, static_cast<Chunk<B>*>(grad_y), grad_weights,
+        const bool narrow = few_chunks(d * t / B);
+        auto* kernel = narrow ? from_clusters_grad_kernel<decltype(value), B, 8> : from_clusters_grad_kernel<decltype(value), B, 32>;
+        kernel<<<row_blocks(at.n, narrow ? 8 : 32), kThreads, 0, stream>>>(grad.p, grad.ld * t, y.p, y.ld * t, at, weights, static_cast<Chunk<B>*>(grad_y), grad_weights,
                                                                                                static_cast<uint32_t>(d * t / B));
     });
     SKM_LAUNCH_CHECK();

@@ -1,7 +1,7 @@
 // Gradient of a lookup: for every row of the table the sum of the gradients of the pairs that took it, scaled.
 //
 // The pairs are sorted by id (rows_group.cu) and cut into tiles of equal length, so that a row that half of the pairs took is no
-// longer to sum than a thousand rows are.  A warp takes a tile and 32 chunks of its columns, reads the rows that the order names,
+// longer to sum than a thousand rows are.  A warp takes a tile and 32 chunks of its columns (eight lanes a tile where rows have no more than eight), reads the rows that the order names,
 // eight ahead, and adds in fp32 registers; a run of equal ids that lies inside the tile goes straight to the output, the tile's first
 // and last run, which may go on in the neighbours, into partial sums.  A second launch adds the partial sums of each id in the order of
 // their tiles and writes the zeros of ids that nobody took.  Nothing depends on the order of atomics.
@@ -97,17 +97,18 @@ struct Lane {
 };
 
 // SCALED: each pair with a factor of its own; otherwise the sums are scaled.
-template <typename T, typename O, int BYTES, bool WINDOWS, bool SCALED>
+template <typename T, typename O, int BYTES, bool WINDOWS, bool SCALED, int LANES>
 __global__ void __launch_bounds__(32 * kWarps) sum_tiles_kernel(const SumParams p) {
     wait_for_the_one_before();
     constexpr uint32_t AHEAD = kAhead;
     using S = Sums<T, BYTES>;
-    const uint32_t lane = threadIdx.x & 31;
-    const size_t unit = static_cast<size_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
+    const Lanes<LANES> lanes;
+    const uint32_t lane = lanes.lane;
+    const size_t unit = static_cast<size_t>(blockIdx.x) * (32 * kWarps / LANES) + threadIdx.x / LANES;
     const size_t tile = unit / p.slabs, begin = tile * p.tile;
     const uint32_t held = __ldcg(p.offsets + p.k);
     if (begin >= held) return;   // (pairs without an id come last)
-    const uint32_t col = static_cast<uint32_t>(unit - tile * p.slabs) * 32 + lane;
+    const uint32_t col = static_cast<uint32_t>(unit - tile * p.slabs) * LANES + lane;
     const bool mine = col < p.width;
     const uint32_t s0 = static_cast<uint32_t>(begin), s1 = min(s0 + p.tile, held);
     const size_t at = static_cast<size_t>(col) * S::N;
@@ -119,34 +120,34 @@ __global__ void __launch_bounds__(32 * kWarps) sum_tiles_kernel(const SumParams 
     sum.clear();
     uint32_t now = __ldcg(p.keys + s0);
     bool first = true;
-    for (uint32_t s = s0; s < s1; s += 32) {
-        // a lane's pair of the next 32, and where runs of equal ids begin
+    for (uint32_t s = s0; s < s1; s += LANES) {
+        // a lane's pair of the next ones, and where runs of equal ids begin
         const uint32_t my = s + lane;
         const uint32_t my_pair = my < s1 ? __ldcg(p.order + my) : 0u, my_key = my < s1 ? __ldcg(p.keys + my) : 0u;
         float my_factor = 0.f;
         if (SCALED && my < s1) my_factor = p.scale * __ldg(p.row_scales + my_pair);
-        const uint32_t above = __shfl_up_sync(0xffffffffu, my_key, 1);
-        const uint32_t begins = __ballot_sync(0xffffffffu, my < s1 && my_key != (lane == 0 ? now : above));
-        const uint32_t count = min(32u, s1 - s);
+        const uint32_t above = lanes.from(my_key, (lane + LANES - 1) % LANES);
+        const uint32_t begins = lanes.ballot(my < s1 && my_key != (lane == 0 ? now : above));
+        const uint32_t count = min(static_cast<uint32_t>(LANES), s1 - s);
         for (uint32_t u0 = 0; u0 < count; u0 += AHEAD) {
             Chunk<BYTES> c[AHEAD];
 #pragma unroll
             for (uint32_t u = 0; u < AHEAD; ++u) {
-                const uint32_t pair = __shfl_sync(0xffffffffu, my_pair, u0 + u);   // (behind the last: row 0, which is not added)
+                const uint32_t pair = lanes.from(my_pair, u0 + u);   // (behind the last: row 0, which is not added)
                 c[u] = chunk.load(grad + pair * p.pitch);
             }
             const uint32_t here = begins >> u0 & ((1u << AHEAD) - 1);
             if (here == 0 && u0 + AHEAD <= count) {
 #pragma unroll
                 for (uint32_t u = 0; u < AHEAD; ++u) {
-                    if (SCALED) sum.add(c[u], __shfl_sync(0xffffffffu, my_factor, u0 + u));
+                    if (SCALED) sum.add(c[u], lanes.from(my_factor, u0 + u));
                     else sum.add(c[u]);
                 }
                 continue;
             }
 #pragma unroll
             for (uint32_t u = 0; u < AHEAD; ++u) {
-                const float f = SCALED ? __shfl_sync(0xffffffffu, my_factor, u0 + u) : 1.f;
+                const float f = SCALED ? lanes.from(my_factor, u0 + u) : 1.f;
                 if (here >> u & 1) {
                     if (mine) {
                         if (first) sum.template store<float>(first_part, scale);
@@ -154,7 +155,7 @@ __global__ void __launch_bounds__(32 * kWarps) sum_tiles_kernel(const SumParams 
                     }
                     sum.clear();
                     first = false;
-                    now = __shfl_sync(0xffffffffu, my_key, u0 + u);
+                    now = lanes.from(my_key, u0 + u);
                 }
                 if (u0 + u < count) {
                     if (SCALED) sum.add(c[u], f);
@@ -379,14 +380,17 @@ void launch_lookup_grad(const Rows& grad, Type type, size_t k, size_t d, const I
         constexpr int B = decltype(width)::bytes;
         constexpr bool W = decltype(in_windows)::value;
         p.width = static_cast<uint32_t>((d * t + B - 1) / B);
-        p.slabs = (p.width + 31) / 32;
+        const uint32_t lanes = p.width <= 8 ? 8 : 32;
+        p.slabs = (p.width + 31) / 32;   // (one, where the lanes are eight)
         if (is_few) {
             launch_after(sum_few_kernel<T, O, B, W>, dim3(static_cast<unsigned>(k), p.slabs), 32 * kFewWarps, 0, stream, p, ids.p, ids.wide);
             return;
         }
         const size_t units = tiles * p.slabs;
-        auto* kernel = row_scales ? sum_tiles_kernel<T, O, B, W, true> : sum_tiles_kernel<T, O, B, W, false>;
-        launch_after(kernel, dim3(static_cast<unsigned>((units + kWarps - 1) / kWarps)), 32 * kWarps, 0, stream, p);
+        auto* kernel = lanes == 8 ? row_scales ? sum_tiles_kernel<T, O, B, W, true, 8> : sum_tiles_kernel<T, O, B, W, false, 8>
+                                  : row_scales ? sum_tiles_kernel<T, O, B, W, true, 32> : sum_tiles_kernel<T, O, B, W, false, 32>;
+        const size_t of_block = 32 * kWarps / lanes;
+        launch_after(kernel, dim3(static_cast<unsigned>((units + of_block - 1) / of_block)), 32 * kWarps, 0, stream, p);
         // a warp takes its ids one after the other: few, as long as there are warps for them
         p.join_ids = 1;
         while (p.join_ids < 32 && k * p.slabs > static_cast<size_t>(p.join_ids) * 148 * 32) p.join_ids *= 2;

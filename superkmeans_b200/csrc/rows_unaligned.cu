@@ -10,8 +10,6 @@
 // Sums along a row (dots) do take the row's own 16-byte chunks by load_window.
 #include "rows_access.cuh"
 
-#include "device_utils.cuh"
-
 namespace skmb {
 namespace rows {
 
@@ -245,20 +243,21 @@ struct SlotRow {
     }
 };
 
-// out[pair] = scale * <a[row], b[partner of the pair]>, a warp to a row
-template <typename T, class Partner>
+// out[pair] = scale * <a[row], b[partner of the pair]>, LANES lanes to a row
+template <typename T, int LANES, class Partner>
 __global__ void __launch_bounds__(kThreads) dots_kernel(const char* __restrict__ a, size_t pitch_a, const char* __restrict__ b, size_t pitch_b, const Partner partner, size_t n, size_t m,
                                                         uint32_t row_bytes, float scale, float* __restrict__ out) {
-    const size_t row = static_cast<size_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
+    const Lanes<LANES> lanes;
+    const size_t row = static_cast<size_t>(blockIdx.x) * (kThreads / LANES) + threadIdx.x / LANES;
     if (row >= n) return;
-    const uint32_t lane = threadIdx.x & 31;
+    const uint32_t lane = lanes.lane;
     for (size_t j = 0; j < m; ++j) {
         size_t other;
         const bool there = partner.at(row * m + j, other);
         float dot = 0.f;
         if (there) {
 #pragma unroll 2
-            for (uint32_t col = lane * 16; col < row_bytes; col += 512) {
+            for (uint32_t col = lane * 16; col < row_bytes; col += LANES * 16) {
                 const uint32_t valid = min(16u, row_bytes - col);
                 Values<T, 16> x, z;
                 x.from(load_window<T>(a + row * pitch_a + col, 0, valid));
@@ -268,7 +267,7 @@ __global__ void __launch_bounds__(kThreads) dots_kernel(const char* __restrict__
                     if ((i + 1) * sizeof(T) <= valid) dot = fmaf(x.v[i], z.v[i], dot);
             }
         }
-        dot = warp_sum(dot);
+        dot = lanes.sum(dot);
         if (lane == 0) out[row * m + j] = there ? scale * dot : 0.f;
     }
 }
@@ -307,7 +306,10 @@ template <class Partner>
 void launch_dots(const Rows& a, const Rows& b, Type type, size_t d, const Partner& partner, size_t n, size_t m, float scale, float* out, cudaStream_t stream) {
     const size_t t = type_bytes(type);
     with_type(type, [&](auto value) {
-        dots_kernel<decltype(value), Partner><<<static_cast<unsigned>((n + kThreads / 32 - 1) / (kThreads / 32)), kThreads, 0, stream>>>(
+        const bool narrow = d * t <= 16 * 16;
+        const size_t of_block = kThreads / (narrow ? 8 : 32);
+        auto* kernel = narrow ? dots_kernel<decltype(value), 8, Partner> : dots_kernel<decltype(value), 32, Partner>;
+        kernel<<<static_cast<unsigned>((n + of_block - 1) / of_block), kThreads, 0, stream>>>(
             static_cast<const char*>(a.p), a.ld * t, static_cast<const char*>(b.p), b.ld * t, partner, n, m, static_cast<uint32_t>(d * t), scale, out);
     });
     SKM_LAUNCH_CHECK();
