@@ -2,13 +2,11 @@
 // out[i][c] = x_scale[i] * w_scale[c] * sum_j x[i][j] w[c][j].  The sums are whole numbers in 32 bits, hence exact however they are
 // split; a result is rounded when its sum becomes a float, at each of the two scales, and once more to the output's type.
 //
-// tcgen05.mma of kind::i8: the matrix's rows ("channels") are the 128 lanes of the accumulator, the rows of x ("rows") its columns.  That
-// way round one kernel serves a single row as well as many: the accumulator is as narrow as there are rows, and a warp's 32 lanes write
-// 32 neighbouring results of a row.
-#include <cmath>
+// tcgen05.mma of kind::i8, in two kernels.  Few rows: the matrix's rows ("channels") are the 128 lanes of the accumulator, the rows of x
+// ("rows") its columns, so that the accumulator is as narrow as there are rows; one row of 768 by 16 384 channels takes 5.4 us.  Many:
+// pairs of CTAs, below.
 #include <map>
 #include <mutex>
-#include <set>
 #include <string>
 
 #include "rows_access.cuh"
@@ -463,8 +461,14 @@ __global__ void __launch_bounds__(P_THREADS) product_kernel(const __grid_constan
 //   warp 1       MMA issuer (the leader's)
 //   warps 4-11   epilogue: 32 lanes and half of the columns each, out of one accumulator while the other is filled
 // Where rows of the result begin on 32 bytes, the lanes are rows of x: a thread then holds 128 neighbouring results of a row and stores
-// 32 bytes at a time.  Elsewhere, and where the tile is narrow because the groups are small, the lanes are channels, and the 32 lanes of
-// a warp store 32 neighbouring results of a row.
+// 32 bytes at a time, or whole lines by way of shared memory.  Elsewhere, and where the tile is narrow because the groups are small, the
+// lanes are channels, and the 32 lanes of a warp store 32 neighbouring results of a row.
+//
+// One B200: 32 768 x 1024 by 10 000 channels to bf16 262 us, 2560 T/s, the tensor pipe 70 % busy (by 10 001 channels 302; to fp32 355; depth
+// 128: 112; depth 4096: 855, 3140 T/s; the single-CTA kernel 1269).  Power is the bound: the clock falls to 1.5 GHz, and operands of
+// zeros, which do not draw it, are through depth 4096 in 709 us.  Without results to store it would be 208.  Measured and not kept: rows
+// resident in shared memory while the channels pass (266), twice the epilogue warps (314), stores with other cache hints (the same).
+// 65 536 x 768 by 256 clusters of 768 channels 55 us, 302 MB of operands and results: HBM.
 constexpr int Q_EPI_WARPS = 8;
 constexpr int Q_THREADS = 128 + 32 * Q_EPI_WARPS;
 constexpr uint32_t Q_TRAY_BYTES = 32 * 128;   // 32 rows of results on their way out, of each epilogue warp
@@ -788,18 +792,6 @@ void throw_if_told(Status& s, cudaStream_t stream) {
     *told = 0;
     SKM_CUDA(cudaMemsetAsync(s.device, 0, sizeof(int), stream));
     throw CudaError("a product in 8 bits gave up waiting on a barrier (code " + std::to_string(code) + "): its results are not valid");
-}
-
-// Lets a kernel have as much shared memory as it needs, once per kernel and device.
-template <typename... A>
-void allow_shared(void (*kernel)(A...), uint32_t bytes) {
-    static std::mutex mutex;
-    static std::set<std::pair<int, const void*>> done;
-    int device = 0;
-    SKM_CUDA(cudaGetDevice(&device));
-    std::lock_guard<std::mutex> lock(mutex);
-    if (!done.insert({device, reinterpret_cast<const void*>(kernel)}).second) return;
-    SKM_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)));
 }
 
 // Blocks of a kernel that are resident at a time, looked up once per kernel and device.

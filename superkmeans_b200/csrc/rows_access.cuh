@@ -7,6 +7,8 @@
 
 #include <algorithm>
 #include <cstdint>
+#include <mutex>
+#include <set>
 #include <utility>
 
 #include "common.cuh"
@@ -177,6 +179,18 @@ void launch_clusters_after(void (*kernel)(P...), dim3 grid, unsigned cluster, un
 template <typename... P, typename... A>
 void launch_after(void (*kernel)(P...), dim3 grid, unsigned threads, size_t shared, cudaStream_t stream, A&&... args) {
     launch_clusters_after(kernel, grid, 0, threads, shared, stream, std::forward<A>(args)...);
+}
+
+// Lets a kernel have as much shared memory as it needs, once per kernel and device.
+template <typename... A>
+void allow_shared(void (*kernel)(A...), uint32_t bytes) {
+    static std::mutex mutex;
+    static std::set<std::pair<int, const void*>> done;
+    int device = 0;
+    SKM_CUDA(cudaGetDevice(&device));
+    std::lock_guard<std::mutex> lock(mutex);
+    if (!done.insert({device, reinterpret_cast<const void*>(kernel)}).second) return;
+    SKM_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)));
 }
 
 // Some neighbouring lanes of a warp, which may have a row of their own.

