@@ -457,16 +457,18 @@ __global__ void __launch_bounds__(kDirectThreads) direct_scatter_kernel(const vo
     }
 }
 
-// Whether the pairs are sorted so, and how.
+// Whether the pairs are sorted so, and how.  The sizes alone decide: a workspace is asked for before a device is current.
+constexpr size_t kDirectBlocks = 148;   // one to an SM
+
 bool make_direct(size_t n, size_t k, Direct& p) {
-    const size_t digits = k + 1, sms = static_cast<size_t>(std::min(sm_count(), 256));
+    const size_t digits = k + 1;
     if (digits * 12 + 4 * 4 > kDirectShared) return false;
     p.digits = static_cast<uint32_t>(digits);
     p.half_pitch = static_cast<uint32_t>((digits + 1) / 2);
     p.units = 32;
     while (p.units > 4 && 4 * (digits + static_cast<size_t>(p.units) * p.half_pitch) > kDirectShared) p.units /= 2;
     if (4 * (digits + static_cast<size_t>(p.units) * p.half_pitch) > kDirectShared) return false;
-    p.blocks = static_cast<uint32_t>(std::min(sms, (n + 1023) / 1024));
+    p.blocks = static_cast<uint32_t>(std::min(kDirectBlocks, (n + 1023) / 1024));
     const size_t share = (n + static_cast<size_t>(p.blocks) * p.units - 1) / (static_cast<size_t>(p.blocks) * p.units);
     p.share = static_cast<uint32_t>((share + 31) / 32 * 32);
     p.n = static_cast<uint32_t>(n);
