@@ -319,7 +319,7 @@ skm_status skm_op_find_nearest_noalloc(int device, const float* x_dev, const flo
  * overlap (two streams, two graphs that are replayed at once) have one each.
  *
  * Values of rows have one of the types below; sums and products are in fp32 and rounded once.  `ld_*` is the number of elements from
- * one row to the next; outputs are contiguous.  Cluster numbers (ids) are int32, uint32 (ids_bits 32) or int64 (64); one outside
+ * one row to the next; outputs are contiguous.  Pointers are aligned to their type, and to nothing more.  Cluster numbers (ids) are int32, uint32 (ids_bits 32) or int64 (64); one outside
  * [0, k) stands for no cluster.  k and the number of ids stay below 2^31, d is at most 2^20. */
 typedef enum skm_dtype { SKM_F32 = 0, SKM_F16 = 1, SKM_BF16 = 2 } skm_dtype;
 

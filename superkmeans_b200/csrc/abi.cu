@@ -1,6 +1,7 @@
 // extern "C" surface of libskm_b200.so (declared in include/skm_b200.h): translates between the C
 // ABI and the Engine class, and between C++ exceptions and status codes.
 #include <algorithm>
+#include <initializer_list>
 #include <cstring>
 #include <memory>
 #include <new>
@@ -63,8 +64,15 @@ rows::Type type_of(int dtype) {
     return static_cast<rows::Type>(dtype);
 }
 
+// Where values of `bytes` bytes can begin (NULL is for others to refuse).
+void aligned(size_t bytes, std::initializer_list<const void*> pointers) {
+    for (const void* p : pointers) need(reinterpret_cast<uintptr_t>(p) % bytes == 0, "a pointer is not aligned to its type");
+}
+void aligned(rows::Type type, std::initializer_list<const void*> pointers) { aligned(rows::type_bytes(type), pointers); }
+
 rows::Ids ids_of(const void* ids, int bits, uint64_t n) {
     need(bits == 32 || bits == 64, "ids_bits must be 32 or 64");
+    aligned(bits / 8, {ids});
     need(ids || n == 0, "ids must not be NULL");
     return {ids, bits == 64};
 }
@@ -88,6 +96,7 @@ rows::Places places_of(const uint32_t* order, const uint32_t* position, const ui
     need(n <= 0x7fffffff / m, "no more than 2^31 - 1 choices");
     check_sizes(n * m, k);
     need(n == 0 || (order && position && offsets), "order, position and offsets must not be NULL");
+    aligned(4, {order, position, offsets});
     return {order, position, offsets ? offsets + k : nullptr, n, m};
 }
 
@@ -427,6 +436,8 @@ skm_status skm_op_lookup(int device, const void* table, uint64_t ld_table, int d
         check_sizes(n, k);
         check_width(d);
         need(n == 0 || (table && out), "table and out must not be NULL");
+        aligned(type, {table, out});
+        aligned(4, {row_scales});
         const Here here(device);
         rows::launch_lookup({table, ld_table}, type, k, d, at, n, scale, row_scales, out, stream_of(cuda_stream));
     });
@@ -446,6 +457,9 @@ skm_status skm_op_lookup_grad(int device, const void* grad, uint64_t ld_grad, in
         check_sizes(n, k);
         check_width(d);
         need(out && (grad || n == 0), "grad and out must not be NULL");
+        aligned(type, {grad});
+        aligned(out_type, {out});
+        aligned(4, {row_scales});
         if (n > 0) check_workspace(workspace, workspace_bytes, rows::lookup_grad_workspace_bytes(n, k, d, type));
         const Here here(device);
         rows::launch_lookup_grad({grad, ld_grad}, type, k, d, at, n, scale, row_scales, out, out_type, workspace, stream_of(cuda_stream));
@@ -460,6 +474,8 @@ skm_status skm_op_lookup_scale_grad(int device, const void* grad, uint64_t ld_gr
         check_sizes(n, k);
         check_width(d);
         need(n == 0 || (grad && table && out), "grad, table and out must not be NULL");
+        aligned(type, {grad, table});
+        aligned(4, {out});
         const Here here(device);
         rows::launch_lookup_scale_grad({grad, ld_grad}, {table, ld_table}, type, k, d, at, n, scale, out, stream_of(cuda_stream));
     });
@@ -473,6 +489,7 @@ skm_status skm_op_group_rows(int device, const void* ids, int ids_bits, uint64_t
         const rows::Ids at = ids_of(ids, ids_bits, n);
         check_sizes(n, k);
         need(offsets && (n == 0 || (order && position)), "order, position and offsets must not be NULL");
+        aligned(4, {order, position, offsets});
         check_workspace(workspace, workspace_bytes, rows::group_workspace_bytes(n, k));
         const Here here(device);
         rows::launch_group(at, n, k, order, position, nullptr, offsets, workspace, stream_of(cuda_stream));
@@ -486,6 +503,7 @@ skm_status skm_op_to_clusters(int device, const void* x, uint64_t ld_x, int dtyp
         check_width(d);
         const rows::Places at = places_of(order, position, offsets, k, n, m);
         need(n == 0 || (x && out), "x and out must not be NULL");
+        aligned(type, {x, out});
         const Here here(device);
         rows::launch_to_clusters({x, ld_x}, type, d, at, out, stream_of(cuda_stream));
     });
@@ -498,6 +516,8 @@ skm_status skm_op_from_clusters(int device, const void* y, uint64_t ld_y, int dt
         check_width(d);
         const rows::Places at = places_of(order, position, offsets, k, n, m);
         need(n == 0 || (y && out), "y and out must not be NULL");
+        aligned(type, {y, out});
+        aligned(4, {weights});
         const Here here(device);
         rows::launch_from_clusters({y, ld_y}, type, d, at, weights, out, stream_of(cuda_stream));
     });
@@ -512,6 +532,8 @@ skm_status skm_op_from_clusters_grad(int device, const void* grad, uint64_t ld_g
         need(n == 0 || grad, "grad must not be NULL");
         need(n == 0 || grad_y || grad_weights, "one of grad_y and grad_weights must not be NULL");
         need(n == 0 || y || !grad_weights, "y must not be NULL where grad_weights is asked for");
+        aligned(type, {grad, y, grad_y});
+        aligned(4, {weights, grad_weights});
         const Here here(device);
         rows::launch_from_clusters_grad({grad, ld_grad}, {y, y ? ld_y : 0}, type, d, at, weights, grad_y, grad_weights, stream_of(cuda_stream));
     });
@@ -523,6 +545,8 @@ skm_status skm_op_quantize_rows(int device, const void* x, uint64_t ld_x, int dt
         check_width(d);
         need(n <= 0x7fffffff, "no more than 2^31 - 1 rows");
         need(n == 0 || (x && q && scales), "x, q and scales must not be NULL");
+        aligned(type, {x});
+        aligned(4, {scales});
         need(n <= 1 || ld_q >= d, "rows of q must not overlap");
         const Here here(device);
         rows::launch_quantize_rows({x, ld_x}, type, n, d, q, n > 1 ? ld_q : d, scales, stream_of(cuda_stream));
@@ -545,6 +569,8 @@ skm_status skm_op_product_8bit(int device, const int8_t* x, uint64_t ld_x, const
         if (n == 0 || m == 0) return;
         need(x && w && x_scales && w_scales && out, "x, w, their scales and out must not be NULL");
         need(groups == 0 || offsets, "offsets must not be NULL where there are groups");
+        aligned(p.out_type, {out});
+        aligned(4, {x_scales, w_scales, offsets});
         check_workspace(workspace, workspace_bytes, rows::product_workspace_bytes(p));
         p.x_scales = x_scales;
         p.w_scales = w_scales;

@@ -123,6 +123,33 @@ def test_product_refusals():
     refused(lib.skm_op_quantize_rows(-1, None, 8, 0, 4, 8, AT, 16, AT, None), "NULL")
 
 
+def test_pointers_between_values_are_refused():
+    """(No kernel has loads for them: until they were refused such a call answered SKM_OK and left its output as it was.)"""
+    def lookup(table=AT, ids=AT, scales=AT, out=AT, dtype=0, bits=32):
+        return lib.skm_op_lookup(-1, table, 8, dtype, 10, 8, ids, bits, 3, 1.0, scales, out, None)
+
+    refused(lookup(table=AT + 2), "aligned")
+    refused(lookup(table=AT + 1, dtype=2), "aligned")
+    refused(lookup(out=AT + 2), "aligned")
+    refused(lookup(ids=AT + 4, bits=64), "aligned")
+    refused(lookup(scales=AT + 2), "aligned")
+    refused(lib.skm_op_lookup_grad(-1, AT + 2, 8, 0, 10, 8, AT, 32, 100, 1.0, None, AT, 0, None, 0, None), "aligned")
+    refused(lib.skm_op_lookup_grad(-1, AT, 8, 2, 10, 8, AT, 32, 100, 1.0, None, AT + 2, 0, None, 0, None), "aligned")
+    refused(lib.skm_op_lookup_scale_grad(-1, AT, 8, AT + 2, 8, 0, 10, 8, AT, 32, 3, 1.0, AT, None), "aligned")
+    refused(lib.skm_op_lookup_scale_grad(-1, AT, 8, AT, 8, 1, 10, 8, AT, 32, 3, 1.0, AT + 2, None), "aligned")
+    refused(lib.skm_op_group_rows(-1, AT, 32, 100, 10, AT, AT, AT + 2, None, 0, None), "aligned")
+    refused(lib.skm_op_to_clusters(-1, AT + 2, 8, 0, 8, AT, AT, AT, 4, 3, 2, AT, None), "aligned")
+    refused(lib.skm_op_to_clusters(-1, AT, 8, 0, 8, AT, AT + 2, AT, 4, 3, 2, AT, None), "aligned")
+    refused(lib.skm_op_from_clusters(-1, AT, 8, 1, 8, AT, AT, AT, 4, 3, 2, AT + 2, AT, None), "aligned")
+    refused(lib.skm_op_from_clusters(-1, AT, 8, 1, 8, AT, AT, AT, 4, 3, 2, None, AT + 1, None), "aligned")
+    refused(lib.skm_op_from_clusters_grad(-1, AT, 8, AT + 1, 8, 1, 8, AT, AT, AT, 4, 3, 2, AT, AT, AT, None), "aligned")
+    refused(lib.skm_op_from_clusters_grad(-1, AT, 8, AT, 8, 1, 8, AT, AT, AT, 4, 3, 2, AT, AT, AT + 2, None), "aligned")
+    refused(lib.skm_op_quantize_rows(-1, AT + 2, 8, 0, 4, 8, AT, 16, AT, None), "aligned")
+    refused(lib.skm_op_quantize_rows(-1, AT, 8, 0, 4, 8, AT, 16, AT + 1, None), "aligned")
+    refused(lib.skm_op_product_8bit(-1, AT, 16, AT, AT, 16, AT + 2, 5, 7, 16, 0, None, AT, 0, None, 0, None), "aligned")
+    refused(lib.skm_op_product_8bit(-1, AT, 16, AT, AT, 16, AT, 5, 7, 16, 0, None, AT + 2, 0, None, 0, None), "aligned")
+
+
 def test_workspaces_grow_with_what_they_hold():
     assert lib.skm_op_product_8bit_workspace(AT, 16, AT, 16, 5, 7, 16, 0) == 0
     assert lib.skm_op_product_8bit_workspace(AT, 17, AT, 16, 5, 7, 16, 0) >= 5 * 16
