@@ -144,7 +144,7 @@ __global__ void __launch_bounds__(kThreads) move_rows_kernel(const char* __restr
         size_t row = 0;
         float f = 0.f;
         const bool there = r < part.rows && index.at(part.row0 + r, row, f);
-        sources[r] = {there ? from + row * pitch : nullptr, f};
+        sources[r] = there ? Source{from + row * pitch, f} : Source{nullptr, 0.f};   // (zeros, whatever the factor of what is not there)
     }
     __syncthreads();
 #pragma unroll 1

@@ -99,6 +99,26 @@ def test_lookup(ops, dtype, n, k, d, scale, scaled):
     assert not got[as_index(ids, k) < 0].any()
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [5, 16, 33, 130, 257])
+def test_scales_that_are_no_numbers_where_the_id_is_none(ops, dtype, d):
+    """Padding may hold anything: zeros come out, and gradients of zero, exactly."""
+    g = rng(31)
+    n, k = 300, 20
+    table, ids = randn(g, k, d, dtype=dtype), some_ids(g, n, k, lost=0.3)
+    lost = (ids < 0) | (ids >= k)
+    scales = torch.rand(n, generator=g, device="cuda")
+    odd = scales.clone()
+    odd[lost] = torch.tensor([float("inf"), float("-inf"), float("nan")], device="cuda").repeat(n)[: int(lost.sum())]
+    out = ops.lookup(table, ids, 1.0, odd)
+    assert lost.any() and not out[lost].any() and torch.equal(out, ops.lookup(table, ids, 1.0, scales))
+    grad = randn(g, n, d, dtype=dtype)
+    assert torch.equal(ops.lookup_grad(grad, ids, k, 1.0, odd), ops.lookup_grad(grad, ids, k, 1.0, scales))
+    grad[lost] = float("nan")
+    assert not ops.lookup_grad(grad, ids, k, 1.0, odd).isnan().any()
+    assert not ops.lookup_scale_grad(grad, table, ids)[lost].any()
+
+
 @pytest.mark.parametrize("id_dtype", [torch.int32, torch.uint32, torch.int64])
 def test_ids_of_every_type_and_shape(ops, id_dtype):
     g = rng(3)
