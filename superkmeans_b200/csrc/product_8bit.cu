@@ -61,13 +61,13 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const void* __restri
         const char* p = static_cast<const char*>(x) + row * pitch + static_cast<size_t>(c) * BYTES;
         if constexpr (WINDOWS) {
             const uint32_t valid = min(16u, row_bytes - c * 16);
-            const uint4 w = load_window<T>(p, 0, valid);
+            const uint4 w = load_window<T, true>(p, 0, valid);
             uint32_t r[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
             for (uint32_t i = 0; i < 4; ++i) r[i] = valid >= 4 * i + 4 ? r[i] : valid <= 4 * i ? 0u : r[i] & 0xffffu;
             return make_uint4(r[0], r[1], r[2], r[3]);
         } else {
-            return load_chunk<BYTES>(reinterpret_cast<const Chunk<BYTES>*>(p));
+            return load_now(reinterpret_cast<const Chunk<BYTES>*>(p));
         }
     };
     Chunk<BYTES> held[HELD], next[HELD];
@@ -159,7 +159,7 @@ __global__ void __launch_bounds__(256) pad_bytes_kernel(const int8_t* __restrict
         uint32_t v = 0;
 #pragma unroll
         for (uint32_t e = 0; e < 4; ++e)
-            if (4 * j + e < d) v |= static_cast<uint32_t>(static_cast<uint8_t>(__ldg(in + row * ld + 4 * j + e))) << (8 * e);
+            if (4 * j + e < d) v |= load_now(reinterpret_cast<const uint8_t*>(in) + row * ld + 4 * j + e) << (8 * e);
         *reinterpret_cast<uint32_t*>(out + row * pitch + 4 * j) = v;
     }
 }
@@ -176,7 +176,7 @@ struct RowTile {
     uint32_t row0, row1, group;
 };
 
-__device__ __forceinline__ RowTile load_tile(const RowTile* p) { return {__ldcg(&p->row0), __ldcg(&p->row1), __ldcg(&p->group)}; }
+__device__ __forceinline__ RowTile load_tile(const RowTile* p) { return {load_new(&p->row0), load_new(&p->row1), load_new(&p->group)}; }
 
 struct ProductMaps {
     CUtensorMap w, x;
@@ -325,7 +325,7 @@ __global__ void __launch_bounds__(P_THREADS) product_kernel(const __grid_constan
     const uint32_t tile = blockIdx.x / split, channel_tile = tile % p.channel_tiles, row_tile = tile / p.channel_tiles;
     RowTile t;
     if (p.groups) {
-        if (row_tile >= __ldcg(p.n_tiles + 1)) return;   // (the whole cluster)
+        if (row_tile >= load_new(p.n_tiles + 1)) return;   // (the whole cluster)
         t = load_tile(p.tiles + row_tile);
     } else {
         t = {row_tile * ROWS, min(row_tile * ROWS + ROWS, p.n), 0};
@@ -350,7 +350,7 @@ __global__ void __launch_bounds__(P_THREADS) product_kernel(const __grid_constan
         fence_proxy_async();
     }
     if (warp == 0) tmem_alloc(&ctrl->tmem_base, COLS);
-    for (uint32_t r = threadIdx.x; r < ROWS; r += P_THREADS) ctrl->x_scales[r] = t.row0 + r < t.row1 ? __ldcg(p.x_scales + t.row0 + r) : 0.f;
+    for (uint32_t r = threadIdx.x; r < ROWS; r += P_THREADS) ctrl->x_scales[r] = t.row0 + r < t.row1 ? load_new(p.x_scales + t.row0 + r) : 0.f;
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -400,7 +400,7 @@ __global__ void __launch_bounds__(P_THREADS) product_kernel(const __grid_constan
     tc_fence_after();
 
     const bool has_channel = channel < p.m;
-    const float w_scale = has_channel ? __ldg(p.w_scales + static_cast<size_t>(t.group) * p.m + channel) : 0.f;
+    const float w_scale = has_channel ? load_new(p.w_scales + static_cast<size_t>(t.group) * p.m + channel) : 0.f;
     const uint32_t taddr = tmem_base + (warp * 32 << 16), count = t.row1 - t.row0;
     out += static_cast<size_t>(t.row0) * p.m;
     if (split == 1) {
@@ -526,7 +526,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Q_THREADS, 1) produc
     tc_fence_after();
     const uint32_t tmem_base = ctrl->tmem_base;
 
-    const uint32_t row_tiles = p.groups ? __ldcg(p.n_tiles) : (p.n + ROWS - 1) / ROWS;   // that have a group
+    const uint32_t row_tiles = p.groups ? load_new(p.n_tiles) : (p.n + ROWS - 1) / ROWS;   // that have a group
     const uint32_t n_tiles = row_tiles * p.channel_tiles;
     const uint32_t first = blockIdx.x >> 1, step = gridDim.x >> 1;
     // the rows of tile t and its first channel
@@ -614,7 +614,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Q_THREADS, 1) produc
                 column = channel;
                 end = p.m;
                 column_scales = w_scales;
-                lane_scale = valid ? __ldcg(p.x_scales + row) : 0.f;
+                lane_scale = valid ? load_new(p.x_scales + row) : 0.f;
             } else {
                 row = tile.row0 + half * MINE;
                 channel = channel0 + at_lane;
@@ -622,11 +622,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Q_THREADS, 1) produc
                 column = row;
                 end = tile.row1;
                 column_scales = p.x_scales;
-                lane_scale = valid ? __ldg(w_scales + channel) : 0.f;
+                lane_scale = valid ? load_new(w_scales + channel) : 0.f;
             }
             count = end > column ? min(end - column, MINE) : 0;
 #pragma unroll
-            for (uint32_t e = 0; e < EACH; ++e) scale[e] = e * 32 + lane < count ? __ldcg(column_scales + column + e * 32 + lane) : 0.f;
+            for (uint32_t e = 0; e < EACH; ++e) scale[e] = e * 32 + lane < count ? load_new(column_scales + column + e * 32 + lane) : 0.f;
         };
         if (first < n_tiles) look_up(first);
         uint32_t i = 0;
@@ -687,7 +687,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Q_THREADS, 1) produc
         if (LANES_ARE_ROWS && lane == 0) tma_stores_done();
         // rows of no group
         if (p.groups) {
-            const uint32_t all = __ldcg(p.n_tiles + 1), threads = threadIdx.x - 128;
+            const uint32_t all = load_new(p.n_tiles + 1), threads = threadIdx.x - 128;
             for (uint32_t t = row_tiles * p.channel_tiles + first; t < all * p.channel_tiles; t += step) {
                 uint32_t channel0;
                 const RowTile tile = tile_at(t, channel0);
@@ -717,13 +717,13 @@ __global__ void __launch_bounds__(1024) row_tiles_kernel(const uint32_t* __restr
         const uint32_t g = g0 + threadIdx.x;
         uint32_t a = 0, b = 0;
         if (g < groups) {
-            a = min(__ldcg(offsets + g), n);
-            b = min(__ldcg(offsets + g + 1), n);
+            a = min(load_new(offsets + g), n);
+            b = min(load_new(offsets + g + 1), n);
         } else if (g == groups) {
-            a = min(__ldcg(offsets + groups), n);
+            a = min(load_new(offsets + groups), n);
             b = n;
         } else if (g == groups + 1) {
-            b = min(__ldcg(offsets), n);
+            b = min(load_new(offsets), n);
         }
         const uint32_t count = b > a ? (b - a + rows - 1) / rows : 0;
         uint32_t upto = count;

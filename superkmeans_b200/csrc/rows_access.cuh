@@ -53,7 +53,52 @@ __device__ __forceinline__ Chunk<BYTES> zero_chunk() {
     return c;
 }
 
-// Global memory that nobody writes meanwhile, and stores.
+// Loads for kernels that start before the one ahead has ended (launch_after) of what that one may have written: a read-only load (__ldg) is
+// for memory that does not change while the kernel lives, and may be moved ahead of the wait.  load_now reads what is visible
+// behind the wait; load_new passes the first-level cache by as well, for what is read once.
+#define SKM_LOADS(TYPE, SUFFIX, REGISTER)                                                                     \
+    __device__ __forceinline__ TYPE load_now(const TYPE* p) {                                                 \
+        TYPE v;                                                                                               \
+        asm volatile("ld.global." SUFFIX " %0, [%1];" : "=" REGISTER(v) : "l"(p));                            \
+        return v;                                                                                             \
+    }                                                                                                         \
+    __device__ __forceinline__ TYPE load_new(const TYPE* p) {                                                 \
+        TYPE v;                                                                                               \
+        asm volatile("ld.global.cg." SUFFIX " %0, [%1];" : "=" REGISTER(v) : "l"(p));                         \
+        return v;                                                                                             \
+    }
+SKM_LOADS(uint16_t, "u16", "h")
+SKM_LOADS(uint32_t, "u32", "r")
+SKM_LOADS(float, "f32", "f")
+SKM_LOADS(unsigned long long, "u64", "l")
+#undef SKM_LOADS
+__device__ __forceinline__ uint32_t load_now(const uint8_t* p) {
+    uint32_t v;
+    asm volatile("ld.global.u8 %0, [%1];" : "=r"(v) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ uint2 load_now(const uint2* p) {
+    uint2 v;
+    asm volatile("ld.global.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ uint2 load_new(const uint2* p) {
+    uint2 v;
+    asm volatile("ld.global.cg.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ uint4 load_now(const uint4* p) {
+    uint4 v;
+    asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ uint4 load_new(const uint4* p) {
+    uint4 v;
+    asm volatile("ld.global.cg.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+
+// Global memory that nobody writes while the kernel lives, and stores.
 template <int BYTES>
 __device__ __forceinline__ Chunk<BYTES> load_chunk(const Chunk<BYTES>* p) {
     if constexpr (BYTES == 32) {
@@ -129,11 +174,15 @@ struct Values {
 // The 16 bytes at p, an address of values of T that need not be a multiple of 16, of which bytes from .. to - 1 are wanted: the one or two
 // aligned blocks that hold some of them, shifted.  (A block that holds a byte of the rows is memory of theirs or of the same 16 bytes:
 // nothing beyond is touched.  The bytes that are not wanted are of no meaning.)
-template <typename T>
+template <typename T, bool NOW = false>
 __device__ __forceinline__ uint4 load_window(const char* p, uint32_t from, uint32_t to) {
     const uint32_t s = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p)) & 15u;
     const uint4* block = reinterpret_cast<const uint4*>(p - s);
-    const uint4 lo = from < 16 - s ? __ldg(block) : make_uint4(0, 0, 0, 0), hi = to > 16 - s ? __ldg(block + 1) : make_uint4(0, 0, 0, 0);
+    auto load = [](const uint4* b) {
+        if constexpr (NOW) return load_now(b);
+        else return __ldg(b);
+    };
+    const uint4 lo = from < 16 - s ? load(block) : make_uint4(0, 0, 0, 0), hi = to > 16 - s ? load(block + 1) : make_uint4(0, 0, 0, 0);
     uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
     for (int i = 0; i < 6; ++i) w[i] = s & 8 ? w[i + 2] : w[i];
@@ -151,8 +200,7 @@ __device__ __forceinline__ uint4 load_window(const char* p, uint32_t from, uint3
 inline bool use_windows(int bytes, size_t row_bytes) { return bytes < 4 && row_bytes >= 32; }
 
 // Kernels that follow one another (launch_after) start before the one ahead has ended and wait for it here, before they touch memory: what
-// that one wrote is visible then.  It is read past the first-level cache (__ldcg), which may hold older lines: a kernel's start, which
-// empties that cache, is no longer behind the end of the one ahead.  (Sort and sums of 500 000 pairs, eight launches: 227 -> 219 us;
+// that one wrote is visible then, to load_now and load_new.  (Sort and sums of 500 000 pairs, eight launches: 227 -> 219 us;
 // routing of 30 001 x 4 rows: 118 -> 108.)
 __device__ __forceinline__ void wait_for_the_one_before() {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -213,10 +261,10 @@ struct Lanes {
 // The cluster of pair i, or k.
 __device__ __forceinline__ uint32_t load_id(const void* ids, bool wide, size_t i, uint32_t k) {
     if (wide) {
-        const unsigned long long v = __ldg(static_cast<const unsigned long long*>(ids) + i);   // (a negative one is large)
+        const unsigned long long v = load_now(static_cast<const unsigned long long*>(ids) + i);   // (a negative one is large)
         return v < k ? static_cast<uint32_t>(v) : k;
     }
-    return min(__ldg(static_cast<const uint32_t*>(ids) + i), k);
+    return min(load_now(static_cast<const uint32_t*>(ids) + i), k);
 }
 
 // Division of small numbers by one that a launch knows: magic is 0 where multiplication would not give the quotient.

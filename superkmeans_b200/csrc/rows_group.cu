@@ -141,7 +141,7 @@ struct PassInput {
     const uint32_t* pairs;
 };
 
-__device__ __forceinline__ uint32_t key_of(const PassInput& in, size_t i, uint32_t k) { return in.keys ? __ldcg(in.keys + i) : load_id(in.ids, in.wide, i, k); }
+__device__ __forceinline__ uint32_t key_of(const PassInput& in, size_t i, uint32_t k) { return in.keys ? load_new(in.keys + i) : load_id(in.ids, in.wide, i, k); }
 
 constexpr int kSortAhead = 4;
 
@@ -181,12 +181,12 @@ __global__ void __launch_bounds__(256) place_kernel(const Pass p, uint32_t* __re
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     uint4* row = reinterpret_cast<uint4*>(table + static_cast<size_t>(blockIdx.x) * p.pitch);
     const uint32_t n4 = p.pitch / 4;
-    uint4 v = threadIdx.x < n4 ? __ldcg(row + threadIdx.x) : make_uint4(0, 0, 0, 0);
+    uint4 v = threadIdx.x < n4 ? load_new(row + threadIdx.x) : make_uint4(0, 0, 0, 0);
     uint32_t before = 0;
     for (uint32_t s = 0; s < n4; s += 256) {
         const uint32_t i = s + threadIdx.x;
         const uint4 c = v;
-        v = i + 256 < n4 ? __ldcg(row + i + 256) : make_uint4(0, 0, 0, 0);
+        v = i + 256 < n4 ? load_new(row + i + 256) : make_uint4(0, 0, 0, 0);
         const uint32_t four = c.x + c.y + c.z + c.w;
         uint32_t upto = four;
 #pragma unroll
@@ -221,7 +221,7 @@ __global__ void __launch_bounds__(32 * WARPS) scatter_kernel(const PassInput in,
     uint32_t* base = next + apart * WARPS;
     const uint32_t each = (digits + 32 * WARPS - 1) / (32 * WARPS), digit0 = threadIdx.x * each;
     uint32_t mine = 0;
-    for (uint32_t e = 0; e < each && digit0 + e < digits; ++e) mine += __ldcg(totals + digit0 + e);
+    for (uint32_t e = 0; e < each && digit0 + e < digits; ++e) mine += load_new(totals + digit0 + e);
     uint32_t upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -235,12 +235,12 @@ __global__ void __launch_bounds__(32 * WARPS) scatter_kernel(const PassInput in,
     for (uint32_t e = 0; e < each && digit0 + e < digits; ++e) {
         base[digit0 + e] = slot0;
         if (offsets && blockIdx.x == 0 && digit0 + e <= p.k) offsets[digit0 + e] = slot0;
-        slot0 += __ldcg(totals + digit0 + e);
+        slot0 += load_new(totals + digit0 + e);
     }
     __syncthreads();
     for (uint32_t i = threadIdx.x; i < digits * WARPS; i += 32 * WARPS) {
         const uint32_t w = i % WARPS, digit = i / WARPS;
-        if (unit0 + w < p.n_units) next[w * apart + digit] = base[digit] + __ldcg(table + static_cast<size_t>(digit) * p.pitch + unit0 + w);
+        if (unit0 + w < p.n_units) next[w * apart + digit] = base[digit] + load_new(table + static_cast<size_t>(digit) * p.pitch + unit0 + w);
     }
     __syncthreads();
     const size_t begin = static_cast<size_t>(unit) * p.unit, end = min(begin + p.unit, p.n);
@@ -251,7 +251,7 @@ __global__ void __launch_bounds__(32 * WARPS) scatter_kernel(const PassInput in,
             const size_t i = s + u * 32 + lane;
             const bool valid = i < end;
             key[u] = valid ? key_of(in, i, p.k) : 0u;
-            pair[u] = valid && in.pairs ? __ldcg(in.pairs + i) : static_cast<uint32_t>(i);
+            pair[u] = valid && in.pairs ? load_new(in.pairs + i) : static_cast<uint32_t>(i);
         }
 #pragma unroll
         for (int u = 0; u < kSortAhead; ++u) {
@@ -275,14 +275,14 @@ __global__ void __launch_bounds__(32 * WARPS) scatter_kernel(const PassInput in,
 __global__ void __launch_bounds__(256) offsets_kernel(const uint32_t* __restrict__ keys, uint32_t n, uint32_t k, uint32_t* __restrict__ offsets) {
     wait_for_the_one_before();
     const uint32_t lane = threadIdx.x & 31, slot = blockIdx.x * 256 + threadIdx.x;
-    const uint32_t key = slot < n ? __ldcg(keys + slot) : 0u, from = slot == 0 ? 0u : slot < n ? __ldcg(keys + slot - 1) + 1 : 1u;
+    const uint32_t key = slot < n ? load_new(keys + slot) : 0u, from = slot == 0 ? 0u : slot < n ? load_new(keys + slot - 1) + 1 : 1u;
     for (uint32_t left = __ballot_sync(0xffffffffu, slot < n && from <= key); left; left &= left - 1) {
         const int l = __ffs(left) - 1;
         const uint32_t f = __shfl_sync(0xffffffffu, from, l), t = __shfl_sync(0xffffffffu, key, l), v = __shfl_sync(0xffffffffu, slot, l);
         for (uint32_t c = f + lane; c <= t; c += 32) offsets[c] = v;
     }
     // behind the last key, by the grid
-    for (uint32_t c = __ldcg(keys + n - 1) + 1 + slot; c <= k; c += gridDim.x * 256) offsets[c] = n;
+    for (uint32_t c = load_new(keys + n - 1) + 1 + slot; c <= k; c += gridDim.x * 256) offsets[c] = n;
 }
 
 // ---------------------------------------------------------------------------------------------- many pairs, not too many clusters
@@ -330,7 +330,7 @@ __global__ void __launch_bounds__(kDirectThreads) direct_place_kernel(const Dire
     uint32_t v[MOST], sum = 0;
 #pragma unroll
     for (uint32_t r = 0; r < MOST; ++r) {
-        v[r] = r < each && row0 + r < p.blocks && digit < p.digits ? __ldcg(table + static_cast<size_t>(row0 + r) * p.pitch + digit) : 0u;
+        v[r] = r < each && row0 + r < p.blocks && digit < p.digits ? load_new(table + static_cast<size_t>(row0 + r) * p.pitch + digit) : 0u;
         sum += v[r];
     }
     sums[warp][lane] = sum;
@@ -361,7 +361,7 @@ __global__ void __launch_bounds__(kDirectThreads) direct_scatter_kernel(const vo
     for (uint32_t i0 = threadIdx.x; i0 < p.digits; i0 += kDirectThreads * AHEAD) {
         uint32_t v[AHEAD];
 #pragma unroll
-        for (uint32_t u = 0; u < AHEAD; ++u) v[u] = i0 + u * kDirectThreads < p.digits ? __ldcg(totals + i0 + u * kDirectThreads) : 0u;
+        for (uint32_t u = 0; u < AHEAD; ++u) v[u] = i0 + u * kDirectThreads < p.digits ? load_new(totals + i0 + u * kDirectThreads) : 0u;
 #pragma unroll
         for (uint32_t u = 0; u < AHEAD; ++u)
             if (i0 + u * kDirectThreads < p.digits) base[i0 + u * kDirectThreads] = v[u];
@@ -408,7 +408,7 @@ __global__ void __launch_bounds__(kDirectThreads) direct_scatter_kernel(const vo
 #pragma unroll
         for (uint32_t e = 0; e < AHEAD; ++e) {
             const uint32_t i = i0 + e * kDirectThreads;
-            v[e] = i < p.digits ? __ldcg(table + static_cast<size_t>(blockIdx.x) * p.pitch + i) : 0u;
+            v[e] = i < p.digits ? load_new(table + static_cast<size_t>(blockIdx.x) * p.pitch + i) : 0u;
         }
 #pragma unroll
         for (uint32_t e = 0; e < AHEAD; ++e) {
@@ -485,7 +485,7 @@ __global__ void __launch_bounds__(256) offsets_search_kernel(const uint32_t* __r
     uint32_t lo = 0, hi = n;
     while (lo < hi) {
         const uint32_t mid = lo + (hi - lo) / 2;
-        if (__ldcg(keys + mid) < c) lo = mid + 1;
+        if (load_new(keys + mid) < c) lo = mid + 1;
         else hi = mid;
     }
     offsets[c] = lo;

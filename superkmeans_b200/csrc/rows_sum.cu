@@ -90,8 +90,8 @@ struct Lane {
 
     __device__ __forceinline__ Lane(uint32_t row_bytes, uint32_t col) : bytes(WINDOWS ? min(16u, row_bytes - col * 16) : BYTES) {}
     __device__ __forceinline__ Chunk<BYTES> load(const char* p) const {
-        if constexpr (WINDOWS) return load_window<T>(p, 0, bytes);
-        else return load_chunk<BYTES>(reinterpret_cast<const Chunk<BYTES>*>(p));
+        if constexpr (WINDOWS) return load_window<T, true>(p, 0, bytes);
+        else return load_now(reinterpret_cast<const Chunk<BYTES>*>(p));
     }
     template <typename O>
     __device__ __forceinline__ void store(const Sums<T, BYTES>& sum, O* to, float scale) const {
@@ -110,7 +110,7 @@ __global__ void __launch_bounds__(32 * kWarps) sum_tiles_kernel(const SumParams 
     const uint32_t lane = lanes.lane;
     const size_t unit = static_cast<size_t>(blockIdx.x) * (32 * kWarps / LANES) + threadIdx.x / LANES;
     const size_t tile = unit / p.slabs, begin = tile * p.tile;
-    const uint32_t held = __ldcg(p.offsets + p.k);
+    const uint32_t held = load_new(p.offsets + p.k);
     if (begin >= held) return;   // (pairs without an id come last)
     const uint32_t col = static_cast<uint32_t>(unit - tile * p.slabs) * LANES + lane;
     const bool mine = col < p.width;
@@ -122,14 +122,14 @@ __global__ void __launch_bounds__(32 * kWarps) sum_tiles_kernel(const SumParams 
     const float scale = SCALED ? 1.f : p.scale;
     S sum;
     sum.clear();
-    uint32_t now = __ldcg(p.keys + s0);
+    uint32_t now = load_new(p.keys + s0);
     bool first = true;
     for (uint32_t s = s0; s < s1; s += LANES) {
         // a lane's pair of the next ones, and where runs of equal ids begin
         const uint32_t my = s + lane;
-        const uint32_t my_pair = my < s1 ? __ldcg(p.order + my) : 0u, my_key = my < s1 ? __ldcg(p.keys + my) : 0u;
+        const uint32_t my_pair = my < s1 ? load_new(p.order + my) : 0u, my_key = my < s1 ? load_new(p.keys + my) : 0u;
         float my_factor = 0.f;
-        if (SCALED && my < s1) my_factor = p.scale * __ldg(p.row_scales + my_pair);
+        if (SCALED && my < s1) my_factor = p.scale * load_now(p.row_scales + my_pair);
         const uint32_t above = lanes.from(my_key, (lane + LANES - 1) % LANES);
         const uint32_t begins = lanes.ballot(my < s1 && my_key != (lane == 0 ? now : above));
         const uint32_t count = min(static_cast<uint32_t>(LANES), s1 - s);
@@ -192,8 +192,8 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_tiles_kernel(const SumPa
     uint32_t begin = 0, t0 = 0, t1 = 0;
     bool todo = false;
     if (lane < p.join_ids && id0 + lane < p.k) {
-        begin = __ldcg(p.offsets + id0 + lane);
-        const uint32_t end = __ldcg(p.offsets + id0 + lane + 1), held = __ldcg(p.offsets + p.k);
+        begin = load_new(p.offsets + id0 + lane);
+        const uint32_t end = load_new(p.offsets + id0 + lane + 1), held = load_new(p.offsets + p.k);
         t0 = begin / p.tile;
         t1 = end > begin ? (end - 1) / p.tile + 1 : t0;
         todo = !(t1 == t0 + 1 && begin > t0 * p.tile && end < min(static_cast<size_t>(t1) * p.tile, static_cast<size_t>(held)));
@@ -209,7 +209,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_tiles_kernel(const SumPa
                 const float* src = p.partials + (tile * 2 + (first > tile * p.tile ? 1 : 0)) * p.apart + at;
 #pragma unroll
                 for (int i = 0; i < S::N / EACH; ++i)
-                    v[u][i].from(t + u < to && mine ? __ldcg(reinterpret_cast<const Chunk<EACH * 4>*>(src) + i) : zero_chunk<EACH * 4>());
+                    v[u][i].from(t + u < to && mine ? load_new(reinterpret_cast<const Chunk<EACH * 4>*>(src) + i) : zero_chunk<EACH * 4>());
             }
 #pragma unroll
             for (uint32_t u = 0; u < AHEAD; ++u)
@@ -230,7 +230,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_tiles_kernel(const SumPa
     for (uint32_t w = 0; w < kJoinWarps; ++w)
         for (uint32_t left = long_ids[w]; left; left &= left - 1) {   // (the same for the whole block)
             const uint32_t id = block0 + w * p.join_ids + __ffs(left) - 1;
-            const uint32_t first = __ldcg(p.offsets + id), from0 = first / p.tile, to0 = (__ldcg(p.offsets + id + 1) - 1) / p.tile + 1;
+            const uint32_t first = load_new(p.offsets + id), from0 = first / p.tile, to0 = (load_new(p.offsets + id + 1) - 1) / p.tile + 1;
             const uint32_t share = (to0 - from0 + kJoinWarps - 1) / kJoinWarps, from = min(from0 + warp * share, to0);
             S sum;
             sum.clear();
@@ -292,7 +292,7 @@ __global__ void __launch_bounds__(32 * kFewWarps) sum_few_kernel(const SumParams
             if (s + u < count) {
                 const uint32_t pair = found[warp][s + u];
                 c[u] = chunk.load(grad + pair * p.pitch);
-                f[u] = p.row_scales ? p.scale * __ldg(p.row_scales + pair) : p.scale;
+                f[u] = p.row_scales ? p.scale * load_now(p.row_scales + pair) : p.scale;
             }
 #pragma unroll
         for (uint32_t u = 0; u < kAhead; ++u)
