@@ -789,8 +789,13 @@ void throw_if_told(Status& s, cudaStream_t stream) {
     volatile int* told = s.host;
     if (*told == 0) return;
     const int code = *told;
-    *told = 0;
-    SKM_CUDA(cudaMemsetAsync(s.device, 0, sizeof(int), stream));
+    // (under capture the word would be cleared by each replay instead of now: that is left to the next call outside)
+    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+    SKM_CUDA(cudaStreamIsCapturing(stream, &capture));
+    if (capture == cudaStreamCaptureStatusNone) {
+        *told = 0;
+        SKM_CUDA(cudaMemsetAsync(s.device, 0, sizeof(int), stream));
+    }
     throw CudaError("a product in 8 bits gave up waiting on a barrier (code " + std::to_string(code) + "): its results are not valid");
 }
 

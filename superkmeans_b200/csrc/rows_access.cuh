@@ -237,8 +237,10 @@ void allow_shared(void (*kernel)(A...), uint32_t bytes) {
     int device = 0;
     SKM_CUDA(cudaGetDevice(&device));
     std::lock_guard<std::mutex> lock(mutex);
-    if (!done.insert({device, reinterpret_cast<const void*>(kernel)}).second) return;
+    const std::pair<int, const void*> key{device, reinterpret_cast<const void*>(kernel)};
+    if (done.count(key)) return;
     SKM_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)));
+    done.insert(key);
 }
 
 // Some neighbouring lanes of a warp, which may have a row of their own.

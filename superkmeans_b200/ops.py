@@ -402,7 +402,8 @@ def from_clusters_grad(grad: torch.Tensor, y: torch.Tensor, groups: RowGroups, w
 
 def quantize_rows(x: torch.Tensor) -> QuantizedRows:
     """Rows in 8 bits: scales[i] = max |x[i]| / 127 (float32), values[i] = x[i] / scales[i] rounded to the nearest whole number, int8.  A row of
-    zeros has scale 0; a row with a value that is no finite number has scale NaN.  The rows of the result begin on 16 bytes."""
+    zeros has scale 0; a row with a value that is no finite number has scale NaN.  The rows of the result begin on 16 bytes.  No gradient is
+    recorded."""
     out = _calls.quantize_rows(x)
     if out is not None:
         return QuantizedRows(*out)
@@ -432,7 +433,7 @@ def product_8bit(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_sca
     With `offsets` (int32, from group_rows) w is n_clusters x m x d and w_scales n_clusters x m: row i is multiplied by the matrix of the cluster c with
     offsets[c] <= i < offsets[c + 1]; rows of no cluster come out as zeros.
 
-    Rows that do not begin on 16 bytes are copied first; quantize_rows makes rows that do.  d is at most 131071."""
+    Rows that do not begin on 16 bytes are copied first; quantize_rows makes rows that do.  d is at most 131071.  No gradient is recorded."""
     kind = _DTYPES.get(dtype)
     if kind is None:
         raise ValueError(f"dtype must be float32, float16 or bfloat16, got {dtype}")

@@ -551,6 +551,27 @@ def test_a_wait_that_runs_out_in_a_product_is_reported(ops):
         check_product(ops.product_8bit(x, xs, w, ws, dtype=torch.float32), x, xs, w, ws, torch.float32)
 
 
+def test_a_wait_that_ran_out_is_told_under_capture_and_after_it(ops):
+    from superkmeans_b200 import _lib
+
+    g = rng(8)
+    x, w, xs, ws = some_bytes(g, 40, 4096), some_bytes(g, 200, 4096), torch.ones(40, device="cuda"), torch.ones(200, device="cuda")
+    _lib.check(_lib.lib.skm_debug_wait_injection(20_000_000, 1))
+    try:
+        ops.product_8bit(x, xs, w, ws)
+        torch.cuda.synchronize()
+    finally:
+        _lib.check(_lib.lib.skm_debug_wait_injection(0, 0))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match="gave up waiting"):
+            ops.product_8bit(x, xs, w, ws)
+    with pytest.raises(RuntimeError, match="gave up waiting"):
+        ops.check_products()
+    check_product(ops.product_8bit(x, xs, w, ws, dtype=torch.float32), x, xs, w, ws, torch.float32)
+    ops.check_products()
+
+
 # ---- refusals
 
 
