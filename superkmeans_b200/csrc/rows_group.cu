@@ -4,11 +4,11 @@
 // call consists of.
 //
 // More, and up to some 18 000 clusters: a counting sort in three launches.  A block has a part of the pairs and counts its clusters in
-// shared memory; the counts of all blocks become places; and the block, whose warps have a part each, counts again for every warp
-// (two bytes a cluster), adds up, and lets the warps rank equal clusters among 32 neighbours by __match_any_sync, in order, so that the
-// sort is stable; no order of atomics matters.  One B200, a call: 300 000 pairs with 5000 clusters 19 us (two passes of the radix sort 36),
-// 262 144 with 256 17 (one pass 26), 4M with 1000 82 (255).  What bounds it is the latency of each launch's few reads, and from a million
-// pairs on the scattered stores.
+// shared memory; the counts of all blocks become places; and the block gives each of its pairs a place, in order, so that the sort is
+// stable; no order of atomics matters.  Up to 1023 clusters it sorts 4096 pairs at a time in shared memory; with more, its warps have
+// a part each, count again for every warp (two bytes a cluster), add up, and rank equal clusters among 32 neighbours by
+// __match_any_sync.  One B200, a call: 262 144 pairs with 255 clusters 11.5 us (one pass of the radix sort 26), 300 000 with 5000 18 (two passes
+// 36), 4M with 1000 78 (255).  What bounds it is the latency of each launch's few reads, and from a million pairs on the scattered stores.
 //
 // More clusters, or very many pairs: a radix sort of the same kind, up to 11 bits at a time.  A unit of a few hundred pairs belongs to a warp, which counts its digits in shared
 // memory; a block for each digit turns the units' counts into places; and the units, read again, rank equal digits as above.
@@ -457,6 +457,141 @@ __global__ void __launch_bounds__(kDirectThreads) direct_scatter_kernel(const vo
     }
 }
 
+// Up to 1023 clusters: 4096 of a block's pairs at a time are sorted by cluster in shared memory, after which neighbours have neighbouring
+// places and both lists are written in runs.  With few clusters the warps of direct_scatter_kernel rank nearly every 32 pairs by
+// __match_any_sync and write each place by itself.  A call with this kernel and with that one: 262 144 pairs with 16 clusters 10.1 and 12.1 us,
+// with 255 11.5 and 17.4, with 1000 13.7 and 20.1; 4M with 255 66 and 87; 10 000 with 256 10.6 both; 30 000 with 256 10.9 and 10.1; 12M with 16 182 and 168.
+// With more clusters a chunk takes two passes, and 300 000 with 5000 20 and 18, 9M 236 and 150.
+constexpr uint32_t kSortedEach = 4, kSortedChunk = kDirectThreads * kSortedEach, kSortedWarps = kDirectThreads / 32;
+template <uint32_t DIGITS>
+constexpr uint32_t kSortedApart = DIGITS + 2;   // from one warp's counts to the next's
+template <uint32_t DIGITS>
+constexpr uint32_t kSortedShared = 4 * DIGITS + 2 * (2 * kSortedChunk + kSortedWarps * kSortedApart<DIGITS>);
+
+template <uint32_t DIGITS>
+__global__ void __launch_bounds__(kDirectThreads) direct_sorted_kernel(const void* __restrict__ ids, bool wide, const Direct p, const uint32_t* __restrict__ table,
+                                                                       const uint32_t* __restrict__ totals, uint32_t* __restrict__ order, uint32_t* __restrict__ position,
+                                                                       uint32_t* __restrict__ keys_out, uint32_t* __restrict__ offsets) {
+    wait_for_the_one_before();
+    constexpr uint32_t APART = kSortedApart<DIGITS>;
+    static_assert(2 * kSortedWarps * APART >= 4 * kSortedChunk, "the slots have room where the counts were");
+    extern __shared__ uint32_t shared[];
+    __shared__ uint32_t sums[kSortedWarps];
+    uint32_t* base = shared;                                                  // of each cluster: the slot of the block's next pair with it
+    uint16_t* sorted_key = reinterpret_cast<uint16_t*>(shared + DIGITS);
+    uint16_t* sorted_pair = sorted_key + kSortedChunk;                        // (its number in the chunk)
+    uint16_t* counts = sorted_pair + kSortedChunk;                            // of each warp and cluster
+    uint32_t* slots = reinterpret_cast<uint32_t*>(counts);                    // of the chunk's pairs
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const size_t share = static_cast<size_t>(p.units) * p.share, begin = blockIdx.x * share, end = min(begin + share, static_cast<size_t>(p.n));
+    auto sum_before = [&](uint32_t mine) {   // of the threads before this one; a barrier lies between a call's end and the next call
+        uint32_t upto = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t t = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= static_cast<uint32_t>(o)) upto += t;
+        }
+        if (lane == 31) sums[warp] = upto;
+        __syncthreads();
+        uint32_t of_warps = sums[lane];
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t t = __shfl_up_sync(0xffffffffu, of_warps, o);
+            if (lane >= static_cast<uint32_t>(o)) of_warps += t;
+        }
+        const uint32_t before = __shfl_sync(0xffffffffu, of_warps, warp == 0 ? 0 : warp - 1);
+        return upto - mine + (warp == 0 ? 0u : before);
+    };
+    // a warp has 128 neighbouring pairs of a chunk
+    const uint32_t item0 = warp * 32 * kSortedEach + lane;
+    uint32_t id[kSortedEach];
+    auto fetch = [&](size_t chunk0) {
+#pragma unroll
+        for (uint32_t u = 0; u < kSortedEach; ++u) id[u] = chunk0 + item0 + u * 32 < end ? load_id(ids, wide, chunk0 + item0 + u * 32, p.k) : 0u;
+    };
+    fetch(begin);
+    // where each cluster begins, and the block's part of it
+    const bool has = threadIdx.x < p.digits;
+    const uint32_t total = has ? load_new(totals + threadIdx.x) : 0u, before_block = has ? load_new(table + static_cast<size_t>(blockIdx.x) * p.pitch + threadIdx.x) : 0u;
+    const uint32_t slot0 = sum_before(total);
+    if (has) {
+        if (blockIdx.x == 0) offsets[threadIdx.x] = slot0;
+        base[threadIdx.x] = slot0 + before_block;
+    }
+    for (size_t chunk0 = begin; chunk0 < end; chunk0 += kSortedChunk) {
+        const uint32_t count = static_cast<uint32_t>(min(static_cast<size_t>(kSortedChunk), end - chunk0));
+        for (uint32_t i = threadIdx.x; i < kSortedWarps * APART / 2; i += kDirectThreads) slots[i] = 0;
+        __syncthreads();
+        uint16_t* row = counts + warp * APART;
+        uint32_t rank[kSortedEach];
+#pragma unroll
+        for (uint32_t u = 0; u < kSortedEach; ++u) {
+            const bool valid = item0 + u * 32 < count;
+            const uint32_t same = __match_any_sync(0xffffffffu, valid ? id[u] : 0xffffffffu), ahead = __popc(same & ((1u << lane) - 1u));
+            uint32_t before = 0;
+            if (valid) before = row[id[u]];
+            __syncwarp();
+            if (valid && ahead == 0) row[id[u]] = static_cast<uint16_t>(before + __popc(same));
+            __syncwarp();
+            rank[u] = before + ahead;
+        }
+        __syncthreads();
+        // the counts become places: a cluster's of WARPS warps to a thread
+        constexpr uint32_t PARTS = kDirectThreads / DIGITS, WARPS = kSortedWarps / PARTS;
+        uint16_t* column = counts + threadIdx.x % PARTS * WARPS * APART + threadIdx.x / PARTS;
+        uint32_t sum = 0;
+#pragma unroll
+        for (uint32_t w = 0; w < WARPS; ++w) sum += column[w * APART];
+        uint32_t place = sum_before(sum);
+#pragma unroll
+        for (uint32_t w = 0; w < WARPS; ++w) {
+            const uint32_t here = column[w * APART];
+            column[w * APART] = static_cast<uint16_t>(place);
+            place += here;
+        }
+        __syncthreads();
+#pragma unroll
+        for (uint32_t u = 0; u < kSortedEach; ++u)
+            if (item0 + u * 32 < count) {
+                const uint32_t to = row[id[u]] + rank[u];
+                sorted_key[to] = static_cast<uint16_t>(id[u]);
+                sorted_pair[to] = static_cast<uint16_t>(item0 + u * 32);
+            }
+        __syncthreads();
+        fetch(chunk0 + kSortedChunk);
+        // a cluster's place less that of its first pair here, which leaves each pair to add its own; and behind its last one
+        uint32_t key[kSortedEach];
+        bool last[kSortedEach];
+#pragma unroll
+        for (uint32_t u = 0; u < kSortedEach; ++u) {
+            const uint32_t i = threadIdx.x + u * kDirectThreads;
+            if (i >= count) break;
+            key[u] = sorted_key[i];
+            last[u] = i + 1 == count || sorted_key[i + 1] != key[u];
+            if (i == 0 || sorted_key[i - 1] != key[u]) base[key[u]] -= i;
+        }
+        __syncthreads();
+#pragma unroll
+        for (uint32_t u = 0; u < kSortedEach; ++u) {
+            const uint32_t i = threadIdx.x + u * kDirectThreads;
+            if (i >= count) break;
+            const uint32_t slot = base[key[u]] + i, in_chunk = sorted_pair[i];
+            order[slot] = static_cast<uint32_t>(chunk0) + in_chunk;
+            if (keys_out) keys_out[slot] = key[u];
+            slots[in_chunk] = slot;
+        }
+        __syncthreads();
+#pragma unroll
+        for (uint32_t u = 0; u < kSortedEach; ++u) {
+            const uint32_t i = threadIdx.x + u * kDirectThreads;
+            if (i >= count) break;
+            if (last[u]) base[key[u]] += i + 1;
+            if (position) position[chunk0 + i] = slots[i];
+        }
+        __syncthreads();   // (the next counts are where the slots are)
+    }
+}
+
 // Whether the pairs are sorted so, and how.  The sizes alone decide: a workspace is asked for before a device is current.
 constexpr size_t kDirectBlocks = 148;   // one to an SM
 
@@ -474,7 +609,7 @@ bool make_direct(size_t n, size_t k, Direct& p) {
     p.n = static_cast<uint32_t>(n);
     p.k = static_cast<uint32_t>(k);
     p.pitch = static_cast<uint32_t>((digits + 31) / 32 * 32);
-    return static_cast<size_t>(p.units) * p.share < 65536;   // (what two bytes hold)
+    return digits <= 1024 || static_cast<size_t>(p.units) * p.share < 65536;   // (what two bytes hold)
 }
 
 // The same by looking each cluster up, for far more clusters than pairs.
@@ -540,7 +675,14 @@ void launch_group(const Ids& ids, size_t n, size_t k, uint32_t* order, uint32_t*
         allow_shared(direct_scatter_kernel, kDirectShared);
         launch_after(direct_count_kernel, dim3(direct.blocks), kDirectThreads, 4 * direct.digits, stream, ids.p, ids.wide, direct, table);
         launch_after(direct_place_kernel, dim3((direct.digits + 31) / 32), kDirectThreads, 0, stream, direct, table, totals);
-        launch_after(direct_scatter_kernel, dim3(direct.blocks), kDirectThreads, shared, stream, ids.p, ids.wide, direct, table, totals, order, position, keys, offsets);
+        auto sorted = [&](auto digits) {
+            auto* kernel = direct_sorted_kernel<decltype(digits)::value>;
+            allow_shared(kernel, kSortedShared<decltype(digits)::value>);
+            launch_after(kernel, dim3(direct.blocks), kDirectThreads, kSortedShared<decltype(digits)::value>, stream, ids.p, ids.wide, direct, table, totals, order, position, keys, offsets);
+        };
+        if (direct.digits <= 256) sorted(std::integral_constant<uint32_t, 256>{});
+        else if (direct.digits <= 1024) sorted(std::integral_constant<uint32_t, 1024>{});
+        else launch_after(direct_scatter_kernel, dim3(direct.blocks), kDirectThreads, shared, stream, ids.p, ids.wide, direct, table, totals, order, position, keys, offsets);
         return;
     }
     const Plan plan = make_plan(n, k);

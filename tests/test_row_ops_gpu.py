@@ -290,7 +290,7 @@ def plain_groups(ids, k):
 
 
 SORTS = [(1, 1), (2, 1), (33, 5), (1000, 65_536), (4095, 300), (4096, 1), (4097, 1), (5000, 2047), (5000, 2048), (70_000, 255), (140_001, 10_000), (300_000, 5_000_000), (1_100_000, 37), (700, 2**20 - 1), (700, 2**20), (4000, 3_000_000), (1, 3_000_000), (2, 65_536), (3000, 65_537), (150_000, 18_700), (150_000, 18_800), (10_000_000, 300),
-         (9_000_000, 5000)]
+         (9_000_000, 5000), (150_000, 47_700), (150_000, 48_000), (4097, 40_000), (700_000, 255), (700_000, 256), (606_209, 30_000), (700_000, 1023), (700_000, 1024), (20_000_003, 500)]
 
 
 @pytest.mark.parametrize("n,k", SORTS)
