@@ -200,7 +200,7 @@ __device__ __forceinline__ uint4 load_window(const char* p, uint32_t from, uint3
 inline bool use_windows(int bytes, size_t row_bytes) { return bytes < 4 && row_bytes >= 32; }
 
 // Kernels that follow one another (launch_after) start before the one ahead has ended and wait for it here, before they touch memory: what
-// that one wrote is visible then, to load_now and load_new.  (Sort and sums of 500 000 pairs, eight launches: 227 -> 219 us;
+// that one wrote is visible then, to load_now and load_new.  (Sort and sums of 500 000 pairs, by eight launches then: 227 -> 219 us;
 // routing of 30 001 x 4 rows: 118 -> 108.)
 __device__ __forceinline__ void wait_for_the_one_before() {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
