@@ -18,10 +18,25 @@ namespace {
 
 constexpr int64_t kMostIds = 0x7fffffff;
 
+// Whether the storage holds all that the tensor reaches (throws where there is none).
+bool has_memory(const at::Tensor& t) {
+    if (t.numel() == 0) return true;
+    const c10::Storage& storage = t.storage();
+    if (storage.device() != t.device() || t._is_zerotensor()) return false;
+    int64_t ends = t.storage_offset() + 1;
+    for (int64_t i = 0; i < t.dim(); ++i) ends += (t.size(i) - 1) * t.stride(i);
+    return storage.nbytes() >= static_cast<size_t>(ends) * t.element_size() && storage.data() != nullptr;
+}
+
+// Nothing that a call has to refuse whatever it goes on to ask for.
+bool is_ordinary(const at::Tensor& t) {
+    return t.defined() && t.layout() == at::kStrided && !t.unsafeGetTensorImpl()->is_python_dispatch() && has_memory(t);
+}
+
 bool plain(PyObject* o) {
     if (!THPVariable_CheckExact(o)) return false;
     const at::Tensor& t = THPVariable_Unpack(o);
-    return t.defined() && t.is_cuda() && t.layout() == at::kStrided && !t.unsafeGetTensorImpl()->is_python_dispatch() && !t.is_neg();
+    return t.is_cuda() && !t.is_neg() && is_ordinary(t);
 }
 bool wants_grad(const at::Tensor& t) { return t.requires_grad() && at::GradMode::is_enabled(); }
 
@@ -129,6 +144,15 @@ PyObject* shortcut(F&& f) {
     } catch (const std::exception&) {
         return none();
     }
+}
+
+// True where all arguments that are tensors are ordinary ones; ops.py says what is wrong with others
+PyObject* ordinary(PyObject*, PyObject* const* a, Py_ssize_t count) {
+    return shortcut([&]() -> PyObject* {
+        for (Py_ssize_t i = 0; i < count; ++i)
+            if (THPVariable_Check(a[i]) && !is_ordinary(THPVariable_Unpack(a[i]))) return none();
+        Py_RETURN_TRUE;
+    });
 }
 
 // table, ids, scale, row_scales
@@ -305,7 +329,7 @@ PyObject* product_8bit(PyObject*, PyObject* const* a, Py_ssize_t count) {
 }
 
 #define SKM_CALL(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {SKM_CALL(lookup),        SKM_CALL(lookup_grad),        SKM_CALL(lookup_scale_grad), SKM_CALL(group_rows), SKM_CALL(to_clusters),
+PyMethodDef methods[] = {SKM_CALL(ordinary),      SKM_CALL(lookup),           SKM_CALL(lookup_grad),        SKM_CALL(lookup_scale_grad), SKM_CALL(group_rows), SKM_CALL(to_clusters),
                          SKM_CALL(from_clusters), SKM_CALL(from_clusters_grad), SKM_CALL(quantize_rows),     SKM_CALL(product_8bit), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_ops_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -12,7 +12,7 @@ device (which need not be the current device), allocates its outputs and its wor
 captured into a CUDA graph.  Calls with tensors that need no conversion take a short cut in C++ (csrc/ops_calls.cpp), which answers None
 where there is something to refuse, copy or record; those are made here.  Tensors that are used on another stream than the one they were made on need `record_stream`, as with
 any operator of torch.  Rows may have any distance from one another; the values of a row lie side by side, or the rows are copied
-first.  Arguments that do not fit raise ValueError.
+first.  Arguments that do not fit raise ValueError, and so do tensors whose memory is not there (a storage that was freed).
 """
 from __future__ import annotations
 
@@ -27,7 +27,7 @@ try:
 except ImportError:   # (not built, or for another torch: every call takes the way through ctypes)
 
     class _calls:   # noqa: N801
-        lookup = lookup_grad = lookup_scale_grad = group_rows = to_clusters = from_clusters = from_clusters_grad = quantize_rows = product_8bit = staticmethod(lambda *_: None)
+        ordinary = lookup = lookup_grad = lookup_scale_grad = group_rows = to_clusters = from_clusters = from_clusters_grad = quantize_rows = product_8bit = staticmethod(lambda *_: None)
 
 
 # (looked up once: a call on a few rows takes as long as the host takes to make it)
@@ -59,6 +59,30 @@ class QuantizedRows(NamedTuple):
 
 
 # ---- checks ---------------------------------------------------------------------------------------------------------------------
+
+
+def _check_memory(t, name: str) -> None:
+    """A storage may be smaller than a tensor of its reaches (freed by `resize_`), or not be there at all (zeros and fakes that torch holds as
+    shapes only): the address of a part of it would be followed all the same."""
+    if t.numel() == 0:
+        return
+    storage = t.untyped_storage()
+    ends = t.storage_offset() + 1 + sum((n - 1) * step for n, step in zip(t.shape, t.stride()))
+    if storage.device != t.device or t._is_zerotensor() or storage.nbytes() < ends * t.element_size() or storage.data_ptr() == 0:
+        raise ValueError(f"{name} has no memory, or less than its shape takes")
+
+
+def _named(groups) -> dict:
+    return dict(zip(RowGroups._fields, groups))
+
+
+def _check_ordinary(**tensors) -> None:
+    """What no call can do without, whatever it goes on to ask for."""
+    if _calls.ordinary(*tensors.values()):
+        return
+    for name, t in tensors.items():
+        if isinstance(t, torch.Tensor):
+            _check_memory(t, name)
 
 
 def _on_gpu(t, name: str, like=None) -> None:
@@ -213,6 +237,7 @@ def lookup(table: torch.Tensor, ids: torch.Tensor, scale: float = 1.0, row_scale
     out = _calls.lookup(table, ids, scale, row_scales)
     if out is not None:
         return out
+    _check_ordinary(table=table, ids=ids, row_scales=row_scales)
     if _wants_grad(table, row_scales):
         return _Lookup.apply(table, ids, scale, row_scales)
     return _lookup(table, ids, scale, row_scales)
@@ -226,6 +251,7 @@ def lookup_grad(grad: torch.Tensor, ids: torch.Tensor, n_rows: int, scale: float
         out = _calls.lookup_grad(grad, ids, n_rows, float(scale), row_scales)
         if out is not None:
             return out
+    _check_ordinary(grad=grad, ids=ids, row_scales=row_scales)
     rows, n, d, ld, kind = _rows(grad, "grad")
     at, bits = _ids(ids, "ids", grad)
     if at.shape != (n,):
@@ -251,6 +277,7 @@ def lookup_scale_grad(grad: torch.Tensor, table: torch.Tensor, ids: torch.Tensor
     out = _calls.lookup_scale_grad(grad, table, ids, float(scale))
     if out is not None:
         return out
+    _check_ordinary(grad=grad, table=table, ids=ids)
     rows, n, d, ld, kind = _rows(grad, "grad")
     t, k, d_t, ld_t, _ = _rows(table, "table", grad, grad.dtype)
     at, bits = _ids(ids, "ids", grad)
@@ -275,6 +302,7 @@ def group_rows(ids: torch.Tensor, n_clusters: int) -> RowGroups:
     out = _calls.group_rows(ids, n_clusters)
     if out is not None:
         return RowGroups(*out)
+    _check_ordinary(ids=ids)
     at, bits = _ids(ids, "ids")
     if at.dim() not in (1, 2) or (at.dim() == 2 and at.shape[1] == 0):
         raise ValueError(f"ids must have shape (n,) or (n, m) with m > 0, got {tuple(at.shape)}")
@@ -355,6 +383,7 @@ class _FromClusters(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
         y, weights, *groups = ctx.saved_tensors
+        _check_ordinary(grad=grad, y=y, weights=weights, **_named(groups))
         grad_y, grad_weights = _from_clusters_grad(grad, y, RowGroups(*groups), weights, ctx.needs_input_grad[0], ctx.needs_input_grad[1])
         return grad_y, grad_weights, None, None, None
 
@@ -366,6 +395,7 @@ def to_clusters(x: torch.Tensor, groups: RowGroups) -> torch.Tensor:
     out = _calls.to_clusters(x, *groups)
     if out is not None:
         return out
+    _check_ordinary(x=x, **_named(groups))
     if _wants_grad(x):
         return _ToClusters.apply(x, *groups)
     return _to_clusters(x, groups)
@@ -375,7 +405,10 @@ def to_clusters_grad(grad: torch.Tensor, groups: RowGroups) -> torch.Tensor:
     """Gradient of the rows of to_clusters: the sum over a row's choices of their slots' gradients (n x d), without those that have no
     cluster."""
     out = _calls.from_clusters(grad, *groups, None)
-    return _from_clusters(grad, groups, None, "grad") if out is None else out
+    if out is not None:
+        return out
+    _check_ordinary(grad=grad, **_named(groups))
+    return _from_clusters(grad, groups, None, "grad")
 
 
 def from_clusters(y: torch.Tensor, groups: RowGroups, weights: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -385,6 +418,7 @@ def from_clusters(y: torch.Tensor, groups: RowGroups, weights: Optional[torch.Te
     out = _calls.from_clusters(y, *groups, weights)
     if out is not None:
         return out
+    _check_ordinary(y=y, weights=weights, **_named(groups))
     if _wants_grad(y, weights):
         return _FromClusters.apply(y, weights, *groups)
     return _from_clusters(y, groups, weights)
@@ -394,7 +428,10 @@ def from_clusters_grad(grad: torch.Tensor, y: torch.Tensor, groups: RowGroups, w
     """Gradients of from_clusters: of y, weights[i, j] * grad[i] at position[i, j] and zeros in the slots of choices without a cluster; and of the
     weights (float32; None where there are none), <grad[i], y[position[i, j]]>."""
     out = _calls.from_clusters_grad(grad, y, *groups, weights)
-    return _from_clusters_grad(grad, y, groups, weights, True, weights is not None) if out is None else out
+    if out is not None:
+        return out
+    _check_ordinary(grad=grad, y=y, weights=weights, **_named(groups))
+    return _from_clusters_grad(grad, y, groups, weights, True, weights is not None)
 
 
 # ---- products in 8 bits ---------------------------------------------------------------------------------------------------------
@@ -407,6 +444,7 @@ def quantize_rows(x: torch.Tensor) -> QuantizedRows:
     out = _calls.quantize_rows(x)
     if out is not None:
         return QuantizedRows(*out)
+    _check_ordinary(x=x)
     rows, n, d, ld, kind = _rows(x, "x")
     if n > _MOST:
         raise ValueError("x must have no more than 2**31 - 1 rows")
@@ -440,6 +478,7 @@ def product_8bit(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_sca
     out = _calls.product_8bit(x, x_scales, w, w_scales, offsets, kind)
     if out is not None:
         return out
+    _check_ordinary(x=x, x_scales=x_scales, w=w, w_scales=w_scales, offsets=offsets)
     _on_gpu(x, "x")
     _on_gpu(w, "w", x)
     if x.dim() != 2:

@@ -1,0 +1,23 @@
+"""More of the operators on rows in device memory (superkmeans_b200.ops): tensors that torch holds in other ways, paths and sums that
+test_row_ops_gpu.py does not reach.  Its helpers and its counting of roundings are used here too."""
+import pytest
+import torch
+
+from tests.test_row_ops_gpu import TYPES, U, as_index, check_product, close, ops, pitched, randn, rng, rounding, some_bytes, some_ids   # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+def test_tensors_without_memory(ops):
+    """A storage that was freed, as sharded training does with parameters, is refused by the host; so is one freed before the backward pass."""
+    table, ids = randn(rng(1), 20, 8), some_ids(rng(2), 30, 20)
+    part = table[1:]
+    table.untyped_storage().resize_(0)
+    for call in (lambda: ops.lookup(part, ids), lambda: ops.quantize_rows(part), lambda: ops.lookup(part.requires_grad_(), ids)):
+        with pytest.raises(ValueError, match="has no memory"):
+            call()
+    y, w = randn(rng(3), 30, 8), randn(rng(4), 30).requires_grad_()
+    out = ops.from_clusters(y, ops.group_rows(ids, 20), w)
+    y.untyped_storage().resize_(0)
+    with pytest.raises(ValueError, match="has no memory"):
+        out.sum().backward()

@@ -1,0 +1,86 @@
+"""Tensors that the operators on rows cannot take as they are (superkmeans_b200.ops): refused before anything is asked of their device, so that
+no GPU is needed here."""
+import pytest
+import torch
+
+from superkmeans_b200 import ops as _ops
+
+
+@pytest.fixture(params=["short cuts", "ctypes"])
+def ops(request, monkeypatch):
+    if request.param == "ctypes":
+
+        class Nothing:
+            def __getattr__(self, _):
+                return lambda *_: None
+
+        monkeypatch.setattr(_ops, "_calls", Nothing())
+    return _ops
+
+
+def calls(ops, change):
+    """Every operator with one of its tensors put through `change`: (what is changed, call)."""
+
+    def make():
+        x, ids, s = torch.ones(6, 8), torch.zeros(6, dtype=torch.int32), torch.ones(6)
+        q = torch.ones(6, 8, dtype=torch.int8)
+        groups = ops.RowGroups(torch.arange(6, dtype=torch.int32), torch.arange(6, dtype=torch.int32), torch.tensor([0, 6], dtype=torch.int32))
+        return x, ids, s, q, groups
+
+    def swapped(groups, i):
+        parts = list(groups)
+        parts[i] = change(parts[i])
+        return ops.RowGroups(*parts)
+
+    x, ids, s, q, groups = make()
+    yield "table", lambda: ops.lookup(change(x), ids, 1.0, s)
+    yield "ids", lambda: ops.lookup(x, change(ids))
+    yield "row_scales", lambda: ops.lookup(x, ids, 1.0, change(s))
+    yield "grad", lambda: ops.lookup_grad(change(x), ids, 3)
+    yield "ids", lambda: ops.lookup_grad(x, change(ids), 3)
+    yield "row_scales", lambda: ops.lookup_grad(x, ids, 3, 1.0, change(s))
+    yield "table", lambda: ops.lookup_scale_grad(x, change(x), ids)
+    yield "ids", lambda: ops.group_rows(change(ids), 3)
+    yield "x", lambda: ops.to_clusters(change(x), groups)
+    yield "y", lambda: ops.from_clusters(change(x), groups)
+    yield "weights", lambda: ops.from_clusters(x, groups, change(s))
+    yield "grad", lambda: ops.to_clusters_grad(change(x), groups)
+    yield "y", lambda: ops.from_clusters_grad(x, change(x), groups, s)
+    yield "weights", lambda: ops.from_clusters_grad(x, x, groups, change(s))
+    for i, name in enumerate(groups._fields):
+        yield name, lambda i=i: ops.to_clusters(x, swapped(groups, i))
+        yield name, lambda i=i: ops.from_clusters(x, swapped(groups, i), s)
+    yield "x", lambda: ops.quantize_rows(change(x))
+    yield "x", lambda: ops.product_8bit(change(q), s, q, s)
+    yield "w_scales", lambda: ops.product_8bit(q, s, q, change(s))
+
+
+def part_of_a_freed_storage(t):
+    room = torch.cat([t.reshape(-1)[:1], t.reshape(-1)])
+    part = room[1:].view(t.shape)
+    room.untyped_storage().resize_(0)
+    return part
+
+
+def part_of_a_shortened_storage(t):
+    room = t.clone()
+    room.untyped_storage().resize_(room.untyped_storage().nbytes() - room.element_size())
+    return room
+
+
+def zeros_without_memory(t):
+    return torch._efficientzerotensor((*t.shape[:-1], t.shape[-1] + 1), dtype=t.dtype)[..., 1:]
+
+
+@pytest.mark.parametrize("change", [part_of_a_freed_storage, part_of_a_shortened_storage, zeros_without_memory])
+def test_tensors_without_memory_are_refused(ops, change):
+    """(The address of a part of a storage that was freed is its distance from the storage's beginning: a kernel would follow it.)"""
+    for name, call in calls(ops, change):
+        with pytest.raises(ValueError, match=f"{name} has no memory"):
+            call()
+
+
+def test_empty_and_spread_out_tensors_have_memory(ops):
+    x = torch.ones(3, 4)
+    for t in (x, x[1:], x[:0], x.t(), x[:1].expand(5, 4), x[1, 2], torch.empty(0), torch.empty(5, 0), x[2:, 3:]):
+        ops._check_ordinary(t=t)
