@@ -108,6 +108,7 @@ def _rows(t, name: str, like=None, dtype=None) -> Tuple[torch.Tensor, int, int, 
     n, d = shape
     if d == 0:
         raise ValueError(f"{name} must have at least one column")
+    t = t.resolve_neg()   # (the imaginary part of a conjugate is a view whose values are the negatives of what lies there)
     ld, step = t.stride()
     if step != 1 and d > 1:
         t = t.contiguous()
@@ -131,6 +132,7 @@ def _floats(t, name: str, shape, like) -> torch.Tensor:
         raise ValueError(f"{name} must have dtype float32, got {t.dtype}")
     if tuple(t.shape) != tuple(shape):
         raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+    t = t.resolve_neg()
     return t if t.is_contiguous() else t.contiguous()
 
 

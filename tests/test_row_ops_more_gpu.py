@@ -21,3 +21,13 @@ def test_tensors_without_memory(ops):
     y.untyped_storage().resize_(0)
     with pytest.raises(ValueError, match="has no memory"):
         out.sum().backward()
+
+
+def test_imaginary_parts_of_conjugates(ops):
+    z = torch.complex(randn(rng(5), 40, 1), randn(rng(6), 40, 1)).conj().imag
+    plain, ids = -(-z), some_ids(rng(7), 40, 40)
+    assert z.is_neg() and not plain.is_neg()
+    groups = ops.group_rows(ids, 40)
+    for f in (lambda t: ops.lookup(t, ids), lambda t: ops.lookup_grad(t, ids, 40), lambda t: ops.to_clusters(t, groups), lambda t: ops.quantize_rows(t).values,
+              lambda t: ops.lookup(plain, ids[:1], 1.0, t[:1, 0]), lambda t: ops.from_clusters(plain[:1], ops.group_rows(ids[:1], 40), t[:1, 0])):
+        assert torch.equal(f(z), f(plain))

@@ -84,3 +84,15 @@ def test_empty_and_spread_out_tensors_have_memory(ops):
     x = torch.ones(3, 4)
     for t in (x, x[1:], x[:0], x.t(), x[:1].expand(5, 4), x[1, 2], torch.empty(0), torch.empty(5, 0), x[2:, 3:]):
         ops._check_ordinary(t=t)
+
+
+def test_imaginary_parts_of_conjugates_are_read_with_their_sign(monkeypatch):
+    """(A view, and a contiguous one where there is one column or one number: what lies in its memory has the other sign.)"""
+    monkeypatch.setattr(_ops, "_on_gpu", lambda *_: None)
+    part = torch.complex(torch.ones(5, 2), torch.arange(10.0).reshape(5, 2)).conj().imag
+    assert part.is_neg()
+    for t in (part, part[:, :1], part[1:2, :1]):
+        rows, n, d, ld, _ = _ops._rows(t, "x")
+        assert not rows.is_neg() and (n, d) == t.shape and torch.equal(rows.as_strided((n, d), (ld, 1)), -(-t))
+        one = _ops._floats(t, "weights", t.shape, t)
+        assert not one.is_neg() and one.is_contiguous() and torch.equal(one, -(-t))
