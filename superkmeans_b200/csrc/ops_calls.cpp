@@ -30,7 +30,7 @@ bool has_memory(const at::Tensor& t) {
 
 // Nothing that a call has to refuse whatever it goes on to ask for.
 bool is_ordinary(const at::Tensor& t) {
-    return t.defined() && t.layout() == at::kStrided && !t.unsafeGetTensorImpl()->is_python_dispatch() && has_memory(t);
+    return t.defined() && t.layout() == at::kStrided && !t.unsafeGetTensorImpl()->is_python_dispatch() && !t._fw_grad(0).defined() && has_memory(t);
 }
 
 bool plain(PyObject* o) {

@@ -12,13 +12,15 @@ device (which need not be the current device), allocates its outputs and its wor
 captured into a CUDA graph.  Calls with tensors that need no conversion take a short cut in C++ (csrc/ops_calls.cpp), which answers None
 where there is something to refuse, copy or record; those are made here.  Tensors that are used on another stream than the one they were made on need `record_stream`, as with
 any operator of torch.  Rows may have any distance from one another; the values of a row lie side by side, or the rows are copied
-first.  Arguments that do not fit raise ValueError, and so do tensors whose memory is not there (a storage that was freed).
+first.  Arguments that do not fit raise ValueError, and so do tensors whose memory is not there (a storage that was freed).  Gradients are
+those of `backward`; a tensor that carries a derivative forward (torch.autograd.forward_ad, torch.func.jvp) raises NotImplementedError.
 """
 from __future__ import annotations
 
 from typing import NamedTuple, Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from ._lib import check, lib
 
@@ -82,6 +84,8 @@ def _check_ordinary(**tensors) -> None:
         return
     for name, t in tensors.items():
         if isinstance(t, torch.Tensor):
+            if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError(f"{name} carries a derivative forward, which the operators on rows would lose: use backward, or unpack_dual")
             _check_memory(t, name)
 
 

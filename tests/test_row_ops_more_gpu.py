@@ -31,3 +31,17 @@ def test_imaginary_parts_of_conjugates(ops):
     for f in (lambda t: ops.lookup(t, ids), lambda t: ops.lookup_grad(t, ids, 40), lambda t: ops.to_clusters(t, groups), lambda t: ops.quantize_rows(t).values,
               lambda t: ops.lookup(plain, ids[:1], 1.0, t[:1, 0]), lambda t: ops.from_clusters(plain[:1], ops.group_rows(ids[:1], 40), t[:1, 0])):
         assert torch.equal(f(z), f(plain))
+
+
+def test_derivatives_carried_forward(ops):
+    table, ids, w = randn(rng(8), 20, 8), some_ids(rng(9), 30, 20), randn(rng(10), 30)
+    groups = ops.group_rows(ids, 20)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(table, table)
+        rows = torch.autograd.forward_ad.make_dual(randn(rng(11), 30, 8), randn(rng(12), 30, 8))
+        for call in (lambda: ops.lookup(dual, ids), lambda: ops.lookup(dual[1:], ids), lambda: ops.lookup(table, ids, 1.0, rows[:, 0].contiguous()), lambda: ops.to_clusters(rows, groups),
+                     lambda: ops.from_clusters(rows, groups, w), lambda: ops.from_clusters(table.repeat(2, 1)[:30], groups, rows[:, 1].contiguous()), lambda: ops.quantize_rows(rows)):
+            with pytest.raises(NotImplementedError, match="derivative forward"):
+                call()
+        assert torch.equal(ops.lookup(torch.autograd.forward_ad.unpack_dual(dual).primal, ids), ops.lookup(table, ids))
+    assert torch.equal(ops.lookup(dual, ids), ops.lookup(table, ids))   # (the level has ended, and the derivative with it)

@@ -96,3 +96,20 @@ def test_imaginary_parts_of_conjugates_are_read_with_their_sign(monkeypatch):
         assert not rows.is_neg() and (n, d) == t.shape and torch.equal(rows.as_strided((n, d), (ld, 1)), -(-t))
         one = _ops._floats(t, "weights", t.shape, t)
         assert not one.is_neg() and one.is_contiguous() and torch.equal(one, -(-t))
+
+
+def test_derivatives_carried_forward_are_refused(ops):
+    """(A result without its tangent would be taken for a constant.)"""
+    with torch.autograd.forward_ad.dual_level():
+
+        def dual(t):
+            return torch.autograd.forward_ad.make_dual(t, torch.ones_like(t)) if t.is_floating_point() else t
+
+        seen = 0
+        for name, call in calls(ops, dual):
+            if name in ("table", "row_scales", "grad", "weights", "y", "w_scales"):
+                seen += 1
+                with pytest.raises(NotImplementedError, match=f"{name} carries a derivative forward"):
+                    call()
+        assert seen >= 10
+        ops._check_ordinary(t=torch.ones(3), ids=torch.zeros(3, dtype=torch.int32))
