@@ -5,8 +5,10 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/TracerMode.h>
 #include <ATen/core/LegacyTypeDispatch.h>
 #include <ATen/core/grad_mode.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -134,9 +136,15 @@ PyObject* failed(skm_status status) {
     return nullptr;
 }
 
+// Whether torch looks on as calls are made, some of whose ways to do so ops.py refuses.
+bool is_watched() {
+    return at::tracer::impl::is_dispatch_enabled() || c10::impl::TorchDispatchModeTLS::any_modes_set() || c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::PreDispatch);
+}
+
 // An exception of torch's (no memory) is the caller's to meet again.
 template <class F>
 PyObject* shortcut(F&& f) {
+    if (is_watched()) return none();
     // (no gradient is recorded here: allocations and views go straight to what makes them)
     const at::AutoDispatchBelowADInplaceOrView direct;
     try {

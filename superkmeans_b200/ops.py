@@ -13,7 +13,9 @@ captured into a CUDA graph.  Calls with tensors that need no conversion take a s
 where there is something to refuse, copy or record; those are made here.  Tensors that are used on another stream than the one they were made on need `record_stream`, as with
 any operator of torch.  Rows may have any distance from one another; the values of a row lie side by side, or the rows are copied
 first.  Arguments that do not fit raise ValueError, and so do tensors whose memory is not there (a storage that was freed).  Gradients are
-those of `backward`; a tensor that carries a derivative forward (torch.autograd.forward_ad, torch.func.jvp) raises NotImplementedError.
+those of `backward`.  NotImplementedError is raised for what torch would record or carry along without the operators' part: tensors with a
+derivative forward (torch.autograd.forward_ad), torch.jit.trace, make_fx and other tracing with fake tensors, transforms of torch.func.
+(torch.compile breaks its graph at a call, and a CUDA graph captures it.)
 """
 from __future__ import annotations
 
@@ -78,12 +80,25 @@ def _named(groups) -> dict:
     return dict(zip(RowGroups._fields, groups))
 
 
+# Modes of torch in which an allocation is recorded, or made as a shape only, and what a kernel writes into it is not.
+_RECORDERS = [getattr(torch._C._TorchDispatchModeKey, name) for name in ("PROXY", "FAKE", "FUNCTIONAL")]
+
+
+def _is_recorded() -> bool:
+    return (torch._C._get_tracing_state() is not None or torch._ops._len_torch_dispatch_stack_pre_dispatch() > 0
+            or any(torch._C._get_dispatch_mode(key) is not None for key in _RECORDERS))
+
+
 def _check_ordinary(**tensors) -> None:
     """What no call can do without, whatever it goes on to ask for."""
     if _calls.ordinary(*tensors.values()):
         return
+    if _is_recorded():
+        raise NotImplementedError("the operators on rows are not recorded by torch.jit.trace, make_fx or tracing with fake tensors: a trace would hold their outputs as allocations only")
     for name, t in tensors.items():
         if isinstance(t, torch.Tensor):
+            if torch._C._functorch.is_functorch_wrapped_tensor(t) or torch._is_functional_tensor(t):
+                raise NotImplementedError(f"{name} is a tensor of a torch.func transform, which the operators on rows do not take")
             if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
                 raise NotImplementedError(f"{name} carries a derivative forward, which the operators on rows would lose: use backward, or unpack_dual")
             _check_memory(t, name)

@@ -45,3 +45,30 @@ def test_derivatives_carried_forward(ops):
                 call()
         assert torch.equal(ops.lookup(torch.autograd.forward_ad.unpack_dual(dual).primal, ids), ops.lookup(table, ids))
     assert torch.equal(ops.lookup(dual, ids), ops.lookup(table, ids))   # (the level has ended, and the derivative with it)
+
+
+def test_where_torch_records_or_looks_on(ops):
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    table, ids = randn(rng(13), 20, 8), some_ids(rng(14), 30, 20)
+    want = ops.lookup(table, ids)
+    for record in (lambda: torch.jit.trace(lambda t: ops.lookup(t, ids), (table,)), lambda: make_fx(lambda t: ops.lookup(t, ids))(table),
+                   lambda: make_fx(lambda t: ops.lookup(t[1:], ids), tracing_mode="fake")(table), lambda: torch.func.vmap(lambda t: ops.lookup(t, ids))(table[None]),
+                   lambda: torch.func.functionalize(lambda t: ops.lookup(t[1:], ids))(table)):
+        with pytest.raises(NotImplementedError):
+            record()
+
+    class LooksOn(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+
+    with LooksOn():
+        assert torch.equal(ops.lookup(table, ids), want)
+        t = table.clone().requires_grad_()
+        ops.lookup(t, ids).sum().backward()
+    assert torch.equal(t.grad, ops.lookup_grad(torch.ones_like(want), ids, 20))
+    for t in (table, table.clone().requires_grad_()):
+        assert torch.equal(torch.compile(lambda t: ops.lookup(t + 0, ids) * 1, backend="eager")(t), want)
+    with torch.inference_mode():
+        assert torch.equal(ops.lookup(table, ids), want)

@@ -113,3 +113,53 @@ def test_derivatives_carried_forward_are_refused(ops):
                     call()
         assert seen >= 10
         ops._check_ordinary(t=torch.ones(3), ids=torch.zeros(3, dtype=torch.int32))
+
+
+def test_calls_are_refused_where_torch_records_them(ops):
+    """(A trace would hold the allocation of the output and nothing else, and give back memory as it finds it.)"""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    x, ids = torch.ones(6, 8), torch.zeros(6, dtype=torch.int32)
+    fs = [lambda t: ops.lookup(t, ids), lambda t: ops.lookup(t[1:], ids), lambda t: ops.lookup_grad(t, ids, 3), lambda t: ops.lookup_scale_grad(t, t, ids),
+          lambda t: ops.group_rows(t[:, 0].int(), 3).order, lambda t: ops.to_clusters(t, (ids, ids, ids)), lambda t: ops.from_clusters(t, (ids, ids, ids)),
+          lambda t: ops.to_clusters_grad(t, (ids, ids, ids)), lambda t: ops.from_clusters_grad(t, t, (ids, ids, ids)), lambda t: ops.quantize_rows(t).values,
+          lambda t: ops.product_8bit(t.to(torch.int8), t[:, 0], t.to(torch.int8), t[:, 0])]
+    for f in fs:
+        with pytest.raises(NotImplementedError, match="not recorded"):
+            torch.jit.trace(f, (x,))
+        for how in (dict(tracing_mode="real"), dict(tracing_mode="fake"), dict(tracing_mode="symbolic"), dict(pre_dispatch=True)):
+            with pytest.raises(NotImplementedError, match="not recorded"):
+                make_fx(f, **how)(x)
+        with pytest.raises(NotImplementedError, match="torch.func"):
+            torch.func.functionalize(f)(x)
+    for f in (fs[0], fs[2], fs[5], fs[9]):
+        with pytest.raises(NotImplementedError, match="torch.func"):
+            torch.func.vmap(f)(torch.ones(2, 6, 8))
+        with pytest.raises(NotImplementedError, match="torch.func"):
+            torch.func.jvp(f, (x,), (x,))
+        with pytest.raises(NotImplementedError, match="torch.func"):
+            torch.func.grad(lambda t: f(t).sum())(x)
+
+
+def test_fake_tensors_are_refused(ops):
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with FakeTensorMode():
+        fake, ids = torch.empty(6, 8, device="cuda"), torch.empty(6, device="cuda", dtype=torch.int32)
+        with pytest.raises(NotImplementedError, match="not recorded"):
+            ops.lookup(fake[1:], ids)
+    with pytest.raises(ValueError, match="table has no memory"):
+        ops.lookup(fake, ids)
+
+
+def test_modes_that_only_look_on_are_none_of_ours(ops):
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class LooksOn(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+
+    with LooksOn():
+        ops._check_ordinary(t=torch.ones(3))
+        with pytest.raises(ValueError, match="CUDA"):
+            ops.lookup(torch.ones(3, 4), torch.zeros(2, dtype=torch.int32))
