@@ -5,6 +5,7 @@
 // tcgen05.mma of kind::i8, in two kernels.  Few rows: the matrix's rows ("channels") are the 128 lanes of the accumulator, the rows of x
 // ("rows") its columns, so that the accumulator is as narrow as there are rows; one row of 768 by 16 384 channels takes 5.4 us.  Many:
 // pairs of CTAs, below.
+#include <atomic>
 #include <map>
 #include <mutex>
 #include <string>
@@ -192,11 +193,37 @@ struct ProductParams {
     uint32_t groups;             // 0: none
     const RowTile* tiles;        // with groups
     const uint32_t* n_tiles;     // that belong to a group, and all
-    int* error;
+    uint32_t* given_up;          // the launch whose wait ran out last
+    uint32_t launch;             // this one: no two have the same number, but for the replays of a graph
     int* told;                   // in host memory
     long long wait_limit;
     uint32_t producer_stop;
 };
+
+// A bounded wait.  One that runs out ends the others of its launch, and those only: what runs beside it on another stream, or after it
+// before anybody was told, is a launch of its own.
+__device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, const ProductParams& p) {
+    if (mbar_try_wait(bar, parity)) return true;
+    const long long t0 = clock64();
+    uint32_t spins = 0;
+    while (!mbar_try_wait(bar, parity)) {
+        if ((++spins & 1023u) == 0) {
+            volatile uint32_t* given_up = p.given_up;
+            if (*given_up == p.launch) return false;
+            if (clock64() - t0 > p.wait_limit) {
+                *given_up = p.launch;
+                return false;
+            }
+        }
+    }
+    return true;
+}
+// A replay of a graph has the number of the one before: what that one may have left is cleared by a thread that has nothing else to do, while the first waits begin
+// (a wait looks at it after a thousand polls, some milliseconds).
+__device__ __forceinline__ void forget_the_replay_before(const ProductParams& p) {
+    volatile uint32_t* given_up = p.given_up;
+    if (blockIdx.x == 0 && *given_up == p.launch) *given_up = 0;
+}
 
 template <int ROWS>
 struct ProductControl {
@@ -318,7 +345,6 @@ __global__ void __launch_bounds__(P_THREADS) product_kernel(const __grid_constan
     const uint32_t smem_base = raw_addr + pad;
     auto* ctrl = reinterpret_cast<ProductControl<ROWS>*>(smem + P_STAGES * kStageBytes<ROWS>);
     constexpr uint32_t COLS = ROWS < 32 ? 32 : ROWS;
-    const WaitCtx wctx{p.error, p.wait_limit};
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t split = cluster_size(), rank = cluster_rank();
 
@@ -362,7 +388,7 @@ __global__ void __launch_bounds__(P_THREADS) product_kernel(const __grid_constan
         const int w_row = static_cast<int>(t.group * p.m + channel_tile * P_CHANNELS), x_row = static_cast<int>(t.row0);
         for (uint32_t k = k0, it = 0; k < k1; ++k, ++it) {
             const uint32_t s = it % P_STAGES, ph = (it / P_STAGES) & 1u;
-            if ((p.producer_stop != 0 && it >= p.producer_stop) || !mbar_wait(&ctrl->empty[s], ph ^ 1u, wctx, 41)) {
+            if ((p.producer_stop != 0 && it >= p.producer_stop) || !wait_for(&ctrl->empty[s], ph ^ 1u, p)) {
                 ok = false;
                 break;
             }
@@ -375,7 +401,7 @@ __global__ void __launch_bounds__(P_THREADS) product_kernel(const __grid_constan
         constexpr uint32_t idesc = make_idesc_i8(P_CHANNELS, ROWS);
         for (uint32_t k = k0, it = 0; k < k1; ++k, ++it) {
             const uint32_t s = it % P_STAGES, ph = (it / P_STAGES) & 1u;
-            if (!mbar_wait(&ctrl->full[s], ph, wctx, 42)) {
+            if (!wait_for(&ctrl->full[s], ph, p)) {
                 ok = false;
                 break;
             }
@@ -386,9 +412,11 @@ __global__ void __launch_bounds__(P_THREADS) product_kernel(const __grid_constan
             umma_commit(&ctrl->empty[s]);
         }
         if (ok) umma_commit(&ctrl->done);
+    } else if (threadIdx.x == P_THREADS - 1) {
+        forget_the_replay_before(p);
     }
     __syncwarp();
-    const bool summed = __all_sync(0xffffffffu, mbar_wait(&ctrl->done, 0, wctx, 43));
+    const bool summed = __all_sync(0xffffffffu, wait_for(&ctrl->done, 0, p));
     if (!summed && lane == 0) *reinterpret_cast<volatile int*>(p.told) = 43;
     if (!ok) {
         // a millisecond for the copies that are in flight before the block's memory is let go
@@ -500,7 +528,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Q_THREADS, 1) produc
     constexpr int STAGES = kPairStages<LANES_ARE_ROWS>;
     constexpr uint32_t TRAYS_AT = STAGES * kPairStageBytes<COLS>;
     auto* ctrl = reinterpret_cast<PairControl<COLS>*>(smem + TRAYS_AT + (LANES_ARE_ROWS ? Q_EPI_WARPS * Q_TRAY_BYTES : 0));
-    const WaitCtx wctx{p.error, p.wait_limit};
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank();
     constexpr uint32_t ROWS = LANES_ARE_ROWS ? 256 : COLS, CHANNELS = LANES_ARE_ROWS ? COLS : 256;   // of a tile
@@ -549,7 +576,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Q_THREADS, 1) produc
             if (t + step < n_tiles) next = tile_at(t + step, next_channel0);
             for (uint32_t k = 0; k < p.depth_blocks; ++k, ++it) {
                 const uint32_t s = it % STAGES, ph = (it / STAGES) & 1u;
-                if ((p.producer_stop != 0 && it >= p.producer_stop) || !mbar_wait(&ctrl->empty[s], ph ^ 1u, wctx, 44)) {
+                if ((p.producer_stop != 0 && it >= p.producer_stop) || !wait_for(&ctrl->empty[s], ph ^ 1u, p)) {
                     ok = false;
                     break;
                 }
@@ -570,14 +597,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Q_THREADS, 1) produc
         uint32_t it = 0, i = 0;
         for (uint32_t t = first; t < n_tiles && ok; t += step, ++i) {
             const uint32_t b = i & 1u, acc = tmem_base + b * 256;
-            if (!mbar_wait(&ctrl->acc_empty[b], ((i >> 1) & 1u) ^ 1u, wctx, 45)) {
+            if (!wait_for(&ctrl->acc_empty[b], ((i >> 1) & 1u) ^ 1u, p)) {
                 ok = false;
                 break;
             }
             tc_fence_after();
             for (uint32_t k = 0; k < p.depth_blocks; ++k, ++it) {
                 const uint32_t s = it % STAGES, ph = (it / STAGES) & 1u;
-                if (!mbar_wait(&ctrl->full[s], ph, wctx, 46)) {
+                if (!wait_for(&ctrl->full[s], ph, p)) {
                     ok = false;
                     break;
                 }
@@ -589,6 +616,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Q_THREADS, 1) produc
             }
             if (ok) umma_commit_pair(&ctrl->acc_full[b]);
         }
+    } else if (threadIdx.x == 127) {
+        forget_the_replay_before(p);
     } else if (warp >= 4) {
         constexpr uint32_t MINE = COLS / 2, EACH = MINE / 32;   // columns of a warp
         const uint32_t quarter = warp & 3u, half = (warp - 4) >> 2;
@@ -639,7 +668,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Q_THREADS, 1) produc
             for (uint32_t e = 0; e < EACH; ++e) scales[e * 32 + lane] = scale[e];
             __syncwarp();
             if (t + step < n_tiles) look_up(t + step);
-            if (!__all_sync(0xffffffffu, mbar_wait(&ctrl->acc_full[b], (i >> 1) & 1u, wctx, 47))) {
+            if (!__all_sync(0xffffffffu, wait_for(&ctrl->acc_full[b], (i >> 1) & 1u, p))) {
                 if (lane == 0) *reinterpret_cast<volatile int*>(p.told) = 47;
                 break;
             }
@@ -748,14 +777,15 @@ __global__ void __launch_bounds__(1024) row_tiles_kernel(const uint32_t* __restr
     if (threadIdx.x == 0) n_tiles[1] = min(base, room);
 }
 
-// Where a kernel records that a wait ran out: for the kernels in device memory, for the host in its own.
+// Where a kernel records that a wait ran out: for its other waits in device memory, for the host in its own.
 struct Status {
-    int* device = nullptr;
+    uint32_t* device = nullptr;
     int* host = nullptr;
     int* host_on_device = nullptr;
 };
 constexpr int kMaxDevices = 64;
-__device__ int g_product_error;   // (in host code a handle, no address)
+__device__ uint32_t g_product_given_up;   // (in host code a handle, no address)
+std::atomic<uint32_t> g_product_launches{0};
 
 Status& status_of_current_device() {
     static std::mutex mutex;
@@ -770,8 +800,8 @@ Status& status_of_current_device() {
         cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
         SKM_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
         void* word = nullptr;
-        cudaError_t e = cudaGetSymbolAddress(&word, g_product_error);
-        s.device = static_cast<int*>(word);
+        cudaError_t e = cudaGetSymbolAddress(&word, g_product_given_up);
+        s.device = static_cast<uint32_t*>(word);
         if (e == cudaSuccess && !s.host) e = cudaHostAlloc(&s.host, sizeof(int), cudaHostAllocMapped | cudaHostAllocPortable);
         if (e == cudaSuccess) {
             *s.host = 0;
@@ -789,13 +819,10 @@ void throw_if_told(Status& s, cudaStream_t stream) {
     volatile int* told = s.host;
     if (*told == 0) return;
     const int code = *told;
-    // (under capture the word would be cleared by each replay instead of now: that is left to the next call outside)
+    // (a capture that fails for this is told, and so is the next call outside)
     cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
     SKM_CUDA(cudaStreamIsCapturing(stream, &capture));
-    if (capture == cudaStreamCaptureStatusNone) {
-        *told = 0;
-        SKM_CUDA(cudaMemsetAsync(s.device, 0, sizeof(int), stream));
-    }
+    if (capture == cudaStreamCaptureStatusNone) *told = 0;
     throw CudaError("a product in 8 bits gave up waiting on a barrier (code " + std::to_string(code) + "): its results are not valid");
 }
 
@@ -924,7 +951,9 @@ void launch_product(const Product& p, void* workspace, cudaStream_t stream) {
     const uint32_t channels = plan.pairs ? 256 : P_CHANNELS;
     k.channel_tiles = static_cast<uint32_t>((p.m + channels - 1) / channels);
     k.groups = static_cast<uint32_t>(p.groups);
-    k.error = status.device;
+    k.given_up = status.device;
+    do k.launch = ++g_product_launches;
+    while (k.launch == 0);   // (no launch)
     k.told = status.host_on_device;
     k.wait_limit = wait_limit();
     k.producer_stop = producer_stop();

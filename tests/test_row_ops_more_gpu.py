@@ -72,3 +72,53 @@ def test_where_torch_records_or_looks_on(ops):
         assert torch.equal(torch.compile(lambda t: ops.lookup(t + 0, ids) * 1, backend="eager")(t), want)
     with torch.inference_mode():
         assert torch.equal(ops.lookup(table, ids), want)
+
+
+@pytest.mark.parametrize("n,m", [(300, 500), (2000, 1200)])   # (one CTA to a tile, and pairs)
+def test_a_wait_that_ran_out_ends_no_other_launch(ops, n, m):
+    """What a launch that gave up leaves behind must not end the waits of the next one, whether or not anybody was told, and on whatever stream: that
+    one's own waits run their time (here all of it, as the injection stops its producer too)."""
+    from superkmeans_b200 import _lib
+
+    g = rng(15)
+    x, w, xs, ws = some_bytes(g, n, 4096), some_bytes(g, m, 4096), torch.ones(n, device="cuda"), torch.ones(m, device="cuda")
+    cycles = 100_000_000   # 50 ms at 2 GHz
+
+    def gives_up(call):
+        start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        start.record()
+        call()
+        end.record()
+        end.synchronize()
+        return start.elapsed_time(end)
+
+    def told():
+        with pytest.raises(RuntimeError, match="gave up waiting"):
+            ops.product_8bit(x, xs, w, ws)
+
+    busy, other = torch.cuda.Stream(), torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    ops.product_8bit(x, xs, w, ws)
+    torch.cuda.synchronize()
+    _lib.check(_lib.lib.skm_debug_wait_injection(cycles, 1))
+    try:
+        assert gives_up(lambda: ops.product_8bit(x, xs, w, ws)) >= 40
+        with torch.cuda.stream(busy):   # told while this stream has other work
+            torch.cuda._sleep(2_000_000_000)
+            told()
+        with torch.cuda.stream(other):
+            assert gives_up(lambda: ops.product_8bit(x, xs, w, ws)) >= 40
+            assert not busy.query(), "the other stream should still be busy"
+            told()
+            with torch.cuda.graph(graph, stream=other):
+                ops.product_8bit(x, xs, w, ws)
+            for _ in range(3):
+                assert gives_up(graph.replay) >= 40
+            told()
+    finally:
+        _lib.check(_lib.lib.skm_debug_wait_injection(0, 0))
+        torch.cuda.synchronize()
+    ops.check_products()
+    check_product(ops.product_8bit(x, xs, w, ws, dtype=torch.float32), x, xs, w, ws, torch.float32)
+    torch.cuda.synchronize()
+    ops.check_products()
