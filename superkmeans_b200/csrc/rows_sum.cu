@@ -7,6 +7,11 @@
 // launch adds the partial sums of each id in the order of their tiles and writes the zeros of ids that nobody took.  Nothing depends on
 // the order of atomics.
 //
+// No chain of sums in 32 bits is long, so that fp32 results keep their last places: eight rows are added to one another and then to the
+// eights before (32 in a tile), partial sums eight at most, or four at a time and the fours in 64 bits.  A sum of any length is off by less than
+// 50 roundings (of few pairs 80) of the sum of the magnitudes; as one chain of a tile's rows and one of the tiles it was off by hundreds.  A
+// million positive normal values come out as if rounded once (rms 0.36 of 2^-24; 3.1 before).  Sums of eights in 64 bits too were 10 % slower.
+//
 // One B200, 500 000 x 1024 bf16 into 16 384 rows: the tiles 162 us, 1.07 GB at 6.6 TB/s (HBM; where runs begin is found for 32 pairs by
 // a ballot: with a comparison for each pair the same took 263), the joins 10, the sort 34.
 #include "rows_access.cuh"
@@ -60,6 +65,10 @@ struct Sums {
 #pragma unroll
         for (int i = 0; i < N; ++i) v[i] = fmaf(f, x.v[i], v[i]);
     }
+    __device__ __forceinline__ void add(const Sums& other) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] += other.v[i];
+    }
     // the first `count` of them
     template <typename O>
     __device__ __forceinline__ void store_some(O* to, float scale, uint32_t count) const {
@@ -100,9 +109,10 @@ struct Lane {
     }
 };
 
-// SCALED: each pair with a factor of its own; otherwise the sums are scaled.
+// SCALED: each pair with a factor of its own; otherwise the sums are scaled.  (Blocks to an SM: 500 000 x 1024 bf16 with factors 227 us where the
+// compiler is told to fit five, 239 where it is not; without factors 213 and 229.  Windows, 112 749 x 39 bf16: 27.6 where told one, 30.2 where not.)
 template <typename T, typename O, int BYTES, bool WINDOWS, bool SCALED, int LANES>
-__global__ void __launch_bounds__(32 * kWarps) sum_tiles_kernel(const SumParams p) {
+__global__ void __launch_bounds__(32 * kWarps, WINDOWS ? 1 : SCALED && LANES == 32 && BYTES == 16 ? 5 : 0) sum_tiles_kernel(const SumParams p) {
     wait_for_the_one_before();
     constexpr uint32_t AHEAD = kAhead;
     using S = Sums<T, BYTES>;
@@ -141,18 +151,23 @@ __global__ void __launch_bounds__(32 * kWarps) sum_tiles_kernel(const SumParams 
                 c[u] = chunk.load(grad + pair * p.pitch);
             }
             const uint32_t here = begins >> u0 & ((1u << AHEAD) - 1);
+            S eight;
+            eight.clear();
             if (here == 0 && u0 + AHEAD <= count) {
 #pragma unroll
                 for (uint32_t u = 0; u < AHEAD; ++u) {
-                    if (SCALED) sum.add(c[u], lanes.from(my_factor, u0 + u));
-                    else sum.add(c[u]);
+                    if (SCALED) eight.add(c[u], lanes.from(my_factor, u0 + u));
+                    else eight.add(c[u]);
                 }
+                sum.add(eight);
                 continue;
             }
 #pragma unroll
             for (uint32_t u = 0; u < AHEAD; ++u) {
                 const float f = SCALED ? lanes.from(my_factor, u0 + u) : 1.f;
                 if (here >> u & 1) {
+                    sum.add(eight);
+                    eight.clear();
                     if (mine) {
                         if (first) sum.template store<float>(first_part, scale);
                         else chunk.store(sum, static_cast<O*>(p.out) + static_cast<size_t>(now) * p.d + at, scale);
@@ -162,24 +177,44 @@ __global__ void __launch_bounds__(32 * kWarps) sum_tiles_kernel(const SumParams 
                     now = lanes.from(my_key, u0 + u);
                 }
                 if (u0 + u < count) {
-                    if (SCALED) sum.add(c[u], f);
-                    else sum.add(c[u]);
+                    if (SCALED) eight.add(c[u], f);
+                    else eight.add(c[u]);
                 }
             }
+            sum.add(eight);
         }
     }
     if (mine) sum.template store<float>(first ? first_part : first_part + p.apart, scale);
 }
+
+// Partial sums are added four at a time, and the fours of ids that have many in 64 bits (there may be thousands, and a chain of so many in 32
+// bits is off by many steps of the last place).
+template <int N>
+struct Total {
+    double v[N];
+
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = 0.0;
+    }
+    template <class S>
+    __device__ __forceinline__ S rounded() const {
+        S sum;
+#pragma unroll
+        for (int i = 0; i < N; ++i) sum.v[i] = static_cast<float>(v[i]);
+        return sum;
+    }
+};
 
 // Up to 32 ids and 32 chunks to a warp; ids whose pairs fill many tiles are taken by all eight warps of a block together.
 constexpr int kJoinWarps = 8;
 constexpr uint32_t kLongRun = 8;   // tiles
 
 template <typename T, typename O, int BYTES, bool WINDOWS>
-__global__ void __launch_bounds__(32 * kJoinWarps) join_tiles_kernel(const SumParams p) {
+__global__ void __launch_bounds__(32 * kJoinWarps, 4) join_tiles_kernel(const SumParams p) {
     wait_for_the_one_before();
     using S = Sums<T, BYTES>;
-    __shared__ float parts[kJoinWarps][32][S::N + 1];
+    __shared__ double parts[kJoinWarps][32][S::N + 1];
     __shared__ uint32_t long_ids[kJoinWarps];
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t block0 = blockIdx.x * (p.join_ids * kJoinWarps), id0 = block0 + warp * p.join_ids, col = blockIdx.y * 32 + lane;
@@ -198,7 +233,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_tiles_kernel(const SumPa
         t1 = end > begin ? (end - 1) / p.tile + 1 : t0;
         todo = !(t1 == t0 + 1 && begin > t0 * p.tile && end < min(static_cast<size_t>(t1) * p.tile, static_cast<size_t>(held)));
     }
-    auto add_tiles = [&](S& sum, uint32_t from, uint32_t to, uint32_t first) {
+    auto add_tiles = [&](auto& sum, uint32_t from, uint32_t to, uint32_t first) {
         constexpr uint32_t AHEAD = 4;
         for (uint32_t t = from; t < to; t += AHEAD) {
             constexpr int EACH = S::N < 4 ? S::N : 4;   // floats of a load
@@ -211,16 +246,24 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_tiles_kernel(const SumPa
                 for (int i = 0; i < S::N / EACH; ++i)
                     v[u][i].from(t + u < to && mine ? load_new(reinterpret_cast<const Chunk<EACH * 4>*>(src) + i) : zero_chunk<EACH * 4>());
             }
+            if constexpr (std::is_same_v<std::decay_t<decltype(sum)>, S>) {
 #pragma unroll
-            for (uint32_t u = 0; u < AHEAD; ++u)
+                for (uint32_t u = 0; u < AHEAD; ++u)
 #pragma unroll
-                for (int i = 0; i < S::N; ++i) sum.v[i] += v[u][i / EACH].v[i % EACH];
+                    for (int i = 0; i < S::N; ++i) sum.v[i] += v[u][i / EACH].v[i % EACH];
+            } else {
+#pragma unroll
+                for (int i = 0; i < S::N; ++i) {
+                    auto of = [&](uint32_t u) { return v[u][i / EACH].v[i % EACH]; };
+                    sum.v[i] += (of(0) + of(1)) + (of(2) + of(3));
+                }
+            }
         }
     };
     const uint32_t long_here = __ballot_sync(0xffffffffu, todo && t1 - t0 > kLongRun);
     for (uint32_t left = __ballot_sync(0xffffffffu, todo) & ~long_here; left; left &= left - 1) {
         const int l = __ffs(left) - 1;
-        S sum;
+        S sum;   // (two fours at most)
         sum.clear();
         add_tiles(sum, __shfl_sync(0xffffffffu, t0, l), __shfl_sync(0xffffffffu, t1, l), __shfl_sync(0xffffffffu, begin, l));
         if (mine) chunk.store(sum, out + static_cast<size_t>(id0 + l) * p.d, 1.f);
@@ -232,7 +275,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_tiles_kernel(const SumPa
             const uint32_t id = block0 + w * p.join_ids + __ffs(left) - 1;
             const uint32_t first = load_new(p.offsets + id), from0 = first / p.tile, to0 = (load_new(p.offsets + id + 1) - 1) / p.tile + 1;
             const uint32_t share = (to0 - from0 + kJoinWarps - 1) / kJoinWarps, from = min(from0 + warp * share, to0);
-            S sum;
+            Total<S::N> sum;
             sum.clear();
             add_tiles(sum, from, min(from + share, to0), first);
 #pragma unroll
@@ -243,7 +286,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_tiles_kernel(const SumPa
                 for (int q = 1; q < kJoinWarps; ++q)
 #pragma unroll
                     for (int e = 0; e < S::N; ++e) sum.v[e] += parts[q][lane][e];
-                if (mine) chunk.store(sum, out + static_cast<size_t>(id) * p.d, 1.f);
+                if (mine) chunk.store(sum.template rounded<S>(), out + static_cast<size_t>(id) * p.d, 1.f);
             }
             __syncthreads();
         }
@@ -294,9 +337,12 @@ __global__ void __launch_bounds__(32 * kFewWarps) sum_few_kernel(const SumParams
                 c[u] = chunk.load(grad + pair * p.pitch);
                 f[u] = p.row_scales ? p.scale * load_now(p.row_scales + pair) : p.scale;
             }
+        S eight;
+        eight.clear();
 #pragma unroll
         for (uint32_t u = 0; u < kAhead; ++u)
-            if (s + u < count) sum.add(c[u], f[u]);
+            if (s + u < count) eight.add(c[u], f[u]);
+        sum.add(eight);
     }
     if (lane == 0) counts[warp] = count;
     if (count != 0)

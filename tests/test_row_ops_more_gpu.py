@@ -122,3 +122,20 @@ def test_a_wait_that_ran_out_ends_no_other_launch(ops, n, m):
     check_product(ops.product_8bit(x, xs, w, ws, dtype=torch.float32), x, xs, w, ws, torch.float32)
     torch.cuda.synchronize()
     ops.check_products()
+
+
+@pytest.mark.parametrize("n,k,small,roundings", [
+    (4096, 1, 2.0**-25, 80),           # one launch: eight rows, the 64 eights of a warp, eight warps
+    (1_300_000, 5, 2.0**-25, 50),      # tiles: eight rows, 32 eights, their factor; and eight tiles at most, or fours of them in 64 bits
+    (1_024_000, 100_000, 2.0**-33, 50),   # (the rows of a tile add up to half a step of one: a chain of tiles loses them all)
+])
+@pytest.mark.parametrize("scaled", [False, True])
+def test_sums_of_many_rows_keep_their_last_places(ops, n, k, small, roundings, scaled):
+    """One row of ones and many of less than half of one's last place each, all for one id: a chain of sums in 32 bits stays at one."""
+    grad = torch.full((n, 8), small, device="cuda")
+    grad[0] = 1.0
+    ids = torch.full((n,), k - 1, dtype=torch.int32, device="cuda")
+    got = ops.lookup_grad(grad, ids, k, 1.0, torch.ones(n, device="cuda") if scaled else None)
+    want = torch.zeros(k, 8, dtype=torch.float64, device="cuda")
+    want[k - 1] = 1.0 + (n - 1) * small
+    close(got, want, roundings * U * want)
