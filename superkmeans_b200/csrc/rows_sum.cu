@@ -361,15 +361,18 @@ __global__ void __launch_bounds__(32 * kFewWarps) sum_few_kernel(const SumParams
 bool few(size_t n, size_t k, size_t d, Type type) { return n <= kFewSumPairs && k * ((d * type_bytes(type) + 511) / 512) <= 4096; }
 
 // Pairs to a tile: enough tiles to fill the chip several times over (148 SMs, 16 warps each), and no shorter than it takes to keep the
-// partial sums' traffic below the rows'.
-uint32_t tile_pairs(size_t n, size_t slabs) {
+// partial sums' traffic below the rows'.  Of narrow rows, which have eight lanes to a tile, twice as many tiles: 2M x 3 fp32 by 1000 ids 83 us (with as many
+// as of wide rows 104, with four times as many 78), 1M x 64 bf16 by 300, half of them one's, 166 (124 and 326: more partial sums to join).
+uint32_t tile_pairs(size_t n, size_t slabs, bool narrow) {
     uint32_t tile = 256;
-    while (tile > 16 && (n + tile - 1) / tile * slabs < 148 * 32) tile /= 2;
+    while (tile > 16 && (n + tile - 1) / tile * slabs < 148 * (narrow ? 64 : 32)) tile /= 2;
     return tile;
 }
 
 // (a chunk is at most 16 bytes: with narrower ones there are more slabs, and tiles no shorter)
-size_t slabs_of(size_t d, Type type, int bytes) { return (d * type_bytes(type) / bytes + 31) / 32; }
+size_t slabs_of(size_t d, Type type, int bytes) { return ((d * type_bytes(type) + bytes - 1) / bytes + 31) / 32; }
+
+uint32_t tile_pairs(size_t n, size_t d, Type type) { return tile_pairs(n, slabs_of(d, type, 16), d * type_bytes(type) <= 8 * 16); }
 
 size_t rounded(size_t bytes) { return (bytes + 255) / 256 * 256; }
 size_t whole_chunks(size_t d) { return (d + 7) / 8 * 8; }
@@ -378,7 +381,7 @@ size_t whole_chunks(size_t d) { return (d + 7) / 8 * 8; }
 
 size_t lookup_grad_workspace_bytes(size_t n, size_t k, size_t d, Type type) {
     if (few(n, k, d, type)) return 0;
-    const size_t tile = tile_pairs(n, slabs_of(d, type, 16)), tiles = (n + tile - 1) / tile;
+    const size_t tile = tile_pairs(n, d, type), tiles = (n + tile - 1) / tile;
     return rounded(n * 4) * 2 + rounded((k + 1) * 4) + rounded(tiles * 2 * whole_chunks(d) * 4) + rounded(group_workspace_bytes(n, k));
 }
 
@@ -402,7 +405,7 @@ void launch_lookup_grad(const Rows& grad, Type type, size_t k, size_t d, const I
         uint32_t* order = reinterpret_cast<uint32_t*>(take(n * 4));
         uint32_t* keys = reinterpret_cast<uint32_t*>(take(n * 4));
         uint32_t* offsets = reinterpret_cast<uint32_t*>(take((k + 1) * 4));
-        p.tile = tile_pairs(n, slabs_of(d, type, 16));
+        p.tile = tile_pairs(n, d, type);
         tiles = (n + p.tile - 1) / p.tile;
         p.partials = reinterpret_cast<float*>(take(tiles * 2 * whole_chunks(d) * 4));
         launch_group(ids, n, k, order, nullptr, keys, offsets, at, stream);

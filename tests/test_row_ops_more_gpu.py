@@ -139,3 +139,17 @@ def test_sums_of_many_rows_keep_their_last_places(ops, n, k, small, roundings, s
     want = torch.zeros(k, 8, dtype=torch.float64, device="cuda")
     want[k - 1] = 1.0 + (n - 1) * small
     close(got, want, roundings * U * want)
+
+
+@pytest.mark.parametrize("dtype,d", [(torch.float32, 3), (torch.float32, 1), (torch.bfloat16, 7), (torch.float16, 2)])
+@pytest.mark.parametrize("k", [20, 3000])
+def test_gradients_of_a_million_narrow_rows(ops, dtype, d, k):
+    n = 1_300_000
+    g = rng(n + d)
+    ids, grad = some_ids(g, n, k, skew=True), randn(g, n, d, dtype=dtype)
+    i = as_index(ids, k)
+    held = i >= 0
+    want = torch.zeros(k, d, dtype=torch.float64, device="cuda").index_add_(0, i[held], grad.double()[held])
+    size = torch.zeros(k, d, dtype=torch.float64, device="cuda").index_add_(0, i[held], grad.double()[held].abs())
+    for out in {dtype, torch.float32}:
+        close(ops.lookup_grad(grad, ids, k, dtype=out), want, rounding(want, out, 50 * U * size))

@@ -163,3 +163,14 @@ def test_modes_that_only_look_on_are_none_of_ours(ops):
         ops._check_ordinary(t=torch.ones(3))
         with pytest.raises(ValueError, match="CUDA"):
             ops.lookup(torch.ones(3, 4), torch.zeros(2, dtype=torch.int32))
+
+
+@pytest.mark.parametrize("dtype,d", [(0, 1), (0, 3), (0, 4), (1, 1), (1, 7), (2, 8)])
+def test_the_workspace_of_narrow_rows_is_mostly_lists(dtype, d):
+    """Two lists of n numbers and what sorts them, the ids' first slots, and for every 256 rows two of partial sums (8 floats, as rows are rounded up)."""
+    from superkmeans_b200._lib import lib
+
+    n, k = 100_000_000, 1000
+    tiles = -(-n // 256)
+    most = 2 * 4 * n + lib.skm_op_group_rows_workspace(n, k) + 4 * (k + 1) + tiles * 2 * 8 * 4
+    assert lib.skm_op_lookup_grad_workspace(n, k, d, dtype) <= most + 5 * 256
