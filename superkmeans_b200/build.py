@@ -1,7 +1,8 @@
 """Builds libskm_b200.so in-tree with nvcc for sm_100a.  Run as `python superkmeans_b200/build.py` (by path: importing the package needs the library).
 
-`_ops_calls.so`, the short cuts of ops.py into that library, is built beside it where torch and Python's headers are there; ops.py
-works without.
+`_ops_calls`, the short cuts of ops.py into that library, is built beside it where torch and Python's headers are there; ops.py works without,
+and so does this where it cannot be compiled or linked (a torch without CUDA).  It is made for one torch and one Python, whose names it carries: it is
+built again for others, and ops.py leaves one that was built for others alone.
 
 Every source file is compiled to an object of its own (in parallel, and only when it or a header changed), then the
 objects are linked into the shared library.  `-v` prints what ptxas reports (registers, spills, shared memory)."""
@@ -9,6 +10,7 @@ from __future__ import annotations
 
 import importlib.util
 import os
+import runpy
 import shutil
 import subprocess
 import sys
@@ -24,7 +26,8 @@ HEADERS = ["common.cuh", "device_utils.cuh", "gemm_simt.cuh", "tc_ptx.cuh", "ker
            os.path.join("..", "..", "include", "skm_b200.h")]
 OUTPUT = os.path.join(HERE, "libskm_b200.so")
 CALLS_SOURCE = os.path.join(CSRC, "ops_calls.cpp")
-CALLS_OUTPUT = os.path.join(HERE, "_ops_calls.so")
+CALLS_OUTPUT = os.path.join(HERE, "_ops_calls" + sysconfig.get_config_var("EXT_SUFFIX"))
+CALLS_BUILT_FOR = os.path.join(HERE, "_ops_calls.built_for")
 
 
 def _nvcc() -> str:
@@ -67,31 +70,57 @@ def _compile_one(nvcc: str, src: str, verbose: bool):
     return src, obj, res
 
 
-def _stale_calls() -> bool:
-    if not os.path.exists(CALLS_OUTPUT):
+def _torch_dir():
+    found = importlib.util.find_spec("torch")
+    return None if found is None else os.path.dirname(found.origin)
+
+
+def calls_built_for(torch_dir: str) -> str:
+    """The torch and the Python that the short cuts are made for (ops.py says the same of those that it runs with)."""
+    version = runpy.run_path(os.path.join(torch_dir, "version.py"))
+    return f"torch {version['__version__']}, CUDA {version['cuda']}, {sysconfig.get_config_var('SOABI')}"
+
+
+def _stale_calls(built_for: str) -> bool:
+    if not os.path.exists(CALLS_OUTPUT) or not os.path.exists(CALLS_BUILT_FOR):
         return True
+    with open(CALLS_BUILT_FOR) as f:
+        if f.read() != built_for:
+            return True
     header = os.path.join(CSRC, "..", "..", "include", "skm_b200.h")
     return max(os.path.getmtime(CALLS_SOURCE), os.path.getmtime(header)) > os.path.getmtime(CALLS_OUTPUT)
 
 
 def build_calls(force: bool = False) -> None:
     """The short cuts between torch tensors and the library (needs the library)."""
-    if not force and not _stale_calls():
-        return
     include = sysconfig.get_paths()["include"]
-    found = importlib.util.find_spec("torch")
-    if found is None or not os.path.exists(os.path.join(include, "Python.h")):
+    torch_dir = _torch_dir()
+    if torch_dir is None or not os.path.exists(os.path.join(include, "Python.h")):
         sys.stderr.write("torch or Python.h is missing: ops.py goes without its short cuts\n")
         return
-    torch_dir = os.path.dirname(found.origin)
-    cuda = os.path.dirname(os.path.dirname(os.path.realpath(_nvcc())))
-    cmd = ["/usr/bin/g++", "-std=c++17", "-O2", "-fPIC", "-shared", "-Wall", f"-I{include}", f"-I{torch_dir}/include", f"-I{torch_dir}/include/torch/csrc/api/include",
-           f"-I{cuda}/include", CALLS_SOURCE, "-o", CALLS_OUTPUT, f"-L{torch_dir}/lib", "-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10", "-lc10_cuda", f"-L{HERE}", "-lskm_b200",
-           "-Wl,-rpath,$ORIGIN"]
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    if res.returncode != 0:
-        sys.stderr.write(res.stdout + res.stderr)
-        raise RuntimeError("compiling ops_calls.cpp failed")
+    built_for = calls_built_for(torch_dir)
+    if not force and not _stale_calls(built_for):
+        return
+    for old in (CALLS_OUTPUT, CALLS_BUILT_FOR, os.path.join(HERE, "_ops_calls.so")):   # (the last: of a build that named no Python)
+        if os.path.exists(old):
+            os.remove(old)
+    try:
+        import torch
+
+        cuda = os.path.dirname(os.path.dirname(os.path.realpath(_nvcc())))
+        cmd = ["/usr/bin/g++", "-std=c++17", "-O2", "-fPIC", "-shared", "-Wall", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f'-DSKM_BUILT_FOR="{built_for}"',
+               f"-I{include}", f"-I{torch_dir}/include", f"-I{torch_dir}/include/torch/csrc/api/include",
+               f"-I{cuda}/include", CALLS_SOURCE, "-o", CALLS_OUTPUT, f"-L{torch_dir}/lib", "-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10", "-lc10_cuda", f"-L{HERE}", "-lskm_b200",
+               "-Wl,-rpath,$ORIGIN"]
+        res = subprocess.run(cmd, capture_output=True, text=True)
+        failed = res.stdout + res.stderr if res.returncode != 0 else None
+    except (ImportError, OSError) as e:
+        failed = f"{e}\n"
+    if failed is not None:
+        sys.stderr.write(failed + "compiling ops_calls.cpp failed: ops.py goes without its short cuts\n")
+        return
+    with open(CALLS_BUILT_FOR, "w") as f:
+        f.write(built_for)
 
 
 def build(force: bool = False, verbose: bool = False) -> str:

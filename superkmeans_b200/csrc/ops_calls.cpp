@@ -343,4 +343,12 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_ops_calls", nullptr, -1, methods,
 
 } // namespace
 
-PyMODINIT_FUNC PyInit__ops_calls() { return PyModule_Create(&module); }
+// `built_for` says for which torch and Python: the layouts of their objects are compiled in.
+PyMODINIT_FUNC PyInit__ops_calls() {
+    PyObject* made = PyModule_Create(&module);
+    if (made && PyModule_AddStringConstant(made, "built_for", SKM_BUILT_FOR) < 0) {
+        Py_DECREF(made);
+        return nullptr;
+    }
+    return made;
+}

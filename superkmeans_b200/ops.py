@@ -19,6 +19,7 @@ derivative forward (torch.autograd.forward_ad), torch.jit.trace, make_fx and oth
 """
 from __future__ import annotations
 
+import sysconfig
 from typing import NamedTuple, Optional, Tuple
 
 import torch
@@ -28,7 +29,10 @@ from ._lib import check, lib
 
 try:
     from . import _ops_calls as _calls
-except ImportError:   # (not built, or for another torch: every call takes the way through ctypes)
+
+    if _calls.built_for != f"torch {torch.__version__}, CUDA {torch.version.cuda}, {sysconfig.get_config_var('SOABI')}":
+        raise ImportError(f"the short cuts were built for {_calls.built_for}")
+except (ImportError, AttributeError):   # (not built, or for another torch or Python: every call takes the way through ctypes)
 
     class _calls:   # noqa: N801
         ordinary = lookup = lookup_grad = lookup_scale_grad = group_rows = to_clusters = from_clusters = from_clusters_grad = quantize_rows = product_8bit = staticmethod(lambda *_: None)
