@@ -153,3 +153,144 @@ def test_gradients_of_a_million_narrow_rows(ops, dtype, d, k):
     size = torch.zeros(k, d, dtype=torch.float64, device="cuda").index_add_(0, i[held], grad.double()[held].abs())
     for out in {dtype, torch.float32}:
         close(ops.lookup_grad(grad, ids, k, dtype=out), want, rounding(want, out, 50 * U * size))
+
+
+# ---- paths of the product by cluster: tiles of 16, 32 and 64 rows, and pairs of CTAs with 128 columns (groups of 65 - 191 rows) or 256
+
+GROUPED = [
+    (200, 20, 77, 48), (3000, 120, 300, 64), (3001, 120, 129, 200), (2500, 50, 1000, 96),   # 10, 25 and 50 rows a group
+    (12_000, 100, 520, 129), (12_000, 100, 521, 160), (9001, 70, 1024, 64),                 # 120 and 129: pairs, odd and even numbers of channels
+    (20_000, 40, 528, 300), (20_000, 40, 521, 96), (16_384, 64, 1040, 128),                 # 500 and 256: rows or channels in lanes
+]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,e,m,d", GROUPED)
+@pytest.mark.parametrize("skew", [False, True])
+def test_product_by_cluster_of_every_type(ops, dtype, n, e, m, d, skew):
+    g = rng(n + e + m)
+    ids = some_ids(g, n, e, lost=0.1, skew=skew)
+    ids[ids == e // 2] = -1   # (a cluster that nobody has)
+    groups = ops.group_rows(ids, e)
+    x, w, xs, ws = some_bytes(g, n, d), some_bytes(g, e, m, d), torch.exp(randn(g, n)) / 4096, torch.exp(randn(g, e, m)) / 64
+    xs[int(groups.offsets[-1]):] = float("nan")   # rows of no cluster: zeros, whatever their scales
+    pitch = -(-d // 16) * 16
+    got = ops.product_8bit(pitched(x, pitch), xs, pitched(w, pitch), ws, groups.offsets, dtype=dtype)
+    ends = groups.offsets.tolist()
+    for c in range(e):
+        a, b = ends[c], ends[c + 1]
+        check_product(got[a:b], x[a:b], xs[a:b], w[c], ws[c], dtype)
+    assert not got[ends[-1]:].any()
+    assert torch.equal(ops.product_8bit(x, xs, w, ws, groups.offsets, dtype=dtype), got)   # (rows that are copied first)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,m", [(40, 33), (9000, 520)])
+def test_product_of_rows_ahead_of_the_first_cluster(ops, dtype, n, m):
+    """Offsets of one's own may begin behind the first row and end before the last; clusters without rows lie at either end."""
+    g = rng(n)
+    x, w, xs, ws = some_bytes(g, n, 64), some_bytes(g, 5, m, 64), torch.exp(randn(g, n)) / 512, torch.exp(randn(g, 5, m)) / 512
+    ends = [n // 10, n // 10, n // 2, n // 2, n - 3, n - 3]
+    got = ops.product_8bit(x, xs, w, ws, torch.tensor(ends, dtype=torch.int32, device="cuda"), dtype=dtype)
+    for c in range(5):
+        check_product(got[ends[c]:ends[c + 1]], x[ends[c]:ends[c + 1]], xs[ends[c]:ends[c + 1]], w[c], ws[c], dtype)
+    assert not got[:ends[0]].any() and not got[ends[-1]:].any()
+
+
+# ---- gradients of scales and weights: eight lanes to a row and 32, chunks of 16 bytes and less, windows
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [2, 4, 8, 16, 20, 24, 33, 64, 72, 128, 136, 137, 256, 512, 768, 1024, 1032, 2048])
+def test_lookup_scale_grad_of_every_width(ops, dtype, d):
+    g = rng(d)
+    n, k = 501, 40
+    grad, table, ids = randn(g, n, d, dtype=dtype), randn(g, k, d, dtype=dtype), some_ids(g, n, k)
+    i = as_index(ids, k)
+    parts = torch.where((i >= 0)[:, None], grad.double() * table.double()[i.clamp(min=0)], 0.0) * 0.75
+    want = parts.sum(1)
+    close(ops.lookup_scale_grad(grad, table, ids, 0.75), want, rounding(want, torch.float32, (d + 2) * U * parts.abs().sum(1)))
+    # and of the weights of the way back: <grad[i], y[position]>
+    groups = ops.group_rows(ids[:500].reshape(250, 2), k)
+    up, y, w = randn(g, 250, d, dtype=dtype), randn(g, 500, d, dtype=dtype), randn(g, 250, 2)
+    there = (as_index(ids[:500], k) >= 0).reshape(250, 2)
+    parts = torch.where(there[..., None], up.double()[:, None] * y.double()[groups.position.long()], 0.0)
+    close(ops.from_clusters_grad(up, y, groups, w)[1], parts.sum(2), rounding(parts.sum(2), torch.float32, (d + 1) * U * parts.abs().sum(2)))
+
+
+# ---- the radix sort of one pass
+
+
+@pytest.mark.parametrize("k", [1024, 1500, 2046])
+def test_many_pairs_of_few_thousand_clusters(ops, k):
+    """(One pass: the clusters' first slots come out of the sort itself, and its list of clusters goes to the gradient.)"""
+    n = 10_000_000
+    ids = some_ids(rng(k), n, k, lost=0.1)
+    i = as_index(ids, k)
+    key = torch.where(i >= 0, i, k)
+    order, position, offsets = ops.group_rows(ids, k)
+    want = torch.argsort(key, stable=True)
+    assert torch.equal(order.long(), want)
+    assert torch.equal(position.long()[want], torch.arange(n, device="cuda"))
+    counts = torch.bincount(key, minlength=k + 1)
+    assert torch.equal(offsets.long()[1:], counts[:k].cumsum(0)) and int(offsets[0]) == 0
+    grad = torch.randint(-8, 9, (n, 4), generator=rng(k + 1), device="cuda").float()
+    sums = torch.zeros(k + 1, 4, dtype=torch.float64, device="cuda").index_add_(0, key, grad.double())[:k]
+    assert torch.equal(ops.lookup_grad(grad, ids, k).double(), sums)   # (whole numbers of less than 2^24)
+
+
+# ---- as they are used
+
+
+def test_ids_that_an_engine_leaves_on_the_gpu(ops):
+    """Assignments stay on the device: as int32 or as the uint32 that they are, for lookup, grouping and gradient."""
+    import numpy as np
+
+    from superkmeans_b200 import Engine
+
+    n, k, d = 5000, 60, 32
+    rows = np.random.default_rng(1).standard_normal((n, d)).astype(np.float32)
+    engine = Engine(k, d)
+    centroids = engine.train(rows)
+    x, table = torch.from_numpy(rows).cuda(), torch.from_numpy(centroids).cuda()
+    want = torch.from_numpy(engine.assign(rows, centroids).astype(np.int64)).cuda()
+    for dtype in (torch.int32, torch.uint32):
+        ids = torch.empty(n, dtype=dtype, device="cuda")
+        engine.assign(x, table, n=n, on_device=True, out=ids)
+        assert torch.equal(as_index(ids, k), want)
+        assert torch.equal(ops.lookup(table, ids), table[want])
+        groups = ops.group_rows(ids, k)
+        assert torch.equal(groups.order.long(), torch.argsort(want, stable=True))
+        back = ops.from_clusters(ops.to_clusters(x, groups), groups)
+        assert torch.equal(back, x)
+        assert torch.equal(ops.lookup_grad(x, ids, k), ops.lookup_grad(x, want, k))
+
+
+def test_two_threads_that_may_fail(ops):
+    """Every turn of both threads ends, and with the right result."""
+    import threading
+
+    from tests.test_row_ops_gpu import make_run, whole_run
+
+    runs = [make_run(s) for s in (21, 22)]
+    want = [whole_run(ops, *r, 9) for r in runs]
+    grads = [ops.lookup_grad(r[0], r[1][:, 0], 9) for r in runs]
+    torch.cuda.synchronize()
+    done, wrong = [0, 0], []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(30):
+                    if not torch.equal(whole_run(ops, *runs[i], 9), want[i]) or not torch.equal(ops.lookup_grad(runs[i][0], runs[i][1][:, 0], 9), grads[i]):
+                        wrong.append((i, "another result"))
+                    done[i] += 1
+        except BaseException as e:
+            wrong.append((i, e))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong and done == [30, 30]
