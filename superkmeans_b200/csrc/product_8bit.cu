@@ -492,11 +492,12 @@ __global__ void __launch_bounds__(P_THREADS) product_kernel(const __grid_constan
 // 32 bytes at a time, or whole lines by way of shared memory.  Elsewhere, and where the tile is narrow because the groups are small, the
 // lanes are channels, and the 32 lanes of a warp store 32 neighbouring results of a row.
 //
-// One B200: 32 768 x 1024 by 10 000 channels to bf16 262 us, 2560 T/s, the tensor pipe 70 % busy (by 10 001 channels 302; to fp32 355; depth
-// 128: 112; depth 4096: 855, 3140 T/s; the single-CTA kernel 1269).  Power is the bound: the clock falls to 1.5 GHz, and operands of
-// zeros, which do not draw it, are through depth 4096 in 709 us.  Without results to store it would be 208.  Measured and not kept: rows
-// resident in shared memory while the channels pass (266), twice the epilogue warps (314), stores with other cache hints (the same).
-// 65 536 x 768 by 256 clusters of 768 channels 55 us, 302 MB of operands and results: HBM.
+// One B200: 32 768 x 1024 by 10 000 channels to bf16 262 us in a short run, 2560 T/s, the tensor pipe 70 % busy, and 310 in a long one, 2170 T/s.  In
+// short runs: by 10 001 channels 302; to fp32 355; depth 128: 112; depth 4096: 855, 3140 T/s; the single-CTA kernel 1269.  Power is the bound:
+// the clock falls to 1.5 GHz, and operands of zeros, which do not draw it, are through depth 4096 in 709 us.  Without results to store it
+// would be 208.  Measured and not kept: rows resident in shared memory while the channels pass (266), twice the epilogue warps (314), stores
+// with other cache hints (the same).  65 536 x 768 by 256 clusters of 768 channels 55 us where all clusters are of one size, 64 where they are
+// as a router makes them, 302 MB of operands and results: HBM.
 constexpr int Q_EPI_WARPS = 8;
 constexpr int Q_THREADS = 128 + 32 * Q_EPI_WARPS;
 constexpr uint32_t Q_TRAY_BYTES = 32 * 128;   // 32 rows of results on their way out, of each epilogue warp
@@ -852,6 +853,15 @@ struct ProductPlan {
     bool pairs, lanes_are_rows;
     uint32_t rows, split, row_tiles;   // row_tiles: with groups at most
 };
+// Which kernel and tile, by the rows that a matrix has on average (one B200, kernels alone, results in bf16, d = 768):
+//   pairs of CTAs from 65 rows and 64 tiles on.  By 16 384 channels (64 tiles and more) 64 rows take 5.7 us with a CTA to a tile and 6.0 with pairs, 65
+//   7.6 and 6.2, 256 12.3 and 7.2, 4096 155 and 47; by 4096 channels 256 rows (32 tiles) 5.6 and 6.0, 512 (64) 7.0 and 6.1, 1024 (128) 12.3 and 7.2.
+//   By 64 clusters of 768 channels each 64 rows 14.2 and 13.6, 65 20.3 and 14.0; by 256 clusters pairs would be ahead from 8 rows on (34 and 32; of 64
+//   55 and 37).
+//   256 columns from 192 rows on, 128 below: of 64 clusters 128 rows 14.4 us with 128 and 16.0 with 256, 192 rows 21.1 and 16.0 (between, 129 rows
+//   20.5 and 15.8: two tiles to a cluster); of 256 clusters 43.6 and 46.2, 59.5 and 50.0.
+//   Without pairs, 16, 32 or 64 rows to a tile, the least that hold them: of 64 clusters 16 rows take 10.5, 12.5 and 12.9 us, 17 14.8, 12.5 and 12.9, 33
+//   19.3, 18.1 and 13.9.
 ProductPlan make_plan(const Product& p) {
     const size_t channel_tiles = (p.m + P_CHANNELS - 1) / P_CHANNELS, depth_blocks = (p.d + P_DEPTH - 1) / P_DEPTH;
     const size_t typical = p.groups ? (p.n + p.groups - 1) / p.groups : p.n;
@@ -867,7 +877,8 @@ ProductPlan make_plan(const Product& p) {
     }
     plan.rows = typical <= 16 ? 16 : typical <= 32 ? 32 : 64;
     plan.row_tiles = static_cast<uint32_t>((p.n + plan.rows - 1) / plan.rows + (p.groups ? p.groups + 1 : 0));
-    // (adding the sums up costs two barriers of the cluster and 2 us: no block gets fewer than four steps)
+    // (adding the sums up costs two barriers of the cluster and 2 us: no block gets fewer than four steps; 64 rows by 1000 channels of depth 4096
+    // 6.8 us, 7.8 with eight steps at least, 12.3 undivided; 1 by 16 384 of 768, which has too many tiles to be divided, 4.9)
     if (!p.groups)
         while (plan.split < 8 && plan.row_tiles * channel_tiles * plan.split * 2 <= 148 && depth_blocks >= 8 * plan.split) plan.split *= 2;
     return plan;

@@ -271,7 +271,8 @@ def lookup(table: torch.Tensor, ids: torch.Tensor, scale: float = 1.0, row_scale
 def lookup_grad(grad: torch.Tensor, ids: torch.Tensor, n_rows: int, scale: float = 1.0, row_scales: Optional[torch.Tensor] = None,
                 dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """Gradient of a table of `n_rows` rows: row c is the sum of scale * row_scales[i] * grad[i] over ids[i] = c, zeros where there is no such
-    i.  Summed in fp32 in an order that depends on the ids alone, and rounded once to `dtype` (that of `grad`, or float32)."""
+    i.  Summed in fp32, in short chains and an order that depends on the ids alone, and rounded once to `dtype` (that of `grad`, or float32).
+    No gradient is recorded (nor by the other functions whose names end in _grad)."""
     if dtype is None:
         out = _calls.lookup_grad(grad, ids, n_rows, float(scale), row_scales)
         if out is not None:
@@ -463,9 +464,9 @@ def from_clusters_grad(grad: torch.Tensor, y: torch.Tensor, groups: RowGroups, w
 
 
 def quantize_rows(x: torch.Tensor) -> QuantizedRows:
-    """Rows in 8 bits: scales[i] = max |x[i]| / 127 (float32), values[i] = x[i] / scales[i] rounded to the nearest whole number, int8.  A row of
-    zeros has scale 0; a row with a value that is no finite number has scale NaN.  The rows of the result begin on 16 bytes.  No gradient is
-    recorded."""
+    """Rows in 8 bits: scales[i] = max |x[i]| / 127 (float32), values[i] = x[i] * (127 / max |x[i]|), both in float32, rounded to the nearest whole number,
+    int8.  A row of zeros has scale 0; a row with a value that is no finite number has scale NaN and zeros.  The rows of the result begin on 16
+    bytes.  No gradient is recorded."""
     out = _calls.quantize_rows(x)
     if out is not None:
         return QuantizedRows(*out)
