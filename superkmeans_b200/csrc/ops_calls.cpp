@@ -22,11 +22,16 @@ constexpr int64_t kMostIds = 0x7fffffff;
 
 // Whether the storage holds all that the tensor reaches (throws where there is none).
 bool has_memory(const at::Tensor& t) {
-    if (t.numel() == 0) return true;
+    const int64_t numel = t.numel();
+    if (numel == 0) return true;
     const c10::Storage& storage = t.storage();
     if (storage.device() != t.device() || t._is_zerotensor()) return false;
-    int64_t ends = t.storage_offset() + 1;
-    for (int64_t i = 0; i < t.dim(); ++i) ends += (t.size(i) - 1) * t.stride(i);
+    int64_t ends = t.storage_offset() + numel;
+    if (!t.is_contiguous()) {
+        const at::IntArrayRef sizes = t.sizes(), strides = t.strides();
+        ends = t.storage_offset() + 1;
+        for (size_t i = 0; i < sizes.size(); ++i) ends += (sizes[i] - 1) * strides[i];
+    }
     return storage.nbytes() >= static_cast<size_t>(ends) * t.element_size() && storage.data() != nullptr;
 }
 
