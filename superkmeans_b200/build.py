@@ -108,7 +108,7 @@ def build_calls(force: bool = False) -> None:
         import torch
 
         cuda = os.path.dirname(os.path.dirname(os.path.realpath(_nvcc())))
-        cmd = ["/usr/bin/g++", "-std=c++17", "-O2", "-fPIC", "-shared", "-Wall", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f'-DSKM_BUILT_FOR="{built_for}"',
+        cmd = ["/usr/bin/g++", "-std=c++17", "-O2", "-fPIC", "-shared", "-Wall", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", f'-DSKM_BUILT_FOR="{built_for}"',
                f"-I{include}", f"-I{torch_dir}/include", f"-I{torch_dir}/include/torch/csrc/api/include",
                f"-I{cuda}/include", CALLS_SOURCE, "-o", CALLS_OUTPUT, f"-L{torch_dir}/lib", "-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10", "-lc10_cuda", f"-L{HERE}", "-lskm_b200",
                "-Wl,-rpath,$ORIGIN"]

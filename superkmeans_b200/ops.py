@@ -84,13 +84,15 @@ def _named(groups) -> dict:
     return dict(zip(RowGroups._fields, groups))
 
 
-# Modes of torch in which an allocation is recorded, or made as a shape only, and what a kernel writes into it is not.
-_RECORDERS = [getattr(torch._C._TorchDispatchModeKey, name) for name in ("PROXY", "FAKE", "FUNCTIONAL")]
+# Modes of torch in which an allocation is recorded, or made as a shape only, and what a kernel writes into it is not.  (Another torch may have
+# other names for them.)
+_RECORDERS = [key for key in (getattr(getattr(torch._C, "_TorchDispatchModeKey", None), name, None) for name in ("PROXY", "FAKE", "FUNCTIONAL")) if key is not None]
+_modes_before_dispatch = getattr(torch._ops, "_len_torch_dispatch_stack_pre_dispatch", lambda: 0)
+_is_wrapped = getattr(torch._C._functorch, "is_functorch_wrapped_tensor", lambda _: False)
 
 
 def _is_recorded() -> bool:
-    return (torch._C._get_tracing_state() is not None or torch._ops._len_torch_dispatch_stack_pre_dispatch() > 0
-            or any(torch._C._get_dispatch_mode(key) is not None for key in _RECORDERS))
+    return torch.jit.is_tracing() or _modes_before_dispatch() > 0 or any(torch._C._get_dispatch_mode(key) is not None for key in _RECORDERS)
 
 
 def _check_ordinary(**tensors) -> None:
@@ -101,7 +103,7 @@ def _check_ordinary(**tensors) -> None:
         raise NotImplementedError("the operators on rows are not recorded by torch.jit.trace, make_fx or tracing with fake tensors: a trace would hold their outputs as allocations only")
     for name, t in tensors.items():
         if isinstance(t, torch.Tensor):
-            if torch._C._functorch.is_functorch_wrapped_tensor(t) or torch._is_functional_tensor(t):
+            if _is_wrapped(t) or torch._is_functional_tensor(t):
                 raise NotImplementedError(f"{name} is a tensor of a torch.func transform, which the operators on rows do not take")
             if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
                 raise NotImplementedError(f"{name} carries a derivative forward, which the operators on rows would lose: use backward, or unpack_dual")
